@@ -84,7 +84,7 @@ enum lse_query_key {
   LSE_Q_NOALLOC_SCRATCH = 5, /* bytes of the static scratch lse_w8a16_gemm_noalloc works in */
 };
 
-#define LSE_ABI_VERSION 13
+#define LSE_ABI_VERSION 14
 #define LSE_NOALLOC_SCRATCH_BYTES (32 << 20)
 #define LSE_K_ALIGN 16
 #define LSE_DECODE_MAX_M 64
@@ -372,6 +372,80 @@ int lse_rope_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride
                 int64_t pool_stride_slot, int64_t pool_stride_head, const int32_t* block_table,
                 int64_t block_table_stride, int64_t block_size, int64_t H, int64_t H_KV, int64_t D,
                 int64_t sequences, int64_t tokens_per_sequence, int64_t start, void* stream);
+
+/*
+ * Rotary positions of q and k rows from fp32 tables, in one launch. With pair i < rotary / 2 of a head at
+ * dims (i, i + rotary / 2), or (2 i, 2 i + 1) when interleaved is 1, and c, s the tables' values for the
+ * row's position and i:  a' = bf16(a c - b s), b' = bf16(b c + a s), products and sums rounded in fp32
+ * without fused forms; the dims from `rotary` on are copied.
+ * q: bf16, element (t, h, d) at t * q_stride_t + h * q_stride_h + d; k likewise with H_KV heads (NULL and
+ *   H_KV 0: no k). cos, sin: (table_rows, rotary / 2) fp32. positions: (tokens) int32; one outside the
+ *   tables gives NaN. q_out: (tokens, H, D), k_out: (tokens, H_KV, D) bf16, no other argument's memory.
+ * D % 16 == 0 up to 1024, rotary % 16 == 0; strides multiples of 8, 16-byte aligned pointers.
+ * Replaces: apply_rotary_pos_emb in `_project_qkv` (model_runner.py:310-326), for the layouts, partial
+ * rotations and scaled tables that the reference's models do not use.
+ */
+int lse_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+             int64_t k_stride_h, const float* cos, const float* sin, int64_t table_rows,
+             const int32_t* positions, void* q_out, void* k_out, int64_t tokens, int64_t H, int64_t H_KV,
+             int64_t D, int64_t rotary, int interleaved, void* stream);
+
+/*
+ * The 8-bit paged K/V cache. Codes are float8 e4m3 (448 the largest), and each group of 16 positions of a K/V
+ * head has one scale for k and one for v, powers of two as e8m0 bytes b = 2^(b - 127) (255 = NaN).
+ * With S = block_size / 16: k_pool, v_pool (blocks, H_KV, S, 16 D) bytes, `pool_stride_block` bytes from a
+ * block to the next; scales (blocks, H_KV, S, 2) bytes (k's, v's), scales_stride_block likewise. Position n
+ * of an entry lies in block block_table[n / block_size], group n % block_size / 16, slot n % 16; in a group
+ * k's element (slot, d) is byte ((slot / 4 * D / 64 + d / 64) * 4 + slot % 4) * 64 + d % 64, v's 16 d + slot.
+ *
+ * lse_append_kv_fp8 rotates a batch plan's new q and k rows (as lse_rope; rotary 0: not at all) and writes k
+ * and v at positions query_offset[e] + m, m < q_len[e], of every entry e, from rows q_start[e] + m.
+ *   scale of a group = the smallest power of two s >= 2^-126 with |x| <= 448 s for every finite new x (k
+ *     after its rotation, in fp32), and no less than the group's former scale where it holds positions
+ *     before query_offset[e]; those are kept, requantised if the scale grew;
+ *   code = rne_e4m3(x / s); infinity and NaN become NaN. Slots behind the last new position of a group are
+ *     zeroed, other groups are not touched.
+ * q (may be NULL), k, v: bf16, element (t, h, d) at t * stride_t + h * stride_h + d. q_out: (tokens, H, D)
+ *   bf16; rows of no entry are not written. Positions outside the table's max_blocks blocks, blocks outside
+ *   the pool and rows outside the `tokens` rows are dropped. Entries must own distinct rows, and the blocks they
+ *   write to must be theirs alone. max_q_len >= every q_len.
+ * D = 64 or 128; block_size % 16 == 0; strides of rows multiples of 8, pool_stride_block of 16; rows, tables
+ *   and pools 16-byte aligned.
+ * Replaces: apply_rotary_pos_emb and the K/V writes in `_project_qkv` and `attend_paged`
+ * (model_runner.py:310-363), for an 8-bit pool, which the reference does not have.
+ */
+int lse_append_kv_fp8(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                      int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                      int64_t v_stride_h, const float* cos, const float* sin, int64_t table_rows,
+                      void* q_out, void* k_pool, void* v_pool, int64_t pool_stride_block, void* scales,
+                      int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
+                      const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                      const int32_t* query_offset, const int32_t* q_start, const int32_t* q_len,
+                      int64_t entries, int64_t tokens, int64_t max_q_len, int64_t H, int64_t H_KV,
+                      int64_t D, int64_t rotary, int interleaved, void* stream);
+
+/*
+ * lse_paged_attention over the 8-bit cache: the same plan, semantics and determinism, k and v being the
+ * values code x scale. q and o have `tokens` rows; entries own distinct ones, and rows of no entry are not
+ * written. A block outside the pool makes the rows that see it NaN; a context longer than the table is cut.
+ * D = 64 or 128; 1 <= H / H_KV <= 16; block_size % 16 == 0; the strides of q and o multiples of 8, q, o and
+ * the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes (-1: invalid sizes),
+ * 16-byte aligned.
+ * Replaces: `paged_attention_forward` (src/llm_serving_engine/kernels/flash_attention.py:287-332) over a pool
+ * the reference does not have.
+ */
+int64_t lse_paged_attention_fp8_workspace_bytes(int64_t entries, int64_t tokens, int64_t H, int64_t H_KV,
+                                                int64_t D, int64_t max_q_len, int64_t max_blocks,
+                                                int64_t block_size);
+int lse_paged_attention_fp8(const void* q, int64_t q_stride_h, int64_t q_stride_t, const void* k_pool,
+                            const void* v_pool, int64_t pool_stride_block, const void* scales,
+                            int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
+                            const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                            const int32_t* context_len, const int32_t* query_offset,
+                            const int32_t* q_start, const int32_t* q_len, void* o, int64_t o_stride_h,
+                            int64_t o_stride_t, int64_t entries, int64_t tokens, int64_t max_q_len,
+                            int64_t H, int64_t H_KV, int64_t D, float softmax_scale, void* workspace,
+                            int64_t workspace_bytes, void* stream);
 
 /* Static properties (enum lse_query_key); -1 for an unknown key. Load-time checks read these,
  * as `ModelRunner.check_custom_kernel_support` (model_runner.py:77-94) checks its kernels. */

@@ -45,6 +45,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lse_add_rmsnorm": (_INT, [_P, _I64, _P, _I64, _P, ctypes.c_float, _P, _P, _I64, _I64, _P]),
     "lse_rope_kv": (_INT, [_P, _I64] * 3 + [_P, _P, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _P]
                     + [_I64] * 3 + [_P] + [_I64] * 8 + [_P]),
+    "lse_rope": (_INT, [_P, _I64, _I64, _P, _I64, _I64, _P, _P, _I64, _P, _P, _P] + [_I64] * 5
+                 + [_INT, _P]),
+    "lse_append_kv_fp8": (_INT, [_P, _I64, _I64] * 3 + [_P, _P, _I64, _P, _P, _P, _I64, _P]
+                          + [_I64] * 3 + [_P, _I64, _I64, _P, _P, _P] + [_I64] * 7 + [_INT, _P]),
+    "lse_paged_attention_fp8_workspace_bytes": (_I64, [_I64] * 8),
+    "lse_paged_attention_fp8": (_INT, [_P, _I64, _I64, _P, _P, _I64, _P, _I64, _I64, _I64, _P, _I64,
+                                       _I64, _P, _P, _P, _P, _P, _I64, _I64] + [_I64] * 6
+                                + [ctypes.c_float, _P, _I64, _P]),
     "lse_query": (_I64, [_INT]),
     "lse_status_string": (ctypes.c_char_p, [_INT]),
 }
@@ -56,7 +64,7 @@ MODE_W8A16, MODE_W8A8 = 0, 1
 E_WORKSPACE, E_SCRATCH = -6, -7
 Q_ABI_VERSION, Q_K_ALIGN, Q_DECODE_MAX_M, Q_MAX_K, Q_GFX_ARCH = 0, 1, 2, 3, 4
 Q_NOALLOC_SCRATCH = 5
-ABI_VERSION = 13
+ABI_VERSION = 14
 NORM_MAX_K = 16384
 
 _lock = threading.Lock()

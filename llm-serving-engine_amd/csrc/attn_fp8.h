@@ -1,0 +1,31 @@
+// Arguments and host entry points shared by the attention kernels over the 8-bit paged K/V cache
+// (attn_fp8.hip: the key-streaming kernel of decode rows and short chunks).
+#pragma once
+
+#include "attention.h"
+#include "fp8_kv.h"
+
+namespace lse {
+
+struct Fp8AttnArgs {
+  const uint16_t* q;  // bf16, element (h, t, d) at h * sq_h + t * sq_t + d
+  int64_t sq_h, sq_t;
+  Fp8Pool pool;
+  const int32_t* block_table;  // (entries, max_blocks), row stride sbt
+  int64_t sbt;
+  const int32_t *context_len, *query_offset, *q_start, *q_len;
+  uint16_t* o;  // bf16, same indexing as q with strides so_h, so_t
+  int64_t so_h, so_t;
+  int entries, H, HKV, G, tokens;
+  int max_ctx;       // positions that the table has room for
+  int max_q_len;     // rows of an entry in the split launch's workspace
+  int tq;            // query tokens per tile: floor(16 / G)
+  int parts;         // 1: a workgroup takes every chunk of its item; > 1: one chunk of each of its waves
+  int sorted;        // entries are taken in descending order of context length...
+  int first_round;   // ...and, where > 0, those from this rank on in ascending order
+  float scale_log2;  // softmax scale x log2(e)
+  float* ws_o;       // parts > 1: chunk states' O [parts x 4][entries][H][max_q_len][D], fp32
+  float* ws_ml;      // parts > 1: chunk states' max and sum [parts x 4][entries][H][max_q_len][2]
+};
+
+}  // namespace lse

@@ -1,0 +1,380 @@
+// Rotary positions from fp32 tables, by themselves (rope_kernel) and on the way into the 8-bit paged K/V cache
+// (append_kv_kernel).
+//
+// The rotation of a pair (a, b) by the angle whose cosine and sine the tables hold is (a c - b s, b c + a s),
+// every product and sum rounded in fp32 (no fused forms, so that a value and its code depend on the formula
+// alone), the result rounded once: to bf16, or to its code. Pair i of the first `rotary` dims is (i, i +
+// rotary / 2), or (2 i, 2 i + 1) interleaved; the dims behind are passed on.
+//
+// A thread's unit is 16 dims of a token's head: eight pairs, or 16 dims to pass on.
+#include <algorithm>
+
+#include "fp8_kv.h"
+
+namespace lse {
+
+// Rows (token, head) of bf16 values: element (t, h, d) at t * st + h * sh + d.
+struct RowsIn {
+  const uint16_t* p;
+  int64_t st, sh;
+};
+
+struct RopeTables {
+  const float *cos, *sin;  // (rows, half) each
+  int64_t rows;
+  int half;  // rotary / 2
+  int interleaved;
+};
+
+// Offsets of a unit's two runs of eight dims.
+struct UnitDims {
+  int a, b;
+  bool turned;
+};
+__device__ __forceinline__ UnitDims unit_dims(const RopeTables& r, int unit) {
+  UnitDims u{16 * unit, 16 * unit + 8, 16 * unit < 2 * r.half};
+  if (u.turned && !r.interleaved) u.a = 8 * unit, u.b = r.half + 8 * unit;
+  return u;
+}
+
+__device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
+  const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __builtin_bit_cast(float, v[i] << 16);
+    x[2 * i + 1] = __builtin_bit_cast(float, v[i] & 0xffff0000u);
+  }
+}
+
+// The 16 dims of a unit as two runs of eight, rotated to `pos`. A position outside the tables gives NaN.
+__device__ __forceinline__ void rotated_unit(const uint16_t* row, const RopeTables& r, const UnitDims& u,
+                                             int unit, int pos, float (&x)[8], float (&y)[8]) {
+#pragma clang fp contract(off)
+  unpack8(*reinterpret_cast<const uint4*>(row + u.a), x);
+  unpack8(*reinterpret_cast<const uint4*>(row + u.b), y);
+  if (!u.turned) return;
+  const bool known = pos >= 0 && pos < r.rows;
+  const int64_t at = (int64_t)(known ? pos : 0) * r.half + 8 * unit;
+  float c[8], s[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 4) {
+    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(r.cos + at + i);
+    *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(r.sin + at + i);
+  }
+  const float none = __builtin_nanf("");
+  auto turn = [&](float& a, float& b, float cc, float ss) {
+    const float p = a * cc - b * ss, q = b * cc + a * ss;
+    a = p, b = q;
+  };
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float cc = known ? c[i] : none, ss = known ? s[i] : none;
+    if (r.interleaved) {
+      float(&v)[8] = i < 4 ? x : y;
+      turn(v[2 * (i & 3)], v[2 * (i & 3) + 1], cc, ss);
+    } else {
+      turn(x[i], y[i], cc, ss);
+    }
+  }
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                    pack_bf16x2(x[6], x[7]));
+}
+
+struct RopeFp32Args {
+  RowsIn q, k;
+  RopeTables r;
+  const int32_t* positions;
+  uint16_t *q_out, *k_out;  // (tokens, heads, D)
+  int H, HKV, D, units;     // units: of one token
+};
+
+// One thread per unit; bound by HBM (each value in and out once).
+__global__ void __launch_bounds__(256) rope_kernel(RopeFp32Args a, int64_t total) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t t = i / a.units;
+  const int u = (int)(i - t * a.units), per = a.D / 16;
+  const int head = u / per, unit = u - head * per;
+  const bool is_q = head < a.H;
+  const RowsIn& in = is_q ? a.q : a.k;
+  const int h = is_q ? head : head - a.H;
+  const UnitDims d = unit_dims(a.r, unit);
+  float x[8], y[8];
+  rotated_unit(in.p + t * in.st + h * in.sh, a.r, d, unit, a.positions[t], x, y);
+  uint16_t* out = (is_q ? a.q_out + (t * a.H + h) * a.D : a.k_out + (t * a.HKV + h) * a.D);
+  *reinterpret_cast<uint4*>(out + d.a) = pack8(x);
+  *reinterpret_cast<uint4*>(out + d.b) = pack8(y);
+}
+
+struct AppendArgs {
+  RowsIn q, k, v;  // q.p may be null
+  RopeTables r;    // half 0: no rotation
+  uint16_t* q_out;  // (tokens, H, D)
+  Fp8Pool pool;
+  const int32_t* block_table;  // (entries, max_blocks), row stride sbt
+  int64_t sbt;
+  const int32_t *query_offset, *q_start, *q_len;
+  int entries, H, HKV, G, max_groups;  // max_groups: groups that the table has room for
+  int64_t tokens;
+  int one;  // every entry has at most one new token
+};
+
+// Groups of 16 positions that n new tokens at `offset` touch.
+__device__ __forceinline__ int groups_of(int offset, int n) {
+  if (n <= 0 || offset < 0) return 0;
+  return (int)(((unsigned)offset + (unsigned)n - 1) / kKvGroup) - offset / kKvGroup + 1;
+}
+
+// A workgroup takes one group of one K/V head: its up to 16 new tokens' k and v rows, and their rows of the G
+// query heads. Threads 0 .. D - 1 hold k's units (16 tokens x D / 16), the next D v's. The group's image (codes
+// in pool order) is built in LDS: what it held of earlier positions, requantised where the scale grew; the new
+// codes; zeros behind them; then it is written whole. At decode sizes this is bound by its chain of
+// dependent loads (lengths, table, scale, codes), at prompt sizes by HBM.
+template <int D>
+__global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
+  constexpr int U = D / 16;      // units of a row
+  constexpr int T = 16 * U;      // threads of k, and of v
+  static_assert(2 * T <= 256, "k's and v's threads in one workgroup");
+  __shared__ __attribute__((aligned(16))) uint8_t image[2][16 * D];
+  __shared__ float wave_max[4];
+
+  const int kvh = blockIdx.x % a.HKV;
+  int slot_id = blockIdx.x / a.HKV, e = -1, first = 0;
+  if (a.one) {
+    e = slot_id;
+  } else {
+    // The entry of this unit, and the unit's place in it: a sum over the entries' groups, 64 at a time.
+    const int lane = threadIdx.x & 63;
+    for (int e0 = 0; e0 < a.entries; e0 += 64) {
+      const int i = e0 + lane;
+      const int mine = i < a.entries ? groups_of(a.query_offset[i], a.q_len[i]) : 0;
+      const int before = kv_wave_scan(mine) - mine;
+      const unsigned long long hit = __ballot((unsigned)(slot_id - before) < (unsigned)mine);
+      if (hit) {
+        const int at = __ffsll(hit) - 1;
+        e = e0 + at;
+        first = slot_id - __builtin_amdgcn_readlane(before, at);
+        break;
+      }
+      slot_id -= __builtin_amdgcn_readlane(before + mine, 63);
+    }
+    if (e < 0) return;
+  }
+  const int offset = a.query_offset[e], n = a.q_len[e], start = a.q_start[e];
+  if (n <= 0 || offset < 0) return;
+  const int group = offset / kKvGroup + first;
+  // New tokens' slots of the group: [lo, hi), slot s being token s + base of the entry.
+  const int base = group * kKvGroup - offset;
+  const int lo = max(0, -base), hi = min(kKvGroup, n - base);
+
+  // The new rows, rotated; tokens of rows outside the call's are dropped.
+  const int what = threadIdx.x / T, unit = threadIdx.x % U, slot = threadIdx.x % T / U;
+  const int64_t row = (int64_t)start + base + slot;
+  const bool mine = what < 2 && slot >= lo && slot < hi && row >= 0 && row < a.tokens;
+  const RowsIn& in = what == 0 ? a.k : a.v;
+  RopeTables tables = a.r;
+  if (what != 0) tables.half = 0;
+  const UnitDims dims = unit_dims(tables, unit);
+  float x[8] = {}, y[8] = {};
+  if (mine)
+    rotated_unit(in.p + row * in.st + (int64_t)kvh * in.sh, tables, dims, unit,
+                 offset + base + slot, x, y);
+  if (a.q.p) {
+    const int count = (hi - lo) * a.G * U;
+    for (int i = threadIdx.x; i < count; i += 256) {
+      const int qu = i % U, h = kvh * a.G + i / U % a.G, s = lo + i / (U * a.G);
+      const int64_t t = (int64_t)start + base + s;
+      if (t < 0 || t >= a.tokens) continue;
+      const UnitDims qd = unit_dims(a.r, qu);
+      float qx[8], qy[8];
+      rotated_unit(a.q.p + t * a.q.st + (int64_t)h * a.q.sh, a.r, qd, qu, offset + base + s, qx, qy);
+      uint16_t* out = a.q_out + (t * a.H + h) * D;
+      *reinterpret_cast<uint4*>(out + qd.a) = pack8(qx);
+      *reinterpret_cast<uint4*>(out + qd.b) = pack8(qy);
+    }
+  }
+  if (group >= a.max_groups) return;
+  const int block = a.block_table[(int64_t)e * a.sbt + group / a.pool.per];
+  if (block < 0 || block >= a.pool.blocks) return;
+  const int64_t inner = (int64_t)kvh * a.pool.per + group % a.pool.per;
+  uint8_t* scale_at = a.pool.scales + (int64_t)block * a.pool.ss + 2 * inner;
+
+  // k's and v's largest finite magnitudes.
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float ax = __builtin_fabsf(x[i]), ay = __builtin_fabsf(y[i]);
+    top = fmaxf(top, ax < __builtin_huge_valf() ? ax : 0.0f);
+    top = fmaxf(top, ay < __builtin_huge_valf() ? ay : 0.0f);
+  }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
+  if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = top;
+  const int old = what < 2 && lo > 0 ? scale_at[what] : 0;
+  __syncthreads();
+  if (what < 2) {
+    constexpr int W = T / 64;  // waves of k, and of v
+    top = wave_max[what * W];
+#pragma unroll
+    for (int i = 1; i < W; ++i) top = fmaxf(top, wave_max[what * W + i]);
+  }
+  const int byte = max(kv_scale_byte(top), old == kKvScaleNan ? 0 : old);
+  const int64_t bytes = (int64_t)block * a.pool.sb + inner * (16 * D) + 16 * (threadIdx.x % T);
+  uint8_t* at = (what == 0 ? a.pool.k : a.pool.v) + bytes;
+  uint4* img = reinterpret_cast<uint4*>(image[what & 1] + 16 * (threadIdx.x % T));
+  if (what < 2) {
+    uint4 kept = make_uint4(0, 0, 0, 0);
+    // A thread's 16 bytes: k, of slot 4 i + j; v, all 16 slots of a dim.
+    const int in_slot = threadIdx.x % T / (D / 64 * 16) * 4 + threadIdx.x % T / 4 % 4;
+    if (lo > 0 && (what == 1 || in_slot < lo)) {
+      kept = *reinterpret_cast<const uint4*>(at);
+      if (byte != old) {
+        const float ratio = old == kKvScaleNan ? __builtin_nanf("")
+                            : byte - old > 126 ? 0.0f
+                                               : kv_scale(127 + old - byte);
+        kept = make_uint4(kv_requantize4(kept.x, ratio), kv_requantize4(kept.y, ratio),
+                          kv_requantize4(kept.z, ratio), kv_requantize4(kept.w, ratio));
+      }
+      if (what == 1) {
+        auto mask = [&](int w) {
+          const int nb = min(max(lo - 4 * w, 0), 4);
+          return nb == 4 ? 0xffffffffu : (1u << (8 * nb)) - 1u;
+        };
+        kept.x &= mask(0), kept.y &= mask(1), kept.z &= mask(2), kept.w &= mask(3);
+      }
+    }
+    *img = kept;
+  }
+  __syncthreads();
+  if (mine) {
+    const float inv = kv_scale_inverse(byte);
+    const uint32_t c[4] = {kv_encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+                           kv_encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv),
+                           kv_encode4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
+                           kv_encode4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)};
+    if (what == 0) {
+      auto put = [&](int d, uint32_t w0, uint32_t w1) {
+        uint8_t* to = image[0] + ((slot / 4 * (D / 64) + d / 64) * 4 + slot % 4) * 64 + d % 64;
+        *reinterpret_cast<uint2*>(to) = make_uint2(w0, w1);
+      };
+      put(dims.a, c[0], c[1]);
+      put(dims.b, c[2], c[3]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        image[1][16 * ((i < 8 ? dims.a : dims.b) + i % 8) + slot] = (uint8_t)(c[i / 4] >> (8 * (i % 4)));
+    }
+  }
+  __syncthreads();
+  if (what < 2) {
+    *reinterpret_cast<uint4*>(at) = *img;
+    if (threadIdx.x % T == 0) scale_at[what] = (uint8_t)byte;
+  }
+}
+
+}  // namespace lse
+
+namespace {
+
+bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+constexpr int64_t kMax31 = 2147483647;
+
+int check_rows(const void* p, int64_t st, int64_t sh) {
+  if (st < 0 || sh < 0) return LSE_E_SHAPE;
+  return st % 8 || sh % 8 || !aligned16(p) ? LSE_E_ALIGN : LSE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int lse_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
+             int64_t k_stride_h, const float* cos, const float* sin, int64_t table_rows,
+             const int32_t* positions, void* q_out, void* k_out, int64_t tokens, int64_t H, int64_t H_KV,
+             int64_t D, int64_t rotary, int interleaved, void* stream) {
+  if (tokens < 0 || tokens > kMax31 || H < 1 || H > 65536 || H_KV < 0 || H_KV > 65536 || D < 16 ||
+      D > 1024 || D % 16 || rotary < 16 || rotary > D || rotary % 16 || table_rows < 1 ||
+      (interleaved != 0 && interleaved != 1))
+    return LSE_E_SHAPE;
+  if (tokens == 0) return LSE_OK;
+  if (!q || !q_out || !cos || !sin || !positions || (H_KV > 0 && (!k || !k_out))) return LSE_E_NULL;
+  if (int st = check_rows(q, q_stride_t, q_stride_h)) return st;
+  if (H_KV > 0)
+    if (int st = check_rows(k, k_stride_t, k_stride_h)) return st;
+  if (!aligned16(cos) || !aligned16(sin) || !aligned16(q_out) || !aligned16(k_out) ||
+      ((uintptr_t)positions & 3))
+    return LSE_E_ALIGN;
+  lse::RopeFp32Args a{};
+  a.q = {(const uint16_t*)q, q_stride_t, q_stride_h};
+  a.k = {(const uint16_t*)k, k_stride_t, k_stride_h};
+  a.r = {cos, sin, table_rows, (int)(rotary / 2), interleaved};
+  a.positions = positions;
+  a.q_out = (uint16_t*)q_out, a.k_out = (uint16_t*)k_out;
+  a.H = (int)H, a.HKV = (int)H_KV, a.D = (int)D;
+  a.units = (int)((H + H_KV) * (D / 16));
+  const int64_t total = tokens * a.units, blocks = lse::ceil_div(total, 256);
+  if (blocks > kMax31) return LSE_E_RANGE;
+  hipLaunchKernelGGL(lse::rope_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, total);
+  return lse::launch_status();
+}
+
+int lse_append_kv_fp8(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
+                      int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
+                      int64_t v_stride_h, const float* cos, const float* sin, int64_t table_rows,
+                      void* q_out, void* k_pool, void* v_pool, int64_t pool_stride_block, void* scales,
+                      int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
+                      const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
+                      const int32_t* query_offset, const int32_t* q_start, const int32_t* q_len,
+                      int64_t entries, int64_t tokens, int64_t max_q_len, int64_t H, int64_t H_KV,
+                      int64_t D, int64_t rotary, int interleaved, void* stream) {
+  if (entries < 0 || entries > kMax31 || tokens < 0 || tokens > kMax31 || max_q_len < 0 ||
+      max_q_len > kMax31 || H < 1 || H > 65536 || H_KV < 1 || H % H_KV || (D != 64 && D != 128) ||
+      rotary < 0 || rotary > D || rotary % 16 || (interleaved != 0 && interleaved != 1) ||
+      num_blocks < 0 || num_blocks > kMax31 || block_size < 16 || block_size % 16 ||
+      max_blocks < 0 || block_table_stride < max_blocks)
+    return LSE_E_SHAPE;
+  if (block_size > kMax31 || max_blocks > kMax31 / block_size) return LSE_E_RANGE;
+  const int64_t per = block_size / 16;
+  if (pool_stride_block < H_KV * per * 16 * D || scales_stride_block < 2 * H_KV * per) return LSE_E_SHAPE;
+  if (entries == 0 || tokens == 0 || max_q_len == 0) return LSE_OK;
+  if (!k || !v || !k_pool || !v_pool || !scales || !block_table || !query_offset || !q_start || !q_len ||
+      (q && !q_out) || (rotary > 0 && (!cos || !sin)))
+    return LSE_E_NULL;
+  if (rotary > 0 && table_rows < 1) return LSE_E_SHAPE;
+  if (q)
+    if (int st = check_rows(q, q_stride_t, q_stride_h)) return st;
+  if (int st = check_rows(k, k_stride_t, k_stride_h)) return st;
+  if (int st = check_rows(v, v_stride_t, v_stride_h)) return st;
+  if (pool_stride_block % 16 || !aligned16(cos) || !aligned16(sin) || !aligned16(q_out) ||
+      !aligned16(k_pool) || !aligned16(v_pool))
+    return LSE_E_ALIGN;
+  lse::AppendArgs a{};
+  a.q = {(const uint16_t*)q, q_stride_t, q_stride_h};
+  a.k = {(const uint16_t*)k, k_stride_t, k_stride_h};
+  a.v = {(const uint16_t*)v, v_stride_t, v_stride_h};
+  a.r = {cos, sin, table_rows, (int)(rotary / 2), interleaved};
+  a.q_out = (uint16_t*)q_out;
+  a.pool = {(uint8_t*)k_pool, (uint8_t*)v_pool, (uint8_t*)scales, pool_stride_block, scales_stride_block,
+            (int)num_blocks, (int)per};
+  a.block_table = block_table, a.sbt = block_table_stride;
+  a.query_offset = query_offset, a.q_start = q_start, a.q_len = q_len;
+  a.entries = (int)entries, a.H = (int)H, a.HKV = (int)H_KV, a.G = (int)(H / H_KV);
+  a.max_groups = (int)(max_blocks * per);
+  a.tokens = tokens;
+  a.one = max_q_len == 1;
+  // An entry of n tokens touches at most (n + 30) / 16 groups; the entries' rows are distinct.
+  const int64_t most = std::min(entries * ((max_q_len + 30) / 16), tokens / 16 + 2 * entries);
+  const int64_t blocks = (a.one ? entries : most) * H_KV;
+  if (blocks > kMax31) return LSE_E_RANGE;
+  const dim3 grid((unsigned)blocks), wg(256);
+  if (D == 64)
+    hipLaunchKernelGGL(lse::append_kv_kernel<64>, grid, wg, 0, (hipStream_t)stream, a);
+  else
+    hipLaunchKernelGGL(lse::append_kv_kernel<128>, grid, wg, 0, (hipStream_t)stream, a);
+  return lse::launch_status();
+}
+
+}  // extern "C"

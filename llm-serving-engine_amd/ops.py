@@ -12,17 +12,24 @@ rows, so one kernel computes both and applies SiLU-mul before anything leaves re
 
 from __future__ import annotations
 
+import math
+from typing import NamedTuple
+
 import torch
 
 from . import _lib
 
 __all__ = [
+    "Fp8KV",
     "add_rmsnorm",
+    "append_kv_fp8",
     "bf16_decode_linear",
+    "fp8_kv_pool",
     "pack_bf16_weight",
     "packed_bf16_shape",
     "unpack_bf16_weight",
     "paged_attention_forward",
+    "paged_attention_fp8",
     "pack_glu",
     "pack_weight",
     "packed_glu_shape",
@@ -30,7 +37,10 @@ __all__ = [
     "quantize_act_per_token",
     "quantize_weight_per_channel",
     "rmsnorm_quantize",
+    "rope",
     "rope_kv",
+    "rope_table",
+    "unpack_fp8_kv",
     "unpack_glu",
     "unpack_weight",
     "w8a8_gemm",
@@ -588,6 +598,290 @@ def rope_kv(
         "lse_rope_kv",
     )
     return out
+
+
+# ---- rotary positions and the 8-bit K/V cache ----------------------------------------------------
+
+KV_GROUP = 16  # positions of a head that share a scale
+
+
+def _launch(dev: int, what: str, *args) -> None:
+    """Calls the entry point `what` with dev's current stream behind the arguments. A kernel goes to the
+    current device, whose default stream has the handle of every other's."""
+    fn = getattr(_lib.library(), what)
+    if torch.cuda.current_device() == dev:
+        status = fn(*args, _stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            status = fn(*args, _stream(dev))
+    _lib.check(status, what)
+
+
+def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dict | None = None,
+               device: torch.device | str | int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """(cos, sin) of positions 0 .. positions - 1, each (positions, rotary / 2) fp32: what `rope` and
+    `append_kv_fp8` rotate by. Angles are computed in fp64, so far positions keep their precision.
+
+    `scaling` is a model configuration's `rope_scaling` for contexts longer than it was trained on:
+    {"rope_type": "linear", "factor"}, {"rope_type": "llama3", "factor", "low_freq_factor",
+    "high_freq_factor", "original_max_position_embeddings"} or {"rope_type": "yarn", "factor",
+    "original_max_position_embeddings"} with yarn's optional "beta_fast", "beta_slow" and
+    "attention_factor" (which multiplies cos and sin)."""
+    _require(rotary >= 2 and rotary % 2 == 0, f"rotary must be even, got {rotary}")
+    _require(positions >= 1, f"a table needs at least one position, got {positions}")
+    pair = torch.arange(0, rotary, 2, dtype=torch.float64, device=device) / rotary
+    freq = 1.0 / theta ** pair
+    gain = 1.0
+    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
+    if kind == "linear":
+        freq = freq / scaling["factor"]
+    elif kind == "llama3":
+        # Wavelengths a context of `original` holds fewer than `low` times are stretched by the factor,
+        # those it holds more than `high` times are kept, linear in between.
+        low, high = scaling["low_freq_factor"], scaling["high_freq_factor"]
+        turns = scaling["original_max_position_embeddings"] * freq / (2.0 * math.pi)
+        keep = ((turns - low) / (high - low)).clamp(0.0, 1.0)
+        freq = keep * freq + (1.0 - keep) * freq / scaling["factor"]
+    elif kind == "yarn":
+        factor, original = scaling["factor"], scaling["original_max_position_embeddings"]
+        # The pair whose wavelength a context of `original` holds `turns` times.
+        where = lambda turns: (rotary * math.log(original / (turns * 2.0 * math.pi))  # noqa: E731
+                               / (2.0 * math.log(theta)))
+        first = max(math.floor(where(scaling.get("beta_fast") or 32.0)), 0)
+        last = min(math.ceil(where(scaling.get("beta_slow") or 1.0)), rotary - 1)
+        index = torch.arange(rotary // 2, dtype=torch.float64, device=device)
+        keep = 1.0 - ((index - first) / max(last - first, 0.001)).clamp(0.0, 1.0)
+        freq = keep * freq + (1.0 - keep) * freq / factor
+        gain = scaling.get("attention_factor")
+        if gain is None:
+            gain = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
+    elif kind != "default":
+        raise RuntimeError(f"unknown rope_type {kind!r}")
+    angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
+    return (gain * torch.cos(angle)).float(), (gain * torch.sin(angle)).float()
+
+
+def _head_rows(t: torch.Tensor, what: str) -> torch.Tensor:
+    """(tokens, heads, D) bf16 as rows of heads the kernels take: D contiguous, strides multiples of 8
+    elements, a 16-byte aligned address."""
+    if t.dtype is not torch.bfloat16 or t.dim() != 3:
+        raise RuntimeError(f"{what} must be a bf16 (tokens, heads, D) tensor, got {tuple(t.shape)} {t.dtype}")
+    strides = t.stride()
+    if strides[2] != 1 or strides[0] % 8 or strides[1] % 8:
+        t = t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+
+
+def _rope_tables(cos: torch.Tensor, sin: torch.Tensor) -> int:
+    """The rotary dims of two tables as `rope_table` makes them."""
+    if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2
+            or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous()):
+        raise RuntimeError("cos and sin must be contiguous fp32 (positions, rotary / 2) tensors")
+    return 2 * cos.shape[1]
+
+
+def _check_rotary(rotary: int, d: int) -> None:
+    _require(16 <= rotary <= d and rotary % 16 == 0 and d % 16 == 0,
+             f"rotary dims and D must be multiples of 16, rotary at most D; got {rotary} of {d}")
+
+
+def rope(
+    q: torch.Tensor, k: torch.Tensor | None, cos: torch.Tensor, sin: torch.Tensor,
+    positions: torch.Tensor, interleaved: bool = False,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """q (tokens, H, D) and k (tokens, H_KV, D) or None, bf16, rotated to `positions` (tokens,) int32, in
+    one kernel: pair i of a head's first R dims, (i, i + R / 2), or (2 i, 2 i + 1) when interleaved, is turned
+    by the angle whose cosine and sine are in row `positions[t]`, column i of cos and sin (`rope_table`,
+    fp32, (rows, R / 2)); the dims from R on are copied. Computed in fp32, rounded once. A position outside
+    the tables gives NaN. D and R are multiples of 16. Tokens and heads may be strided."""
+    dev = _on_gpu(q, cos, sin, positions) if k is None else _on_gpu(q, k, cos, sin, positions)
+    rotary = _rope_tables(cos, sin)
+    q2 = _head_rows(q, "q")
+    tokens, h, d = q2.shape
+    _check_rotary(rotary, d)
+    if positions.dtype is not torch.int32 or positions.shape != (tokens,):
+        raise RuntimeError(f"positions must be int32 ({tokens},)")
+    at = positions.contiguous()
+    q_out = torch.empty((tokens, h, d), dtype=torch.bfloat16, device=dev)
+    k2 = k_out = None
+    if k is not None:
+        k2 = _head_rows(k, "k")
+        _require(k2.shape[0] == tokens and k2.shape[2] == d, "q and k must have the same tokens and D")
+        k_out = torch.empty(k2.shape, dtype=torch.bfloat16, device=dev)
+    k_args = (k2.data_ptr(), *k2.stride()[:2]) if k2 is not None else (None, 0, 0)
+    _launch(
+        dev, "lse_rope", q2.data_ptr(), *q2.stride()[:2], *k_args, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+        at.data_ptr(), q_out.data_ptr(), k_out.data_ptr() if k_out is not None else None, tokens, h,
+        k2.shape[1] if k2 is not None else 0, d, rotary, int(interleaved))
+    return q_out, k_out
+
+
+class Fp8KV(NamedTuple):
+    """A layer's paged K/V cache in 8 bits, in the layout its kernels stream (`fp8_kv_pool`): float8 e4m3
+    codes k and v (blocks, H_KV, S, 16 D), S = block_size / 16 groups of 16 positions in a block, and their
+    scales, powers of two (e8m0), (blocks, H_KV, S, 2) for k and v. `unpack_fp8_kv` gives the values."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    scales: torch.Tensor
+
+    @property
+    def block_size(self) -> int:
+        return KV_GROUP * self.k.shape[2]
+
+
+def fp8_kv_pool(num_blocks: int, block_size: int, n_kv: int, d: int,
+                device: torch.device | str | int) -> Fp8KV:
+    """An 8-bit K/V pool of zeros: 1 byte per value and 1/(16 D) for the scales."""
+    _require(block_size >= KV_GROUP and block_size % KV_GROUP == 0,
+             f"block_size must be a multiple of {KV_GROUP}, got {block_size}")
+    _require(d in (64, 128), f"D must be 64 or 128, got {d}")
+    shape = (num_blocks, n_kv, block_size // KV_GROUP)
+    code = lambda: torch.zeros((*shape, KV_GROUP * d), dtype=torch.uint8,  # noqa: E731
+                               device=device).view(torch.float8_e4m3fn)
+    scales = torch.ones((*shape, 2), dtype=torch.uint8, device=device)  # 2^-126, the least
+    return Fp8KV(code(), code(), scales.view(torch.float8_e8m0fnu))
+
+
+def unpack_fp8_kv(pool: Fp8KV) -> tuple[torch.Tensor, torch.Tensor]:
+    """The values a pool stands for, as two bf16 (blocks, block_size, H_KV, D) tensors (the layout of
+    `paged_attention_forward`'s pools; exact, done with torch operations)."""
+    blocks, n_kv, per, size = pool.k.shape
+    d = size // KV_GROUP
+    k = pool.k.view(torch.uint8).reshape(blocks, n_kv, per, 4, d // 64, 4, 64).transpose(4, 5)
+    v = pool.v.view(torch.uint8).reshape(blocks, n_kv, per, d, KV_GROUP).transpose(3, 4)
+    got = []
+    for what, codes in enumerate((k, v)):
+        codes = codes.reshape(blocks, n_kv, per, KV_GROUP, d).contiguous().view(torch.float8_e4m3fn)
+        values = codes.float() * pool.scales[..., what].float()[..., None, None]
+        got.append(values.permute(0, 2, 3, 1, 4).reshape(blocks, per * KV_GROUP, n_kv, d)
+                   .to(torch.bfloat16))
+    return got[0], got[1]
+
+
+def _check_fp8_pool(pool: Fp8KV) -> tuple[int, int, int, int, int, int]:
+    """(blocks, H_KV, S, D, bytes from a block to the next in k and v, and in scales) of a pool."""
+    k, v, s = pool
+    if k.dtype is not torch.float8_e4m3fn or v.dtype is not k.dtype or k.dim() != 4 or v.shape != k.shape:
+        raise RuntimeError("pool codes must be two float8_e4m3fn (blocks, H_KV, S, 16 D) tensors")
+    blocks, n_kv, per, size = k.shape
+    if s.dtype is not torch.float8_e8m0fnu or s.shape != (blocks, n_kv, per, 2):
+        raise RuntimeError(f"pool scales must be float8_e8m0fnu ({blocks}, {n_kv}, {per}, 2)")
+    if size not in (64 * KV_GROUP, 128 * KV_GROUP) or per < 1 or n_kv < 1:
+        raise RuntimeError(f"pool groups of {size} bytes: D must be 64 or 128")
+    if blocks < 2:
+        stride, s_stride = n_kv * per * size, 2 * n_kv * per
+    else:
+        stride, s_stride = k.stride(0), s.stride(0)
+        if v.stride(0) != stride:
+            raise RuntimeError("a pool's k and v must have their blocks equally far apart")
+    if not (k[:1].is_contiguous() and v[:1].is_contiguous() and s[:1].is_contiguous()):
+        raise RuntimeError("a pool's blocks must be contiguous")
+    return blocks, n_kv, per, size // KV_GROUP, stride, s_stride
+
+
+def _check_plan(table: torch.Tensor, entry: dict[str, torch.Tensor]) -> int:
+    """The entries of a batch plan: block_table (entries, blocks) and int32 (entries,) tensors."""
+    for name, t in (("block_table", table), *entry.items()):
+        if t.dtype is not torch.int32:
+            raise RuntimeError(f"{name} must be int32, got {t.dtype}")
+    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
+        raise RuntimeError("block_table must be (E, B) with unit column stride")
+    entries = table.shape[0]
+    for name, t in entry.items():
+        if t.shape != (entries,) or (entries > 1 and t.stride(0) != 1):
+            raise RuntimeError(f"{name} must be a contiguous ({entries},) tensor")
+    return entries
+
+
+def _table_stride(table: torch.Tensor) -> int:
+    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+
+
+def append_kv_fp8(
+    q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, cos: torch.Tensor | None,
+    sin: torch.Tensor | None, pool: Fp8KV, block_table: torch.Tensor, query_offset: torch.Tensor,
+    q_start: torch.Tensor, q_len: torch.Tensor, max_q_len: int, interleaved: bool = False,
+) -> torch.Tensor | None:
+    """Writes a batch plan's new k and v rows into an 8-bit paged pool, rotating q and k on the way (as
+    `rope`, by the entries' positions; cos and sin None: not at all), in one kernel.
+
+    q (tokens, H, D) or None, k and v (tokens, H_KV, D): bf16, tokens and heads may be strided. Entry e's rows
+    are q_start[e] + m, m < q_len[e] <= max_q_len, at positions query_offset[e] + m of the blocks that
+    block_table[e] names; entries own their rows and the blocks they write to. A group of 16 positions
+    takes the smallest power-of-two scale that keeps its finite values within 448 scales; positions it held
+    before are requantised when its scale grows, and slots behind the last new one are zeroed. Infinities
+    and NaN are held as NaN. Positions outside the table, blocks outside the pool and rows outside q, k
+    and v are dropped. Returns the rotated q (tokens, H, D), of which rows of no entry are not written."""
+    entry = dict(query_offset=query_offset, q_start=q_start, q_len=q_len)
+    dev = _on_gpu(k, v, *pool, block_table, *entry.values(),
+                  *(t for t in (q, cos, sin) if t is not None))
+    blocks, n_kv, per, d, stride, s_stride = _check_fp8_pool(pool)
+    entries = _check_plan(block_table, entry)
+    k2, v2 = _head_rows(k, "k"), _head_rows(v, "v")
+    tokens = k2.shape[0]
+    if k2.shape[1:] != (n_kv, d) or v2.shape != k2.shape:
+        raise RuntimeError(f"k and v must be (tokens, {n_kv}, {d}) for this pool")
+    if (cos is None) != (sin is None):
+        raise RuntimeError("cos and sin go together")
+    rotary = 0
+    if cos is not None:
+        rotary = _rope_tables(cos, sin)
+        _check_rotary(rotary, d)
+    q_args, h, q_out = (None, 0, 0), n_kv, None
+    if q is not None:
+        q2 = _head_rows(q, "q")
+        h = q2.shape[1]
+        if q2.shape[0] != tokens or q2.shape[2] != d or h % n_kv or h == 0:
+            raise RuntimeError(f"q must be ({tokens}, H, {d}), H a multiple of {n_kv}")
+        q_args = (q2.data_ptr(), *q2.stride()[:2])
+        q_out = torch.empty((tokens, h, d), dtype=torch.bfloat16, device=dev)
+    _launch(
+        dev, "lse_append_kv_fp8", *q_args, k2.data_ptr(), *k2.stride()[:2], v2.data_ptr(), *v2.stride()[:2],
+        cos.data_ptr() if rotary else None, sin.data_ptr() if rotary else None,
+        cos.shape[0] if rotary else 0, q_out.data_ptr() if q_out is not None else None,
+        pool.k.data_ptr(), pool.v.data_ptr(), stride, pool.scales.data_ptr(), s_stride,
+        blocks, KV_GROUP * per, block_table.data_ptr(), _table_stride(block_table),
+        block_table.shape[1], query_offset.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), entries,
+        tokens, max_q_len, h, n_kv, d, rotary, int(interleaved))
+    return q_out
+
+
+def paged_attention_fp8(
+    q: torch.Tensor, pool: Fp8KV, block_table: torch.Tensor, context_len: torch.Tensor,
+    query_offset: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor, max_q_len: int,
+) -> torch.Tensor:
+    """`paged_attention_forward` over an 8-bit pool: one call for a whole batch plan's attention at one
+    layer, the same plan tensors and meaning, k and v being the values the pool stands for.
+
+    q: (H, tokens, D) bf16, D contiguous; D = 64 or 128, 1 <= H / H_KV <= 16. block_table (entries,
+    max_blocks), context_len, query_offset, q_start, q_len (entries,): int32 on the device; entries own
+    distinct rows of q; max_q_len >= every q_len. Returns o like q; rows of no entry are not written. Softmax
+    scale 1/sqrt(D)."""
+    entry = dict(context_len=context_len, query_offset=query_offset, q_start=q_start, q_len=q_len)
+    dev = _on_gpu(q, *pool, block_table, *entry.values())
+    blocks, n_kv, per, d, stride, s_stride = _check_fp8_pool(pool)
+    entries = _check_plan(block_table, entry)
+    if q.dim() != 3 or q.dtype is not torch.bfloat16 or q.shape[2] != d or q.stride(2) != 1:
+        raise RuntimeError(f"q must be bf16 (H, tokens, {d}) with a contiguous head dim")
+    h, tokens, _ = q.shape
+    if h == 0 or h % n_kv or h // n_kv > 16:
+        raise RuntimeError(f"unsupported attention shape: H={h} H_KV={n_kv} D={d}")
+    o = torch.empty_like(q)
+    lib = _lib.library()
+    width, size = block_table.shape[1], KV_GROUP * per
+    nbytes = lib.lse_paged_attention_fp8_workspace_bytes(entries, tokens, h, n_kv, d, max_q_len, width,
+                                                         size)
+    if nbytes < 0:
+        raise RuntimeError(f"unsupported attention sizes: max_q_len={max_q_len}, {width} blocks of {size}")
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(
+        dev, "lse_paged_attention_fp8", q.data_ptr(), q.stride(0), q.stride(1), pool.k.data_ptr(), pool.v.data_ptr(), stride,
+        pool.scales.data_ptr(), s_stride, blocks, size, block_table.data_ptr(),
+        _table_stride(block_table), width, context_len.data_ptr(), query_offset.data_ptr(),
+        q_start.data_ptr(), q_len.data_ptr(), o.data_ptr(), o.stride(0), o.stride(1), entries, tokens,
+        max_q_len, h, n_kv, d, 1.0 / d ** 0.5, *_ws_args(ws))
+    return o
 
 
 def packed_bf16_shape(n: int, k: int) -> tuple[int, int, int]:

@@ -1,0 +1,296 @@
+"""Paged attention over the 8-bit K/V cache on the GPU against the fp64 oracle on the values the cache stands
+for. Tolerance (`fp8_kv_helpers.check_attention`): bf16 probabilities and a bf16 output, as for the bf16 cache."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from fp8_kv_helpers import (attend, attend_args, attention_case, attention_golden, bf16_rows, check_attention,
+                            i32, pool_to_dev, to_dev)
+from helpers import bf16_bits, to_bf16_tensor
+from oracle import kv_cache as kv
+from oracle import numerics as ora
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("ctxs", [[1, 2, 15, 16, 17], [63, 64, 65, 255, 256, 257], [1023, 1024, 1025, 3, 700],
+                                  [1279, 1281, 2047, 2050, 4095]])
+def test_decode_rows(pkg, dev, d, ctxs):
+    """One row a sequence at every edge of a group, a tile, a window and a round of four chunks."""
+    check_attention(pkg, dev, attention_case(d + len(ctxs), [(1, c - 1, c) for c in ctxs], d=d), f"{ctxs}")
+
+
+@pytest.mark.parametrize("h,h_kv", [(8, 8), (16, 8), (24, 8), (40, 8), (32, 2), (16, 1), (10, 2), (7, 1), (26, 2)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_head_groupings(pkg, dev, h, h_kv, d):
+    """1 to 16 query heads per K/V head, those that do not divide a tile's 16 rows among them."""
+    entries = [(5, 10, 15), (1, 40, 41), (20, 0, 20), (7, 600, 607), (1, 1300, 1301)]
+    check_attention(pkg, dev, attention_case(h * d + h_kv, entries, h=h, h_kv=h_kv, d=d), f"{h} over {h_kv}")
+
+
+@pytest.mark.parametrize("block_size", [16, 32, 48, 64, 80, 256])
+def test_block_sizes(pkg, dev, block_size):
+    entries = [(1, 500, 501), (9, 70, 79), (30, 0, 30), (1, 0, 1), (1, 47, 48), (2, 255, 257)]
+    check_attention(pkg, dev, attention_case(block_size, entries, h=8, h_kv=2, block_size=block_size))
+
+
+def test_mixed_chunks_and_decode(pkg, dev):
+    entries = [(50, 0, 50), (33, 64, 97), (1, 200, 201), (7, 5, 12), (1, 0, 1), (129, 3, 132), (0, 9, 9),
+               (1, 1500, 1501), (64, 1000, 1064)]
+    check_attention(pkg, dev, attention_case(3, entries, h=24, h_kv=8, block_size=32), "mixed")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_prompts(pkg, dev, d):
+    """Fresh prompts and later chunks of several hundred tokens."""
+    entries = [(300, 0, 300), (257, 130, 387), (128, 1000, 1128), (1, 60, 61)]
+    check_attention(pkg, dev, attention_case(20 + d, entries, h=8, h_kv=2, d=d), "prompts")
+
+
+def test_contexts_end_before_the_rows_do(pkg, dev):
+    """context_len below query_offset + q_len: later rows see no more than the context; none at all gives
+    zeros; a context longer than the table is cut to it."""
+    case = attention_case(30, [(20, 0, 20), (6, 40, 46), (1, 99, 100), (3, 10, 13)], h=8, h_kv=2)
+    case["ctx"][:] = [7, 0, 50, 13]
+    o = check_attention(pkg, dev, case)
+    assert not o[:, 20:26].any()
+    long = dict(case, ctx=case["ctx"].copy())
+    case["ctx"][2], long["ctx"][2] = 100, 5000
+    case["table"], long["table"] = (np.ascontiguousarray(c["table"][:, :7]) for c in (case, long))
+    case["qo"][2] = long["qo"][2] = 111
+    case["ctx"][2] = 112
+    np.testing.assert_array_equal(attend(pkg, dev, long), attend(pkg, dev, case))
+
+
+def test_nothing_outside_the_context_is_read_into_a_row(pkg, dev):
+    """NaN codes in every slot behind a context and in every other block, NaN scales in groups behind it."""
+    entries = [(1, 20, 21), (1, 63, 64), (40, 7, 47), (1, 300, 301), (18, 0, 18)]
+    case = attention_case(31, entries, h=8, h_kv=2, block_size=32)
+    want = attend(pkg, dev, case)
+    k, v, s = (a.copy() for a in case["pool"])
+    used = np.zeros((case["blocks"], 2, 16), bool)
+    for e, (_, _, ctx) in enumerate(entries):
+        for n in range(ctx):
+            used[case["table"][e, n // 32], n % 32 // 16, n % 16] = True
+    for b, sub, slot in np.argwhere(~used):
+        dims = np.arange(128)
+        k[b, :, sub, kv.k_index(slot, dims, 128)] = 127
+        v[b, :, sub, kv.v_index(slot, dims, 128)] = 255
+        if not used[b, sub].any():
+            s[b, :, sub] = kv.NAN_SCALE
+    np.testing.assert_array_equal(attend(pkg, dev, dict(case, pool=(k, v, s))), want)
+
+
+def test_bad_blocks_reach_their_own_entry_only(pkg, dev):
+    """A block outside the pool, and a NaN scale: the rows that see them are NaN, everything else as before."""
+    case = attention_case(32, [(1, 99, 100), (1, 99, 100), (1, 1999, 2000), (4, 30, 34)], h=8, h_kv=2)
+    want = attend(pkg, dev, case)
+    bad = dict(case, table=case["table"].copy())
+    bad["table"][0, 2], bad["table"][2, 100] = case["blocks"], -7
+    pool = tuple(a.copy() for a in case["pool"])
+    pool[2][case["table"][3, 0], :, 0, 0] = kv.NAN_SCALE
+    o = ora.bf16_bits_to_f32(attend(pkg, dev, dict(bad, pool=pool)))
+    assert np.isnan(o[:, [0, 2]]).all() and np.isnan(o[:, 3:7]).all()
+    np.testing.assert_array_equal(ora.f32_to_bf16_bits(o[:, 1]), want[:, 1])
+
+
+@pytest.mark.parametrize("q_scale", [0.0, 4.0, 2.0 ** 12, 2.0 ** 40, 2.0 ** -40])
+def test_flat_and_peaked_scores(pkg, dev, q_scale):
+    case = attention_case(33, [(1, 699, 700), (40, 300, 340)], h=8, h_kv=2, q_scale=q_scale)
+    check_attention(pkg, dev, case, f"q x {q_scale}")
+
+
+def _bits(pkg, dev, case, rows, most=None):
+    return attend(pkg, dev, case, most)[:, rows]
+
+
+def test_a_rows_bits_depend_on_its_entry_alone(pkg, dev):
+    """Alone (a split launch), among 70 others (an unsplit one), in a padded bucket under a table as wide as
+    the pool, in another order: the same bits."""
+    rng = np.random.default_rng(34)
+    ctxs = [2100, 1, 513, 300, 1030] + [int(c) for c in rng.integers(1, 400, 70)]
+    case = attention_case(34, [(1, c - 1, c) for c in ctxs])
+    everything = check_attention(pkg, dev, case)
+    lib = pkg.library()
+    size = lambda e, w: lib.lse_paged_attention_fp8_workspace_bytes(e, e, 32, 8, 128, 1, w, 16)  # noqa: E731
+    width = case["table"].shape[1]
+    assert size(5, width) > 0 and size(75, width) == 0
+    few = dict(case, q=case["q"][:, :5], **{n: case[n][:5] for n in ("table", "ctx", "qo", "qs", "ql")})
+    np.testing.assert_array_equal(attend(pkg, dev, few), everything[:, :5])
+    wide = np.full((16, case["blocks"]), case["blocks"] - 1, np.int32)
+    wide[:5, :width] = case["table"][:5]
+    pad = dict(few, table=wide, **{n: np.concatenate([few[n], np.zeros(11, np.int32)])
+                                   for n in ("ctx", "qo", "qs", "ql")})
+    np.testing.assert_array_equal(attend(pkg, dev, pad), everything[:, :5])
+    np.testing.assert_array_equal(attend(pkg, dev, pad, most=9), everything[:, :5])
+    back = dict(case, q=case["q"][:, ::-1].copy(), **{n: case[n][::-1].copy() for n in ("table", "ctx", "qo", "ql")})
+    np.testing.assert_array_equal(attend(pkg, dev, back), everything[:, ::-1])
+
+
+@pytest.mark.parametrize("ctx", [32768, 32769, 70000])
+def test_long_contexts(pkg, dev, ctx):
+    """Around the length from which chunks grow, split and unsplit (the same bits), beside a short one."""
+    case = attention_case(ctx, [(1, ctx - 1, ctx), (2, 98, 100)], h=3, h_kv=1, d=64, block_size=64)
+    split = check_attention(pkg, dev, case, f"ctx {ctx}")
+    n = 520  # entries that fill the CUs, all but two of them empty
+    pad = dict(case, **{k: np.concatenate([case[k], np.zeros(n, np.int32)]) for k in ("ctx", "qo", "qs", "ql")})
+    pad["table"] = np.concatenate([case["table"], np.zeros((n, case["table"].shape[1]), np.int32)])
+    lib = pkg.library()
+    assert lib.lse_paged_attention_fp8_workspace_bytes(2, 3, 3, 1, 64, 2, case["table"].shape[1], 64) > 0
+    # The bound on items by rows keeps few tokens split however many entries there are.
+    pad["q"] = np.concatenate([case["q"], np.repeat(case["q"][:, :1], 3000, 1)], 1)
+    np.testing.assert_array_equal(attend(pkg, dev, pad)[:, :3], split)
+
+
+def test_rows_of_no_entry_are_left_alone(pkg, dev):
+    """Through the C entry point into a caller's o: rows before, between and behind the entries' keep what
+    they held."""
+    case = attention_case(36, [(3, 40, 43), (1, 1200, 1201), (2, 0, 2)], h=8, h_kv=2)
+    want = attend(pkg, dev, case)
+    q = np.zeros((8, 20, 128), np.uint16)
+    at = [2, 3, 4, 9, 15, 16]
+    q[:, at] = case["q"]
+    qs = np.array([2, 9, 15], np.int32)
+    pool = pool_to_dev(pkg, case["pool"], dev)
+    qd = to_bf16_tensor(q, dev)
+    o = torch.full((8, 20, 128), 7.0, dtype=torch.bfloat16, device=dev)
+    table, ctx, qo, _, ql = attend_args(case, dev)
+    lib = pkg.library()
+    nbytes = lib.lse_paged_attention_fp8_workspace_bytes(3, 20, 8, 2, 128, 3, table.shape[1], 16)
+    ws = torch.full((max(nbytes, 16),), 0xff, dtype=torch.uint8, device=dev)  # NaN in what nobody writes
+    start = i32(qs, dev)
+    status = lib.lse_paged_attention_fp8(
+        qd.data_ptr(), qd.stride(0), qd.stride(1), pool.k.data_ptr(), pool.v.data_ptr(), pool.k.stride(0),
+        pool.scales.data_ptr(), pool.scales.stride(0), case["blocks"], 16, table.data_ptr(), table.stride(0),
+        table.shape[1], ctx.data_ptr(), qo.data_ptr(), start.data_ptr(), ql.data_ptr(), o.data_ptr(),
+        o.stride(0), o.stride(1), 3, 20, 3, 8, 2, 128, 1.0 / 128 ** 0.5, ws.data_ptr(), nbytes,
+        torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert status == 0
+    np.testing.assert_array_equal(bf16_bits(o[:, at]), want)
+    rest = [t for t in range(20) if t not in at]
+    assert (o[:, rest] == 7.0).all()
+
+
+def test_pool_past_32_bits(pkg, dev):
+    """A pool of more than 4 GiB a side whose used blocks lie at its far end."""
+    h_kv, d, bs = 8, 128, 64
+    per, blocks = bs // 16, 70000
+    case = attention_case(37, [(1, 199, 200), (70, 30, 100)], h=16, h_kv=h_kv, block_size=bs)
+    want = attend(pkg, dev, case)
+    own = case["pool"][0].shape[0]
+    far = [torch.empty((blocks, h_kv, per, n), dtype=torch.uint8, device=dev) for n in (16 * d, 16 * d, 2)]
+    assert far[0].numel() > 1 << 32
+    for t, a in zip(far, case["pool"]):
+        t[-own:] = torch.from_numpy(a).to(dev)
+    pool = pkg.ops.Fp8KV(far[0].view(torch.float8_e4m3fn), far[1].view(torch.float8_e4m3fn),
+                         far[2].view(torch.float8_e8m0fnu))
+    table, *rest = attend_args(dict(case, table=case["table"] + blocks - own), dev)
+    o = pkg.ops.paged_attention_fp8(to_bf16_tensor(case["q"], dev), pool, table, *rest, 70)
+    torch.cuda.synchronize()
+    np.testing.assert_array_equal(bf16_bits(o), want)
+    # The append at the same far end.
+    rng = np.random.default_rng(37)
+    x = to_dev(bf16_rows(rng, 71, h_kv, d), dev)
+    plan = [i32(case[n], dev) for n in ("qo", "qs", "ql")]
+    near = pool_to_dev(pkg, case["pool"], dev)
+    pkg.ops.append_kv_fp8(None, x, x, None, None, near, i32(case["table"], dev), *plan, 70)
+    pkg.ops.append_kv_fp8(None, x, x, None, None, pool, table, *plan, 70)
+    for a, b in zip(pool, near):
+        assert torch.equal(a.view(torch.uint8)[-own:], b.view(torch.uint8))
+
+
+def test_strided_q_and_two_streams(pkg, dev):
+    """q and k as slices of a stacked projection in token-major order, and two calls in flight at once."""
+    case = attention_case(38, [(1, 5999, 6000), (3, 40, 43)], h=8, h_kv=2)
+    want = attend(pkg, dev, case)
+    stacked = torch.zeros(4, 12, 128, dtype=torch.bfloat16, device=dev)
+    stacked[:, :8] = to_bf16_tensor(case["q"], dev).transpose(0, 1)
+    pool, plan = pool_to_dev(pkg, case["pool"], dev), attend_args(case, dev)
+    q = stacked[:, :8].transpose(0, 1)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(3):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                got.append(pkg.ops.paged_attention_fp8(q, pool, *plan, 3))
+    torch.cuda.synchronize()
+    for o in got:
+        assert o.shape == q.shape and o.stride(1) == 8 * 128  # token-major, as q
+        np.testing.assert_array_equal(bf16_bits(o), want)
+
+
+def test_attention_replays_from_a_graph(pkg, dev):
+    """A split decode captured once, replayed over growing contexts with eager calls between; two graphs."""
+    case = attention_case(39, [(1, 1500, 1501), (1, 30, 31)], h=8, h_kv=2)
+    case["table"] = np.concatenate([case["table"], np.zeros_like(case["table"][:, :1])], 1)
+    pool = pool_to_dev(pkg, case["pool"], dev)
+    q = to_bf16_tensor(case["q"], dev)
+    table, ctx, qo, qs, ql = attend_args(case, dev)
+    call = lambda: pkg.ops.paged_attention_fp8(q, pool, table, ctx, qo, qs, ql, 1)  # noqa: E731
+    call()
+    graphs, outs = [], []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(call())
+        graphs.append(g)
+    for step in range(3):
+        for g, o in zip(graphs, outs):
+            q.mul_(-1.25)
+            g.replay()
+            want = call()
+            torch.cuda.synchronize()
+            assert torch.equal(o, want)
+        ctx.add_(1)
+        qo.add_(1)
+
+
+def test_append_then_attend(pkg, dev):
+    """The operators as a serving loop uses them: prompts appended in chunks beside decoding sequences, then
+    decode steps, each step's rows attended; against fp64 attention over the unpacked cache, and that cache
+    against the rotated rows within its codes' rounding."""
+    rng = np.random.default_rng(40)
+    h, h_kv, d, bs, rotary = 8, 2, 128, 32, 64
+    cos, sin = pkg.ops.rope_table(512, rotary, 10000.0, device=dev)
+    pool = pkg.ops.fp8_kv_pool(40, bs, h_kv, d, dev)
+    table = rng.permutation(40)[:36].reshape(3, 12).astype(np.int32)
+    lens = [0, 0, 0]
+    kept = [[], [], []]
+    for step in [(70, 0, 1), (50, 33, 1), (1, 64, 1), (1, 1, 1), (1, 1, 0), (1, 1, 17)]:
+        ql = np.array(step, np.int32)
+        tokens = int(ql.sum())
+        x = bf16_rows(rng, tokens, h + 2 * h_kv, d)
+        qkv = to_dev(x, dev)
+        plan = dict(qo=np.array(lens, np.int32), ql=ql, ctx=np.array(lens, np.int32) + ql, table=table,
+                    qs=np.concatenate([[0], np.cumsum(ql)[:-1]]).astype(np.int32))
+        qo, qs, qlen, ctx, tab = (i32(plan[n], dev) for n in ("qo", "qs", "ql", "ctx", "table"))
+        most = int(ql.max())
+        q = pkg.ops.append_kv_fp8(qkv[:, :h], qkv[:, h:h + h_kv], qkv[:, h + h_kv:], cos, sin, pool, tab, qo,
+                                  qs, qlen, most, interleaved=True)
+        o = pkg.ops.paged_attention_fp8(q.transpose(0, 1), pool, tab, ctx, qo, qs, qlen, most)
+        torch.cuda.synchronize()
+        pos = np.concatenate([np.arange(a, a + n) for a, n in zip(lens, ql)]).astype(np.int64)
+        c, s = cos.cpu().numpy(), sin.cpu().numpy()
+        krot = kv.rotate(x[:, h:h + h_kv], c, s, pos, True)
+        host = tuple(t.view(torch.uint8).cpu().numpy() for t in pool)
+        golden, covered, vmax = attention_golden(dict(plan, q=bf16_bits(q.transpose(0, 1)), pool=host, bs=bs))
+        ok, msg = ora.attention_within_tolerance(bf16_bits(o), golden, vmax, covered)
+        assert ok, msg
+        for e, n in enumerate(ql):
+            rows = slice(int(plan["qs"][e]), int(plan["qs"][e]) + int(n))
+            kept[e] += list(krot[rows])
+            lens[e] += int(n)
+        values, _ = kv.unpack(host, bs)
+        for e in range(3):
+            for p in range(lens[e]):
+                block, sub = table[e, p // bs], p % bs // 16
+                scale = 2.0 ** (host[2][block, :, sub, 0].astype(np.int64) - 127)[:, None]
+                want = kept[e][p].astype(np.float64)
+                assert (np.abs(values[block, p % bs] - want)
+                        <= 2.0 ** -4 * np.abs(want) + 2.0 ** -9 * scale).all()
