@@ -1,5 +1,6 @@
 // Arguments and host entry points shared by the attention kernels over the 8-bit paged K/V cache
-// (attn_fp8.hip: the key-streaming kernel of decode rows and short chunks).
+// (attn_fp8.hip: the key-streaming kernel of decode rows and short chunks, attn_fp8_tile.hip: the row-tiled
+// kernel of prompts and longer chunks).
 #pragma once
 
 #include "attention.h"
@@ -18,14 +19,28 @@ struct Fp8AttnArgs {
   int64_t so_h, so_t;
   int entries, H, HKV, G, tokens;
   int max_ctx;       // positions that the table has room for
-  int max_q_len;     // rows of an entry in the split launch's workspace
+  int max_q_len;
+  int ws_q;          // rows of an entry in the split launch's workspace
+  int tiled;         // the row-tiled kernel runs too and takes the long entries (f8_is_long)
   int tq;            // query tokens per tile: floor(16 / G)
   int parts;         // 1: a workgroup takes every chunk of its item; > 1: one chunk of each of its waves
   int sorted;        // entries are taken in descending order of context length...
   int first_round;   // ...and, where > 0, those from this rank on in ascending order
   float scale_log2;  // softmax scale x log2(e)
-  float* ws_o;       // parts > 1: chunk states' O [parts x 4][entries][H][max_q_len][D], fp32
-  float* ws_ml;      // parts > 1: chunk states' max and sum [parts x 4][entries][H][max_q_len][2]
+  float* ws_o;       // parts > 1: chunk states' O [parts x 4][entries][H][ws_q][D], fp32
+  float* ws_ml;      // parts > 1: chunk states' max and sum [parts x 4][entries][H][ws_q][2]
 };
+
+// Whether the row-tiled kernel takes an entry of q_len tokens; the key-streaming kernel takes it otherwise.
+constexpr int kF8LongRows = 256;  // query rows per K/V head
+__host__ __device__ inline bool f8_is_long(int64_t q_len, int G) { return q_len * G >= kF8LongRows; }
+
+// The keys [0, end) that an entry's first `tokens` rows may see.
+__device__ __forceinline__ int f8_end(const Fp8AttnArgs& a, int qo, int ctx, int tokens) {
+  return max(min((int)min((int64_t)qo + tokens, (int64_t)ctx), a.max_ctx), 0);
+}
+
+// Launches the row-tiled kernel over every long entry.
+int launch_fp8_attn_tile(const Fp8AttnArgs& a, int64_t D, hipStream_t stream);
 
 }  // namespace lse

@@ -89,11 +89,6 @@ __device__ __forceinline__ int f8_sorted_entry(const Fp8AttnArgs& a, int slot) {
   return __ffsll(__ballot(rank == slot && lane < a.entries)) - 1;
 }
 
-// An entry's tile: the keys [0, end) that its rows may see.
-__device__ __forceinline__ int f8_end(const Fp8AttnArgs& a, int qo, int qlen, int ctx, int qt) {
-  return max(min((int)min((int64_t)qo + min(qlen, (qt + 1) * a.tq), (int64_t)ctx), a.max_ctx), 0);
-}
-
 // ONE: every entry has at most one tile (decode); the grid is K/V heads, entries, parts. Otherwise items are
 // counted entry by entry over their tiles and parts, without empty slots.
 template <int D, bool ONE>
@@ -122,11 +117,11 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
       int tiles = 0, parts = 1;
       if (i < a.entries) {
         const int qlen = min(a.q_len[i], a.max_q_len);
-        tiles = qlen > 0 ? (qlen + a.tq - 1) / a.tq : 0;
+        tiles = qlen > 0 && !(a.tiled && f8_is_long(qlen, a.G)) ? (qlen + a.tq - 1) / a.tq : 0;
         if (a.parts > 1) {
           const int ctx = a.context_len[i];
           const int64_t span = (int64_t)(kF8Window * kF8Waves) << f8_chunk_shift(ctx);
-          const int end = f8_end(a, a.query_offset[i], qlen, ctx, tiles);
+          const int end = f8_end(a, a.query_offset[i], ctx, qlen);
           parts = min(max((int)((end + span - 1) / span), 1), a.parts);
         }
       }
@@ -148,7 +143,7 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
   const int qlen = min(a.q_len[e], a.max_q_len);
   if (qt * a.tq >= qlen) return;
   const int ctx = a.context_len[e], qo = a.query_offset[e], qs = a.q_start[e];
-  const int end_n = f8_end(a, qo, qlen, ctx, qt);
+  const int end_n = f8_end(a, qo, ctx, min(qlen, (qt + 1) * a.tq));
   const int shift = f8_chunk_shift(ctx);
   // The wave's windows: j-th has keys [win(j), win(j) + 256); from j0 on, one chunk's in a split launch.
   auto win = [&](int j) -> int64_t {
@@ -338,7 +333,7 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
   if (a.parts > 1) {
     if (row_ok && (((int64_t)part * kF8Waves + wave) << shift) * kF8Window < end_n) {
       const int64_t slot =
-          (((int64_t)(part * kF8Waves + wave) * a.entries + e) * a.H + head) * a.max_q_len + m_row;
+          (((int64_t)(part * kF8Waves + wave) * a.entries + e) * a.H + head) * a.ws_q + m_row;
       float* dst = a.ws_o + slot * D + 4 * g;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
@@ -381,18 +376,18 @@ __global__ void __launch_bounds__(64 * kF8Waves) attn_fp8_merge(Fp8AttnArgs a) {
   __shared__ float mbuf[kF8Waves][64], lbuf[kF8Waves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t t = (int64_t)blockIdx.x * 64 + lane;
-  const int64_t rows = (int64_t)a.entries * a.H * a.max_q_len;
+  const int64_t rows = (int64_t)a.entries * a.H * a.ws_q;
   const int c8 = 8 * (int)(t % C);
   const int64_t r = t / C;
-  const int m_row = (int)(r % a.max_q_len), h = (int)(r / a.max_q_len % a.H);
-  const int e = (int)min(r / a.max_q_len / a.H, (int64_t)a.entries - 1);
+  const int m_row = (int)(r % a.ws_q), h = (int)(r / a.ws_q % a.H);
+  const int e = (int)min(r / a.ws_q / a.H, (int64_t)a.entries - 1);
   const int qlen = min(a.q_len[e], a.max_q_len);
   const int64_t row = (int64_t)a.q_start[e] + m_row;
-  const bool ok = r < rows && m_row < qlen && row >= 0 && row < a.tokens;
+  const bool ok = r < rows && m_row < qlen && !(a.tiled && f8_is_long(qlen, a.G)) && row >= 0 && row < a.tokens;
   float M = kNegInf, L = 0.0f, O[8] = {0, 0, 0, 0, 0, 0, 0, 0};
   if (ok) {
     const int ctx = a.context_len[e];
-    const int end_n = f8_end(a, a.query_offset[e], qlen, ctx, m_row / a.tq);
+    const int end_n = f8_end(a, a.query_offset[e], ctx, min(qlen, (m_row / a.tq + 1) * a.tq));
     const int64_t chunk = (int64_t)kF8Window << f8_chunk_shift(ctx);
     const int chunks = (int)((end_n + chunk - 1) / chunk);
     const int mine = chunks > wave ? (chunks - wave + kF8Waves - 1) / kF8Waves : 0;
@@ -430,6 +425,8 @@ __global__ void __launch_bounds__(64 * kF8Waves) attn_fp8_merge(Fp8AttnArgs a) {
 
 struct Fp8AttnPlan {
   int tq, parts;
+  bool tiled;       // some entry may be the row-tiled kernel's
+  int64_t short_q;  // the most tokens of an entry that is not
   int64_t tiles;  // at most, over all entries
   int64_t ws_o_bytes, ws_bytes;
 };
@@ -451,11 +448,14 @@ static Fp8AttnPlan fp8_attn_plan(int64_t entries, int64_t tokens, int64_t H, int
                                  int64_t max_q_len, int64_t max_ctx, int cus) {
   Fp8AttnPlan pl{};
   pl.tq = (int)(16 / (H / HKV));
-  pl.tiles = std::min(entries * ceil_div(max_q_len, (int64_t)pl.tq), tokens / pl.tq + entries);
+  const int64_t G = H / HKV;
+  pl.tiled = f8_is_long(max_q_len, (int)G);
+  pl.short_q = pl.tiled ? (kF8LongRows - 1) / G : max_q_len;
+  pl.tiles = std::min(entries * ceil_div(pl.short_q, (int64_t)pl.tq), tokens / pl.tq + entries);
   const int64_t rounds = std::min<int64_t>(ceil_div(max_ctx, (int64_t)kF8Window * kF8Waves), kF8MaxParts);
   pl.parts = pl.tiles * HKV < 2 * (int64_t)cus && rounds > 1 ? (int)rounds : 1;
   if (pl.parts > 1) {
-    const int64_t slots = (int64_t)pl.parts * kF8Waves * entries * H * max_q_len;
+    const int64_t slots = (int64_t)pl.parts * kF8Waves * entries * H * pl.short_q;
     pl.ws_o_bytes = slots * D * 4;
     pl.ws_bytes = pl.ws_o_bytes + slots * 2 * 4;
   }
@@ -465,13 +465,15 @@ static Fp8AttnPlan fp8_attn_plan(int64_t entries, int64_t tokens, int64_t H, int
 template <int D>
 static int launch_fp8_attention(const Fp8AttnArgs& a, int64_t blocks, hipStream_t stream) {
   const dim3 wg(64 * kF8Waves);
-  if (a.max_q_len <= a.tq)
+  if (a.tiled)
+    if (int st = launch_fp8_attn_tile(a, D, stream)) return st;
+  if (a.ws_q <= a.tq)
     hipLaunchKernelGGL((attn_fp8_kernel<D, true>), dim3((unsigned)blocks), wg, 0, stream, a);
   else
     hipLaunchKernelGGL((attn_fp8_kernel<D, false>), dim3((unsigned)blocks), wg, 0, stream, a);
   if (int st = launch_status()) return st;
   if (a.parts > 1) {
-    const int64_t pieces = (int64_t)a.entries * a.H * a.max_q_len * (D / 8);
+    const int64_t pieces = (int64_t)a.entries * a.H * a.ws_q * (D / 8);
     hipLaunchKernelGGL(attn_fp8_merge<D>, dim3((unsigned)ceil_div(pieces, 64)), wg, 0, stream, a);
   }
   return launch_status();
@@ -550,7 +552,7 @@ int lse_paged_attention_fp8(const void* q, int64_t q_stride_h, int64_t q_stride_
   a.o = (uint16_t*)o, a.so_h = o_stride_h, a.so_t = o_stride_t;
   a.entries = (int)entries, a.H = (int)H, a.HKV = (int)H_KV, a.G = (int)(H / H_KV), a.tokens = (int)tokens;
   a.max_ctx = (int)(max_blocks * block_size);
-  a.max_q_len = (int)max_q_len;
+  a.max_q_len = (int)max_q_len, a.ws_q = (int)pl.short_q, a.tiled = pl.tiled;
   a.tq = pl.tq, a.parts = pl.parts;
   a.scale_log2 = softmax_scale * 1.4426950408889634f;
   a.ws_o = pl.parts > 1 ? (float*)workspace : nullptr;
@@ -558,8 +560,8 @@ int lse_paged_attention_fp8(const void* q, int64_t q_stride_h, int64_t q_stride_
   const int64_t items = entries * H_KV;
   a.sorted = a.parts == 1 && entries <= 64 && items > cus && a.max_ctx > 256;
   a.first_round = items > cus && items <= 2 * (int64_t)cus && cus % a.HKV == 0 ? cus / a.HKV : 0;
-  const int64_t blocks = (max_q_len <= pl.tq ? entries : pl.tiles) * H_KV * pl.parts;
-  if (blocks > kMax31 || entries * H * max_q_len * (D / 8) / 64 > kMax31) return LSE_E_RANGE;
+  const int64_t blocks = (pl.short_q <= pl.tq ? entries : pl.tiles) * H_KV * pl.parts;
+  if (blocks > kMax31 || entries * H * pl.short_q * (D / 8) / 64 > kMax31) return LSE_E_RANGE;
   return D == 64 ? lse::launch_fp8_attention<64>(a, blocks, (hipStream_t)stream)
                  : lse::launch_fp8_attention<128>(a, blocks, (hipStream_t)stream);
 }
