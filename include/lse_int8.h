@@ -374,6 +374,8 @@ int lse_rope_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride
                 int64_t sequences, int64_t tokens_per_sequence, int64_t start, void* stream);
 
 /*
+ * The entry points from here on take their arguments in a struct, whose fields are all eight bytes wide.
+ *
  * Rotary positions of q and k rows from fp32 tables, in one launch. With pair i < rotary / 2 of a head at
  * dims (i, i + rotary / 2), or (2 i, 2 i + 1) when interleaved is 1, and c, s the tables' values for the
  * row's position and i:  a' = bf16(a c - b s), b' = bf16(b c + a s), products and sums rounded in fp32
@@ -385,10 +387,18 @@ int lse_rope_kv(const void* q, int64_t q_stride, const void* k, int64_t k_stride
  * Replaces: apply_rotary_pos_emb in `_project_qkv` (model_runner.py:310-326), for the layouts, partial
  * rotations and scaled tables that the reference's models do not use.
  */
-int lse_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
-             int64_t k_stride_h, const float* cos, const float* sin, int64_t table_rows,
-             const int32_t* positions, void* q_out, void* k_out, int64_t tokens, int64_t H, int64_t H_KV,
-             int64_t D, int64_t rotary, int interleaved, void* stream);
+struct lse_rope_args {
+  const void* q;
+  int64_t q_stride_t, q_stride_h;
+  const void* k;
+  int64_t k_stride_t, k_stride_h;
+  const float *cos, *sin;
+  int64_t table_rows;
+  const int32_t* positions;
+  void *q_out, *k_out;
+  int64_t tokens, H, H_KV, D, rotary, interleaved;
+};
+int lse_rope(const struct lse_rope_args* args, void* stream);
 
 /*
  * The 8-bit paged K/V cache. Codes are float8 e4m3 (448 the largest), and each group of 16 positions of a K/V
@@ -414,37 +424,52 @@ int lse_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* 
  * Replaces: apply_rotary_pos_emb and the K/V writes in `_project_qkv` and `attend_paged`
  * (model_runner.py:310-363), for an 8-bit pool, which the reference does not have.
  */
-int lse_append_kv_fp8(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
-                      int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
-                      int64_t v_stride_h, const float* cos, const float* sin, int64_t table_rows,
-                      void* q_out, void* k_pool, void* v_pool, int64_t pool_stride_block, void* scales,
-                      int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
-                      const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
-                      const int32_t* query_offset, const int32_t* q_start, const int32_t* q_len,
-                      int64_t entries, int64_t tokens, int64_t max_q_len, int64_t H, int64_t H_KV,
-                      int64_t D, int64_t rotary, int interleaved, void* stream);
+struct lse_append_kv_fp8_args {
+  const void* q;
+  int64_t q_stride_t, q_stride_h;
+  const void* k;
+  int64_t k_stride_t, k_stride_h;
+  const void* v;
+  int64_t v_stride_t, v_stride_h;
+  const float *cos, *sin;
+  int64_t table_rows;
+  void *q_out, *k_pool, *v_pool;
+  int64_t pool_stride_block;
+  void* scales;
+  int64_t scales_stride_block, num_blocks, block_size;
+  const int32_t* block_table;
+  int64_t block_table_stride, max_blocks;
+  const int32_t *query_offset, *q_start, *q_len;
+  int64_t entries, tokens, max_q_len, H, H_KV, D, rotary, interleaved;
+};
+int lse_append_kv_fp8(const struct lse_append_kv_fp8_args* args, void* stream);
 
 /*
  * lse_paged_attention over the 8-bit cache: the same plan, semantics and determinism, k and v being the
  * values code x scale. q and o have `tokens` rows; entries own distinct ones, and rows of no entry are not
  * written. A block outside the pool makes the rows that see it NaN; a context longer than the table is cut.
  * D = 64 or 128; 1 <= H / H_KV <= 16; block_size % 16 == 0; the strides of q and o multiples of 8, q, o and
- * the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes (-1: invalid sizes),
- * 16-byte aligned.
+ * the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes (it reads the
+ * sizes in args only; -1: invalid ones), 16-byte aligned.
  * Replaces: `paged_attention_forward` (src/llm_serving_engine/kernels/flash_attention.py:287-332) over a pool
  * the reference does not have.
  */
-int64_t lse_paged_attention_fp8_workspace_bytes(int64_t entries, int64_t tokens, int64_t H, int64_t H_KV,
-                                                int64_t D, int64_t max_q_len, int64_t max_blocks,
-                                                int64_t block_size);
-int lse_paged_attention_fp8(const void* q, int64_t q_stride_h, int64_t q_stride_t, const void* k_pool,
-                            const void* v_pool, int64_t pool_stride_block, const void* scales,
-                            int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
-                            const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
-                            const int32_t* context_len, const int32_t* query_offset,
-                            const int32_t* q_start, const int32_t* q_len, void* o, int64_t o_stride_h,
-                            int64_t o_stride_t, int64_t entries, int64_t tokens, int64_t max_q_len,
-                            int64_t H, int64_t H_KV, int64_t D, float softmax_scale, void* workspace,
+struct lse_paged_attention_fp8_args {
+  const void* q;
+  int64_t q_stride_h, q_stride_t;
+  const void *k_pool, *v_pool;
+  int64_t pool_stride_block;
+  const void* scales;
+  int64_t scales_stride_block, num_blocks, block_size;
+  const int32_t* block_table;
+  int64_t block_table_stride, max_blocks;
+  const int32_t *context_len, *query_offset, *q_start, *q_len;
+  void* o;
+  int64_t o_stride_h, o_stride_t, entries, tokens, max_q_len, H, H_KV, D;
+  double softmax_scale;
+};
+int64_t lse_paged_attention_fp8_workspace_bytes(const struct lse_paged_attention_fp8_args* args);
+int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, void* workspace,
                             int64_t workspace_bytes, void* stream);
 
 /* Static properties (enum lse_query_key); -1 for an unknown key. Load-time checks read these,

@@ -486,84 +486,83 @@ namespace {
 constexpr int64_t kMax31 = 2147483647;
 bool aligned(const void* p, uintptr_t bytes) { return ((uintptr_t)p % bytes) == 0; }
 
-int check_sizes(int64_t entries, int64_t tokens, int64_t H, int64_t HKV, int64_t D, int64_t max_q_len,
-                int64_t max_blocks, int64_t block_size) {
-  if (entries < 0 || entries > kMax31 || tokens < 0 || tokens > kMax31 || H < 1 || H > 65536 || HKV < 1 ||
-      H % HKV || H / HKV > 16 || (D != 64 && D != 128) || max_q_len < 0 || max_q_len > kMax31 ||
-      max_blocks < 0 || block_size < 16 || block_size % 16)
+typedef lse_paged_attention_fp8_args Args;
+
+int check_sizes(const Args& x) {
+  if (x.entries < 0 || x.entries > kMax31 || x.tokens < 0 || x.tokens > kMax31 || x.H < 1 || x.H > 65536 ||
+      x.H_KV < 1 || x.H % x.H_KV || x.H / x.H_KV > 16 || (x.D != 64 && x.D != 128) || x.max_q_len < 0 ||
+      x.max_q_len > kMax31 || x.max_blocks < 0 || x.block_size < 16 || x.block_size % 16)
     return LSE_E_SHAPE;
-  return block_size > kMax31 || max_blocks > kMax31 / block_size ? LSE_E_RANGE : LSE_OK;
+  return x.block_size > kMax31 || x.max_blocks > kMax31 / x.block_size ? LSE_E_RANGE : LSE_OK;
+}
+
+lse::Fp8AttnPlan plan_of(const Args& x, int cus) {
+  return lse::fp8_attn_plan(x.entries, x.tokens, x.H, x.H_KV, x.D, x.max_q_len, x.max_blocks * x.block_size,
+                            cus);
 }
 
 }  // namespace
 
 extern "C" {
 
-int64_t lse_paged_attention_fp8_workspace_bytes(int64_t entries, int64_t tokens, int64_t H, int64_t H_KV,
-                                                int64_t D, int64_t max_q_len, int64_t max_blocks,
-                                                int64_t block_size) {
-  if (check_sizes(entries, tokens, H, H_KV, D, max_q_len, max_blocks, block_size)) return -1;
-  if (entries == 0 || tokens == 0 || max_q_len == 0) return 0;
-  return lse::fp8_attn_plan(entries, tokens, H, H_KV, D, max_q_len, max_blocks * block_size,
-                            lse::fp8_attn_cus())
-      .ws_bytes;
+int64_t lse_paged_attention_fp8_workspace_bytes(const struct lse_paged_attention_fp8_args* args) {
+  if (!args || check_sizes(*args)) return -1;
+  if (args->entries == 0 || args->tokens == 0 || args->max_q_len == 0) return 0;
+  return plan_of(*args, lse::fp8_attn_cus()).ws_bytes;
 }
 
-int lse_paged_attention_fp8(const void* q, int64_t q_stride_h, int64_t q_stride_t, const void* k_pool,
-                            const void* v_pool, int64_t pool_stride_block, const void* scales,
-                            int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
-                            const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
-                            const int32_t* context_len, const int32_t* query_offset,
-                            const int32_t* q_start, const int32_t* q_len, void* o, int64_t o_stride_h,
-                            int64_t o_stride_t, int64_t entries, int64_t tokens, int64_t max_q_len,
-                            int64_t H, int64_t H_KV, int64_t D, float softmax_scale, void* workspace,
+int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, void* workspace,
                             int64_t workspace_bytes, void* stream) {
-  if (int st = check_sizes(entries, tokens, H, H_KV, D, max_q_len, max_blocks, block_size)) return st;
-  if (num_blocks < 0 || num_blocks > kMax31 || block_table_stride < max_blocks) return LSE_E_SHAPE;
-  const int64_t per = block_size / 16;
-  if (pool_stride_block < H_KV * per * 16 * D || scales_stride_block < 2 * H_KV * per) return LSE_E_SHAPE;
-  if (entries == 0 || tokens == 0 || max_q_len == 0) return LSE_OK;
-  if (num_blocks < 1) return LSE_E_SHAPE;
-  if (!q || !k_pool || !v_pool || !scales || !block_table || !context_len || !query_offset || !q_start ||
-      !q_len || !o)
+  if (!args) return LSE_E_NULL;
+  const Args& x = *args;
+  if (int st = check_sizes(x)) return st;
+  if (x.num_blocks < 0 || x.num_blocks > kMax31 || x.block_table_stride < x.max_blocks) return LSE_E_SHAPE;
+  const int64_t per = x.block_size / 16;
+  if (x.pool_stride_block < x.H_KV * per * 16 * x.D || x.scales_stride_block < 2 * x.H_KV * per)
+    return LSE_E_SHAPE;
+  if (x.entries == 0 || x.tokens == 0 || x.max_q_len == 0) return LSE_OK;
+  if (x.num_blocks < 1) return LSE_E_SHAPE;
+  if (!x.q || !x.k_pool || !x.v_pool || !x.scales || !x.block_table || !x.context_len || !x.query_offset ||
+      !x.q_start || !x.q_len || !x.o)
     return LSE_E_NULL;
   // Groups are addressed in 16-byte units by 32 bits.
-  if (num_blocks > (((int64_t)1 << 36) - 1) / pool_stride_block) return LSE_E_RANGE;
-  const int64_t strides[] = {q_stride_h, q_stride_t, o_stride_h, o_stride_t};
+  if (x.num_blocks > (((int64_t)1 << 36) - 1) / x.pool_stride_block) return LSE_E_RANGE;
+  const int64_t strides[] = {x.q_stride_h, x.q_stride_t, x.o_stride_h, x.o_stride_t};
   for (int64_t s : strides)
     if (s < 0) return LSE_E_SHAPE;
   for (int64_t s : strides)
     if (s % 8) return LSE_E_ALIGN;
-  if (pool_stride_block % 16 || scales_stride_block % 2 || !aligned(q, 16) || !aligned(o, 16) ||
-      !aligned(k_pool, 16) || !aligned(v_pool, 16) || !aligned(scales, 2) || !aligned(block_table, 4) ||
-      !aligned(context_len, 4) || !aligned(query_offset, 4) || !aligned(q_start, 4) || !aligned(q_len, 4))
+  if (x.pool_stride_block % 16 || x.scales_stride_block % 2 || !aligned(x.q, 16) || !aligned(x.o, 16) ||
+      !aligned(x.k_pool, 16) || !aligned(x.v_pool, 16) || !aligned(x.scales, 2) ||
+      !aligned(x.block_table, 4) || !aligned(x.context_len, 4) || !aligned(x.query_offset, 4) ||
+      !aligned(x.q_start, 4) || !aligned(x.q_len, 4))
     return LSE_E_ALIGN;
   if (workspace_bytes < 0 || (workspace && !aligned(workspace, 16))) return LSE_E_WORKSPACE;
   const int cus = lse::fp8_attn_cus();
-  const lse::Fp8AttnPlan pl =
-      lse::fp8_attn_plan(entries, tokens, H, H_KV, D, max_q_len, max_blocks * block_size, cus);
+  const lse::Fp8AttnPlan pl = plan_of(x, cus);
   if (pl.ws_bytes > 0 && (workspace_bytes < pl.ws_bytes || !workspace)) return LSE_E_WORKSPACE;
   lse::Fp8AttnArgs a{};
-  a.q = (const uint16_t*)q, a.sq_h = q_stride_h, a.sq_t = q_stride_t;
-  a.pool = {(uint8_t*)k_pool, (uint8_t*)v_pool, (uint8_t*)scales, pool_stride_block, scales_stride_block,
-            (int)num_blocks, (int)per};
-  a.block_table = block_table, a.sbt = block_table_stride;
-  a.context_len = context_len, a.query_offset = query_offset, a.q_start = q_start, a.q_len = q_len;
-  a.o = (uint16_t*)o, a.so_h = o_stride_h, a.so_t = o_stride_t;
-  a.entries = (int)entries, a.H = (int)H, a.HKV = (int)H_KV, a.G = (int)(H / H_KV), a.tokens = (int)tokens;
-  a.max_ctx = (int)(max_blocks * block_size);
-  a.max_q_len = (int)max_q_len, a.ws_q = (int)pl.short_q, a.tiled = pl.tiled;
+  a.q = (const uint16_t*)x.q, a.sq_h = x.q_stride_h, a.sq_t = x.q_stride_t;
+  a.pool = {(uint8_t*)x.k_pool, (uint8_t*)x.v_pool, (uint8_t*)x.scales, x.pool_stride_block,
+            x.scales_stride_block, (int)x.num_blocks, (int)per};
+  a.block_table = x.block_table, a.sbt = x.block_table_stride;
+  a.context_len = x.context_len, a.query_offset = x.query_offset, a.q_start = x.q_start, a.q_len = x.q_len;
+  a.o = (uint16_t*)x.o, a.so_h = x.o_stride_h, a.so_t = x.o_stride_t;
+  a.entries = (int)x.entries, a.H = (int)x.H, a.HKV = (int)x.H_KV, a.G = (int)(x.H / x.H_KV);
+  a.tokens = (int)x.tokens;
+  a.max_ctx = (int)(x.max_blocks * x.block_size);
+  a.max_q_len = (int)x.max_q_len, a.ws_q = (int)pl.short_q, a.tiled = pl.tiled;
   a.tq = pl.tq, a.parts = pl.parts;
-  a.scale_log2 = softmax_scale * 1.4426950408889634f;
+  a.scale_log2 = (float)x.softmax_scale * 1.4426950408889634f;
   a.ws_o = pl.parts > 1 ? (float*)workspace : nullptr;
   a.ws_ml = pl.parts > 1 ? (float*)((char*)workspace + pl.ws_o_bytes) : nullptr;
-  const int64_t items = entries * H_KV;
-  a.sorted = a.parts == 1 && entries <= 64 && items > cus && a.max_ctx > 256;
+  const int64_t items = x.entries * x.H_KV;
+  a.sorted = a.parts == 1 && x.entries <= 64 && items > cus && a.max_ctx > 256;
   a.first_round = items > cus && items <= 2 * (int64_t)cus && cus % a.HKV == 0 ? cus / a.HKV : 0;
-  const int64_t blocks = (pl.short_q <= pl.tq ? entries : pl.tiles) * H_KV * pl.parts;
-  if (blocks > kMax31 || entries * H * pl.short_q * (D / 8) / 64 > kMax31) return LSE_E_RANGE;
-  return D == 64 ? lse::launch_fp8_attention<64>(a, blocks, (hipStream_t)stream)
-                 : lse::launch_fp8_attention<128>(a, blocks, (hipStream_t)stream);
+  const int64_t blocks = (pl.short_q <= pl.tq ? x.entries : pl.tiles) * x.H_KV * pl.parts;
+  if (blocks > kMax31 || x.entries * x.H * pl.short_q * (x.D / 8) / 64 > kMax31) return LSE_E_RANGE;
+  return x.D == 64 ? lse::launch_fp8_attention<64>(a, blocks, (hipStream_t)stream)
+                   : lse::launch_fp8_attention<128>(a, blocks, (hipStream_t)stream);
 }
 
 }  // extern "C"

@@ -291,86 +291,81 @@ int check_rows(const void* p, int64_t st, int64_t sh) {
 
 extern "C" {
 
-int lse_rope(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k, int64_t k_stride_t,
-             int64_t k_stride_h, const float* cos, const float* sin, int64_t table_rows,
-             const int32_t* positions, void* q_out, void* k_out, int64_t tokens, int64_t H, int64_t H_KV,
-             int64_t D, int64_t rotary, int interleaved, void* stream) {
-  if (tokens < 0 || tokens > kMax31 || H < 1 || H > 65536 || H_KV < 0 || H_KV > 65536 || D < 16 ||
-      D > 1024 || D % 16 || rotary < 16 || rotary > D || rotary % 16 || table_rows < 1 ||
-      (interleaved != 0 && interleaved != 1))
+int lse_rope(const struct lse_rope_args* args, void* stream) {
+  if (!args) return LSE_E_NULL;
+  const lse_rope_args& x = *args;
+  if (x.tokens < 0 || x.tokens > kMax31 || x.H < 1 || x.H > 65536 || x.H_KV < 0 || x.H_KV > 65536 ||
+      x.D < 16 || x.D > 1024 || x.D % 16 || x.rotary < 16 || x.rotary > x.D || x.rotary % 16 ||
+      x.table_rows < 1 || (x.interleaved != 0 && x.interleaved != 1))
     return LSE_E_SHAPE;
-  if (tokens == 0) return LSE_OK;
-  if (!q || !q_out || !cos || !sin || !positions || (H_KV > 0 && (!k || !k_out))) return LSE_E_NULL;
-  if (int st = check_rows(q, q_stride_t, q_stride_h)) return st;
-  if (H_KV > 0)
-    if (int st = check_rows(k, k_stride_t, k_stride_h)) return st;
-  if (!aligned16(cos) || !aligned16(sin) || !aligned16(q_out) || !aligned16(k_out) ||
-      ((uintptr_t)positions & 3))
+  if (x.tokens == 0) return LSE_OK;
+  if (!x.q || !x.q_out || !x.cos || !x.sin || !x.positions || (x.H_KV > 0 && (!x.k || !x.k_out)))
+    return LSE_E_NULL;
+  if (int st = check_rows(x.q, x.q_stride_t, x.q_stride_h)) return st;
+  if (x.H_KV > 0)
+    if (int st = check_rows(x.k, x.k_stride_t, x.k_stride_h)) return st;
+  if (!aligned16(x.cos) || !aligned16(x.sin) || !aligned16(x.q_out) || !aligned16(x.k_out) ||
+      ((uintptr_t)x.positions & 3))
     return LSE_E_ALIGN;
   lse::RopeFp32Args a{};
-  a.q = {(const uint16_t*)q, q_stride_t, q_stride_h};
-  a.k = {(const uint16_t*)k, k_stride_t, k_stride_h};
-  a.r = {cos, sin, table_rows, (int)(rotary / 2), interleaved};
-  a.positions = positions;
-  a.q_out = (uint16_t*)q_out, a.k_out = (uint16_t*)k_out;
-  a.H = (int)H, a.HKV = (int)H_KV, a.D = (int)D;
-  a.units = (int)((H + H_KV) * (D / 16));
-  const int64_t total = tokens * a.units, blocks = lse::ceil_div(total, 256);
+  a.q = {(const uint16_t*)x.q, x.q_stride_t, x.q_stride_h};
+  a.k = {(const uint16_t*)x.k, x.k_stride_t, x.k_stride_h};
+  a.r = {x.cos, x.sin, x.table_rows, (int)(x.rotary / 2), (int)x.interleaved};
+  a.positions = x.positions;
+  a.q_out = (uint16_t*)x.q_out, a.k_out = (uint16_t*)x.k_out;
+  a.H = (int)x.H, a.HKV = (int)x.H_KV, a.D = (int)x.D;
+  a.units = (int)((x.H + x.H_KV) * (x.D / 16));
+  const int64_t total = x.tokens * a.units, blocks = lse::ceil_div(total, 256);
   if (blocks > kMax31) return LSE_E_RANGE;
   hipLaunchKernelGGL(lse::rope_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream, a, total);
   return lse::launch_status();
 }
 
-int lse_append_kv_fp8(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* k,
-                      int64_t k_stride_t, int64_t k_stride_h, const void* v, int64_t v_stride_t,
-                      int64_t v_stride_h, const float* cos, const float* sin, int64_t table_rows,
-                      void* q_out, void* k_pool, void* v_pool, int64_t pool_stride_block, void* scales,
-                      int64_t scales_stride_block, int64_t num_blocks, int64_t block_size,
-                      const int32_t* block_table, int64_t block_table_stride, int64_t max_blocks,
-                      const int32_t* query_offset, const int32_t* q_start, const int32_t* q_len,
-                      int64_t entries, int64_t tokens, int64_t max_q_len, int64_t H, int64_t H_KV,
-                      int64_t D, int64_t rotary, int interleaved, void* stream) {
-  if (entries < 0 || entries > kMax31 || tokens < 0 || tokens > kMax31 || max_q_len < 0 ||
-      max_q_len > kMax31 || H < 1 || H > 65536 || H_KV < 1 || H % H_KV || (D != 64 && D != 128) ||
-      rotary < 0 || rotary > D || rotary % 16 || (interleaved != 0 && interleaved != 1) ||
-      num_blocks < 0 || num_blocks > kMax31 || block_size < 16 || block_size % 16 ||
-      max_blocks < 0 || block_table_stride < max_blocks)
+int lse_append_kv_fp8(const struct lse_append_kv_fp8_args* args, void* stream) {
+  if (!args) return LSE_E_NULL;
+  const lse_append_kv_fp8_args& x = *args;
+  if (x.entries < 0 || x.entries > kMax31 || x.tokens < 0 || x.tokens > kMax31 || x.max_q_len < 0 ||
+      x.max_q_len > kMax31 || x.H < 1 || x.H > 65536 || x.H_KV < 1 || x.H % x.H_KV ||
+      (x.D != 64 && x.D != 128) || x.rotary < 0 || x.rotary > x.D || x.rotary % 16 ||
+      (x.interleaved != 0 && x.interleaved != 1) || x.num_blocks < 0 || x.num_blocks > kMax31 ||
+      x.block_size < 16 || x.block_size % 16 || x.max_blocks < 0 || x.block_table_stride < x.max_blocks)
     return LSE_E_SHAPE;
-  if (block_size > kMax31 || max_blocks > kMax31 / block_size) return LSE_E_RANGE;
-  const int64_t per = block_size / 16;
-  if (pool_stride_block < H_KV * per * 16 * D || scales_stride_block < 2 * H_KV * per) return LSE_E_SHAPE;
-  if (entries == 0 || tokens == 0 || max_q_len == 0) return LSE_OK;
-  if (!k || !v || !k_pool || !v_pool || !scales || !block_table || !query_offset || !q_start || !q_len ||
-      (q && !q_out) || (rotary > 0 && (!cos || !sin)))
+  if (x.block_size > kMax31 || x.max_blocks > kMax31 / x.block_size) return LSE_E_RANGE;
+  const int64_t per = x.block_size / 16;
+  if (x.pool_stride_block < x.H_KV * per * 16 * x.D || x.scales_stride_block < 2 * x.H_KV * per)
+    return LSE_E_SHAPE;
+  if (x.entries == 0 || x.tokens == 0 || x.max_q_len == 0) return LSE_OK;
+  if (!x.k || !x.v || !x.k_pool || !x.v_pool || !x.scales || !x.block_table || !x.query_offset ||
+      !x.q_start || !x.q_len || (x.q && !x.q_out) || (x.rotary > 0 && (!x.cos || !x.sin)))
     return LSE_E_NULL;
-  if (rotary > 0 && table_rows < 1) return LSE_E_SHAPE;
-  if (q)
-    if (int st = check_rows(q, q_stride_t, q_stride_h)) return st;
-  if (int st = check_rows(k, k_stride_t, k_stride_h)) return st;
-  if (int st = check_rows(v, v_stride_t, v_stride_h)) return st;
-  if (pool_stride_block % 16 || !aligned16(cos) || !aligned16(sin) || !aligned16(q_out) ||
-      !aligned16(k_pool) || !aligned16(v_pool))
+  if (x.rotary > 0 && x.table_rows < 1) return LSE_E_SHAPE;
+  if (x.q)
+    if (int st = check_rows(x.q, x.q_stride_t, x.q_stride_h)) return st;
+  if (int st = check_rows(x.k, x.k_stride_t, x.k_stride_h)) return st;
+  if (int st = check_rows(x.v, x.v_stride_t, x.v_stride_h)) return st;
+  if (x.pool_stride_block % 16 || !aligned16(x.cos) || !aligned16(x.sin) || !aligned16(x.q_out) ||
+      !aligned16(x.k_pool) || !aligned16(x.v_pool))
     return LSE_E_ALIGN;
   lse::AppendArgs a{};
-  a.q = {(const uint16_t*)q, q_stride_t, q_stride_h};
-  a.k = {(const uint16_t*)k, k_stride_t, k_stride_h};
-  a.v = {(const uint16_t*)v, v_stride_t, v_stride_h};
-  a.r = {cos, sin, table_rows, (int)(rotary / 2), interleaved};
-  a.q_out = (uint16_t*)q_out;
-  a.pool = {(uint8_t*)k_pool, (uint8_t*)v_pool, (uint8_t*)scales, pool_stride_block, scales_stride_block,
-            (int)num_blocks, (int)per};
-  a.block_table = block_table, a.sbt = block_table_stride;
-  a.query_offset = query_offset, a.q_start = q_start, a.q_len = q_len;
-  a.entries = (int)entries, a.H = (int)H, a.HKV = (int)H_KV, a.G = (int)(H / H_KV);
-  a.max_groups = (int)(max_blocks * per);
-  a.tokens = tokens;
-  a.one = max_q_len == 1;
+  a.q = {(const uint16_t*)x.q, x.q_stride_t, x.q_stride_h};
+  a.k = {(const uint16_t*)x.k, x.k_stride_t, x.k_stride_h};
+  a.v = {(const uint16_t*)x.v, x.v_stride_t, x.v_stride_h};
+  a.r = {x.cos, x.sin, x.table_rows, (int)(x.rotary / 2), (int)x.interleaved};
+  a.q_out = (uint16_t*)x.q_out;
+  a.pool = {(uint8_t*)x.k_pool, (uint8_t*)x.v_pool, (uint8_t*)x.scales, x.pool_stride_block,
+            x.scales_stride_block, (int)x.num_blocks, (int)per};
+  a.block_table = x.block_table, a.sbt = x.block_table_stride;
+  a.query_offset = x.query_offset, a.q_start = x.q_start, a.q_len = x.q_len;
+  a.entries = (int)x.entries, a.H = (int)x.H, a.HKV = (int)x.H_KV, a.G = (int)(x.H / x.H_KV);
+  a.max_groups = (int)(x.max_blocks * per);
+  a.tokens = x.tokens;
+  a.one = x.max_q_len == 1;
   // An entry of n tokens touches at most (n + 30) / 16 groups; the entries' rows are distinct.
-  const int64_t most = std::min(entries * ((max_q_len + 30) / 16), tokens / 16 + 2 * entries);
-  const int64_t blocks = (a.one ? entries : most) * H_KV;
+  const int64_t most = std::min(x.entries * ((x.max_q_len + 30) / 16), x.tokens / 16 + 2 * x.entries);
+  const int64_t blocks = (a.one ? x.entries : most) * x.H_KV;
   if (blocks > kMax31) return LSE_E_RANGE;
   const dim3 grid((unsigned)blocks), wg(256);
-  if (D == 64)
+  if (x.D == 64)
     hipLaunchKernelGGL(lse::append_kv_kernel<64>, grid, wg, 0, (hipStream_t)stream, a);
   else
     hipLaunchKernelGGL(lse::append_kv_kernel<128>, grid, wg, 0, (hipStream_t)stream, a);

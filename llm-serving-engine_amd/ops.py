@@ -603,18 +603,29 @@ def rope_kv(
 # ---- rotary positions and the 8-bit K/V cache ----------------------------------------------------
 
 KV_GROUP = 16  # positions of a head that share a scale
+_F8, _E8, _BF16, _I32 = torch.float8_e4m3fn, torch.float8_e8m0fnu, torch.bfloat16, torch.int32
 
 
-def _launch(dev: int, what: str, *args) -> None:
-    """Calls the entry point `what` with dev's current stream behind the arguments. A kernel goes to the
-    current device, whose default stream has the handle of every other's."""
-    fn = getattr(_lib.library(), what)
-    if torch.cuda.current_device() == dev:
-        status = fn(*args, _stream(dev))
+def _one_gpu(first: torch.Tensor, *others: torch.Tensor) -> int:
+    """`_on_gpu` in one call a tensor (get_device is -1 on the host)."""
+    dev = first.get_device()
+    for t in others:
+        if t.get_device() != dev:
+            return _on_gpu(first, *others)
+    return dev if dev >= 0 else _on_gpu(first)
+
+
+def _launch(dev: int, what: str, args: bytes, *more) -> None:
+    """Calls the entry point `what` with packed args and dev's current stream. A kernel goes to the current
+    device, whose default stream has the handle of every other's."""
+    fn = getattr(_lib._lib or _lib.library(), what)
+    if torch._C._cuda_getDevice() == dev:
+        status = fn(args, *more, torch._C._cuda_getCurrentRawStream(dev))
     else:
         with torch.cuda.device(dev):
-            status = fn(*args, _stream(dev))
-    _lib.check(status, what)
+            status = fn(args, *more, torch._C._cuda_getCurrentRawStream(dev))
+    if status:
+        _lib.check(status, what)
 
 
 def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dict | None = None,
@@ -661,15 +672,16 @@ def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dic
     return (gain * torch.cos(angle)).float(), (gain * torch.sin(angle)).float()
 
 
-def _head_rows(t: torch.Tensor, what: str) -> torch.Tensor:
-    """(tokens, heads, D) bf16 as rows of heads the kernels take: D contiguous, strides multiples of 8
-    elements, a 16-byte aligned address."""
-    if t.dtype is not torch.bfloat16 or t.dim() != 3:
+def _head_rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
+    """(tokens, heads, D) bf16 as rows of heads the kernels take (D contiguous, strides multiples of 8
+    elements, a 16-byte aligned address), with the strides of tokens and heads."""
+    if t.dtype is not _BF16 or t.dim() != 3:
         raise RuntimeError(f"{what} must be a bf16 (tokens, heads, D) tensor, got {tuple(t.shape)} {t.dtype}")
-    strides = t.stride()
-    if strides[2] != 1 or strides[0] % 8 or strides[1] % 8:
-        t = t.contiguous()
-    return t.clone(memory_format=torch.contiguous_format) if t.data_ptr() % 16 else t
+    st, sh, sd = t.stride()
+    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+        t = t.clone(memory_format=torch.contiguous_format)
+        st, sh, _ = t.stride()
+    return t, st, sh
 
 
 def _rope_tables(cos: torch.Tensor, sin: torch.Tensor) -> int:
@@ -694,25 +706,26 @@ def rope(
     by the angle whose cosine and sine are in row `positions[t]`, column i of cos and sin (`rope_table`,
     fp32, (rows, R / 2)); the dims from R on are copied. Computed in fp32, rounded once. A position outside
     the tables gives NaN. D and R are multiples of 16. Tokens and heads may be strided."""
-    dev = _on_gpu(q, cos, sin, positions) if k is None else _on_gpu(q, k, cos, sin, positions)
+    dev = _one_gpu(q, cos, sin, positions) if k is None else _one_gpu(q, k, cos, sin, positions)
     rotary = _rope_tables(cos, sin)
-    q2 = _head_rows(q, "q")
+    q2, qt, qh = _head_rows(q, "q")
     tokens, h, d = q2.shape
     _check_rotary(rotary, d)
-    if positions.dtype is not torch.int32 or positions.shape != (tokens,):
+    if positions.dtype is not _I32 or positions.shape != (tokens,):
         raise RuntimeError(f"positions must be int32 ({tokens},)")
-    at = positions.contiguous()
-    q_out = torch.empty((tokens, h, d), dtype=torch.bfloat16, device=dev)
-    k2 = k_out = None
+    at = positions if positions.is_contiguous() else positions.contiguous()
+    q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
+    k2, kt, kh, n_kv, k_out = None, 0, 0, 0, None
     if k is not None:
-        k2 = _head_rows(k, "k")
-        _require(k2.shape[0] == tokens and k2.shape[2] == d, "q and k must have the same tokens and D")
-        k_out = torch.empty(k2.shape, dtype=torch.bfloat16, device=dev)
-    k_args = (k2.data_ptr(), *k2.stride()[:2]) if k2 is not None else (None, 0, 0)
-    _launch(
-        dev, "lse_rope", q2.data_ptr(), *q2.stride()[:2], *k_args, cos.data_ptr(), sin.data_ptr(), cos.shape[0],
-        at.data_ptr(), q_out.data_ptr(), k_out.data_ptr() if k_out is not None else None, tokens, h,
-        k2.shape[1] if k2 is not None else 0, d, rotary, int(interleaved))
+        k2, kt, kh = _head_rows(k, "k")
+        n_kv = k2.shape[1]
+        if k2.shape[0] != tokens or k2.shape[2] != d:
+            raise RuntimeError("q and k must have the same tokens and D")
+        k_out = torch.empty_like(k2, memory_format=torch.contiguous_format)
+    _launch(dev, "lse_rope", _lib.ROPE_ARGS.pack(
+        q2.data_ptr(), qt, qh, k2.data_ptr() if n_kv else 0, kt, kh, cos.data_ptr(), sin.data_ptr(),
+        cos.shape[0], at.data_ptr(), q_out.data_ptr(), k_out.data_ptr() if n_kv else 0, tokens, h, n_kv, d,
+        rotary, int(interleaved)))
     return q_out, k_out
 
 
@@ -762,40 +775,39 @@ def unpack_fp8_kv(pool: Fp8KV) -> tuple[torch.Tensor, torch.Tensor]:
 def _check_fp8_pool(pool: Fp8KV) -> tuple[int, int, int, int, int, int]:
     """(blocks, H_KV, S, D, bytes from a block to the next in k and v, and in scales) of a pool."""
     k, v, s = pool
-    if k.dtype is not torch.float8_e4m3fn or v.dtype is not k.dtype or k.dim() != 4 or v.shape != k.shape:
+    if k.dtype is not _F8 or v.dtype is not _F8 or k.dim() != 4 or v.shape != k.shape:
         raise RuntimeError("pool codes must be two float8_e4m3fn (blocks, H_KV, S, 16 D) tensors")
     blocks, n_kv, per, size = k.shape
-    if s.dtype is not torch.float8_e8m0fnu or s.shape != (blocks, n_kv, per, 2):
+    if s.dtype is not _E8 or s.shape != (blocks, n_kv, per, 2):
         raise RuntimeError(f"pool scales must be float8_e8m0fnu ({blocks}, {n_kv}, {per}, 2)")
     if size not in (64 * KV_GROUP, 128 * KV_GROUP) or per < 1 or n_kv < 1:
         raise RuntimeError(f"pool groups of {size} bytes: D must be 64 or 128")
-    if blocks < 2:
-        stride, s_stride = n_kv * per * size, 2 * n_kv * per
-    else:
-        stride, s_stride = k.stride(0), s.stride(0)
-        if v.stride(0) != stride:
-            raise RuntimeError("a pool's k and v must have their blocks equally far apart")
-    if not (k[:1].is_contiguous() and v[:1].is_contiguous() and s[:1].is_contiguous()):
-        raise RuntimeError("a pool's blocks must be contiguous")
+    stride, s_stride = n_kv * per * size, 2 * n_kv * per
+    if not (k.is_contiguous() and v.is_contiguous() and s.is_contiguous()):
+        if blocks > 1:
+            stride, s_stride = k.stride(0), s.stride(0)
+            if v.stride(0) != stride:
+                raise RuntimeError("a pool's k and v must have their blocks equally far apart")
+        if not (k[:1].is_contiguous() and v[:1].is_contiguous() and s[:1].is_contiguous()):
+            raise RuntimeError("a pool's blocks must be contiguous")
     return blocks, n_kv, per, size // KV_GROUP, stride, s_stride
 
 
-def _check_plan(table: torch.Tensor, entry: dict[str, torch.Tensor]) -> int:
-    """The entries of a batch plan: block_table (entries, blocks) and int32 (entries,) tensors."""
-    for name, t in (("block_table", table), *entry.items()):
-        if t.dtype is not torch.int32:
-            raise RuntimeError(f"{name} must be int32, got {t.dtype}")
-    if table.dim() != 2 or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise RuntimeError("block_table must be (E, B) with unit column stride")
-    entries = table.shape[0]
-    for name, t in entry.items():
-        if t.shape != (entries,) or (entries > 1 and t.stride(0) != 1):
-            raise RuntimeError(f"{name} must be a contiguous ({entries},) tensor")
-    return entries
-
-
-def _table_stride(table: torch.Tensor) -> int:
-    return table.stride(0) if table.shape[0] > 1 else table.shape[1]
+def _check_plan(table: torch.Tensor, *entry: torch.Tensor) -> tuple[int, int, int]:
+    """(entries, blocks, row stride) of a batch plan's block_table (entries, blocks); the others are int32
+    (entries,) tensors."""
+    if table.dtype is not _I32 or table.dim() != 2:
+        raise RuntimeError(f"block_table must be an int32 (E, B) tensor, got {tuple(table.shape)} {table.dtype}")
+    entries, width = table.shape
+    stride, column = table.stride()
+    if column != 1 and width > 1:
+        raise RuntimeError("block_table must have unit column stride")
+    want = (entries,)
+    for t in entry:
+        if t.dtype is not _I32 or t.shape != want or not t.is_contiguous():
+            raise RuntimeError(f"context_len, query_offset, q_start and q_len must be contiguous int32 "
+                               f"({entries},) tensors")
+    return entries, width, stride if entries > 1 else width
 
 
 def append_kv_fp8(
@@ -813,37 +825,35 @@ def append_kv_fp8(
     before are requantised when its scale grows, and slots behind the last new one are zeroed. Infinities
     and NaN are held as NaN. Positions outside the table, blocks outside the pool and rows outside q, k
     and v are dropped. Returns the rotated q (tokens, H, D), of which rows of no entry are not written."""
-    entry = dict(query_offset=query_offset, q_start=q_start, q_len=q_len)
-    dev = _on_gpu(k, v, *pool, block_table, *entry.values(),
-                  *(t for t in (q, cos, sin) if t is not None))
+    dev = _one_gpu(k, v, *pool, block_table, query_offset, q_start, q_len)
     blocks, n_kv, per, d, stride, s_stride = _check_fp8_pool(pool)
-    entries = _check_plan(block_table, entry)
-    k2, v2 = _head_rows(k, "k"), _head_rows(v, "v")
+    entries, width, t_stride = _check_plan(block_table, query_offset, q_start, q_len)
+    k2, kt, kh = _head_rows(k, "k")
+    v2, vt, vh = _head_rows(v, "v")
     tokens = k2.shape[0]
-    if k2.shape[1:] != (n_kv, d) or v2.shape != k2.shape:
+    if k2.shape != (tokens, n_kv, d) or v2.shape != (tokens, n_kv, d):
         raise RuntimeError(f"k and v must be (tokens, {n_kv}, {d}) for this pool")
     if (cos is None) != (sin is None):
         raise RuntimeError("cos and sin go together")
-    rotary = 0
+    rotary = rows = cos_at = sin_at = 0
     if cos is not None:
-        rotary = _rope_tables(cos, sin)
+        _one_gpu(k, cos, sin)
+        rotary, rows, cos_at, sin_at = _rope_tables(cos, sin), cos.shape[0], cos.data_ptr(), sin.data_ptr()
         _check_rotary(rotary, d)
-    q_args, h, q_out = (None, 0, 0), n_kv, None
+    h, q_at, qt, qh, q_out, out_at = n_kv, 0, 0, 0, None, 0
     if q is not None:
-        q2 = _head_rows(q, "q")
+        _one_gpu(k, q)
+        q2, qt, qh = _head_rows(q, "q")
         h = q2.shape[1]
-        if q2.shape[0] != tokens or q2.shape[2] != d or h % n_kv or h == 0:
+        if q2.shape != (tokens, h, d) or h % n_kv or h == 0:
             raise RuntimeError(f"q must be ({tokens}, H, {d}), H a multiple of {n_kv}")
-        q_args = (q2.data_ptr(), *q2.stride()[:2])
-        q_out = torch.empty((tokens, h, d), dtype=torch.bfloat16, device=dev)
-    _launch(
-        dev, "lse_append_kv_fp8", *q_args, k2.data_ptr(), *k2.stride()[:2], v2.data_ptr(), *v2.stride()[:2],
-        cos.data_ptr() if rotary else None, sin.data_ptr() if rotary else None,
-        cos.shape[0] if rotary else 0, q_out.data_ptr() if q_out is not None else None,
-        pool.k.data_ptr(), pool.v.data_ptr(), stride, pool.scales.data_ptr(), s_stride,
-        blocks, KV_GROUP * per, block_table.data_ptr(), _table_stride(block_table),
-        block_table.shape[1], query_offset.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), entries,
-        tokens, max_q_len, h, n_kv, d, rotary, int(interleaved))
+        q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
+        q_at, out_at = q2.data_ptr(), q_out.data_ptr()
+    _launch(dev, "lse_append_kv_fp8", _lib.APPEND_KV_FP8_ARGS.pack(
+        q_at, qt, qh, k2.data_ptr(), kt, kh, v2.data_ptr(), vt, vh, cos_at, sin_at, rows, out_at,
+        pool.k.data_ptr(), pool.v.data_ptr(), stride, pool.scales.data_ptr(), s_stride, blocks,
+        KV_GROUP * per, block_table.data_ptr(), t_stride, width, query_offset.data_ptr(), q_start.data_ptr(),
+        q_len.data_ptr(), entries, tokens, max_q_len, h, n_kv, d, rotary, int(interleaved)))
     return q_out
 
 
@@ -858,29 +868,30 @@ def paged_attention_fp8(
     max_blocks), context_len, query_offset, q_start, q_len (entries,): int32 on the device; entries own
     distinct rows of q; max_q_len >= every q_len. Returns o like q; rows of no entry are not written. Softmax
     scale 1/sqrt(D)."""
-    entry = dict(context_len=context_len, query_offset=query_offset, q_start=q_start, q_len=q_len)
-    dev = _on_gpu(q, *pool, block_table, *entry.values())
+    dev = _one_gpu(q, *pool, block_table, context_len, query_offset, q_start, q_len)
     blocks, n_kv, per, d, stride, s_stride = _check_fp8_pool(pool)
-    entries = _check_plan(block_table, entry)
-    if q.dim() != 3 or q.dtype is not torch.bfloat16 or q.shape[2] != d or q.stride(2) != 1:
+    entries, width, t_stride = _check_plan(block_table, context_len, query_offset, q_start, q_len)
+    if q.dim() != 3 or q.dtype is not _BF16:
         raise RuntimeError(f"q must be bf16 (H, tokens, {d}) with a contiguous head dim")
-    h, tokens, _ = q.shape
+    h, tokens, dq = q.shape
+    sh, st, sd = q.stride()
+    if dq != d or sd != 1:
+        raise RuntimeError(f"q must be bf16 (H, tokens, {d}) with a contiguous head dim")
     if h == 0 or h % n_kv or h // n_kv > 16:
         raise RuntimeError(f"unsupported attention shape: H={h} H_KV={n_kv} D={d}")
     o = torch.empty_like(q)
-    lib = _lib.library()
-    width, size = block_table.shape[1], KV_GROUP * per
-    nbytes = lib.lse_paged_attention_fp8_workspace_bytes(entries, tokens, h, n_kv, d, max_q_len, width,
-                                                         size)
+    oh, ot, _ = o.stride()
+    args = _lib.PAGED_ATTENTION_FP8_ARGS.pack(
+        q.data_ptr(), sh, st, pool.k.data_ptr(), pool.v.data_ptr(), stride, pool.scales.data_ptr(), s_stride,
+        blocks, KV_GROUP * per, block_table.data_ptr(), t_stride, width, context_len.data_ptr(),
+        query_offset.data_ptr(), q_start.data_ptr(), q_len.data_ptr(), o.data_ptr(), oh, ot, entries, tokens,
+        max_q_len, h, n_kv, d, d ** -0.5)
+    nbytes = (_lib._lib or _lib.library()).lse_paged_attention_fp8_workspace_bytes(args)
     if nbytes < 0:
-        raise RuntimeError(f"unsupported attention sizes: max_q_len={max_q_len}, {width} blocks of {size}")
+        raise RuntimeError(f"unsupported attention sizes: max_q_len={max_q_len}, {width} blocks of "
+                           f"{KV_GROUP * per}")
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _launch(
-        dev, "lse_paged_attention_fp8", q.data_ptr(), q.stride(0), q.stride(1), pool.k.data_ptr(), pool.v.data_ptr(), stride,
-        pool.scales.data_ptr(), s_stride, blocks, size, block_table.data_ptr(),
-        _table_stride(block_table), width, context_len.data_ptr(), query_offset.data_ptr(),
-        q_start.data_ptr(), q_len.data_ptr(), o.data_ptr(), o.stride(0), o.stride(1), entries, tokens,
-        max_q_len, h, n_kv, d, 1.0 / d ** 0.5, *_ws_args(ws))
+    _launch(dev, "lse_paged_attention_fp8", args, *_ws_args(ws))
     return o
 
 

@@ -3,7 +3,8 @@ call is made."""
 
 from __future__ import annotations
 
-import ctypes
+import re
+from pathlib import Path
 
 import pytest
 import torch
@@ -20,12 +21,52 @@ APPEND = dict(q=FAKE, q_t=512, q_h=64, k=FAKE, k_t=128, k_h=64, v=FAKE, v_t=128,
 ATTEND = dict(q=FAKE, q_h=256, q_t=64, k_pool=FAKE, v_pool=FAKE, stride=2048, scales=FAKE, s_stride=4,
               blocks=10, block_size=16, table=FAKE, t_stride=5, max_blocks=5, ctx=FAKE, offset=FAKE, start=FAKE,
               length=FAKE, o=FAKE, o_h=256, o_t=64, entries=3, tokens=4, most=2, h=8, h_kv=2, d=64,
-              scale=ctypes.c_float(0.125), ws=None, ws_bytes=0)
+              scale=0.125)
+
+
+def _pack(pkg, layout, base, changes):
+    """The packed argument struct: null pointers are 0."""
+    assert set(changes) <= set(base)
+    return layout.pack(*(0 if v is None else v for v in {**base, **changes}.values()))
 
 
 def _call(pkg, name, base, changes):
-    assert set(changes) <= set(base)
-    return getattr(pkg.library(), name)(*{**base, **changes}.values(), None)
+    from llm_serving_engine_amd import _lib
+
+    layout = dict(lse_rope=_lib.ROPE_ARGS, lse_append_kv_fp8=_lib.APPEND_KV_FP8_ARGS)[name]
+    return getattr(pkg.library(), name)(_pack(pkg, layout, base, changes), None)
+
+
+def _attend(pkg, changes, ws=None, ws_bytes=0):
+    from llm_serving_engine_amd import _lib
+
+    args = _pack(pkg, _lib.PAGED_ATTENTION_FP8_ARGS, ATTEND, changes)
+    return pkg.library().lse_paged_attention_fp8(args, ws, ws_bytes, None)
+
+
+def test_the_structs_are_the_headers(pkg):
+    """As many fields as the header's structs have, each of eight bytes."""
+    from llm_serving_engine_amd import _lib
+
+    text = (Path(__file__).resolve().parent.parent / "include" / "lse_int8.h").read_text()
+    for name, layout, base in (("lse_rope_args", _lib.ROPE_ARGS, ROPE),
+                               ("lse_append_kv_fp8_args", _lib.APPEND_KV_FP8_ARGS, APPEND),
+                               ("lse_paged_attention_fp8_args", _lib.PAGED_ATTENTION_FP8_ARGS, ATTEND)):
+        body = re.search(r"struct " + name + r" \{(.*?)\};", text, re.S).group(1)
+        fields = 0
+        for line in body.split(";"):
+            line = line.strip()
+            if line:
+                assert re.match(r"(const )?(void|float|int32_t)( ?\*)|int64_t |double ", line), line
+                fields += line.count(",") + 1
+        assert layout.size == 8 * fields == 8 * len(base)
+
+
+def test_no_arguments_at_all(pkg):
+    lib = pkg.library()
+    assert lib.lse_rope(None, None) == lib.lse_append_kv_fp8(None, None) == E_NULL
+    assert lib.lse_paged_attention_fp8(None, None, 0, None) == E_NULL
+    assert lib.lse_paged_attention_fp8_workspace_bytes(None) == -1
 
 
 @pytest.mark.parametrize("changes,status", [
@@ -61,22 +102,37 @@ def test_append_refusals(pkg, changes, status):
     (dict(k_pool=FAKE + 8), E_ALIGN), (dict(stride=2056), E_ALIGN), (dict(s_stride=5), E_ALIGN),
     (dict(scales=FAKE + 1), E_ALIGN), (dict(table=FAKE + 2), E_ALIGN),
     (dict(blocks=1 << 26), E_RANGE),  # a pool of 2^37 bytes a side
-    (dict(max_blocks=1 << 28, t_stride=1 << 28), E_RANGE), (dict(ws_bytes=-1), E_WORKSPACE),
+    (dict(max_blocks=1 << 28, t_stride=1 << 28), E_RANGE),
     (dict(max_blocks=500, t_stride=500), E_WORKSPACE),  # splits, and has no workspace
     (dict(entries=0), 0), (dict(tokens=0), 0), (dict(most=0), 0)])
 def test_attention_refusals(pkg, changes, status):
-    assert _call(pkg, "lse_paged_attention_fp8", ATTEND, changes) == status
+    assert _attend(pkg, changes) == status
+
+
+def test_workspace_refusals(pkg):
+    assert _attend(pkg, {}, None, -1) == E_WORKSPACE
+    assert _attend(pkg, {}, FAKE + 8, 1 << 20) == E_WORKSPACE
+    split = dict(max_blocks=500, t_stride=500)
+    need = _size(pkg, **split)
+    assert need > 0
+    assert _attend(pkg, split, FAKE, need - 1) == _attend(pkg, split, None, need) == E_WORKSPACE
+
+
+def _size(pkg, **changes):
+    from llm_serving_engine_amd import _lib
+
+    return pkg.library().lse_paged_attention_fp8_workspace_bytes(
+        _pack(pkg, _lib.PAGED_ATTENTION_FP8_ARGS, ATTEND, changes))
 
 
 def test_workspace_sizes(pkg):
-    size = pkg.library().lse_paged_attention_fp8_workspace_bytes
-    assert size(3, 4, 8, 2, 96, 2, 5, 16) == -1 and size(-1, 4, 8, 2, 64, 2, 5, 16) == -1
-    assert size(0, 4, 8, 2, 64, 2, 5, 16) == 0
-    assert size(3, 4, 8, 2, 64, 2, 64, 16) == 0  # one round of chunks
-    two = size(3, 4, 8, 2, 64, 2, 65, 16)
+    assert _size(pkg, d=96) == _size(pkg, entries=-1) == -1
+    assert _size(pkg, entries=0) == 0
+    assert _size(pkg, max_blocks=64) == 0  # one round of chunks
+    two = _size(pkg, max_blocks=65)
     assert two == 2 * 4 * 3 * 8 * 2 * (64 + 2) * 4
-    assert size(3, 4, 8, 2, 64, 2, 1 << 20, 16) == 16 * two  # at most 32 chunks a wave
-    assert size(4096, 4096, 32, 8, 128, 1, 4096, 16) == 0  # enough entries to fill any card
+    assert _size(pkg, max_blocks=1 << 20) == 16 * two  # at most 32 chunks a wave
+    assert _size(pkg, entries=4096, tokens=4096, h=32, h_kv=8, d=128, most=1, max_blocks=4096) == 0
 
 
 def test_tensors_are_checked(pkg):
@@ -107,7 +163,8 @@ def test_tensors_are_checked(pkg):
     assert ops._check_fp8_pool(ops.Fp8KV(*(t[3:] for t in wide))) == (1, 2, 2, 64, 4096, 8)
     for t, e in ((table.long(), i), (table[0], i), (table, torch.zeros(2, dtype=torch.int32)), (table, i.float())):
         with pytest.raises(RuntimeError):
-            ops._check_plan(t, dict(q_len=e))
+            ops._check_plan(t, e)
+    assert ops._check_plan(table, i, i) == (1, 4, 4)
     for cos, sin in ((torch.zeros(4, 32), torch.zeros(4, 31)), (torch.zeros(4, 32).double(), torch.zeros(4, 32)),
                      (torch.zeros(32, 4).t(), torch.zeros(32, 4).t())):
         with pytest.raises(RuntimeError):

@@ -104,8 +104,12 @@ def test_flat_and_peaked_scores(pkg, dev, q_scale):
     check_attention(pkg, dev, case, f"q x {q_scale}")
 
 
-def _bits(pkg, dev, case, rows, most=None):
-    return attend(pkg, dev, case, most)[:, rows]
+def _workspace(pkg, entries, tokens, h, h_kv, d, most, width, block_size):
+    from llm_serving_engine_amd import _lib
+
+    args = [0] * 26
+    args[9], args[12], args[20:26] = block_size, width, (entries, tokens, most, h, h_kv, d)
+    return pkg.library().lse_paged_attention_fp8_workspace_bytes(_lib.PAGED_ATTENTION_FP8_ARGS.pack(*args, 1.0))
 
 
 def test_a_rows_bits_depend_on_its_entry_alone(pkg, dev):
@@ -115,10 +119,9 @@ def test_a_rows_bits_depend_on_its_entry_alone(pkg, dev):
     ctxs = [2100, 1, 513, 300, 1030] + [int(c) for c in rng.integers(1, 400, 70)]
     case = attention_case(34, [(1, c - 1, c) for c in ctxs])
     everything = check_attention(pkg, dev, case)
-    lib = pkg.library()
-    size = lambda e, w: lib.lse_paged_attention_fp8_workspace_bytes(e, e, 32, 8, 128, 1, w, 16)  # noqa: E731
     width = case["table"].shape[1]
-    assert size(5, width) > 0 and size(75, width) == 0
+    size = lambda e: _workspace(pkg, e, e, 32, 8, 128, 1, width, 16)  # noqa: E731
+    assert size(5) > 0 and size(75) == 0
     few = dict(case, q=case["q"][:, :5], **{n: case[n][:5] for n in ("table", "ctx", "qo", "qs", "ql")})
     np.testing.assert_array_equal(attend(pkg, dev, few), everything[:, :5])
     wide = np.full((16, case["blocks"]), case["blocks"] - 1, np.int32)
@@ -139,8 +142,7 @@ def test_long_contexts(pkg, dev, ctx):
     n = 520  # entries that fill the CUs, all but two of them empty
     pad = dict(case, **{k: np.concatenate([case[k], np.zeros(n, np.int32)]) for k in ("ctx", "qo", "qs", "ql")})
     pad["table"] = np.concatenate([case["table"], np.zeros((n, case["table"].shape[1]), np.int32)])
-    lib = pkg.library()
-    assert lib.lse_paged_attention_fp8_workspace_bytes(2, 3, 3, 1, 64, 2, case["table"].shape[1], 64) > 0
+    assert _workspace(pkg, 2, 3, 3, 1, 64, 2, case["table"].shape[1], 64) > 0
     # The bound on items by rows keeps few tokens split however many entries there are.
     pad["q"] = np.concatenate([case["q"], np.repeat(case["q"][:, :1], 3000, 1)], 1)
     np.testing.assert_array_equal(attend(pkg, dev, pad)[:, :3], split)
@@ -159,16 +161,18 @@ def test_rows_of_no_entry_are_left_alone(pkg, dev):
     qd = to_bf16_tensor(q, dev)
     o = torch.full((8, 20, 128), 7.0, dtype=torch.bfloat16, device=dev)
     table, ctx, qo, _, ql = attend_args(case, dev)
-    lib = pkg.library()
-    nbytes = lib.lse_paged_attention_fp8_workspace_bytes(3, 20, 8, 2, 128, 3, table.shape[1], 16)
+    nbytes = _workspace(pkg, 3, 20, 8, 2, 128, 3, table.shape[1], 16)
     ws = torch.full((max(nbytes, 16),), 0xff, dtype=torch.uint8, device=dev)  # NaN in what nobody writes
     start = i32(qs, dev)
-    status = lib.lse_paged_attention_fp8(
+    from llm_serving_engine_amd import _lib
+
+    args = _lib.PAGED_ATTENTION_FP8_ARGS.pack(
         qd.data_ptr(), qd.stride(0), qd.stride(1), pool.k.data_ptr(), pool.v.data_ptr(), pool.k.stride(0),
         pool.scales.data_ptr(), pool.scales.stride(0), case["blocks"], 16, table.data_ptr(), table.stride(0),
         table.shape[1], ctx.data_ptr(), qo.data_ptr(), start.data_ptr(), ql.data_ptr(), o.data_ptr(),
-        o.stride(0), o.stride(1), 3, 20, 3, 8, 2, 128, 1.0 / 128 ** 0.5, ws.data_ptr(), nbytes,
-        torch.cuda.current_stream().cuda_stream)
+        o.stride(0), o.stride(1), 3, 20, 3, 8, 2, 128, 128 ** -0.5)
+    status = pkg.library().lse_paged_attention_fp8(args, ws.data_ptr(), nbytes,
+                                                   torch.cuda.current_stream().cuda_stream)
     torch.cuda.synchronize()
     assert status == 0
     np.testing.assert_array_equal(bf16_bits(o[:, at]), want)
