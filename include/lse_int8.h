@@ -445,8 +445,10 @@ struct lse_append_kv_fp8_args {
 int lse_append_kv_fp8(const struct lse_append_kv_fp8_args* args, void* stream);
 
 /*
- * lse_paged_attention over the 8-bit cache: the same plan, semantics and determinism, k and v being the
- * values code x scale. q and o have `tokens` rows; entries own distinct ones, and rows of no entry are not
+ * lse_paged_attention over the 8-bit cache: the same plan and semantics, k and v being the values code x scale.
+ * Equal calls give equal bits. A row's do not depend on padding entries (q_len 0), the order of the entries, the
+ * table's width or, below 256 query rows per K/V head, max_q_len; in a call of so few entries that their keys
+ * are split over workgroups as well they depend on the lengths of the other entries. q and o have `tokens` rows; entries own distinct ones, and rows of no entry are not
  * written. A block outside the pool makes the rows that see it NaN; a context longer than the table is cut.
  * D = 64 or 128; 1 <= H / H_KV <= 16; block_size % 16 == 0; the strides of q and o multiples of 8, q, o and
  * the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes (it reads the

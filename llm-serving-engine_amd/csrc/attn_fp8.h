@@ -20,15 +20,14 @@ struct Fp8AttnArgs {
   int entries, H, HKV, G, tokens;
   int max_ctx;       // positions that the table has room for
   int max_q_len;
-  int ws_q;          // rows of an entry in the split launch's workspace
   int tiled;         // the row-tiled kernel runs too and takes the long entries (f8_is_long)
   int tq;            // query tokens per tile: floor(16 / G)
-  int parts;         // 1: a workgroup takes every chunk of its item; > 1: one chunk of each of its waves
+  int slots;         // units of a split launch (f8_unit); 0: keys are not split
   int sorted;        // entries are taken in descending order of context length...
   int first_round;   // ...and, where > 0, those from this rank on in ascending order
   float scale_log2;  // softmax scale x log2(e)
-  float* ws_o;       // parts > 1: chunk states' O [parts x 4][entries][H][ws_q][D], fp32
-  float* ws_ml;      // parts > 1: chunk states' max and sum [parts x 4][entries][H][ws_q][2]
+  float* ws_o;       // split launch: the units' O [slots][HKV][16 rows][D], fp32
+  float* ws_ml;      // split launch: their max and sum [slots][HKV][16 rows][2]
 };
 
 // Whether the row-tiled kernel takes an entry of q_len tokens; the key-streaming kernel takes it otherwise.

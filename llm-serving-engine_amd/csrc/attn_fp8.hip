@@ -15,11 +15,11 @@
 // the lane's row of Q again, so the softmax's factors are per-lane scalars. Codes become bf16 in registers,
 // times their scale, at two values an instruction.
 //
-// Order of summation. Wave w of the four takes chunks w, w + 4, ... of L keys, each with an online-softmax state
-// of its own, folded into the wave's in chunk order; the four waves' are merged in wave order at the end. L is
-// 256, twice that for every doubling of the entry's context past 32768 (so at most 32 chunks a wave). In a split
-// launch every workgroup takes one chunk per wave and a second kernel does the same folds in the same order,
-// so a row's bits depend on its own entry only, not on the batch, the table's width or the launch.
+// Wave w of the four takes the tiles of 64 keys w, w + 4, w + 8, ... with an online-softmax state of its own; the four
+// are merged in wave order at the end. Where a call has fewer (entry, K/V head, query tile) items than the card
+// takes workgroups, the keys are split too (f8_units): into ranges of one length for all entries, chosen so
+// that all ranges run at once, each leaving its state to a second kernel. With ranges of a fixed 1024 or 2048
+// keys, four sequences behind 7500 to 60000 positions took 44 + 7 us.
 #include <algorithm>
 
 #include "attn_fp8.h"
@@ -28,51 +28,34 @@ namespace lse {
 
 constexpr int kF8Waves = 4;
 constexpr int kF8Keys = 64;      // keys of a wave's tile: one group per 16 lanes
-constexpr int kF8Window = 256;   // keys whose blocks and scales a wave holds: one group per lane of 16
-constexpr int kF8MaxParts = 32;  // chunks of a wave
+constexpr int kF8Round = kF8Keys * kF8Waves;
+constexpr int kF8Window = 4 * kF8Round;  // keys of four tiles of every wave, whose blocks and scales it holds
+constexpr int kF8Groups = 512;   // workgroups of a split launch: two per CU
+// Fewest keys of a range, and contexts up to which nothing is split: a wave takes 0.5 us a tile, the second
+// kernel 4 us and more.
+constexpr int kF8MinRange = 1024, kF8MinSplit = 2048;
 constexpr float kNegInf = -__builtin_huge_valf();
-
-// log2 of a chunk's windows, for an entry of `ctx` positions.
-__host__ __device__ inline int f8_chunk_shift(int ctx) {
-  int k = 0;
-  while (((int64_t)kF8Window * kF8Waves * kF8MaxParts << k) < ctx) ++k;
-  return k;
-}
-
-// Folds the next chunk's state (max m in the base-2 domain, sum l, unnormalised O) into the state before it;
-// from (-inf, 0, 0) the first fold gives the chunk's state exactly.
-struct FoldFactors {
-  float a, b;
-};
-__device__ __forceinline__ FoldFactors f8_fold_ml(float& M, float& L, float m, float l) {
-  const float mn = fmaxf(M, m), ref = mn == kNegInf ? 0.0f : mn;
-  const FoldFactors f{exp2_fast(M - ref), exp2_fast(m - ref)};
-  L = __builtin_fmaf(l, f.b, L * f.a);
-  M = mn;
-  return f;
-}
-__device__ __forceinline__ float f8_fold(float O, float o, FoldFactors f) {
-  return __builtin_fmaf(o, f.b, O * f.a);
-}
 
 // The four waves' states of a row merged in wave order.
 struct WaveFactors {
-  float f[kF8Waves], inv;
+  float f[kF8Waves], m, sum;
 };
 __device__ __forceinline__ WaveFactors f8_merge_factors(const float (&m)[kF8Waves],
                                                         const float (&l)[kF8Waves]) {
-  float top = kNegInf, sum = 0.0f;
-#pragma unroll
-  for (int w = 0; w < kF8Waves; ++w) top = fmaxf(top, m[w]);
-  const float ref = top == kNegInf ? 0.0f : top;
   WaveFactors r;
+  r.m = kNegInf, r.sum = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kF8Waves; ++w) r.m = fmaxf(r.m, m[w]);
+  const float ref = r.m == kNegInf ? 0.0f : r.m;
 #pragma unroll
   for (int w = 0; w < kF8Waves; ++w) {
     r.f[w] = exp2_fast(m[w] - ref);
-    sum = __builtin_fmaf(l[w], r.f[w], sum);
+    r.sum = __builtin_fmaf(l[w], r.f[w], r.sum);
   }
-  r.inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that saw no key gives zeros
   return r;
+}
+__device__ __forceinline__ float f8_inverse(float sum) {
+  return sum == 0.0f ? 0.0f : 1.0f / sum;  // a row that saw no key gives zeros
 }
 
 // The entry of rank `slot` by context length, longest first (attention.hip's attn_sorted_entry has the
@@ -89,9 +72,79 @@ __device__ __forceinline__ int f8_sorted_entry(const Fp8AttnArgs& a, int slot) {
   return __ffsll(__ballot(rank == slot && lane < a.entries)) - 1;
 }
 
-// ONE: every entry has at most one tile (decode); the grid is K/V heads, entries, parts. Otherwise items are
-// counted entry by entry over their tiles and parts, without empty slots.
-template <int D, bool ONE>
+// The units of a launch that counts them: entry by entry, its query tiles times its key ranges (the tiles that
+// read a range together).
+struct F8Unit {
+  int e, qt, part, parts, tiles, first;  // first: number of the entry's first unit; e < 0: no such unit
+  int64_t range;                         // keys of a range
+};
+struct F8Work {
+  int tiles, end;
+};
+__device__ __forceinline__ F8Work f8_entry_work(const Fp8AttnArgs& a, int i) {
+  if (i >= a.entries) return {0, 0};
+  const int qlen = min(a.q_len[i], a.max_q_len);
+  if (qlen <= 0 || (a.tiled && f8_is_long(qlen, a.G))) return {0, 0};
+  return {(qlen + a.tq - 1) / a.tq, f8_end(a, a.query_offset[i], a.context_len[i], qlen)};
+}
+__device__ __forceinline__ int f8_wave_total(int v) { return __builtin_amdgcn_readlane(kv_wave_scan(v), 63); }
+
+// Unit b, or (of_entry) the units of entry b. Every wave counts for itself, 64 entries at a time.
+__device__ __forceinline__ F8Unit f8_unit(const Fp8AttnArgs& a, int b, bool of_entry) {
+  const int lane = threadIdx.x & 63;
+  const F8Work w0 = f8_entry_work(a, lane);
+  int64_t range = (int64_t)1 << 40;
+  if (a.slots > 0) {
+    // With ranges of W / (slots - T) keys, T tiles of W keys in all (each counted as often as it has tiles) make up
+    // at most slots units.
+    int T = 0, W = 0;
+    for (int e0 = 0; e0 < a.entries; e0 += 64) {
+      const F8Work w = e0 ? f8_entry_work(a, e0 + lane) : w0;
+      T += f8_wave_total(min(w.tiles, kF8Groups));
+      W += f8_wave_total(min(w.tiles, kF8Groups) * min((w.end + kF8Round - 1) / kF8Round, 1 << 15));
+      if (T >= a.slots) break;
+    }
+    if (T < a.slots)
+      range = max((int64_t)kF8Round * ((W + a.slots - T - 1) / (a.slots - T)), (int64_t)kF8MinRange);
+    // So long a context that its length above was cut, or so many units: no more ranges than slots.
+    while (T < a.slots) {
+      int n = 0;
+      for (int e0 = 0; e0 < a.entries; e0 += 64) {
+        const F8Work w = e0 ? f8_entry_work(a, e0 + lane) : w0;
+        n += f8_wave_total(w.tiles * max((int)min((w.end + range - 1) / range, (int64_t)kF8Groups), 1));
+      }
+      if (n <= a.slots) break;
+      range *= 2;
+    }
+  }
+  int before0 = 0;
+  for (int e0 = 0; e0 < a.entries; e0 += 64) {
+    const F8Work w = e0 ? f8_entry_work(a, e0 + lane) : w0;
+    const int parts = max((int)((w.end + range - 1) / range), 1);
+    const int units = w.tiles * parts, before = before0 + kv_wave_scan(units) - units;
+    const unsigned long long hit = __ballot(of_entry ? e0 + lane == b && units > 0
+                                                     : (unsigned)(b - before) < (unsigned)units);
+    if (hit) {
+      const int at = __ffsll(hit) - 1;
+      F8Unit u;
+      u.e = e0 + at;
+      u.first = __builtin_amdgcn_readlane(before, at);
+      u.tiles = __builtin_amdgcn_readlane(w.tiles, at);
+      u.parts = __builtin_amdgcn_readlane(parts, at);
+      u.range = range;
+      const int i = of_entry ? 0 : b - u.first;
+      u.qt = i % u.tiles;
+      u.part = i / u.tiles;
+      return u;
+    }
+    before0 = __builtin_amdgcn_readlane(before + units, 63);
+  }
+  return {-1, 0, 0, 1, 0, 0, range};
+}
+
+// NT: K and V stream with the nt cache policy, where each is read by one workgroup only (one query tile: decode).
+// COUNT: workgroups find their unit (f8_unit); otherwise the grid is K/V heads, then entries of one tile.
+template <int D, bool NT, bool COUNT>
 __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs a) {
   constexpr int J = D / 64, DT = D / 16;  // 64-dim runs of a key; 16-dim tiles of O
   constexpr int OROW = D + 4;             // floats of a row of O in LDS: rows start on other banks
@@ -102,56 +155,25 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int n16 = lane & 15, g = lane >> 4;
 
-  int b = blockIdx.x, e, qt = 0, part = 0;
-  const int kvh = b % a.HKV;
-  b /= a.HKV;
-  if constexpr (ONE) {
-    e = b % a.entries;
-    part = b / a.entries;
-    if (a.sorted) e = f8_sorted_entry(a, e);
+  const int kvh = blockIdx.x % a.HKV, slot = blockIdx.x / a.HKV;
+  int e, qt = 0, parts = 1;
+  int64_t first_key = 0, end_key = (int64_t)1 << 40;
+  if constexpr (COUNT) {
+    const F8Unit u = f8_unit(a, slot, false);
+    if (u.e < 0) return;
+    e = u.e, qt = u.qt, parts = u.parts;
+    first_key = u.part * u.range, end_key = first_key + u.range;
   } else {
-    e = -1;
-    int chunk_parts = 1;
-    for (int e0 = 0; e0 < a.entries; e0 += 64) {
-      const int i = e0 + lane;
-      int tiles = 0, parts = 1;
-      if (i < a.entries) {
-        const int qlen = min(a.q_len[i], a.max_q_len);
-        tiles = qlen > 0 && !(a.tiled && f8_is_long(qlen, a.G)) ? (qlen + a.tq - 1) / a.tq : 0;
-        if (a.parts > 1) {
-          const int ctx = a.context_len[i];
-          const int64_t span = (int64_t)(kF8Window * kF8Waves) << f8_chunk_shift(ctx);
-          const int end = f8_end(a, a.query_offset[i], ctx, qlen);
-          parts = min(max((int)((end + span - 1) / span), 1), a.parts);
-        }
-      }
-      const int items = tiles * parts, before = kv_wave_scan(items) - items;
-      const unsigned long long hit = __ballot((unsigned)(b - before) < (unsigned)items);
-      if (hit) {
-        const int at = __ffsll(hit) - 1;
-        e = e0 + at;
-        b -= __builtin_amdgcn_readlane(before, at);
-        chunk_parts = __builtin_amdgcn_readlane(tiles, at);
-        break;
-      }
-      b -= __builtin_amdgcn_readlane(before + items, 63);
-    }
-    if (e < 0) return;
-    qt = b % chunk_parts;  // the tiles that read a chunk together
-    part = b / chunk_parts;
+    e = a.sorted ? f8_sorted_entry(a, slot) : slot;
   }
   const int qlen = min(a.q_len[e], a.max_q_len);
   if (qt * a.tq >= qlen) return;
   const int ctx = a.context_len[e], qo = a.query_offset[e], qs = a.q_start[e];
-  const int end_n = f8_end(a, qo, ctx, min(qlen, (qt + 1) * a.tq));
-  const int shift = f8_chunk_shift(ctx);
-  // The wave's windows: j-th has keys [win(j), win(j) + 256); from j0 on, one chunk's in a split launch.
-  auto win = [&](int j) -> int64_t {
-    return ((((int64_t)(j >> shift) * kF8Waves + wave) << shift) + (j & ((1 << shift) - 1))) * kF8Window;
-  };
-  const int j0 = a.parts > 1 ? part << shift : 0;
-  const int j_end = a.parts > 1 ? (part + 1) << shift : 0x7fffffff;
-  if (a.parts > 1 && part > 0 && ((int64_t)part * kF8Waves << shift) * kF8Window >= end_n) return;
+  int end_n = f8_end(a, qo, ctx, min(qlen, (qt + 1) * a.tq));
+  if (first_key > 0 && first_key >= end_n) return;  // the tile has no keys in this range
+  end_n = (int)min((int64_t)end_n, end_key);
+  // The wave's windows: tile t of the j-th has keys 1024 j + 256 t + 64 wave on, from the range's first.
+  auto win = [&](int j) -> int64_t { return first_key + (int64_t)j * kF8Window + kF8Keys * wave; };
 
   // This lane's row: token tq, head gq of the group; rows from tq G on are idle (G not dividing 16).
   const int G = a.G;
@@ -174,13 +196,13 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
       }
   }
 
-  // Blocks and scales of the wave's windows: lane i of 16 holds those of group i. `off` is the group's place
-  // in the pool in 16-byte units; a block that is not the pool's reads block 0 with NaN for a scale.
+  // Blocks and scales of the wave's windows: lane i of 16 holds those of group i % 4 of its tile i / 4. `off` is the
+  // group's place in the pool in 16-byte units; a block that is not the pool's reads block 0 with NaN for a scale.
   const int32_t* bt = a.block_table + (int64_t)e * a.sbt;
   const int last_group = (end_n - 1) / kKvGroup;
   const int per = a.pool.per;
   auto table_at = [&](int j, int& sub) {
-    const int64_t first = win(j) / kKvGroup + n16;
+    const int64_t first = (win(j) + kF8Round * (n16 >> 2)) / kKvGroup + (n16 & 3);
     const int grp = (int)min(first, (int64_t)last_group);
     const int bi = per == 1 ? grp : grp / per;
     sub = grp - bi * per;
@@ -203,7 +225,7 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         const uint8_t* src = p + (bk * J + j) * 256;
-        kr[bk][j] = ONE ? load16_stream(src) : *reinterpret_cast<const uint4*>(src);
+        kr[bk][j] = NT ? load16_stream(src) : *reinterpret_cast<const uint4*>(src);
       }
   };
   auto load_v = [&](uint32_t off, int t) {
@@ -212,33 +234,33 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
 #pragma unroll
     for (int i = 0; i < DT; ++i) {
       const uint8_t* src = p + i * 256;
-      vr[i] = ONE ? load16_stream(src) : *reinterpret_cast<const uint4*>(src);
+      vr[i] = NT ? load16_stream(src) : *reinterpret_cast<const uint4*>(src);
     }
   };
 
-  float M = kNegInf, L = 0.0f, m_run = kNegInf, l_run = 0.0f;
-  f32x4 oacc[DT], ofold[DT];
+  float m_run = kNegInf, l_run = 0.0f;
+  f32x4 oacc[DT];
 #pragma unroll
-  for (int t = 0; t < DT; ++t) oacc[t] = ofold[t] = f32x4{0, 0, 0, 0};
+  for (int t = 0; t < DT; ++t) oacc[t] = f32x4{0, 0, 0, 0};
 
-  if (win(j0) < end_n) {
+  if (win(0) < end_n) {
     // Window j's off and scales, window j + 1's off (and its scales on their way), window j + 2's block.
     int sub0, sub1, sub2, bad0, bad1;
     uint32_t off0, off1;
-    const int blk0 = table_at(j0, sub0), blk1 = table_at(j0 + 1, sub1);
-    int blk2 = table_at(j0 + 2, sub2);
+    const int blk0 = table_at(0, sub0), blk1 = table_at(1, sub1);
+    int blk2 = table_at(2, sub2);
     int sc0 = place(blk0, sub0, off0, bad0);
     load_k(off0, 0);
     load_v(off0, 0);
     int sc1 = place(blk1, sub1, off1, bad1);
     if (bad0) sc0 = 0xffff;
 
-    for (int j = j0;; ) {
+    for (int j = 0;;) {
       const int64_t start = win(j);
-      const int tiles = (int)min((int64_t)4, (end_n - start + kF8Keys - 1) / kF8Keys);
-      const bool more = j + 1 < j_end && win(j + 1) < end_n;
+      const int tiles = (int)min((int64_t)4, (end_n - start + kF8Round - 1) / kF8Round);
+      const bool more = win(j + 1) < end_n;
       for (int t = 0; t < tiles; ++t) {
-        const int n0 = (int)start + kF8Keys * t;
+        const int n0 = (int)start + kF8Round * t;
         const bool last = t + 1 == tiles;
         // The scores of key n0 + 16 g + 4 bk + r and row n16.
         const float ks = kv_scale(__shfl(sc0, 4 * t + (n16 >> 2)) & 255);
@@ -282,7 +304,7 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
           sum += p;
           if (i < 8) p0[i] = p; else p1[i - 8] = p;
         }
-        l_run = __builtin_fmaf(l_run, alpha, sum);  // this lane's keys; its row's others' at the chunk's end
+        l_run = __builtin_fmaf(l_run, alpha, sum);  // this lane's keys; its row's others' at the end
         if (__ballot(m_new != m_run)) {
 #pragma unroll
           for (int d = 0; d < DT; ++d) oacc[d] *= alpha;
@@ -308,19 +330,6 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
         }
         load_v(next_off, next_t);
       }
-      // The end of a chunk: its state into the wave's.
-      if (!more || ((j + 1) >> shift) != (j >> shift)) {
-        l_run += __shfl_xor(l_run, 16);
-        l_run += __shfl_xor(l_run, 32);
-        const FoldFactors f = f8_fold_ml(M, L, m_run, l_run);
-#pragma unroll
-        for (int d = 0; d < DT; ++d) {
-#pragma unroll
-          for (int r = 0; r < 4; ++r) ofold[d][r] = f8_fold(ofold[d][r], oacc[d][r], f);
-          oacc[d] = f32x4{0, 0, 0, 0};
-        }
-        m_run = kNegInf, l_run = 0.0f;
-      }
       if (!more) break;
       ++j;
       off0 = off1, sc0 = bad1 ? 0xffff : sc1;
@@ -330,24 +339,13 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
   }
 
   // Lane (n16, g) holds row n16's dims 16 t + 4 g + r.
-  if (a.parts > 1) {
-    if (row_ok && (((int64_t)part * kF8Waves + wave) << shift) * kF8Window < end_n) {
-      const int64_t slot =
-          (((int64_t)(part * kF8Waves + wave) * a.entries + e) * a.H + head) * a.ws_q + m_row;
-      float* dst = a.ws_o + slot * D + 4 * g;
-#pragma unroll
-      for (int t = 0; t < DT; ++t)
-        *reinterpret_cast<float4*>(dst + 16 * t) =
-            make_float4(ofold[t][0], ofold[t][1], ofold[t][2], ofold[t][3]);
-      if (g == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * slot) = make_float2(M, L);
-    }
-    return;
-  }
-  if (g == 0) mbuf[wave][n16] = M, lbuf[wave][n16] = L;
+  l_run += __shfl_xor(l_run, 16);
+  l_run += __shfl_xor(l_run, 32);
+  if (g == 0) mbuf[wave][n16] = m_run, lbuf[wave][n16] = l_run;
 #pragma unroll
   for (int t = 0; t < DT; ++t)
     *reinterpret_cast<float4*>(&obuf[wave][n16 * OROW + 16 * t + 4 * g]) =
-        make_float4(ofold[t][0], ofold[t][1], ofold[t][2], ofold[t][3]);
+        make_float4(oacc[t][0], oacc[t][1], oacc[t][2], oacc[t][3]);
   __syncthreads();
   if (threadIdx.x >= 16 * (D / 8)) return;
   const int orow = threadIdx.x / (D / 8), c8 = 8 * (threadIdx.x % (D / 8));
@@ -362,72 +360,92 @@ __global__ void __launch_bounds__(64 * kF8Waves, 2) attn_fp8_kernel(Fp8AttnArgs 
   for (int w = 0; w < kF8Waves; ++w)
 #pragma unroll
     for (int i = 0; i < 8; ++i) o[i] = __builtin_fmaf(obuf[w][orow * OROW + c8 + i], f.f[w], o[i]);
+  if (COUNT && parts > 1) {
+    const int64_t at = ((int64_t)slot * a.HKV + kvh) * 16 + orow;
+    *reinterpret_cast<float4*>(a.ws_o + at * D + c8) = make_float4(o[0], o[1], o[2], o[3]);
+    *reinterpret_cast<float4*>(a.ws_o + at * D + c8 + 4) = make_float4(o[4], o[5], o[6], o[7]);
+    if (c8 == 0) *reinterpret_cast<float2*>(a.ws_ml + 2 * at) = make_float2(f.m, f.sum);
+    return;
+  }
+  const float inv = f8_inverse(f.sum);
   *reinterpret_cast<uint4*>(a.o + (int64_t)(kvh * G + orow - otok * G) * a.so_h + out_row * a.so_t + c8) =
-      make_uint4(pack_bf16x2(o[0] * f.inv, o[1] * f.inv), pack_bf16x2(o[2] * f.inv, o[3] * f.inv),
-                 pack_bf16x2(o[4] * f.inv, o[5] * f.inv), pack_bf16x2(o[6] * f.inv, o[7] * f.inv));
+      make_uint4(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv),
+                 pack_bf16x2(o[4] * inv, o[5] * inv), pack_bf16x2(o[6] * inv, o[7] * inv));
 }
 
-// Second pass of a split launch: a workgroup takes 64 (entry, head, query row, 8 dims) pieces; wave w folds the
-// chunk states of the first pass's waves w in order, then the four are merged as in the single pass.
+// Second pass of a split launch, a workgroup per query tile, K/V head and 64 (row, 4 dims) pieces: wave w adds up the
+// states of ranges w, w + 4, ..., then the four are merged. Bound by latency: a thread's loads, eight ranges at
+// a time, do not wait for each other.
 template <int D>
 __global__ void __launch_bounds__(64 * kF8Waves) attn_fp8_merge(Fp8AttnArgs a) {
-  constexpr int C = D / 8;
-  __shared__ float obuf[kF8Waves][64][9];
+  __shared__ float obuf[kF8Waves][64][5];
   __shared__ float mbuf[kF8Waves][64], lbuf[kF8Waves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t t = (int64_t)blockIdx.x * 64 + lane;
-  const int64_t rows = (int64_t)a.entries * a.H * a.ws_q;
-  const int c8 = 8 * (int)(t % C);
-  const int64_t r = t / C;
-  const int m_row = (int)(r % a.ws_q), h = (int)(r / a.ws_q % a.H);
-  const int e = (int)min(r / a.ws_q / a.H, (int64_t)a.entries - 1);
-  const int qlen = min(a.q_len[e], a.max_q_len);
-  const int64_t row = (int64_t)a.q_start[e] + m_row;
-  const bool ok = r < rows && m_row < qlen && !(a.tiled && f8_is_long(qlen, a.G)) && row >= 0 && row < a.tokens;
-  float M = kNegInf, L = 0.0f, O[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const int kvh = blockIdx.x % a.HKV;
+  int e = blockIdx.x / a.HKV;
+  const int qt = blockIdx.z;
+  const F8Unit u = f8_unit(a, e, true);
+  if (u.e < 0 || u.parts <= 1 || qt >= u.tiles) return;
+  const int qlen = min(a.q_len[e], a.max_q_len), G = a.G;
+  const int piece = blockIdx.y * 64 + lane, orow = piece / (D / 4), c4 = 4 * (piece % (D / 4));
+  const int otok = orow / G, om = qt * a.tq + otok;
+  const int64_t row = (int64_t)a.q_start[e] + om;
+  const bool ok = orow < a.tq * G && om < qlen && row >= 0 && row < a.tokens;
+  const int end_n = f8_end(a, a.query_offset[e], a.context_len[e], min(qlen, (qt + 1) * a.tq));
+  const int n = max((int)((end_n + u.range - 1) / u.range), 1);  // ranges with keys of this tile
+  float M = kNegInf, L = 0.0f, O[4] = {0, 0, 0, 0};
   if (ok) {
-    const int ctx = a.context_len[e];
-    const int end_n = f8_end(a, a.query_offset[e], ctx, min(qlen, (m_row / a.tq + 1) * a.tq));
-    const int64_t chunk = (int64_t)kF8Window << f8_chunk_shift(ctx);
-    const int chunks = (int)((end_n + chunk - 1) / chunk);
-    const int mine = chunks > wave ? (chunks - wave + kF8Waves - 1) / kF8Waves : 0;
-#pragma unroll 4
-    for (int p = 0; p < mine; ++p) {
-      const int64_t slot = (int64_t)(p * kF8Waves + wave) * rows + r;
-      const float2 ml = *reinterpret_cast<const float2*>(a.ws_ml + 2 * slot);
-      const float4 x = *reinterpret_cast<const float4*>(a.ws_o + slot * D + c8);
-      const float4 y = *reinterpret_cast<const float4*>(a.ws_o + slot * D + c8 + 4);
-      const FoldFactors f = f8_fold_ml(M, L, ml.x, ml.y);
-      const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+    for (int p0 = wave; p0 < n; p0 += 8 * kF8Waves) {
+      float2 ml[8];
+      float4 v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) O[i] = f8_fold(O[i], v[i], f);
+      for (int i = 0; i < 8; ++i) {  // past the last range the first one again, without weight
+        const int p = p0 + kF8Waves * i < n ? p0 + kF8Waves * i : p0;
+        const int64_t at = ((int64_t)(u.first + p * u.tiles + qt) * a.HKV + kvh) * 16 + orow;
+        ml[i] = *reinterpret_cast<const float2*>(a.ws_ml + 2 * at);
+        v[i] = *reinterpret_cast<const float4*>(a.ws_o + at * D + c4);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const bool real = p0 + kF8Waves * i < n;
+        const float m = real ? ml[i].x : kNegInf, mn = fmaxf(M, m), ref = mn == kNegInf ? 0.0f : mn;
+        const float fa = exp2_fast(M - ref), fb = exp2_fast(m - ref);
+        L = __builtin_fmaf(real ? ml[i].y : 0.0f, fb, L * fa);
+        O[0] = __builtin_fmaf(real ? v[i].x : 0.0f, fb, O[0] * fa);
+        O[1] = __builtin_fmaf(real ? v[i].y : 0.0f, fb, O[1] * fa);
+        O[2] = __builtin_fmaf(real ? v[i].z : 0.0f, fb, O[2] * fa);
+        O[3] = __builtin_fmaf(real ? v[i].w : 0.0f, fb, O[3] * fa);
+        M = mn;
+      }
     }
   }
   mbuf[wave][lane] = M, lbuf[wave][lane] = L;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) obuf[wave][lane][i] = O[i];
+  for (int i = 0; i < 4; ++i) obuf[wave][lane][i] = O[i];
   __syncthreads();
   if (wave != 0 || !ok) return;
-  float m[kF8Waves], l[kF8Waves], o[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  float m[kF8Waves], l[kF8Waves], o[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int w = 0; w < kF8Waves; ++w) m[w] = mbuf[w][lane], l[w] = lbuf[w][lane];
   const WaveFactors f = f8_merge_factors(m, l);
+  const float inv = f8_inverse(f.sum);
 #pragma unroll
   for (int w = 0; w < kF8Waves; ++w)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) o[i] = __builtin_fmaf(obuf[w][lane][i], f.f[w], o[i]);
-  *reinterpret_cast<uint4*>(a.o + (int64_t)h * a.so_h + row * a.so_t + c8) =
-      make_uint4(pack_bf16x2(o[0] * f.inv, o[1] * f.inv), pack_bf16x2(o[2] * f.inv, o[3] * f.inv),
-                 pack_bf16x2(o[4] * f.inv, o[5] * f.inv), pack_bf16x2(o[6] * f.inv, o[7] * f.inv));
+    for (int i = 0; i < 4; ++i) o[i] = __builtin_fmaf(obuf[w][lane][i], f.f[w], o[i]);
+  *reinterpret_cast<uint2*>(a.o + (int64_t)(kvh * G + orow - otok * G) * a.so_h + row * a.so_t + c4) =
+      make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
 
 // ---- host side -----------------------------------------------------------------------------
 
 struct Fp8AttnPlan {
-  int tq, parts;
+  int tq;
   bool tiled;       // some entry may be the row-tiled kernel's
   int64_t short_q;  // the most tokens of an entry that is not
-  int64_t tiles;  // at most, over all entries
+  int64_t tiles;    // query tiles of all entries, at most
+  int slots;        // units of a split launch, 0: keys are not split
   int64_t ws_o_bytes, ws_bytes;
 };
 
@@ -441,40 +459,44 @@ static int fp8_attn_cus() {
   return cus;
 }
 
-// One workgroup per (entry, K/V head, query tile) once those fill the CUs twice over; otherwise, where the
-// table has room for more than one round of chunks, one per round, and a second pass. The choice changes no
-// result.
+// One workgroup per (entry, K/V head, query tile) once those fill the card; otherwise, where contexts may be long
+// enough, the keys are split as well.
 static Fp8AttnPlan fp8_attn_plan(int64_t entries, int64_t tokens, int64_t H, int64_t HKV, int64_t D,
-                                 int64_t max_q_len, int64_t max_ctx, int cus) {
+                                 int64_t max_q_len, int64_t max_ctx) {
   Fp8AttnPlan pl{};
-  pl.tq = (int)(16 / (H / HKV));
   const int64_t G = H / HKV;
+  pl.tq = (int)(16 / G);
   pl.tiled = f8_is_long(max_q_len, (int)G);
   pl.short_q = pl.tiled ? (kF8LongRows - 1) / G : max_q_len;
   pl.tiles = std::min(entries * ceil_div(pl.short_q, (int64_t)pl.tq), tokens / pl.tq + entries);
-  const int64_t rounds = std::min<int64_t>(ceil_div(max_ctx, (int64_t)kF8Window * kF8Waves), kF8MaxParts);
-  pl.parts = pl.tiles * HKV < 2 * (int64_t)cus && rounds > 1 ? (int)rounds : 1;
-  if (pl.parts > 1) {
-    const int64_t slots = (int64_t)pl.parts * kF8Waves * entries * H * pl.short_q;
-    pl.ws_o_bytes = slots * D * 4;
-    pl.ws_bytes = pl.ws_o_bytes + slots * 2 * 4;
+  const int64_t slots = kF8Groups / HKV;
+  if (pl.tiles < slots && max_ctx > kF8MinSplit) {
+    pl.slots = (int)slots;
+    pl.ws_o_bytes = slots * HKV * 16 * D * 4;
+    pl.ws_bytes = pl.ws_o_bytes + slots * HKV * 16 * 2 * 4;
   }
   return pl;
 }
 
 template <int D>
-static int launch_fp8_attention(const Fp8AttnArgs& a, int64_t blocks, hipStream_t stream) {
+static int launch_fp8_attention(const Fp8AttnArgs& a, const Fp8AttnPlan& pl, hipStream_t stream) {
   const dim3 wg(64 * kF8Waves);
   if (a.tiled)
     if (int st = launch_fp8_attn_tile(a, D, stream)) return st;
-  if (a.ws_q <= a.tq)
-    hipLaunchKernelGGL((attn_fp8_kernel<D, true>), dim3((unsigned)blocks), wg, 0, stream, a);
+  const bool one = pl.short_q <= pl.tq;
+  const dim3 grid((unsigned)((pl.slots ? pl.slots : one ? a.entries : pl.tiles) * a.HKV));
+  if (!one)
+    hipLaunchKernelGGL((attn_fp8_kernel<D, false, true>), grid, wg, 0, stream, a);
+  else if (pl.slots)
+    hipLaunchKernelGGL((attn_fp8_kernel<D, true, true>), grid, wg, 0, stream, a);
   else
-    hipLaunchKernelGGL((attn_fp8_kernel<D, false>), dim3((unsigned)blocks), wg, 0, stream, a);
+    hipLaunchKernelGGL((attn_fp8_kernel<D, true, false>), grid, wg, 0, stream, a);
   if (int st = launch_status()) return st;
-  if (a.parts > 1) {
-    const int64_t pieces = (int64_t)a.entries * a.H * a.ws_q * (D / 8);
-    hipLaunchKernelGGL(attn_fp8_merge<D>, dim3((unsigned)ceil_div(pieces, 64)), wg, 0, stream, a);
+  if (pl.slots) {
+    const int64_t rows = std::min<int64_t>(pl.short_q, pl.tq) * a.G;
+    const dim3 pieces((unsigned)(a.entries * a.HKV), (unsigned)ceil_div(rows * (D / 4), 64),
+                      (unsigned)ceil_div(pl.short_q, (int64_t)pl.tq));
+    hipLaunchKernelGGL(attn_fp8_merge<D>, pieces, wg, 0, stream, a);
   }
   return launch_status();
 }
@@ -496,9 +518,8 @@ int check_sizes(const Args& x) {
   return x.block_size > kMax31 || x.max_blocks > kMax31 / x.block_size ? LSE_E_RANGE : LSE_OK;
 }
 
-lse::Fp8AttnPlan plan_of(const Args& x, int cus) {
-  return lse::fp8_attn_plan(x.entries, x.tokens, x.H, x.H_KV, x.D, x.max_q_len, x.max_blocks * x.block_size,
-                            cus);
+lse::Fp8AttnPlan plan_of(const Args& x) {
+  return lse::fp8_attn_plan(x.entries, x.tokens, x.H, x.H_KV, x.D, x.max_q_len, x.max_blocks * x.block_size);
 }
 
 }  // namespace
@@ -508,7 +529,7 @@ extern "C" {
 int64_t lse_paged_attention_fp8_workspace_bytes(const struct lse_paged_attention_fp8_args* args) {
   if (!args || check_sizes(*args)) return -1;
   if (args->entries == 0 || args->tokens == 0 || args->max_q_len == 0) return 0;
-  return plan_of(*args, lse::fp8_attn_cus()).ws_bytes;
+  return plan_of(*args).ws_bytes;
 }
 
 int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, void* workspace,
@@ -539,7 +560,7 @@ int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, voi
     return LSE_E_ALIGN;
   if (workspace_bytes < 0 || (workspace && !aligned(workspace, 16))) return LSE_E_WORKSPACE;
   const int cus = lse::fp8_attn_cus();
-  const lse::Fp8AttnPlan pl = plan_of(x, cus);
+  const lse::Fp8AttnPlan pl = plan_of(x);
   if (pl.ws_bytes > 0 && (workspace_bytes < pl.ws_bytes || !workspace)) return LSE_E_WORKSPACE;
   lse::Fp8AttnArgs a{};
   a.q = (const uint16_t*)x.q, a.sq_h = x.q_stride_h, a.sq_t = x.q_stride_t;
@@ -551,18 +572,16 @@ int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, voi
   a.entries = (int)x.entries, a.H = (int)x.H, a.HKV = (int)x.H_KV, a.G = (int)(x.H / x.H_KV);
   a.tokens = (int)x.tokens;
   a.max_ctx = (int)(x.max_blocks * x.block_size);
-  a.max_q_len = (int)x.max_q_len, a.ws_q = (int)pl.short_q, a.tiled = pl.tiled;
-  a.tq = pl.tq, a.parts = pl.parts;
+  a.max_q_len = (int)x.max_q_len, a.tiled = pl.tiled, a.tq = pl.tq, a.slots = pl.slots;
   a.scale_log2 = (float)x.softmax_scale * 1.4426950408889634f;
-  a.ws_o = pl.parts > 1 ? (float*)workspace : nullptr;
-  a.ws_ml = pl.parts > 1 ? (float*)((char*)workspace + pl.ws_o_bytes) : nullptr;
+  a.ws_o = pl.slots ? (float*)workspace : nullptr;
+  a.ws_ml = pl.slots ? (float*)((char*)workspace + pl.ws_o_bytes) : nullptr;
   const int64_t items = x.entries * x.H_KV;
-  a.sorted = a.parts == 1 && x.entries <= 64 && items > cus && a.max_ctx > 256;
+  a.sorted = x.entries <= 64 && items > cus && a.max_ctx > 256;
   a.first_round = items > cus && items <= 2 * (int64_t)cus && cus % a.HKV == 0 ? cus / a.HKV : 0;
-  const int64_t blocks = (pl.short_q <= pl.tq ? x.entries : pl.tiles) * x.H_KV * pl.parts;
-  if (blocks > kMax31 || x.entries * x.H * pl.short_q * (x.D / 8) / 64 > kMax31) return LSE_E_RANGE;
-  return x.D == 64 ? lse::launch_fp8_attention<64>(a, blocks, (hipStream_t)stream)
-                   : lse::launch_fp8_attention<128>(a, blocks, (hipStream_t)stream);
+  if (std::max(x.entries, pl.tiles) * x.H_KV > kMax31) return LSE_E_RANGE;
+  return x.D == 64 ? lse::launch_fp8_attention<64>(a, pl, (hipStream_t)stream)
+                   : lse::launch_fp8_attention<128>(a, pl, (hipStream_t)stream);
 }
 
 }  // extern "C"

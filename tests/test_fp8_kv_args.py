@@ -128,10 +128,9 @@ def _size(pkg, **changes):
 def test_workspace_sizes(pkg):
     assert _size(pkg, d=96) == _size(pkg, entries=-1) == -1
     assert _size(pkg, entries=0) == 0
-    assert _size(pkg, max_blocks=64) == 0  # one round of chunks
-    two = _size(pkg, max_blocks=65)
-    assert two == 2 * 4 * 3 * 8 * 2 * (64 + 2) * 4
-    assert _size(pkg, max_blocks=1 << 20) == 16 * two  # at most 32 chunks a wave
+    assert _size(pkg, max_blocks=128) == 0  # contexts too short to split
+    split = _size(pkg, max_blocks=129)
+    assert split == 512 * 16 * (64 + 2) * 4 == _size(pkg, max_blocks=1 << 20)
     assert _size(pkg, entries=4096, tokens=4096, h=32, h_kv=8, d=128, most=1, max_blocks=4096) == 0
 
 

@@ -112,40 +112,65 @@ def _workspace(pkg, entries, tokens, h, h_kv, d, most, width, block_size):
     return pkg.library().lse_paged_attention_fp8_workspace_bytes(_lib.PAGED_ATTENTION_FP8_ARGS.pack(*args, 1.0))
 
 
-def test_a_rows_bits_depend_on_its_entry_alone(pkg, dev):
-    """Alone (a split launch), among 70 others (an unsplit one), in a padded bucket under a table as wide as
-    the pool, in another order: the same bits."""
+def test_what_a_rows_bits_depend_on(pkg, dev):
+    """A batch whose keys are split (few entries) and one whose are not: the same bits in a padded bucket
+    under a table as wide as the pool, with a larger max_q_len, in another order; unsplit also among other
+    entries."""
     rng = np.random.default_rng(34)
     ctxs = [2100, 1, 513, 300, 1030] + [int(c) for c in rng.integers(1, 400, 70)]
     case = attention_case(34, [(1, c - 1, c) for c in ctxs])
-    everything = check_attention(pkg, dev, case)
     width = case["table"].shape[1]
     size = lambda e: _workspace(pkg, e, e, 32, 8, 128, 1, width, 16)  # noqa: E731
     assert size(5) > 0 and size(75) == 0
-    few = dict(case, q=case["q"][:, :5], **{n: case[n][:5] for n in ("table", "ctx", "qo", "qs", "ql")})
-    np.testing.assert_array_equal(attend(pkg, dev, few), everything[:, :5])
-    wide = np.full((16, case["blocks"]), case["blocks"] - 1, np.int32)
-    wide[:5, :width] = case["table"][:5]
-    pad = dict(few, table=wide, **{n: np.concatenate([few[n], np.zeros(11, np.int32)])
-                                   for n in ("ctx", "qo", "qs", "ql")})
-    np.testing.assert_array_equal(attend(pkg, dev, pad), everything[:, :5])
-    np.testing.assert_array_equal(attend(pkg, dev, pad, most=9), everything[:, :5])
-    back = dict(case, q=case["q"][:, ::-1].copy(), **{n: case[n][::-1].copy() for n in ("table", "ctx", "qo", "ql")})
-    np.testing.assert_array_equal(attend(pkg, dev, back), everything[:, ::-1])
+    fields = ("table", "ctx", "qo", "qs", "ql")
+    few = dict(case, q=case["q"][:, :5], **{n: case[n][:5] for n in fields})
+    for c, entries, bucket in ((few, 5, 16), (case, 75, 96)):
+        want = check_attention(pkg, dev, c, f"{entries} entries")
+        wide = np.full((bucket, case["blocks"]), case["blocks"] - 1, np.int32)
+        wide[:entries, :width] = c["table"]
+        pad = dict(c, table=wide, **{n: np.concatenate([c[n], np.zeros(bucket - entries, np.int32)])
+                                     for n in fields[1:]})
+        np.testing.assert_array_equal(attend(pkg, dev, pad), want)
+        np.testing.assert_array_equal(attend(pkg, dev, pad, most=9), want)
+        back = dict(c, q=c["q"][:, ::-1].copy(), **{n: c[n][::-1].copy() for n in ("table", "ctx", "qo", "ql")})
+        np.testing.assert_array_equal(attend(pkg, dev, back), want[:, ::-1])
+    some = dict(case, q=case["q"][:, :68], **{n: case[n][:68] for n in fields})
+    np.testing.assert_array_equal(attend(pkg, dev, some), want[:, :68])
 
 
-@pytest.mark.parametrize("ctx", [32768, 32769, 70000])
+@pytest.mark.parametrize("ctx", [2049, 32768, 32769, 70000])
 def test_long_contexts(pkg, dev, ctx):
-    """Around the length from which chunks grow, split and unsplit (the same bits), beside a short one."""
+    """Split and unsplit, beside a short entry."""
     case = attention_case(ctx, [(1, ctx - 1, ctx), (2, 98, 100)], h=3, h_kv=1, d=64, block_size=64)
-    split = check_attention(pkg, dev, case, f"ctx {ctx}")
-    n = 520  # entries that fill the CUs, all but two of them empty
+    assert _workspace(pkg, 2, 3, 3, 1, 64, 2, case["table"].shape[1], 64) > 0
+    check_attention(pkg, dev, case, f"ctx {ctx} split")
+    n = 520  # entries that fill the card, all but two of them empty
     pad = dict(case, **{k: np.concatenate([case[k], np.zeros(n, np.int32)]) for k in ("ctx", "qo", "qs", "ql")})
     pad["table"] = np.concatenate([case["table"], np.zeros((n, case["table"].shape[1]), np.int32)])
-    assert _workspace(pkg, 2, 3, 3, 1, 64, 2, case["table"].shape[1], 64) > 0
-    # The bound on items by rows keeps few tokens split however many entries there are.
-    pad["q"] = np.concatenate([case["q"], np.repeat(case["q"][:, :1], 3000, 1)], 1)
-    np.testing.assert_array_equal(attend(pkg, dev, pad)[:, :3], split)
+    assert _workspace(pkg, n + 2, 3, 3, 1, 64, 2, case["table"].shape[1], 64) == 0
+    check_attention(pkg, dev, pad, f"ctx {ctx} unsplit")
+
+
+@pytest.mark.parametrize("h_kv", [1, 2, 8])
+def test_split_ranges(pkg, dev, h_kv):
+    """Short chunks and decode rows of very different contexts in one split call, some with no key in later
+    ranges, one without any; ranges and tiles that end together."""
+    entries = [(20, 4076, 4096), (1, 9999, 10000), (3, 0, 3), (1, 1023, 1024), (33, 2100, 2133), (1, 4999, 5000),
+               (5, 3000, 3005)]
+    case = attention_case(50 + h_kv, entries, h=4 * h_kv, h_kv=h_kv, d=64, block_size=32)
+    case["ctx"][6] = 0
+    assert _workspace(pkg, 7, 64, 4 * h_kv, h_kv, 64, 33, case["table"].shape[1], 32) > 0
+    o = check_attention(pkg, dev, case)
+    assert not o[:, 59:64].any()
+    # More entries than one wave looks at in a step, most of them empty.
+    pad = {k: np.zeros((len(entries) + 60, *case[k].shape[1:]), np.int32) for k in ("table", "ctx", "qo", "qs", "ql")}
+    at = np.arange(len(entries)) * 10 + 3
+    for k in pad:
+        pad[k][at] = case[k]
+    if h_kv < 8:
+        np.testing.assert_array_equal(attend(pkg, dev, dict(case, **pad)), o)
+    else:
+        check_attention(pkg, dev, dict(case, **pad))
 
 
 def test_rows_of_no_entry_are_left_alone(pkg, dev):
