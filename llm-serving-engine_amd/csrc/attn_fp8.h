@@ -1,6 +1,5 @@
-// Arguments and host entry points shared by the attention kernels over the 8-bit paged K/V cache
-// (attn_fp8.hip: the key-streaming kernel of decode rows and short chunks, attn_fp8_tile.hip: the row-tiled
-// kernel of prompts and longer chunks).
+// Arguments and helpers shared by the two attention kernels over the 8-bit paged K/V cache (attn_fp8_stream.h: decode
+// rows and short chunks, attn_fp8_tile.h: prompts and longer chunks; attn_fp8.hip launches them).
 #pragma once
 
 #include "attention.h"
@@ -28,6 +27,10 @@ struct Fp8AttnArgs {
   float scale_log2;  // softmax scale x log2(e)
   float* ws_o;       // split launch: the units' O [slots][HKV][16 rows][D], fp32
   float* ws_ml;      // split launch: their max and sum [slots][HKV][16 rows][2]
+  int tile_blocks;   // workgroups of the row-tiled kernel, which come first
+  int tile_parts;    // parts its items may be cut into
+  float* ws_tile_o;  // their O [items][parts][HKV][128 rows][D], fp32
+  float* ws_tile_ml;  // their max and sum [items][parts][HKV][128 rows][2]
 };
 
 // Whether the row-tiled kernel takes an entry of q_len tokens; the key-streaming kernel takes it otherwise.
@@ -39,7 +42,8 @@ __device__ __forceinline__ int f8_end(const Fp8AttnArgs& a, int qo, int ctx, int
   return max(min((int)min((int64_t)qo + tokens, (int64_t)ctx), a.max_ctx), 0);
 }
 
-// Launches the row-tiled kernel over every long entry.
-int launch_fp8_attn_tile(const Fp8AttnArgs& a, int64_t D, hipStream_t stream);
+__device__ __forceinline__ int f8_wave_total(int v) { return __builtin_amdgcn_readlane(kv_wave_scan(v), 63); }
+
+constexpr float kNegInf = -__builtin_huge_valf();
 
 }  // namespace lse

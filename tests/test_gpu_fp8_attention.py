@@ -323,3 +323,69 @@ def test_append_then_attend(pkg, dev):
                 want = kept[e][p].astype(np.float64)
                 assert (np.abs(values[block, p % bs] - want)
                         <= 2.0 ** -4 * np.abs(want) + 2.0 ** -9 * scale).all()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("h,h_kv", [(8, 2), (3, 1), (16, 1), (8, 8)])
+def test_long_entries(pkg, dev, h, h_kv, d):
+    """Entries on both sides of the first row-tiled length and of the next row tile, key tiles one short of and
+    one over, few items (cut into parts), decode rows beside them."""
+    g = h // h_kv
+    first = -(-256 // g)
+    entries = [(first - 1, 5, first + 4), (first, 0, first), (first + 1, 3000, first + 3001),
+               (384 // g, 63, 384 // g + 63), (384 // g + 1, 64, 384 // g + 65), (1, 2600, 2601), (1, 0, 1)]
+    case = attention_case(h + d, entries, h=h, h_kv=h_kv, d=d, block_size=48)
+    check_attention(pkg, dev, case, f"{h} over {h_kv}, D={d}")
+    alone = dict(case, q=case["q"][:, 2 * first - 1:3 * first], qs=np.zeros(1, np.int32),
+                 **{n: case[n][2:3] for n in ("table", "ctx", "qo", "ql")})
+    check_attention(pkg, dev, alone, "alone")
+
+
+@pytest.mark.parametrize("end", [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 385, 1000])
+def test_long_entries_key_edges(pkg, dev, end):
+    """Contexts one short of and one over a key tile; the second entry's rows see less and less, the third's
+    nothing."""
+    case = attention_case(end, [(64, max(end - 64, 0), max(end, 64)), (70, 11, 81), (64, 0, 64)], h=8, h_kv=2, d=64)
+    case["ctx"][:] = [end, min(end, 81), 0]
+    o = check_attention(pkg, dev, case, f"end {end}")
+    assert not o[:, 134:].any()
+
+
+@pytest.mark.parametrize("q_scale", [0.0, 3.0, 2.0 ** 12, 2.0 ** 40, 2.0 ** -40])
+def test_long_entries_flat_and_peaked_scores(pkg, dev, q_scale):
+    case = attention_case(61, [(150, 450, 600), (64, 0, 64)], h=8, h_kv=2, q_scale=q_scale)
+    check_attention(pkg, dev, case, f"q x {q_scale}")
+
+
+def test_long_entries_read_nothing_behind_their_context(pkg, dev):
+    """NaN codes in every slot behind a context, NaN scales in groups behind it, a bad block in one entry."""
+    entries = [(80, 20, 100), (64, 300, 364), (70, 0, 70), (1, 40, 41)]
+    case = attention_case(62, entries, h=8, h_kv=2, d=128, block_size=16)
+    want = attend(pkg, dev, case)
+    k, v, s = (a.copy() for a in case["pool"])
+    used = np.zeros((case["blocks"], 16), bool)
+    for e, (_, _, ctx) in enumerate(entries):
+        for n in range(ctx):
+            used[case["table"][e, n // 16], n % 16] = True
+    dims = np.arange(128)
+    for b, slot in np.argwhere(~used):
+        k[b, :, 0, kv.k_index(slot, dims, 128)] = 127
+        v[b, :, 0, kv.v_index(slot, dims, 128)] = 255
+        if not used[b].any():
+            s[b] = kv.NAN_SCALE
+    case["pool"] = (k, v, s)
+    np.testing.assert_array_equal(attend(pkg, dev, case), want)
+    case["table"] = case["table"].copy()
+    case["table"][1, 3] = case["blocks"] + 5
+    o = ora.bf16_bits_to_f32(attend(pkg, dev, case))
+    assert np.isnan(o[:, 80:144]).all()
+    np.testing.assert_array_equal(ora.f32_to_bf16_bits(o[:, :80]), want[:, :80])
+    np.testing.assert_array_equal(ora.f32_to_bf16_bits(o[:, 144:]), want[:, 144:])
+
+
+def test_many_long_entries(pkg, dev):
+    """More entries than a wave looks at in a step: prompts of 64 to 100 tokens among decode rows."""
+    rng = np.random.default_rng(63)
+    entries = [(int(n), int(o), int(n + o)) for n, o in zip(rng.integers(64, 100, 70), rng.integers(0, 90, 70))]
+    entries = [x for e in entries for x in (e, (1, e[2], e[2] + 1))]
+    check_attention(pkg, dev, attention_case(63, entries, h=4, h_kv=1, d=64), "many")
