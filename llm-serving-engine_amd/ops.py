@@ -672,29 +672,29 @@ def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dic
     return (gain * torch.cos(angle)).float(), (gain * torch.sin(angle)).float()
 
 
-def _head_rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int]:
+def _head_rows(t: torch.Tensor, what: str) -> tuple[torch.Tensor, int, int, int]:
     """(tokens, heads, D) bf16 as rows of heads the kernels take (D contiguous, strides multiples of 8
-    elements, a 16-byte aligned address), with the strides of tokens and heads."""
+    elements, a 16-byte aligned address): owner, address, strides of tokens and heads."""
     if t.dtype is not _BF16 or t.dim() != 3:
         raise RuntimeError(f"{what} must be a bf16 (tokens, heads, D) tensor, got {tuple(t.shape)} {t.dtype}")
     st, sh, sd = t.stride()
-    if sd != 1 or st % 8 or sh % 8 or t.data_ptr() % 16:
+    at = t.data_ptr()
+    if sd != 1 or (st | sh) & 7 or at & 15:
         t = t.clone(memory_format=torch.contiguous_format)
         st, sh, _ = t.stride()
-    return t, st, sh
+        at = t.data_ptr()
+    return t, at, st, sh
 
 
-def _rope_tables(cos: torch.Tensor, sin: torch.Tensor) -> int:
-    """The rotary dims of two tables as `rope_table` makes them."""
+def _rope_tables(cos: torch.Tensor, sin: torch.Tensor, d: int) -> tuple[int, int]:
+    """(rows, rotary dims) of two tables as `rope_table` makes them, for heads of d dims."""
     if (cos.dtype is not torch.float32 or sin.dtype is not torch.float32 or cos.dim() != 2
             or cos.shape != sin.shape or not cos.is_contiguous() or not sin.is_contiguous()):
         raise RuntimeError("cos and sin must be contiguous fp32 (positions, rotary / 2) tensors")
-    return 2 * cos.shape[1]
-
-
-def _check_rotary(rotary: int, d: int) -> None:
-    _require(16 <= rotary <= d and rotary % 16 == 0 and d % 16 == 0,
-             f"rotary dims and D must be multiples of 16, rotary at most D; got {rotary} of {d}")
+    rows, half = cos.shape
+    if half < 8 or half & 7 or 2 * half > d or d & 15:
+        raise RuntimeError(f"rotary dims and D must be multiples of 16, rotary at most D; got {2 * half} of {d}")
+    return rows, 2 * half
 
 
 def rope(
@@ -706,26 +706,26 @@ def rope(
     by the angle whose cosine and sine are in row `positions[t]`, column i of cos and sin (`rope_table`,
     fp32, (rows, R / 2)); the dims from R on are copied. Computed in fp32, rounded once. A position outside
     the tables gives NaN. D and R are multiples of 16. Tokens and heads may be strided."""
-    dev = _one_gpu(q, cos, sin, positions) if k is None else _one_gpu(q, k, cos, sin, positions)
-    rotary = _rope_tables(cos, sin)
-    q2, qt, qh = _head_rows(q, "q")
+    dev = _one_gpu(q, cos, sin, positions)
+    q2, q_at, qt, qh = _head_rows(q, "q")
     tokens, h, d = q2.shape
-    _check_rotary(rotary, d)
+    rows, rotary = _rope_tables(cos, sin, d)
     if positions.dtype is not _I32 or positions.shape != (tokens,):
         raise RuntimeError(f"positions must be int32 ({tokens},)")
     at = positions if positions.is_contiguous() else positions.contiguous()
     q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
-    k2, kt, kh, n_kv, k_out = None, 0, 0, 0, None
+    k_out, k_at, kt, kh, n_kv, k_out_at = None, 0, 0, 0, 0, 0
     if k is not None:
-        k2, kt, kh = _head_rows(k, "k")
-        n_kv = k2.shape[1]
-        if k2.shape[0] != tokens or k2.shape[2] != d:
+        _one_gpu(q, k)
+        k2, k_at, kt, kh = _head_rows(k, "k")
+        k_tokens, n_kv, dk = k2.shape
+        if k_tokens != tokens or dk != d:
             raise RuntimeError("q and k must have the same tokens and D")
         k_out = torch.empty_like(k2, memory_format=torch.contiguous_format)
+        k_out_at = k_out.data_ptr()
     _launch(dev, "lse_rope", _lib.ROPE_ARGS.pack(
-        q2.data_ptr(), qt, qh, k2.data_ptr() if n_kv else 0, kt, kh, cos.data_ptr(), sin.data_ptr(),
-        cos.shape[0], at.data_ptr(), q_out.data_ptr(), k_out.data_ptr() if n_kv else 0, tokens, h, n_kv, d,
-        rotary, int(interleaved)))
+        q_at, qt, qh, k_at, kt, kh, cos.data_ptr(), sin.data_ptr(), rows, at.data_ptr(), q_out.data_ptr(),
+        k_out_at, tokens, h, n_kv, d, rotary, int(interleaved)))
     return q_out, k_out
 
 
@@ -775,12 +775,13 @@ def unpack_fp8_kv(pool: Fp8KV) -> tuple[torch.Tensor, torch.Tensor]:
 def _check_fp8_pool(pool: Fp8KV) -> tuple[int, int, int, int, int, int]:
     """(blocks, H_KV, S, D, bytes from a block to the next in k and v, and in scales) of a pool."""
     k, v, s = pool
-    if k.dtype is not _F8 or v.dtype is not _F8 or k.dim() != 4 or v.shape != k.shape:
+    shape = k.shape
+    if k.dtype is not _F8 or v.dtype is not _F8 or len(shape) != 4 or v.shape != shape:
         raise RuntimeError("pool codes must be two float8_e4m3fn (blocks, H_KV, S, 16 D) tensors")
-    blocks, n_kv, per, size = k.shape
+    blocks, n_kv, per, size = shape
     if s.dtype is not _E8 or s.shape != (blocks, n_kv, per, 2):
         raise RuntimeError(f"pool scales must be float8_e8m0fnu ({blocks}, {n_kv}, {per}, 2)")
-    if size not in (64 * KV_GROUP, 128 * KV_GROUP) or per < 1 or n_kv < 1:
+    if size != 128 * KV_GROUP and size != 64 * KV_GROUP or per < 1 or n_kv < 1:
         raise RuntimeError(f"pool groups of {size} bytes: D must be 64 or 128")
     stride, s_stride = n_kv * per * size, 2 * n_kv * per
     if not (k.is_contiguous() and v.is_contiguous() and s.is_contiguous()):
@@ -802,9 +803,8 @@ def _check_plan(table: torch.Tensor, *entry: torch.Tensor) -> tuple[int, int, in
     stride, column = table.stride()
     if column != 1 and width > 1:
         raise RuntimeError("block_table must have unit column stride")
-    want = (entries,)
     for t in entry:
-        if t.dtype is not _I32 or t.shape != want or not t.is_contiguous():
+        if t.dtype is not _I32 or t.dim() != 1 or t.numel() != entries or not t.is_contiguous():
             raise RuntimeError(f"context_len, query_offset, q_start and q_len must be contiguous int32 "
                                f"({entries},) tensors")
     return entries, width, stride if entries > 1 else width
@@ -828,32 +828,32 @@ def append_kv_fp8(
     dev = _one_gpu(k, v, *pool, block_table, query_offset, q_start, q_len)
     blocks, n_kv, per, d, stride, s_stride = _check_fp8_pool(pool)
     entries, width, t_stride = _check_plan(block_table, query_offset, q_start, q_len)
-    k2, kt, kh = _head_rows(k, "k")
-    v2, vt, vh = _head_rows(v, "v")
-    tokens = k2.shape[0]
-    if k2.shape != (tokens, n_kv, d) or v2.shape != (tokens, n_kv, d):
+    k2, k_at, kt, kh = _head_rows(k, "k")
+    v2, v_at, vt, vh = _head_rows(v, "v")
+    tokens, heads, dk = shape = k2.shape
+    if heads != n_kv or dk != d or v2.shape != shape:
         raise RuntimeError(f"k and v must be (tokens, {n_kv}, {d}) for this pool")
-    if (cos is None) != (sin is None):
-        raise RuntimeError("cos and sin go together")
-    rotary = rows = cos_at = sin_at = 0
-    if cos is not None:
+    rows = rotary = cos_at = sin_at = 0
+    if cos is not None and sin is not None:
         _one_gpu(k, cos, sin)
-        rotary, rows, cos_at, sin_at = _rope_tables(cos, sin), cos.shape[0], cos.data_ptr(), sin.data_ptr()
-        _check_rotary(rotary, d)
+        rows, rotary = _rope_tables(cos, sin, d)
+        cos_at, sin_at = cos.data_ptr(), sin.data_ptr()
+    elif cos is not sin:
+        raise RuntimeError("cos and sin go together")
     h, q_at, qt, qh, q_out, out_at = n_kv, 0, 0, 0, None, 0
     if q is not None:
         _one_gpu(k, q)
-        q2, qt, qh = _head_rows(q, "q")
-        h = q2.shape[1]
-        if q2.shape != (tokens, h, d) or h % n_kv or h == 0:
+        q2, q_at, qt, qh = _head_rows(q, "q")
+        q_tokens, h, dq = q2.shape
+        if q_tokens != tokens or dq != d or h % n_kv or h == 0:
             raise RuntimeError(f"q must be ({tokens}, H, {d}), H a multiple of {n_kv}")
         q_out = torch.empty_like(q2, memory_format=torch.contiguous_format)
-        q_at, out_at = q2.data_ptr(), q_out.data_ptr()
+        out_at = q_out.data_ptr()
     _launch(dev, "lse_append_kv_fp8", _lib.APPEND_KV_FP8_ARGS.pack(
-        q_at, qt, qh, k2.data_ptr(), kt, kh, v2.data_ptr(), vt, vh, cos_at, sin_at, rows, out_at,
-        pool.k.data_ptr(), pool.v.data_ptr(), stride, pool.scales.data_ptr(), s_stride, blocks,
-        KV_GROUP * per, block_table.data_ptr(), t_stride, width, query_offset.data_ptr(), q_start.data_ptr(),
-        q_len.data_ptr(), entries, tokens, max_q_len, h, n_kv, d, rotary, int(interleaved)))
+        q_at, qt, qh, k_at, kt, kh, v_at, vt, vh, cos_at, sin_at, rows, out_at, pool.k.data_ptr(),
+        pool.v.data_ptr(), stride, pool.scales.data_ptr(), s_stride, blocks, KV_GROUP * per,
+        block_table.data_ptr(), t_stride, width, query_offset.data_ptr(), q_start.data_ptr(), q_len.data_ptr(),
+        entries, tokens, max_q_len, h, n_kv, d, rotary, int(interleaved)))
     return q_out
 
 

@@ -165,6 +165,7 @@ def test_tensors_are_checked(pkg):
             ops._check_plan(t, e)
     assert ops._check_plan(table, i, i) == (1, 4, 4)
     for cos, sin in ((torch.zeros(4, 32), torch.zeros(4, 31)), (torch.zeros(4, 32).double(), torch.zeros(4, 32)),
-                     (torch.zeros(32, 4).t(), torch.zeros(32, 4).t())):
+                     (torch.zeros(32, 4).t(), torch.zeros(32, 4).t()), (torch.zeros(4, 4),) * 2,
+                     (torch.zeros(4, 12),) * 2, (torch.zeros(4, 40),) * 2):
         with pytest.raises(RuntimeError):
-            ops._rope_tables(cos, sin)
+            ops._rope_tables(cos, sin, 64)
