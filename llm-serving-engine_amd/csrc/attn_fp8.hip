@@ -37,30 +37,31 @@ __device__ __forceinline__ void f8_add_state(float& M, float& L, float (&O)[4], 
 }
 
 struct Fp8MergeGrid {
-  int stream;  // workgroups of f8_merge_stream, which come first
-  int pieces;  // workgroups of one query tile
+  int stream;    // workgroups of f8_merge_stream, which come first
+  int pieces;    // workgroups of one query tile
+  int by_entry;  // they go by entries, of one query tile each; otherwise by units, the first of each tile's
 };
 
 // The second kernel of calls whose keys are split. Bound by latency: a thread's loads, eight states at a time, do not
 // wait for each other.
 //
-// f8_stream's ranges, a workgroup per entry, K/V head, query tile and 64 (row, 4 dims) pieces: wave w adds up the states
+// f8_stream's ranges, a workgroup per query tile, K/V head and 64 (row, 4 dims) pieces: wave w adds up the states
 // of ranges w, w + 4, ..., then the four are merged.
 template <int D>
 __device__ __forceinline__ void f8_merge_stream(const Fp8AttnArgs& a, const Fp8MergeGrid& g, int block) {
   __shared__ float obuf[kF8Waves][64][5];
   __shared__ float mbuf[kF8Waves][64], lbuf[kF8Waves][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int kvh = block % a.HKV, e = block / a.HKV % a.entries;
-  const int rest = block / a.HKV / a.entries, qt = rest / g.pieces;
-  const F8Unit u = f8_unit(a, e, true);
-  if (u.e < 0 || u.parts <= 1 || qt >= u.tiles) return;
-  const int qlen = min(a.q_len[e], a.max_q_len), G = a.G;
-  const int piece = rest % g.pieces * 64 + lane, orow = piece / (D / 4), c4 = 4 * (piece % (D / 4));
+  const int kvh = block % a.HKV, item = block / a.HKV / g.pieces;
+  const F8Unit u = f8_unit(a, item, g.by_entry);
+  if (u.e < 0 || u.parts <= 1 || u.part > 0) return;
+  const int qt = u.qt;
+  const int qlen = u.qlen, G = a.G;
+  const int piece = block / a.HKV % g.pieces * 64 + lane, orow = piece / (D / 4), c4 = 4 * (piece % (D / 4));
   const int otok = orow / G, om = qt * a.tq + otok;
-  const int64_t row = (int64_t)a.q_start[e] + om;
+  const int64_t row = (int64_t)u.qs + om;
   const bool ok = orow < a.tq * G && om < qlen && row >= 0 && row < a.tokens;
-  const int end_n = f8_end(a, a.query_offset[e], a.context_len[e], min(qlen, (qt + 1) * a.tq));
+  const int end_n = f8_end(a, u.qo, u.ctx, min(qlen, (qt + 1) * a.tq));
   const int n = max((int)((end_n + u.range - 1) / u.range), 1);  // ranges with keys of this tile
   float M = kNegInf, L = 0.0f, O[4] = {0, 0, 0, 0};
   if (ok) {
@@ -97,39 +98,43 @@ __device__ __forceinline__ void f8_merge_stream(const Fp8AttnArgs& a, const Fp8M
       make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
 
-// f8_tile's parts, a workgroup per item, K/V head and 256 (row, 4 dims) pieces.
+// f8_tile's parts, a workgroup per item, K/V head and quarter of its (row, 4 dims) pieces.
+constexpr int kF8TileMerges = 4;
 template <int D>
 __device__ __forceinline__ void f8_merge_tile(const Fp8AttnArgs& a, int block) {
-  constexpr int kPieces = kF8TileRows * (D / 4) / 256;
-  const int kvh = block % a.HKV, rank = block / a.HKV / kPieces;
+  constexpr int kPieces = kF8TileRows * (D / 4) / kF8TileMerges;
+  const int kvh = block % a.HKV, rank = block / a.HKV / kF8TileMerges;
   const F8Item item = f8_tile_item(a, rank);
   if (item.e < 0) return;
-  const int e = item.e, G = a.G, qlen = min(a.q_len[e], a.max_q_len);
-  const int end_n = f8_tile_end(a, a.query_offset[e], a.context_len[e], qlen, item.qt);
+  const int G = a.G, qlen = item.qlen;
+  const int end_n = f8_tile_end(a, item.qo, item.ctx, qlen, item.qt);
   const int parts = f8_tile_parts(a, (end_n + 63) / 64);
   if (parts <= 1) return;
-  const int piece = block / a.HKV % kPieces * 256 + threadIdx.x, irow = piece / (D / 4), c4 = 4 * (piece % (D / 4));
-  const int r = item.qt * kF8TileRows + irow, tok = r / G;
-  const int64_t row = (int64_t)a.q_start[e] + tok;
-  if (r >= (int64_t)qlen * G || row < 0 || row >= a.tokens) return;
-  float M = kNegInf, L = 0.0f, O[4] = {0, 0, 0, 0};
-  for (int p0 = 0; p0 < parts; p0 += 8) {
-    float2 ml[8];
-    float4 v[8];
+  for (int i0 = threadIdx.x; i0 < kPieces; i0 += 256) {
+    const int piece = block / a.HKV % kF8TileMerges * kPieces + i0;
+    const int irow = piece / (D / 4), c4 = 4 * (piece % (D / 4));
+    const int r = item.qt * kF8TileRows + irow, tok = r / G;
+    const int64_t row = (int64_t)item.qs + tok;
+    if (r >= (int64_t)qlen * G || row < 0 || row >= a.tokens) continue;
+    float M = kNegInf, L = 0.0f, O[4] = {0, 0, 0, 0};
+    for (int p0 = 0; p0 < parts; p0 += 8) {
+      float2 ml[8];
+      float4 v[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {  // past the last part the first one again, without weight
-      const int p = p0 + i < parts ? p0 + i : p0;
-      const int64_t at = (((int64_t)rank * a.tile_parts + p) * a.HKV + kvh) * kF8TileRows + irow;
-      ml[i] = *reinterpret_cast<const float2*>(a.ws_tile_ml + 2 * at);
-      v[i] = *reinterpret_cast<const float4*>(a.ws_tile_o + at * D + c4);
+      for (int i = 0; i < 8; ++i) {  // past the last part the first one again, without weight
+        const int p = p0 + i < parts ? p0 + i : p0;
+        const int64_t at = (((int64_t)rank * a.tile_parts + p) * a.HKV + kvh) * kF8TileRows + irow;
+        ml[i] = *reinterpret_cast<const float2*>(a.ws_tile_ml + 2 * at);
+        v[i] = *reinterpret_cast<const float4*>(a.ws_tile_o + at * D + c4);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f8_add_state(M, L, O, ml[i], v[i], p0 + i < parts);
     }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f8_add_state(M, L, O, ml[i], v[i], p0 + i < parts);
+    const float inv = f8_inverse(L);
+    *reinterpret_cast<uint2*>(a.o + (int64_t)(kvh * G + r - tok * G) * a.so_h + row * a.so_t + c4) =
+        make_uint2(pack_bf16x2(O[0] * inv, O[1] * inv), pack_bf16x2(O[2] * inv, O[3] * inv));
   }
-  const float inv = f8_inverse(L);
-  *reinterpret_cast<uint2*>(a.o + (int64_t)(kvh * G + r - tok * G) * a.so_h + row * a.so_t + c4) =
-      make_uint2(pack_bf16x2(O[0] * inv, O[1] * inv), pack_bf16x2(O[2] * inv, O[3] * inv));
 }
 
 template <int D>
@@ -217,9 +222,10 @@ static int launch_fp8_attention(const Fp8AttnArgs& a, const Fp8AttnPlan& pl, hip
     if (pl.slots) {
       const int64_t rows = std::min<int64_t>(pl.short_q, pl.tq) * a.G;
       g.pieces = (int)ceil_div(rows * (D / 4), 64);
-      g.stream = (int)(a.entries * a.HKV * g.pieces * ceil_div(pl.short_q, (int64_t)pl.tq));
+      g.by_entry = one;
+      g.stream = (int)((one ? a.entries : pl.slots) * (int64_t)a.HKV * g.pieces);
     }
-    const int64_t tile = pl.tile_parts > 1 ? pl.tile_items * a.HKV * (kF8TileRows * (D / 4) / 256) : 0;
+    const int64_t tile = pl.tile_parts > 1 ? pl.tile_items * a.HKV * kF8TileMerges : 0;
     hipLaunchKernelGGL(attn_fp8_merge_kernel<D>, dim3((unsigned)(g.stream + tile)), dim3(256), 0, stream, a, g);
   }
   return launch_status();

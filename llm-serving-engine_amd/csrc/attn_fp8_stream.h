@@ -75,16 +75,21 @@ __device__ __forceinline__ int f8_sorted_entry(const Fp8AttnArgs& a, int slot) {
 // read a range together).
 struct F8Unit {
   int e, qt, part, parts, tiles, first;  // first: number of the entry's first unit; e < 0: no such unit
+  int qlen, ctx, qo, qs;
   int64_t range;                         // keys of a range
 };
 struct F8Work {
-  int tiles, end;
+  int tiles, end, qlen, ctx, qo, qs;
 };
 __device__ __forceinline__ F8Work f8_entry_work(const Fp8AttnArgs& a, int i) {
-  if (i >= a.entries) return {0, 0};
-  const int qlen = min(a.q_len[i], a.max_q_len);
-  if (qlen <= 0 || (a.tiled && f8_is_long(qlen, a.G))) return {0, 0};
-  return {(qlen + a.tq - 1) / a.tq, f8_end(a, a.query_offset[i], a.context_len[i], qlen)};
+  F8Work w{0, 0, 0, 0, 0, 0};
+  if (i >= a.entries) return w;
+  w.qlen = min(a.q_len[i], a.max_q_len), w.ctx = a.context_len[i];
+  w.qo = a.query_offset[i], w.qs = a.q_start[i];
+  if (w.qlen <= 0 || (a.tiled && f8_is_long(w.qlen, a.G))) return w;
+  w.tiles = (w.qlen + a.tq - 1) / a.tq;
+  w.end = f8_end(a, w.qo, w.ctx, w.qlen);
+  return w;
 }
 
 // Unit b, or (of_entry) the units of entry b. Every wave counts for itself, 64 entries at a time.
@@ -130,6 +135,10 @@ __device__ __forceinline__ F8Unit f8_unit(const Fp8AttnArgs& a, int b, bool of_e
       u.tiles = __builtin_amdgcn_readlane(w.tiles, at);
       u.parts = __builtin_amdgcn_readlane(parts, at);
       u.range = range;
+      u.qlen = __builtin_amdgcn_readlane(w.qlen, at);
+      u.ctx = __builtin_amdgcn_readlane(w.ctx, at);
+      u.qo = __builtin_amdgcn_readlane(w.qo, at);
+      u.qs = __builtin_amdgcn_readlane(w.qs, at);
       const int i = of_entry ? 0 : b - u.first;
       u.qt = i % u.tiles;
       u.part = i / u.tiles;
@@ -137,7 +146,7 @@ __device__ __forceinline__ F8Unit f8_unit(const Fp8AttnArgs& a, int b, bool of_e
     }
     before0 = __builtin_amdgcn_readlane(before + units, 63);
   }
-  return {-1, 0, 0, 1, 0, 0, range};
+  return {-1, 0, 0, 1, 0, 0, 0, 0, 0, 0, range};
 }
 
 // NT: K and V stream with the nt cache policy, where each is read by one workgroup only (one query tile: decode).
@@ -157,19 +166,18 @@ __device__ __forceinline__ void f8_stream(const Fp8AttnArgs& a, int block, unsig
   const int n16 = lane & 15, g = lane >> 4;
 
   const int kvh = block % a.HKV, slot = block / a.HKV;
-  int e, qt = 0, parts = 1;
+  int e, qt = 0, parts = 1, qlen, ctx, qo, qs;
   int64_t first_key = 0, end_key = (int64_t)1 << 40;
   if constexpr (COUNT) {
     const F8Unit u = f8_unit(a, slot, false);
     if (u.e < 0) return;
-    e = u.e, qt = u.qt, parts = u.parts;
+    e = u.e, qt = u.qt, parts = u.parts, qlen = u.qlen, ctx = u.ctx, qo = u.qo, qs = u.qs;
     first_key = u.part * u.range, end_key = first_key + u.range;
   } else {
     e = a.sorted ? f8_sorted_entry(a, slot) : slot;
+    qlen = min(a.q_len[e], a.max_q_len), ctx = a.context_len[e], qo = a.query_offset[e], qs = a.q_start[e];
   }
-  const int qlen = min(a.q_len[e], a.max_q_len);
   if (qt * a.tq >= qlen) return;
-  const int ctx = a.context_len[e], qo = a.query_offset[e], qs = a.q_start[e];
   int end_n = f8_end(a, qo, ctx, min(qlen, (qt + 1) * a.tq));
   if (first_key > 0 && first_key >= end_n) return;  // the tile has no keys in this range
   end_n = (int)min((int64_t)end_n, end_key);

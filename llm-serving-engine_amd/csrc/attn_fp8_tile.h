@@ -67,19 +67,25 @@ __device__ __forceinline__ F8Halves f8_halves(float v) {
 // offset in tiles + its tile) first. Entries are looked at 64 at a time, one per lane.
 struct F8Item {
   int e, qt;  // e < 0: no such item
+  int qlen, ctx, qo, qs;
 };
 __device__ __forceinline__ F8Item f8_tile_item(const Fp8AttnArgs& a, int p) {
   const int lane = threadIdx.x & 63;
+  struct Entry {
+    int qlen, ctx, qo, qs;
+  };
   auto entry = [&](int i, int& base, int& tiles) {
     base = tiles = 0;
-    if (i >= a.entries) return;
-    const int qlen = min(a.q_len[i], a.max_q_len);
-    if (!f8_is_long(qlen, a.G)) return;
-    tiles = (int)(((int64_t)qlen * a.G + kF8TileRows - 1) / kF8TileRows);
-    base = (int)((int64_t)min(max(a.query_offset[i], 0), a.max_ctx) * a.G / kF8TileRows);
+    Entry x{0, 0, 0, 0};
+    if (i >= a.entries) return x;
+    x = Entry{min(a.q_len[i], a.max_q_len), a.context_len[i], a.query_offset[i], a.q_start[i]};
+    if (!f8_is_long(x.qlen, a.G)) return x;
+    tiles = (int)(((int64_t)x.qlen * a.G + kF8TileRows - 1) / kF8TileRows);
+    base = (int)((int64_t)min(max(x.qo, 0), a.max_ctx) * a.G / kF8TileRows);
+    return x;
   };
   int base0, tiles0;
-  entry(lane, base0, tiles0);
+  const Entry entry0 = entry(lane, base0, tiles0);
   // Tiles at level L or above it, over all entries.
   auto above = [&](int L) {
     int n = min(max(base0 + tiles0 - L, 0), tiles0);
@@ -90,7 +96,7 @@ __device__ __forceinline__ F8Item f8_tile_item(const Fp8AttnArgs& a, int p) {
     }
     return f8_wave_total(n);
   };
-  if (above(0) <= p) return {-1, 0};
+  if (above(0) <= p) return {-1, 0, 0, 0, 0, 0};
   int top = base0 + tiles0;
   for (int e0 = 64; e0 < a.entries; e0 += 64) {
     int b, t;
@@ -107,17 +113,22 @@ __device__ __forceinline__ F8Item f8_tile_item(const Fp8AttnArgs& a, int p) {
   p -= above(lo + 1);  // among the entries that have a tile at level lo
   for (int e0 = 0; e0 < a.entries; e0 += 64) {
     int b = base0, t = tiles0;
-    if (e0) entry(e0 + lane, b, t);
+    const Entry x = e0 ? entry(e0 + lane, b, t) : entry0;
     const int mine = t > 0 && b <= lo && lo < b + t;
     const int before = kv_wave_scan(mine) - mine;
     const unsigned long long hit = __ballot(mine && before == p);
     if (hit) {
       const int at = __ffsll(hit) - 1;
-      return {e0 + at, lo - __builtin_amdgcn_readlane(b, at)};
+      return {e0 + at,
+              lo - __builtin_amdgcn_readlane(b, at),
+              __builtin_amdgcn_readlane(x.qlen, at),
+              __builtin_amdgcn_readlane(x.ctx, at),
+              __builtin_amdgcn_readlane(x.qo, at),
+              __builtin_amdgcn_readlane(x.qs, at)};
     }
     p -= __builtin_amdgcn_readlane(before + mine, 63);
   }
-  return {-1, 0};
+  return {-1, 0, 0, 0, 0, 0};
 }
 
 // Key tiles of an item, and the parts they are cut into.
@@ -145,8 +156,7 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
   const F8Item item = f8_tile_item(a, rank);
   if (item.e < 0) return;
   const int e = item.e;
-  const int qlen = min(a.q_len[e], a.max_q_len), ctx = a.context_len[e];
-  const int qo = a.query_offset[e], qs = a.q_start[e];
+  const int qlen = item.qlen, ctx = item.ctx, qo = item.qo, qs = item.qs;
   const int row0 = item.qt * kF8TileRows;
   const int end_n = f8_tile_end(a, qo, ctx, qlen, item.qt);
   const int all_tiles = (end_n + 63) / 64, parts = f8_tile_parts(a, all_tiles);
