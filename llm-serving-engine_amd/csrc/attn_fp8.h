@@ -19,7 +19,7 @@ struct Fp8AttnArgs {
   int entries, H, HKV, G, tokens;
   int max_ctx;       // positions that the table has room for
   int max_q_len;
-  int tiled;         // the row-tiled kernel runs too and takes the long entries (f8_is_long)
+  int tiled;         // the row-tiled kernel takes the long entries
   int tq;            // query tokens per tile: floor(16 / G)
   int slots;         // units of a split launch (f8_unit); 0: keys are not split
   int sorted;        // entries are taken in descending order of context length...
@@ -33,16 +33,17 @@ struct Fp8AttnArgs {
   float* ws_tile_ml;  // their max and sum [items][parts][HKV][128 rows][2]
 };
 
-// Whether the row-tiled kernel takes an entry of q_len tokens; the key-streaming kernel takes it otherwise.
-constexpr int kF8LongRows = 256;  // query rows per K/V head
+// In a call that is tiled (fp8_attn_tiled, attn_fp8.hip) the row-tiled kernel takes the entries of 128 query rows per K/V
+// head or more, the key-streaming kernel the others; otherwise the latter takes all.
+constexpr int kF8LongRows = 128;
 __host__ __device__ inline bool f8_is_long(int64_t q_len, int G) { return q_len * G >= kF8LongRows; }
+
+__device__ __forceinline__ int f8_wave_total(int v) { return __builtin_amdgcn_readlane(kv_wave_scan(v), 63); }
 
 // The keys [0, end) that an entry's first `tokens` rows may see.
 __device__ __forceinline__ int f8_end(const Fp8AttnArgs& a, int qo, int ctx, int tokens) {
   return max(min((int)min((int64_t)qo + tokens, (int64_t)ctx), a.max_ctx), 0);
 }
-
-__device__ __forceinline__ int f8_wave_total(int v) { return __builtin_amdgcn_readlane(kv_wave_scan(v), 63); }
 
 constexpr float kNegInf = -__builtin_huge_valf();
 

@@ -157,8 +157,8 @@ __global__ void __launch_bounds__(256) attn_fp8_merge_kernel(Fp8AttnArgs a, Fp8M
 
 struct Fp8AttnPlan {
   int tq;
-  bool tiled;       // some entry may be the row-tiled kernel's
-  int64_t short_q;  // the most tokens of an entry that is not
+  bool tiled;       // the row-tiled kernel takes long entries
+  int64_t short_q;  // the most tokens of an entry that is not its
   int64_t tiles;    // query tiles of the others, at most
   int slots;        // units of a split launch, 0: keys are not split
   int64_t tile_items;  // row tiles of the long entries, at most
@@ -176,6 +176,35 @@ static int fp8_attn_cus() {
   return cus;
 }
 
+// Whether a call's long entries go to the row-tiled kernel: where it has, as far as its sizes tell, so many items of them
+// (128 rows of a K/V head) or so many (query row, key) pairs that this is faster. Measured on MI355X, us, row-tiled /
+// key-streaming, 32 heads over 8 unless said:
+//  * fresh prompts, items: 4 x 64 tokens (64) 9.5 / 7.7, 1 x 512 (128) 19 / 17, 2 x 256 (128) 13 / 14, 1 x 1024, 24 heads
+//    (192) 30 / 30, 1 x 1024 (256) 29 / 35, 4 x 256 (256) 14 / 25, 8 x 512 (1024) 42 / 95; 8 over 8, 1 x 2048 (128) 38 / 26;
+//  * behind 500 positions: 512 tokens (128) 30 / 23, 1024 (256) 39 / 45, 2048 (512) 74 / 111;
+//  * behind 2000, pairs: 512 tokens (37 million) 46 / 41, 768 (59) 57 / 60, 1024 (82) 65 / 80; 8 over 8, 1024 (21) 34 / 25,
+//    2048 (50) 57 / 51; behind 8000, where the query tiles read more than the L2s hold and pairs count twice: 128 tokens
+//    (8) 26 / 26, 256 (17) 28 / 34; behind 16000: 128 (66) 57 / 75; 8 over 8, 128 (16) 35 / 32, 256 (33) 39 / 51;
+//  * one chunk beside 40 decoding sequences, which the two kernels share the card for: 256 tokens behind 1000 (11)
+//    36 / 36, 512 (22) 47 / 47, 735 behind 1300, 24 heads (28) 57 / 74.
+// Contexts are taken to be as long as the table, rows to be the entries' (a call with others may take the slower one). Left
+// to the kernel, which knows the lengths, the choice costs every such call more than a wrong one: a launch for either
+// outcome is 1.1 to 1.6 times as long as the right one.
+static bool fp8_attn_tiled(int64_t entries, int64_t tokens, int64_t G, int64_t HKV, int64_t max_q_len,
+                           int64_t max_ctx) {
+  constexpr int64_t kItems = 200, kFar = 6000, kMixed = 128;
+  constexpr double kPairs = 40e6, kPairsMixed = 20e6;
+  if (!f8_is_long(max_q_len, (int)G)) return false;
+  // The longest entry's items, and those of all rows where the mean entry is long, else of those that short ones
+  // cannot have.
+  const int64_t q = std::min(max_q_len, tokens), rows = tokens * G;
+  const int64_t left = rows >= entries * kF8LongRows ? rows : rows - entries * (kF8LongRows - 1);
+  if (std::max(ceil_div(q * G, (int64_t)kF8TileRows), left / kF8TileRows) * HKV >= kItems) return true;
+  const int64_t keys = std::max<int64_t>(max_ctx - q / 2, 0);
+  const double pairs = (double)rows * HKV * keys * (keys < kFar ? 1 : 2);
+  return pairs >= ((entries - 1) * HKV >= kMixed ? kPairsMixed : kPairs);
+}
+
 // One workgroup per (entry, K/V head, query tile) once those fill the card; otherwise, where contexts may be long
 // enough, the keys are split as well. A lone entry of a call made for long ones is taken to be long.
 static Fp8AttnPlan fp8_attn_plan(int64_t entries, int64_t tokens, int64_t H, int64_t HKV, int64_t D,
@@ -183,7 +212,7 @@ static Fp8AttnPlan fp8_attn_plan(int64_t entries, int64_t tokens, int64_t H, int
   Fp8AttnPlan pl{};
   const int64_t G = H / HKV;
   pl.tq = (int)(16 / G);
-  pl.tiled = f8_is_long(max_q_len, (int)G);
+  pl.tiled = fp8_attn_tiled(entries, tokens, G, HKV, max_q_len, max_ctx);
   pl.short_q = pl.tiled ? (kF8LongRows - 1) / G : max_q_len;
   pl.tiles = std::min(entries * ceil_div(pl.short_q, (int64_t)pl.tq), tokens / pl.tq + entries);
   const int64_t slots = kF8Groups / HKV;
@@ -197,7 +226,10 @@ static Fp8AttnPlan fp8_attn_plan(int64_t entries, int64_t tokens, int64_t H, int
     // Every long entry's rows round up to a tile; it has at least kF8LongRows rows.
     const int64_t rows = tokens * G;
     pl.tile_items = rows / kF8TileRows + std::min(entries, rows / kF8LongRows);
-    const int64_t parts = kF8Groups / std::max<int64_t>(pl.tile_items * HKV, 1);
+    // Parts so that all run at once, if one entry is long and the others decode (which are done in a quarter of a
+    // part's time): 1, 2 and 3 parts of 144 items beside 320 decoding ones 64, 57 and 73 us.
+    const int64_t likely = (std::max<int64_t>(tokens - entries + 1, 1) * G / kF8TileRows + 1) * HKV;
+    const int64_t parts = kF8Groups / (likely + (entries - 1) * HKV / 4);
     const int64_t most = max_ctx / (64 * kF8PartTiles);
     pl.tile_parts = (int)std::max<int64_t>(std::min({parts, most, (int64_t)16}), 1);
     if (pl.tile_parts > 1) {
@@ -214,7 +246,7 @@ template <int D>
 static int launch_fp8_attention(const Fp8AttnArgs& a, const Fp8AttnPlan& pl, hipStream_t stream) {
   const dim3 wg(64 * kF8Waves);
   const bool one = pl.short_q <= pl.tq;
-  const int64_t units = (pl.slots ? pl.slots : one ? a.entries : pl.tiles) * (int64_t)a.HKV;
+  const int64_t units = (pl.slots ? pl.slots : one && !a.tiled ? a.entries : pl.tiles) * (int64_t)a.HKV;
   const dim3 grid((unsigned)(units + a.tile_blocks));
   if (a.tiled)
     hipLaunchKernelGGL(attn_fp8_mixed_kernel<D>, grid, wg, 0, stream, a);

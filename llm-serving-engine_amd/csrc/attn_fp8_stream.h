@@ -17,7 +17,7 @@
 //
 // Wave w of the four takes the tiles of 64 keys w, w + 4, w + 8, ... with an online-softmax state of its own; the four
 // are merged in wave order at the end. Where a call has fewer (entry, K/V head, query tile) items than the card
-// takes workgroups, the keys are split too (f8_units): into ranges of one length for all entries, chosen so
+// takes workgroups, the keys are split too (f8_unit): into ranges of one length for all entries, chosen so
 // that all ranges run at once, each leaving its state to a second kernel. With ranges of a fixed 1024 or 2048
 // keys, four sequences behind 7500 to 60000 positions took 44 + 7 us.
 #pragma once
@@ -30,7 +30,9 @@ constexpr int kF8Waves = 4;
 constexpr int kF8Keys = 64;      // keys of a wave's tile: one group per 16 lanes
 constexpr int kF8Round = kF8Keys * kF8Waves;
 constexpr int kF8Window = 4 * kF8Round;  // keys of four tiles of every wave, whose blocks and scales it holds
-constexpr int kF8Groups = 512;   // workgroups of a split launch: two per CU
+// Workgroups of a split launch, two per CU: all there is room for (204 registers; with 168, three, the kernel spills:
+// four sequences behind 7500 to 60000 positions 42 -> 54 us), and with twice as many, half of them wait (48 us).
+constexpr int kF8Groups = 512;
 // Fewest keys of a range, and contexts up to which nothing is split: a wave takes 0.5 us a tile, the second
 // kernel 4 us and more.
 constexpr int kF8MinRange = 1024, kF8MinSplit = 2048;
@@ -92,7 +94,7 @@ __device__ __forceinline__ F8Work f8_entry_work(const Fp8AttnArgs& a, int i) {
   return w;
 }
 
-// Unit b, or (of_entry) the units of entry b. Every wave counts for itself, 64 entries at a time.
+// Unit b, or (of_entry) the first of entry b's. Every wave counts for itself, 64 entries at a time.
 __device__ __forceinline__ F8Unit f8_unit(const Fp8AttnArgs& a, int b, bool of_entry) {
   const int lane = threadIdx.x & 63;
   const F8Work w0 = f8_entry_work(a, lane);
