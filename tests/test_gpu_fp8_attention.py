@@ -3,6 +3,9 @@ for. Tolerance (`fp8_kv_helpers.check_attention`): bf16 probabilities and a bf16
 
 from __future__ import annotations
 
+import re
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -325,27 +328,61 @@ def test_append_then_attend(pkg, dev):
                         <= 2.0 ** -4 * np.abs(want) + 2.0 ** -9 * scale).all()
 
 
+SOURCES = Path(__file__).resolve().parent.parent / "llm-serving-engine_amd" / "csrc"
+
+
+def _tiled(case, most=None):
+    """Whether the row-tiled kernel takes the case's long entries (128 rows per K/V head), by the library's own
+    bounds."""
+    text = (SOURCES / "attn_fp8.hip").read_text() + (SOURCES / "attn_fp8.h").read_text()
+    bound = {n: float(v) for n, v in re.findall(r"\bk(\w+) = ([\d.e]+)[,;]", text)}
+    h, tokens, _ = case["q"].shape
+    h_kv, entries = case["pool"][0].shape[1], len(case["ql"])
+    g, most = h // h_kv, most or int(case["ql"].max())
+    if most * g < bound["F8LongRows"]:
+        return False
+    q, rows = min(most, tokens), tokens * g
+    left = rows if rows >= entries * bound["F8LongRows"] else rows - entries * (bound["F8LongRows"] - 1)
+    if max(-(-q * g // 128), left // 128) * h_kv >= bound["Items"]:
+        return True
+    keys = max(case["table"].shape[1] * case["bs"] - q // 2, 0)
+    pairs = rows * h_kv * keys * (1 if keys < bound["Far"] else 2)
+    return pairs >= (bound["PairsMixed"] if (entries - 1) * h_kv >= bound["Mixed"] else bound["Pairs"])
+
+
+def _long_case(*args, **kw):
+    case = attention_case(*args, **kw)
+    assert _tiled(case)
+    return case
+
+
 @pytest.mark.parametrize("d", [64, 128])
-@pytest.mark.parametrize("h,h_kv", [(8, 2), (3, 1), (16, 1), (8, 8)])
+@pytest.mark.parametrize("h,h_kv", [(80, 20), (99, 33), (240, 15), (105, 105)])
 def test_long_entries(pkg, dev, h, h_kv, d):
     """Entries on both sides of the first row-tiled length and of the next row tile, key tiles one short of and
-    one over, few items (cut into parts), decode rows beside them."""
+    one over, decode rows beside them."""
     g = h // h_kv
-    first = -(-256 // g)
-    entries = [(first - 1, 5, first + 4), (first, 0, first), (first + 1, 3000, first + 3001),
-               (384 // g, 63, 384 // g + 63), (384 // g + 1, 64, 384 // g + 65), (1, 2600, 2601), (1, 0, 1)]
-    case = attention_case(h + d, entries, h=h, h_kv=h_kv, d=d, block_size=48)
-    check_attention(pkg, dev, case, f"{h} over {h_kv}, D={d}")
-    alone = dict(case, q=case["q"][:, 2 * first - 1:3 * first], qs=np.zeros(1, np.int32),
-                 **{n: case[n][2:3] for n in ("table", "ctx", "qo", "ql")})
-    check_attention(pkg, dev, alone, "alone")
+    first = -(-128 // g)
+    entries = [(first - 1, 5, first + 4), (first, 0, first), (first + 1, 700, first + 701),
+               (384 // g, 63, 384 // g + 63), (384 // g + 1, 64, 384 // g + 65), (1, 600, 601), (1, 0, 1),
+               (640 // g, 0, 640 // g)]
+    check_attention(pkg, dev, _long_case(h + d, entries, h=h, h_kv=h_kv, d=d, block_size=48), f"{h} over {h_kv}")
 
 
-@pytest.mark.parametrize("end", [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 385, 1000])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("entries", [[(300, 17000, 17300)], [(300, 19000, 19300), (1, 18000, 18001), (40, 70, 110)]])
+def test_parts_of_few_items(pkg, dev, entries, d):
+    """Few items behind long contexts are cut into 16 parts by their keys; beside a decode row whose keys are
+    split too, and a long entry that has one part."""
+    case = _long_case(70 + len(entries), entries, h=4, h_kv=1, d=d, block_size=64)
+    check_attention(pkg, dev, case, "parts")
+
+
+@pytest.mark.parametrize("end", [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 385, 500])
 def test_long_entries_key_edges(pkg, dev, end):
     """Contexts one short of and one over a key tile; the second entry's rows see less and less, the third's
     nothing."""
-    case = attention_case(end, [(64, max(end - 64, 0), max(end, 64)), (70, 11, 81), (64, 0, 64)], h=8, h_kv=2, d=64)
+    case = _long_case(end, [(64, max(end - 64, 0), max(end, 64)), (70, 11, 81), (64, 0, 64)], h=136, h_kv=34, d=64)
     case["ctx"][:] = [end, min(end, 81), 0]
     o = check_attention(pkg, dev, case, f"end {end}")
     assert not o[:, 134:].any()
@@ -353,14 +390,14 @@ def test_long_entries_key_edges(pkg, dev, end):
 
 @pytest.mark.parametrize("q_scale", [0.0, 3.0, 2.0 ** 12, 2.0 ** 40, 2.0 ** -40])
 def test_long_entries_flat_and_peaked_scores(pkg, dev, q_scale):
-    case = attention_case(61, [(150, 450, 600), (64, 0, 64)], h=8, h_kv=2, q_scale=q_scale)
+    case = _long_case(61, [(150, 450, 600), (64, 0, 64)], h=136, h_kv=34, q_scale=q_scale)
     check_attention(pkg, dev, case, f"q x {q_scale}")
 
 
 def test_long_entries_read_nothing_behind_their_context(pkg, dev):
     """NaN codes in every slot behind a context, NaN scales in groups behind it, a bad block in one entry."""
     entries = [(80, 20, 100), (64, 300, 364), (70, 0, 70), (1, 40, 41)]
-    case = attention_case(62, entries, h=8, h_kv=2, d=128, block_size=16)
+    case = _long_case(62, entries, h=136, h_kv=34, d=128, block_size=16)
     want = attend(pkg, dev, case)
     k, v, s = (a.copy() for a in case["pool"])
     used = np.zeros((case["blocks"], 16), bool)
@@ -383,9 +420,47 @@ def test_long_entries_read_nothing_behind_their_context(pkg, dev):
     np.testing.assert_array_equal(ora.f32_to_bf16_bits(o[:, 144:]), want[:, 144:])
 
 
-def test_many_long_entries(pkg, dev):
+@pytest.mark.parametrize("h,h_kv,tiled", [(16, 1, True), (4, 1, False)])
+def test_many_entries(pkg, dev, h, h_kv, tiled):
     """More entries than a wave looks at in a step: prompts of 64 to 100 tokens among decode rows."""
     rng = np.random.default_rng(63)
     entries = [(int(n), int(o), int(n + o)) for n, o in zip(rng.integers(64, 100, 70), rng.integers(0, 90, 70))]
     entries = [x for e in entries for x in (e, (1, e[2], e[2] + 1))]
-    check_attention(pkg, dev, attention_case(63, entries, h=4, h_kv=1, d=64), "many")
+    case = attention_case(63, entries, h=h, h_kv=h_kv, d=64)
+    assert _tiled(case) == tiled
+    check_attention(pkg, dev, case, "many")
+
+
+def test_long_entries_replay_from_a_graph(pkg, dev):
+    """A mixed call whose items are cut into parts, captured once, replayed with other q, against eager calls."""
+    case = _long_case(64, [(300, 17000, 17300), (1, 3000, 3001), (2, 7, 9)], h=4, h_kv=1, d=64, block_size=64)
+    pool, q, plan = pool_to_dev(pkg, case["pool"], dev), to_bf16_tensor(case["q"], dev), attend_args(case, dev)
+    call = lambda: pkg.ops.paged_attention_fp8(q, pool, *plan, 300)  # noqa: E731
+    call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = call()
+    for _ in range(3):
+        q.mul_(-1.25)
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(o, want)
+
+
+def test_how_far_a_nan_value_reaches(pkg, dev):
+    """NaN in a token's v: the rows that see it, and earlier rows of its own query tile at most (16 query rows, or
+    128 of a long entry); no other entry or K/V head."""
+    for h, h_kv, reach in ((8, 2, 16), (128, 32, 128)):
+        case = attention_case(65, [(150, 0, 150), (150, 0, 150)], h=h, h_kv=h_kv, d=64)
+        assert _tiled(case) == (reach == 128)
+        want = attend(pkg, dev, case)
+        v = case["pool"][1].copy()
+        v[case["table"][0, 120 // 16], 1, 0, kv.v_index(120 % 16, np.arange(64), 64)] = 127
+        o = attend(pkg, dev, dict(case, pool=(case["pool"][0], v, case["pool"][2])))
+        nan = np.isnan(ora.bf16_bits_to_f32(o)).any(-1)
+        g = h // h_kv
+        assert nan[g:2 * g, 120:150].all()
+        assert not nan[:, 150:].any() and not nan[:g].any() and not nan[2 * g:].any()
+        assert not nan[:, :max(0, 120 - reach // g + 1)].any()
+        np.testing.assert_array_equal(o[~nan], want[~nan])
