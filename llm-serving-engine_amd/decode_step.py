@@ -33,10 +33,12 @@ lm_head stays bf16 in every back end: the vendor BLAS's `nn.Linear` on "bf16" an
 on "int8", in either quantization mode. Attention has two implementations: "torch", fp32 over a
 contiguous per-layer KV cache (the reference's `contiguous_attention` path,
 model_runner.py:400-418), the same arithmetic for both linear back ends so only the linears
-differ; and "paged", the HIP paged attention (`ops.paged_attention_forward`, the reference's
+differ; "paged", the HIP paged attention (`ops.paged_attention_forward`, the reference's
 `attend_paged`, model_runner.py:357-363) over a per-layer pool of 16-slot blocks handed to the
 sequences in shuffled order, kept in step with the contiguous cache once `enable_paged()` has
-allocated it.
+allocated it; and, after `enable_fp8_kv()`, "paged-fp8" over an 8-bit pool that takes the place of
+both: per layer one `ops.append_kv_fp8` (rotary embedding and K/V writes) and one
+`ops.paged_attention_fp8`.
 """
 
 from __future__ import annotations
@@ -90,7 +92,7 @@ class DecodeRunner:
         self.n_heads = cfg.num_attention_heads
         self.n_kv = cfg.num_key_value_heads
         self.head_dim = getattr(cfg, "head_dim", None) or cfg.hidden_size // self.n_heads
-        dev = next(model.parameters()).device
+        self.device = dev = next(model.parameters()).device
         shape = (batch, self.n_kv, capacity, self.head_dim)
         self.k_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         self.v_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
@@ -101,28 +103,81 @@ class DecodeRunner:
         self.attention = "torch"
         self.k_pool: list[torch.Tensor] | None = None
         self.v_pool: list[torch.Tensor] | None = None
+        self.fp8_kv: list[ops.Fp8KV] | None = None
 
     def enable_paged(self, block_size: int = 16, seed: int = 0) -> None:
         """Allocates a paged K/V pool per layer (the reference's allocate_kv_pool,
         model_runner.py:107-116: (num_blocks + 1, block_size, H_KV, D), the last block a
         scratch row) with each sequence's blocks drawn in shuffled order, and copies in what the
         contiguous cache holds. Call before prefill, or after: both caches then stay in step."""
-        dev = self.k_cache[0].device
-        per_seq = -(-self.capacity // block_size)
-        num_blocks = self.batch * per_seq
-        g = torch.Generator().manual_seed(seed)
-        perm = torch.randperm(num_blocks, generator=g)
-        self.block_size = block_size
-        self.tables = perm.reshape(self.batch, per_seq).to(torch.int32).to(dev)
+        if self.fp8_kv is not None:
+            raise RuntimeError("the K/V cache is 8-bit")
+        dev = self.device
+        num_blocks = self._deal_blocks(block_size, seed)
         shape = (num_blocks + 1, block_size, self.n_kv, self.head_dim)
         self.k_pool = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         self.v_pool = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         for i in range(len(self.layers)):
             self._write_pool(i, self.k_cache[i], self.v_cache[i], 0, self.capacity, slice(None))
 
+    def _deal_blocks(self, block_size: int, seed: int) -> int:
+        """Block tables of `capacity` positions a sequence, in shuffled order; the number of blocks."""
+        per_seq = -(-self.capacity // block_size)
+        num_blocks = self.batch * per_seq
+        g = torch.Generator().manual_seed(seed)
+        perm = torch.randperm(num_blocks, generator=g)
+        self.block_size = block_size
+        self.tables = perm.reshape(self.batch, per_seq).to(torch.int32).to(self.device)
+        return num_blocks
+
+    @torch.no_grad()
+    def enable_fp8_kv(self, block_size: int = 16, seed: int = 0) -> None:
+        """Holds K/V in an 8-bit paged pool per layer (about half the bytes) from here on: what the contiguous
+        cache holds is copied in, it and the bf16 pools are freed, and attention is "paged-fp8". Call before
+        prefill, or after."""
+        if self.fp8_kv is not None:
+            raise RuntimeError("the K/V cache is 8-bit already")
+        d, groups = self.head_dim, self.n_heads // self.n_kv
+        if self.device.type != "cuda" or d not in (64, 128) or groups > 16:
+            raise ValueError(f"an 8-bit cache needs a GPU, heads of 64 or 128 dims and at most 16 query heads per "
+                             f"K/V head, got {self.device}, {d}, {groups}")
+        if block_size < ops.KV_GROUP or block_size % ops.KV_GROUP:
+            raise ValueError(f"block_size must be a multiple of {ops.KV_GROUP}, got {block_size}")
+        self.rope = self._rope_table()
+        num_blocks = self._deal_blocks(block_size, seed)
+        self.k_pool = self.v_pool = None
+        self._rows = slice(None)
+        plan = self._paged_plan(0, self.capacity, self.batch, self.capacity)
+        pools = []
+        for i in range(len(self.layers)):
+            pools.append(ops.fp8_kv_pool(num_blocks, block_size, self.n_kv, d, self.device))
+            k, v = (c[i].transpose(1, 2).reshape(-1, self.n_kv, d) for c in (self.k_cache, self.v_cache))
+            self.k_cache[i] = self.v_cache[i] = None
+            table, _, offset, q_start, q_len, ntok = plan
+            ops.append_kv_fp8(None, k, v, None, None, pools[i], table, offset, q_start, q_len, ntok)
+        self.fp8_kv = pools
+        self.attention = "paged-fp8"
+
+    def _rope_table(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(cos, sin) of every position, (capacity, D / 2) fp32, by the model's own frequencies."""
+        from transformers.models.llama.modeling_llama import LlamaRotaryEmbedding
+
+        rotary = self.model.model.rotary_emb
+        kind = getattr(rotary, "rope_type", None)
+        if type(rotary) is not LlamaRotaryEmbedding or kind not in ("default", "linear", "llama3", "yarn"):
+            raise ValueError(f"an 8-bit cache needs a rotary embedding of fixed frequencies, got "
+                             f"{type(rotary).__name__} ({kind})")
+        position = torch.arange(self.capacity, dtype=torch.float64, device=self.device)
+        angle = position[:, None] * rotary.inv_freq.to(self.device, torch.float64)
+        return tuple((f(angle) * rotary.attention_scaling).float() for f in (torch.cos, torch.sin))
+
     def use_attention(self, kind: str) -> None:
-        if kind not in ("torch", "paged"):
+        if kind not in ("torch", "paged", "paged-fp8"):
             raise ValueError(f"unknown attention {kind!r}")
+        if kind == "paged-fp8" and self.fp8_kv is None:
+            raise RuntimeError("enable_fp8_kv() first")
+        if kind != "paged-fp8" and self.fp8_kv is not None:
+            raise RuntimeError("the K/V cache is 8-bit")
         if kind == "paged" and self.k_pool is None:
             raise RuntimeError("enable_paged() first")
         self.attention = kind
@@ -144,9 +199,19 @@ class DecodeRunner:
                                         offset, q_start, q_len, self.block_size, ntok)
         return o.transpose(0, 1).reshape(1, q.shape[0], self.n_heads * self.head_dim)
 
+    def _attend_fp8(self, i: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
+        """The projections of one call's tokens (tokens, heads * D) -> (1, tokens, H * D): rotates q and k, appends
+        k and v to layer i's 8-bit pool and attends over it."""
+        table, ctx, offset, q_start, q_len, ntok = self._plan
+        q, k, v = (t.unflatten(-1, (-1, self.head_dim)) for t in (q, k, v))
+        pool = self.fp8_kv[i]
+        q = ops.append_kv_fp8(q, k, v, *self.rope, pool, table, offset, q_start, q_len, ntok)
+        o = ops.paged_attention_fp8(q.transpose(0, 1), pool, table, ctx, offset, q_start, q_len, ntok)
+        return o.transpose(0, 1).reshape(1, q.shape[0], -1)
+
     def _paged_plan(self, start: int, end: int, nseq: int, ntok: int):
         """The paging tensors every layer of one call shares."""
-        dev = self.k_cache[0].device
+        dev = self.device
         full = lambda v: torch.full((nseq,), v, dtype=torch.int32, device=dev)  # noqa: E731
         q_start = torch.arange(0, nseq * ntok, ntok, dtype=torch.int32, device=dev)
         return (self.tables[self._rows].contiguous(), full(end), full(start), q_start, full(ntok),
@@ -215,6 +280,8 @@ class DecodeRunner:
         [start, start + ntok). Writes K/V there and attends causally over [0, end). The
         positions come in as a host int, so a step captures into a graph."""
         q, k, v = self._qkv(i, normed)
+        if self.fp8_kv is not None:
+            return self._o(i, self._attend_fp8(i, q[0], k[0], v[0]))
         end = start + ntok
         rows = self._rows
         pool = None
@@ -275,11 +342,11 @@ class DecodeRunner:
         model = self.model.model
         norms = [model.norm, *(n for layer in self.layers
                                for n in (layer.input_layernorm, layer.post_attention_layernorm))]
-        cache, size = self.k_cache[0], model.embed_tokens.weight.shape[-1]
-        return (cache.is_cuda and self.head_dim % 16 == 0 and self.head_dim <= 1024
+        size = model.embed_tokens.weight.shape[-1]
+        return (self.device.type == "cuda" and self.head_dim % 16 == 0 and self.head_dim <= 1024
                 and size % 8 == 0 and size <= _lib.NORM_MAX_K
                 and all(plain_norm(n) and n.weight.shape == (size,)
-                        and n.weight.device == cache.device for n in norms))
+                        and n.weight.device == self.device for n in norms))
 
     @torch.no_grad()
     def forward(self, tokens: torch.Tensor, start: int, rows: slice | None = None) -> torch.Tensor:
@@ -289,12 +356,17 @@ class DecodeRunner:
         nseq, ntok = tokens.shape
         model = self.model.model
         ids = tokens.reshape(1, nseq * ntok)
-        pos = torch.arange(start, start + ntok, device=tokens.device).repeat(nseq, 1)
         hidden = model.embed_tokens(ids)
-        cos, sin = model.rotary_emb(hidden, pos.reshape(1, -1))
-        self._fused = self._fusable() and hidden.dtype == cos.dtype == torch.bfloat16
-        rope = (cos[0], sin[0])
-        if self.attention == "paged":
+        rope = None
+        self._fused = self._fusable() and hidden.dtype == torch.bfloat16
+        if self.fp8_kv is None:
+            pos = torch.arange(start, start + ntok, device=tokens.device).repeat(nseq, 1)
+            cos, sin = model.rotary_emb(hidden, pos.reshape(1, -1))
+            self._fused = self._fused and cos.dtype == torch.bfloat16
+            rope = (cos[0], sin[0])
+        elif start < 0 or start + ntok > self.capacity:
+            raise ValueError(f"positions [{start}, {start + ntok}) do not fit a capacity of {self.capacity}")
+        if self.attention != "torch":
             self._plan = self._paged_plan(start, start + ntok, nseq, ntok)
         norms = [layer.input_layernorm for layer in self.layers] + [model.norm]
         hidden, normed = self._add_norm(norms[0], hidden, None)
