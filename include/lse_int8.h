@@ -417,8 +417,8 @@ int lse_rope(const struct lse_rope_args* args, void* stream);
  *     zeroed, other groups are not touched.
  * q (may be NULL), k, v: bf16, element (t, h, d) at t * stride_t + h * stride_h + d. q_out: (tokens, H, D)
  *   bf16; rows of no entry are not written. Positions outside the table's max_blocks blocks, blocks outside
- *   the pool and rows outside the `tokens` rows are dropped. Entries must own distinct rows, and the blocks they
- *   write to must be theirs alone. max_q_len >= every q_len.
+ *   the pool and rows outside the `tokens` rows are dropped; a group of none but such is not touched. Entries
+ *   must own distinct rows, and the blocks they write to must be theirs alone. max_q_len >= every q_len.
  * D = 64 or 128; block_size % 16 == 0; strides of rows multiples of 8, pool_stride_block of 16; rows, tables
  *   and pools 16-byte aligned.
  * Replaces: apply_rotary_pos_emb and the K/V writes in `_project_qkv` and `attend_paged`
@@ -445,11 +445,16 @@ struct lse_append_kv_fp8_args {
 int lse_append_kv_fp8(const struct lse_append_kv_fp8_args* args, void* stream);
 
 /*
- * lse_paged_attention over the 8-bit cache: the same plan and semantics, k and v being the values code x scale.
- * Equal calls give equal bits. A row's do not depend on padding entries (q_len 0), the order of the entries, the
- * table's width or, below 256 query rows per K/V head, max_q_len; in a call of so few entries that their keys
- * are split over workgroups as well they depend on the lengths of the other entries. q and o have `tokens` rows; entries own distinct ones, and rows of no entry are not
- * written. A block outside the pool makes the rows that see it NaN; a context longer than the table is cut.
+ * lse_paged_attention over the 8-bit cache: the same plan and semantics, k and v being the values code x scale. q
+ * and o have `tokens` rows; entries own distinct ones, and rows of no entry are not written. A block outside the
+ * pool makes the rows that see it NaN; a context longer than the table is cut.
+ * Determinism: equal calls give equal bits. Which kernel takes the entries of 128 query rows per K/V head or more, and
+ *   whether keys are split over workgroups, follows from the sizes in args alone: entries, tokens, max_q_len, the
+ *   heads and the table's width. Where that comes out alike, a row's bits do not depend on padding entries
+ *   (q_len 0), the entries' order or anything behind its entry's context; where keys are split, they do depend
+ *   on the lengths of the other entries.
+ * Non-finite values: as lse_paged_attention's; infinity or NaN in a V row may reach rows of the same entry and K/V
+ *   head up to 127 query rows before it, and no others.
  * D = 64 or 128; 1 <= H / H_KV <= 16; block_size % 16 == 0; the strides of q and o multiples of 8, q, o and
  * the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes (it reads the
  * sizes in args only; -1: invalid ones), 16-byte aligned.

@@ -18,9 +18,8 @@
 
 namespace lse {
 
-constexpr int kKvGroup = 16;         // positions that share a scale
-constexpr int kKvScaleNan = 255;     // e8m0
-constexpr float kKvMaxCode = 448.0f;  // largest finite e4m3 value
+constexpr int kKvGroup = 16;      // positions that share a scale
+constexpr int kKvScaleNan = 255;  // e8m0
 
 struct Fp8Pool {
   uint8_t *k, *v, *scales;

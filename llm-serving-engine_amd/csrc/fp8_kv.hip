@@ -122,10 +122,19 @@ struct AppendArgs {
   int one;  // every entry has at most one new token
 };
 
-// Groups of 16 positions that n new tokens at `offset` touch.
-__device__ __forceinline__ int groups_of(int offset, int n) {
-  if (n <= 0 || offset < 0) return 0;
-  return (int)(((unsigned)offset + (unsigned)n - 1) / kKvGroup) - offset / kKvGroup + 1;
+// An entry's new tokens whose rows are the call's, [m0, m1), and the groups of 16 positions that they touch.
+struct NewTokens {
+  int offset, start, m0, m1;
+  __device__ __forceinline__ int first_group() const { return (int)(((unsigned)offset + (unsigned)m0) / kKvGroup); }
+  __device__ __forceinline__ int groups() const {
+    if (m0 >= m1 || offset < 0) return 0;
+    return (int)(((unsigned)offset + (unsigned)m1 - 1) / kKvGroup) - first_group() + 1;
+  }
+};
+__device__ __forceinline__ NewTokens new_tokens(const AppendArgs& a, int e) {
+  const int start = a.q_start[e];
+  return {a.query_offset[e], start, (int)min(max(-(int64_t)start, (int64_t)0), (int64_t)0x7fffffff),
+          (int)min((int64_t)a.q_len[e], a.tokens - start)};
 }
 
 // A workgroup takes one group of one K/V head: its up to 16 new tokens' k and v rows, and their rows of the G
@@ -150,7 +159,7 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
     const int lane = threadIdx.x & 63;
     for (int e0 = 0; e0 < a.entries; e0 += 64) {
       const int i = e0 + lane;
-      const int mine = i < a.entries ? groups_of(a.query_offset[i], a.q_len[i]) : 0;
+      const int mine = i < a.entries ? new_tokens(a, i).groups() : 0;
       const int before = kv_wave_scan(mine) - mine;
       const unsigned long long hit = __ballot((unsigned)(slot_id - before) < (unsigned)mine);
       if (hit) {
@@ -163,9 +172,10 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
     }
     if (e < 0) return;
   }
-  const int offset = a.query_offset[e], n = a.q_len[e], start = a.q_start[e];
-  if (n <= 0 || offset < 0) return;
-  const int group = offset / kKvGroup + first;
+  const NewTokens entry = new_tokens(a, e);
+  const int offset = entry.offset, n = entry.m1, start = entry.start;
+  if (entry.groups() == 0) return;
+  const int group = entry.first_group() + first;
   // New tokens' slots of the group: [lo, hi), slot s being token s + base of the entry.
   const int base = group * kKvGroup - offset;
   const int lo = max(0, -base), hi = min(kKvGroup, n - base);

@@ -75,7 +75,8 @@ def rotate(x: np.ndarray, cos: np.ndarray, sin: np.ndarray, positions, interleav
 
 def append(pool, k, v, table, query_offset, q_start, q_len, block_size: int) -> None:
     """Writes fp32 rows k (already rotated) and v (tokens, H_KV, D) into pool = (k codes, v codes, scales), uint8
-    arrays in the pool's layout, in place. Positions past the table and blocks outside the pool are dropped."""
+    arrays in the pool's layout, in place. Positions past the table, blocks outside the pool and rows outside k and v
+    are dropped."""
     kc, vc, scales = pool
     d, n_kv, tokens = k.shape[2], k.shape[1], k.shape[0]
     per = block_size // GROUP
@@ -92,6 +93,8 @@ def append(pool, k, v, table, query_offset, q_start, q_len, block_size: int) -> 
                 continue
             slots = [s for s in range(GROUP) if off <= g * GROUP + s < off + n]
             rows = [int(q_start[e]) + g * GROUP + s - off for s in slots]
+            if not any(0 <= r < tokens for r in rows):
+                continue
             lo = slots[0]
             for what, (codes, rows_of, index) in enumerate(((kc, k, k_index), (vc, v, v_index))):
                 for h in range(n_kv):

@@ -213,6 +213,15 @@ def test_what_is_dropped_and_what_stays(pkg, dev):
     same_pool(pool_to_host(pool), _want(case, None, None))
 
 
+@pytest.mark.parametrize("start", [150, 90, -70, -300])
+def test_rows_outside_take_no_other_entrys_place(pkg, dev, start):
+    """An entry of many rows outside the call's, before entries whose rows all lie inside."""
+    case = _append_case(10, [(100, 7), (5, 40), (60, 3), (1, 0)])
+    case["qs"][0] = start
+    q, pool = _append(pkg, dev, case, None, None)
+    same_pool(pool_to_host(pool), _want(case, None, None))
+
+
 def test_padding_rows_and_entries(pkg, dev):
     """A graph bucket: entries of no tokens behind the real ones, rows of no entry, a table as wide as the
     pool, a larger max_q_len."""
