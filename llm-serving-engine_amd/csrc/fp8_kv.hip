@@ -46,34 +46,41 @@ __device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
   }
 }
 
-// The 16 dims of a unit as two runs of eight, rotated to `pos`. A position outside the tables gives NaN.
-__device__ __forceinline__ void rotated_unit(const uint16_t* row, const RopeTables& r, const UnitDims& u,
-                                             int unit, int pos, float (&x)[8], float (&y)[8]) {
-#pragma clang fp contract(off)
-  unpack8(*reinterpret_cast<const uint4*>(row + u.a), x);
-  unpack8(*reinterpret_cast<const uint4*>(row + u.b), y);
-  if (!u.turned) return;
+// The cosines and sines of a unit's eight pairs at `pos`; of a position outside the tables NaN.
+struct Turn {
+  float c[8], s[8];
+};
+__device__ __forceinline__ Turn turn_at(const RopeTables& r, int unit, int pos) {
+  Turn t;
   const bool known = pos >= 0 && pos < r.rows;
   const int64_t at = (int64_t)(known ? pos : 0) * r.half + 8 * unit;
-  float c[8], s[8];
 #pragma unroll
   for (int i = 0; i < 8; i += 4) {
-    *reinterpret_cast<float4*>(c + i) = *reinterpret_cast<const float4*>(r.cos + at + i);
-    *reinterpret_cast<float4*>(s + i) = *reinterpret_cast<const float4*>(r.sin + at + i);
+    *reinterpret_cast<float4*>(t.c + i) = *reinterpret_cast<const float4*>(r.cos + at + i);
+    *reinterpret_cast<float4*>(t.s + i) = *reinterpret_cast<const float4*>(r.sin + at + i);
   }
-  const float none = __builtin_nanf("");
-  auto turn = [&](float& a, float& b, float cc, float ss) {
-    const float p = a * cc - b * ss, q = b * cc + a * ss;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    t.c[i] = known ? t.c[i] : __builtin_nanf("");
+    t.s[i] = known ? t.s[i] : __builtin_nanf("");
+  }
+  return t;
+}
+
+// Turns the 16 dims of a unit, two runs of eight.
+__device__ __forceinline__ void turn_unit(const Turn& t, bool interleaved, float (&x)[8], float (&y)[8]) {
+#pragma clang fp contract(off)
+  auto turn = [&](float& a, float& b, float c, float s) {
+    const float p = a * c - b * s, q = b * c + a * s;
     a = p, b = q;
   };
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float cc = known ? c[i] : none, ss = known ? s[i] : none;
-    if (r.interleaved) {
+    if (interleaved) {
       float(&v)[8] = i < 4 ? x : y;
-      turn(v[2 * (i & 3)], v[2 * (i & 3) + 1], cc, ss);
+      turn(v[2 * (i & 3)], v[2 * (i & 3) + 1], t.c[i], t.s[i]);
     } else {
-      turn(x[i], y[i], cc, ss);
+      turn(x[i], y[i], t.c[i], t.s[i]);
     }
   }
 }
@@ -102,8 +109,11 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeFp32Args a, int64_t total
   const RowsIn& in = is_q ? a.q : a.k;
   const int h = is_q ? head : head - a.H;
   const UnitDims d = unit_dims(a.r, unit);
+  const uint16_t* row = in.p + t * in.st + h * in.sh;
+  const uint4 lo = *reinterpret_cast<const uint4*>(row + d.a), hi = *reinterpret_cast<const uint4*>(row + d.b);
   float x[8], y[8];
-  rotated_unit(in.p + t * in.st + h * in.sh, a.r, d, unit, a.positions[t], x, y);
+  unpack8(lo, x), unpack8(hi, y);
+  if (d.turned) turn_unit(turn_at(a.r, unit, a.positions[t]), a.r.interleaved, x, y);
   uint16_t* out = (is_q ? a.q_out + (t * a.H + h) * a.D : a.k_out + (t * a.HKV + h) * a.D);
   *reinterpret_cast<uint4*>(out + d.a) = pack8(x);
   *reinterpret_cast<uint4*>(out + d.b) = pack8(y);
@@ -138,10 +148,11 @@ __device__ __forceinline__ NewTokens new_tokens(const AppendArgs& a, int e) {
 }
 
 // A workgroup takes one group of one K/V head: its up to 16 new tokens' k and v rows, and their rows of the G
-// query heads. Threads 0 .. D - 1 hold k's units (16 tokens x D / 16), the next D v's. The group's image (codes
-// in pool order) is built in LDS: what it held of earlier positions, requantised where the scale grew; the new
-// codes; zeros behind them; then it is written whole. At decode sizes this is bound by its chain of
-// dependent loads (lengths, table, scale, codes), at prompt sizes by HBM.
+// query heads. A thread has one (token, unit): of k in the first T threads, of v in the next T, and of every (256 / T)th
+// query head, whose cosines and sines are loaded once. The group's image (codes in pool order) is built in
+// LDS: what it held of earlier positions, requantised where the scale grew; the new codes; zeros behind them;
+// then it is written whole. At decode sizes this is bound by its chain of dependent loads (lengths, table, scale and
+// codes), which are issued as soon as their addresses are known, at prompt sizes by HBM.
 template <int D>
 __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
   constexpr int U = D / 16;      // units of a row
@@ -150,8 +161,13 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
   __shared__ __attribute__((aligned(16))) uint8_t image[2][16 * D];
   __shared__ float wave_max[4];
 
-  const int kvh = blockIdx.x % a.HKV;
-  int slot_id = blockIdx.x / a.HKV, e = -1, first = 0;
+  // A group's K/V heads go to one XCD (workgroups are dealt to the eight in turn), which then reads the rows of cos and
+  // sin once.
+  int kvh = blockIdx.x % a.HKV, slot_id = blockIdx.x / a.HKV, e = -1, first = 0;
+  if (!a.one) {
+    kvh = blockIdx.x / 8 % a.HKV;
+    slot_id = blockIdx.x / 8 / a.HKV * 8 + blockIdx.x % 8;
+  }
   if (a.one) {
     e = slot_id;
   } else {
@@ -180,37 +196,66 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
   const int base = group * kKvGroup - offset;
   const int lo = max(0, -base), hi = min(kKvGroup, n - base);
 
-  // The new rows, rotated; tokens of rows outside the call's are dropped.
+  // The group's place, and what it held, if it holds earlier positions.
   const int what = threadIdx.x / T, unit = threadIdx.x % U, slot = threadIdx.x % T / U;
+  const int block =
+      group < a.max_groups ? a.block_table[(int64_t)e * a.sbt + group / a.pool.per] : -1;
+  const bool held = block >= 0 && block < a.pool.blocks;  // dropped otherwise
+  const int64_t inner = (int64_t)kvh * a.pool.per + group % a.pool.per;
+
+  // The new rows; tokens of rows outside the call's are dropped.
   const int64_t row = (int64_t)start + base + slot;
-  const bool mine = what < 2 && slot >= lo && slot < hi && row >= 0 && row < a.tokens;
-  const RowsIn& in = what == 0 ? a.k : a.v;
-  RopeTables tables = a.r;
-  if (what != 0) tables.half = 0;
-  const UnitDims dims = unit_dims(tables, unit);
-  float x[8] = {}, y[8] = {};
-  if (mine)
-    rotated_unit(in.p + row * in.st + (int64_t)kvh * in.sh, tables, dims, unit,
-                 offset + base + slot, x, y);
-  if (a.q.p) {
-    const int count = (hi - lo) * a.G * U;
-    for (int i = threadIdx.x; i < count; i += 256) {
-      const int qu = i % U, h = kvh * a.G + i / U % a.G, s = lo + i / (U * a.G);
-      const int64_t t = (int64_t)start + base + s;
-      if (t < 0 || t >= a.tokens) continue;
-      const UnitDims qd = unit_dims(a.r, qu);
-      float qx[8], qy[8];
-      rotated_unit(a.q.p + t * a.q.st + (int64_t)h * a.q.sh, a.r, qd, qu, offset + base + s, qx, qy);
-      uint16_t* out = a.q_out + (t * a.H + h) * D;
-      *reinterpret_cast<uint4*>(out + qd.a) = pack8(qx);
-      *reinterpret_cast<uint4*>(out + qd.b) = pack8(qy);
+  const bool in = slot >= lo && slot < hi && row >= 0 && row < a.tokens, mine = in && what < 2;
+  const RowsIn& from = what == 0 ? a.k : a.v;
+  const UnitDims turned = unit_dims(a.r, unit);
+  const UnitDims dims = what == 0 ? turned : UnitDims{16 * unit, 16 * unit + 8, false};
+  uint4 xa = make_uint4(0, 0, 0, 0), xb = xa;
+  if (mine) {
+    const uint16_t* p = from.p + row * from.st + (int64_t)kvh * from.sh;
+    xa = *reinterpret_cast<const uint4*>(p + dims.a);
+    xb = *reinterpret_cast<const uint4*>(p + dims.b);
+  }
+  Turn turn{};
+  if (in && turned.turned && (a.q.p || what == 0)) turn = turn_at(a.r, unit, offset + base + slot);
+  uint8_t* scale_at = a.pool.scales + (int64_t)(held ? block : 0) * a.pool.ss + 2 * inner;
+  const int64_t bytes = (int64_t)(held ? block : 0) * a.pool.sb + inner * (16 * D) + 16 * (threadIdx.x % T);
+  uint8_t* at = (what == 0 ? a.pool.k : a.pool.v) + bytes;
+  // A thread's 16 bytes: k, of slot 4 i + j; v, all 16 slots of a dim.
+  const int in_slot = threadIdx.x % T / (D / 64 * 16) * 4 + threadIdx.x % T / 4 % 4;
+  uint4 kept = make_uint4(0, 0, 0, 0);
+  int old = 0;
+  if (held && what < 2 && lo > 0) {
+    old = scale_at[what];
+    if (what == 1 || in_slot < lo) kept = *reinterpret_cast<const uint4*>(at);
+  }
+  if (a.q.p && in) {
+    constexpr int P = 256 / T, B = 2;
+    for (int g0 = what; g0 < a.G; g0 += B * P) {
+      uint4 qa[B], qb[B];
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int g = min(g0 + i * P, a.G - 1);
+        const uint16_t* p = a.q.p + row * a.q.st + (int64_t)(kvh * a.G + g) * a.q.sh;
+        qa[i] = *reinterpret_cast<const uint4*>(p + turned.a);
+        qb[i] = *reinterpret_cast<const uint4*>(p + turned.b);
+      }
+#pragma unroll
+      for (int i = 0; i < B; ++i) {
+        const int g = g0 + i * P;
+        if (g >= a.G) break;
+        float qx[8], qy[8];
+        unpack8(qa[i], qx), unpack8(qb[i], qy);
+        if (turned.turned) turn_unit(turn, a.r.interleaved, qx, qy);
+        uint16_t* out = a.q_out + (row * a.H + kvh * a.G + g) * D;
+        *reinterpret_cast<uint4*>(out + turned.a) = pack8(qx);
+        *reinterpret_cast<uint4*>(out + turned.b) = pack8(qy);
+      }
     }
   }
-  if (group >= a.max_groups) return;
-  const int block = a.block_table[(int64_t)e * a.sbt + group / a.pool.per];
-  if (block < 0 || block >= a.pool.blocks) return;
-  const int64_t inner = (int64_t)kvh * a.pool.per + group % a.pool.per;
-  uint8_t* scale_at = a.pool.scales + (int64_t)block * a.pool.ss + 2 * inner;
+  if (!held) return;
+  float x[8], y[8];
+  unpack8(xa, x), unpack8(xb, y);
+  if (dims.turned) turn_unit(turn, a.r.interleaved, x, y);
 
   // k's and v's largest finite magnitudes.
   float top = 0.0f;
@@ -223,7 +268,6 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
 #pragma unroll
   for (int off = 1; off < 64; off <<= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
   if ((threadIdx.x & 63) == 0) wave_max[threadIdx.x >> 6] = top;
-  const int old = what < 2 && lo > 0 ? scale_at[what] : 0;
   __syncthreads();
   if (what < 2) {
     constexpr int W = T / 64;  // waves of k, and of v
@@ -232,15 +276,9 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
     for (int i = 1; i < W; ++i) top = fmaxf(top, wave_max[what * W + i]);
   }
   const int byte = max(kv_scale_byte(top), old == kKvScaleNan ? 0 : old);
-  const int64_t bytes = (int64_t)block * a.pool.sb + inner * (16 * D) + 16 * (threadIdx.x % T);
-  uint8_t* at = (what == 0 ? a.pool.k : a.pool.v) + bytes;
   uint4* img = reinterpret_cast<uint4*>(image[what & 1] + 16 * (threadIdx.x % T));
   if (what < 2) {
-    uint4 kept = make_uint4(0, 0, 0, 0);
-    // A thread's 16 bytes: k, of slot 4 i + j; v, all 16 slots of a dim.
-    const int in_slot = threadIdx.x % T / (D / 64 * 16) * 4 + threadIdx.x % T / 4 % 4;
     if (lo > 0 && (what == 1 || in_slot < lo)) {
-      kept = *reinterpret_cast<const uint4*>(at);
       if (byte != old) {
         const float ratio = old == kKvScaleNan ? __builtin_nanf("")
                             : byte - old > 126 ? 0.0f
@@ -372,7 +410,7 @@ int lse_append_kv_fp8(const struct lse_append_kv_fp8_args* args, void* stream) {
   a.one = x.max_q_len == 1;
   // An entry of n tokens touches at most (n + 30) / 16 groups; the entries' rows are distinct.
   const int64_t most = std::min(x.entries * ((x.max_q_len + 30) / 16), x.tokens / 16 + 2 * x.entries);
-  const int64_t blocks = (a.one ? x.entries : most) * x.H_KV;
+  const int64_t blocks = (a.one ? x.entries : lse::ceil_div(most, 8) * 8) * x.H_KV;
   if (blocks > kMax31) return LSE_E_RANGE;
   const dim3 grid((unsigned)blocks), wg(256);
   if (x.D == 64)
