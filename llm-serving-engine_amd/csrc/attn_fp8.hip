@@ -98,9 +98,10 @@ __device__ __forceinline__ void f8_merge_stream(const Fp8AttnArgs& a, const Fp8M
       make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
 
-// f8_tile's parts, a workgroup per item, K/V head and sixteenth of its (row, 4 dims) pieces. Two parts, the most common
-// number, are loaded without the repeats that fill up eight: 15 -> 10 us for 288 parts.
-constexpr int kF8TileMerges = 16;
+// f8_tile's parts, a workgroup per item, K/V head and eighth of its (row, 4 dims) pieces (16 workgroups of half the work
+// each: two us more for 288 parts). Two parts, the most common number, are loaded without the repeats that fill up
+// eight: 15 -> 10 us.
+constexpr int kF8TileMerges = 8;
 template <int D>
 __device__ __forceinline__ void f8_merge_tile(const Fp8AttnArgs& a, int block) {
   constexpr int kPieces = kF8TileRows * (D / 4) / kF8TileMerges;
@@ -111,6 +112,7 @@ __device__ __forceinline__ void f8_merge_tile(const Fp8AttnArgs& a, int block) {
   const int end_n = f8_tile_end(a, item.qo, item.ctx, qlen, item.qt);
   const int parts = f8_tile_parts(a, (end_n + 63) / 64);
   if (parts <= 1) return;
+#pragma unroll
   for (int i0 = threadIdx.x; i0 < kPieces; i0 += 256) {
     const int piece = block / a.HKV % kF8TileMerges * kPieces + i0;
     const int irow = piece / (D / 4), c4 = 4 * (piece % (D / 4));

@@ -164,31 +164,6 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
   const int tile0 = (int)((int64_t)all_tiles * part / parts);
   const int tiles = (int)((int64_t)all_tiles * (part + 1) / parts) - tile0;
 
-  // The lane's row and the last position it sees.
-  const int r = row0 + 32 * wave + n32, tok = r / G, gq = r - tok * G;
-  const int64_t row = (int64_t)qs + tok;
-  const bool row_ok = r < (int64_t)qlen * G && row >= 0 && row < a.tokens;
-  const int lim = (int)min((int64_t)qo + tok, (int64_t)end_n - 1);
-  // Keys up to here are seen by every row of the wave.
-  const int all_see = (int)min((int64_t)qo + (row0 + 32 * wave) / G, (int64_t)end_n - 1);
-
-  // A negative softmax scale moves into Q, a zero one makes Q zero (exactly), so that a maximum can be
-  // taken before the scaling.
-  const float sc = a.scale_log2 == 0.0f ? 1.0f : __builtin_fabsf(a.scale_log2);
-  bf16x8 qf[KK];
-  {
-    const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
-    const bool keep = row_ok && a.scale_log2 != 0.0f;
-    const uint16_t* qp =
-        a.q + (int64_t)(kvh * G + (row_ok ? gq : 0)) * a.sq_h + (row_ok ? row : 0) * a.sq_t + 8 * half;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      const uint4 v = *reinterpret_cast<const uint4*>(qp + 16 * kk);
-      qf[kk] = as_bf16x8(keep ? make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip)
-                              : make_uint4(0, 0, 0, 0));
-    }
-  }
-
   // The wave stages group `wave` of every tile. Lane i of 64 holds place (16-byte units) and scales of that
   // group in tile tile0 + 64 w + i, for the window w of the tile to load and the one behind it.
   const int32_t* bt = a.block_table + (int64_t)e * a.sbt;
@@ -200,6 +175,29 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
     sub = grp - bi * per;
     return bt[bi];
   };
+  int blk0 = 0, blk1 = 0, blk2 = 0, sub0 = 0, sub1 = 0, sub2 = 0;
+  if (tiles > 0) blk0 = table_at(0, sub0), blk1 = table_at(1, sub1), blk2 = table_at(2, sub2);
+
+  // The lane's row and the last position it sees.
+  const int r = row0 + 32 * wave + n32, tok = r / G, gq = r - tok * G;
+  const int64_t row = (int64_t)qs + tok;
+  const bool row_ok = r < (int64_t)qlen * G && row >= 0 && row < a.tokens;
+  const int lim = (int)min((int64_t)qo + tok, (int64_t)end_n - 1);
+  // Keys up to here are seen by every row of the wave.
+  const int all_see = (int)min((int64_t)qo + (row0 + 32 * wave) / G, (int64_t)end_n - 1);
+
+  // A negative softmax scale moves into Q, a zero one makes Q zero (exactly), so that a maximum can be
+  // taken before the scaling.
+  const float sc = a.scale_log2 == 0.0f ? 1.0f : __builtin_fabsf(a.scale_log2);
+  const bool keep = row_ok && a.scale_log2 != 0.0f;
+  uint4 qw[KK];
+  {
+    const uint16_t* qp =
+        a.q + (int64_t)(kvh * G + (row_ok ? gq : 0)) * a.sq_h + (row_ok ? row : 0) * a.sq_t + 8 * half;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) qw[kk] = *reinterpret_cast<const uint4*>(qp + 16 * kk);
+  }
+
   auto place = [&](int blk, int sub, uint32_t& off) {
     const bool bad = blk < 0 || blk >= a.pool.blocks;
     blk = bad ? 0 : blk;
@@ -209,7 +207,7 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
     return bad ? 0xffff : s;
   };
   uint32_t off0 = 0, off1 = 0;
-  int sc0 = 0, sc1 = 0, blk2 = 0, sub2 = 0;
+  int sc0 = 0, sc1 = 0;
   // The codes on their way to LDS, and the scales of these groups.
   uint4 kc[P], vc[P];
   uint32_t at_k = 0, at_v = 0;
@@ -281,6 +279,7 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
     return as_bf16x8(*reinterpret_cast<const uint4*>(vread + slot + f / DB * (32 * D) + f % DB * 512));
   };
 
+  bf16x8 qf[KK];
   f32x16 oacc[DB], cur[2], next[2], zero;  // scores: of 32-key block b, keys 16 (i / 8) + 8 half + i % 8
 #pragma unroll
   for (int i = 0; i < 16; ++i) zero[i] = 0.0f;
@@ -411,15 +410,14 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
   };
 
   if (tiles > 0) {
-    {
-      int sub0, sub1;
-      const int blk0 = table_at(0, sub0), blk1 = table_at(1, sub1);
-      blk2 = table_at(2, sub2);
-      sc0 = place(blk0, sub0, off0);
-      sc1 = place(blk1, sub1, off1);
-    }
-    load_k(0);
-    load_v();
+    // The first tile's codes are on their way before its scales are waited for.
+    sc0 = place(blk0, sub0, off0);
+    at_k = __builtin_amdgcn_readfirstlane(off0);
+    load(a.pool.k, at_k, kc);
+    load(a.pool.v, at_k, vc);
+    __builtin_amdgcn_sched_barrier(0);
+    sc1 = place(blk1, sub1, off1);
+    scale_k = scale_v = __builtin_amdgcn_readfirstlane(sc0);
 #pragma unroll
     for (int x = 0; x < 2 * P; ++x) stage_k(x >> 1, x & 1, 0);
     load_k(1);
@@ -430,6 +428,13 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
 #pragma unroll
     for (int x = 0; x < 2 * P; ++x) stage_k(x >> 1, x & 1, kSlot);
     load_k(2);
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
+      const uint4 v = qw[kk];
+      qf[kk] = as_bf16x8(keep ? make_uint4(v.x ^ flip, v.y ^ flip, v.z ^ flip, v.w ^ flip)
+                              : make_uint4(0, 0, 0, 0));
+    }
     f8_barrier();
 #pragma unroll
     for (int f = 0; f < N; ++f) {
@@ -464,8 +469,8 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
 
   const F8Halves h = f8_halves(l);
   const float sum = h.a + h.b;
-  if (!row_ok) return;
   if (parts > 1) {
+    if (!row_ok) return;
     const int64_t at = (((int64_t)rank * a.tile_parts + part) * a.HKV + kvh) * kF8TileRows + 32 * wave + n32;
     float* to = a.ws_tile_o + at * D + 4 * half;
 #pragma unroll
@@ -478,14 +483,25 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
     return;
   }
   const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;  // no key: zeros
-  uint16_t* out = a.o + (int64_t)(kvh * G + gq) * a.so_h + row * a.so_t + 4 * half;
+  // Of each 16 dims a lane has two fours, lane l ^ 32 the others: an exchange gives each eight in a row.
+  uint16_t* out = a.o + (int64_t)(kvh * G + gq) * a.so_h + row * a.so_t + 8 * half;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll
-    for (int b = 0; b < 4; ++b)
-      *reinterpret_cast<uint2*>(out + 32 * d + 8 * b) =
-          make_uint2(pack_bf16x2(oacc[d][4 * b] * inv, oacc[d][4 * b + 1] * inv),
-                     pack_bf16x2(oacc[d][4 * b + 2] * inv, oacc[d][4 * b + 3] * inv));
+    for (int b = 0; b < 4; b += 2) {
+      uint32_t w[2][2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int x = 4 * (b + i);
+        w[i][0] = pack_bf16x2(oacc[d][x] * inv, oacc[d][x + 1] * inv);
+        w[i][1] = pack_bf16x2(oacc[d][x + 2] * inv, oacc[d][x + 3] * inv);
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(w[0][i]), "+v"(w[1][i]));
+      if (row_ok)
+        *reinterpret_cast<uint4*>(out + 32 * d + 8 * b) = make_uint4(w[0][0], w[0][1], w[1][0], w[1][1]);
+    }
 }
 
 }  // namespace lse
