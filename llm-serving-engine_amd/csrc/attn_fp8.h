@@ -33,8 +33,8 @@ struct Fp8AttnArgs {
   float* ws_tile_ml;  // their max and sum [items][parts][HKV][128 rows][2]
 };
 
-// In a call that is tiled (fp8_attn_tiled, attn_fp8.hip) the row-tiled kernel takes the entries of 128 query rows per K/V
-// head or more, the key-streaming kernel the others; otherwise the latter takes all.
+// In a call that is tiled (fp8_attn_tiled, attn_fp8.hip) the row-tiled kernel takes the entries of 128 query rows per
+// K/V head or more, the key-streaming kernel the others; otherwise the latter takes all.
 constexpr int kF8LongRows = 128;
 __host__ __device__ inline bool f8_is_long(int64_t q_len, int G) { return q_len * G >= kF8LongRows; }
 

@@ -98,8 +98,8 @@ __device__ __forceinline__ void f8_merge_stream(const Fp8AttnArgs& a, const Fp8M
       make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
 }
 
-// f8_tile's parts, a workgroup per item, K/V head and eighth of its (row, 4 dims) pieces (16 workgroups of half the work
-// each: two us more for 288 parts). Two parts, the most common number, are loaded without the repeats that fill up
+// f8_tile's parts, a workgroup per item, K/V head and eighth of its (row, 4 dims) pieces (16 workgroups of half the
+// work each: two us more for 288 parts). Two parts, the most common number, are loaded without the repeats that fill up
 // eight: 15 -> 10 us.
 constexpr int kF8TileMerges = 8;
 template <int D>
@@ -178,20 +178,22 @@ static int fp8_attn_cus() {
   return cus;
 }
 
-// Whether a call's long entries go to the row-tiled kernel: where it has, as far as its sizes tell, so many items of them
-// (128 rows of a K/V head) or so many (query row, key) pairs that this is faster. Measured on MI355X, us, row-tiled /
-// key-streaming, 32 heads over 8 unless said:
-//  * fresh prompts, items: 4 x 64 tokens (64) 9.5 / 7.7, 1 x 512 (128) 19 / 17, 2 x 256 (128) 13 / 14, 1 x 1024, 24 heads
-//    (192) 30 / 30, 1 x 1024 (256) 29 / 35, 4 x 256 (256) 14 / 25, 8 x 512 (1024) 42 / 95; 8 over 8, 1 x 2048 (128) 38 / 26;
+// Whether a call's long entries go to the row-tiled kernel: where it has, as far as its sizes tell, so many items of
+// them (128 rows of a K/V head) or so many (query row, key) pairs that this is faster. Measured on MI355X, us,
+// row-tiled / key-streaming, 32 heads over 8 unless said:
+//  * fresh prompts, items: 4 x 64 tokens (64) 9.5 / 7.7, 1 x 512 (128) 19 / 17, 2 x 256 (128) 13 / 14, 1 x 1024, 24
+//    heads (192) 30 / 30, 1 x 1024 (256) 29 / 35, 4 x 256 (256) 14 / 25, 8 x 512 (1024) 42 / 95; 8 over 8, 1 x 2048
+//    (128) 38 / 26;
 //  * behind 500 positions: 512 tokens (128) 30 / 23, 1024 (256) 39 / 45, 2048 (512) 74 / 111;
-//  * behind 2000, pairs: 512 tokens (37 million) 46 / 41, 768 (59) 57 / 60, 1024 (82) 65 / 80; 8 over 8, 1024 (21) 34 / 25,
-//    2048 (50) 57 / 51; behind 8000, where the query tiles read more than the L2s hold and pairs count twice: 128 tokens
-//    (8) 26 / 26, 256 (17) 28 / 34; behind 16000: 128 (66) 57 / 75; 8 over 8, 128 (16) 35 / 32, 256 (33) 39 / 51;
+//  * behind 2000, pairs: 512 tokens (37 million) 46 / 41, 768 (59) 57 / 60, 1024 (82) 65 / 80; 8 over 8, 1024 (21) 34
+//    / 25, 2048 (50) 57 / 51; behind 8000, where the query tiles read more than the L2s hold and pairs count twice:
+//    128 tokens (8) 26 / 26, 256 (17) 28 / 34; behind 16000: 128 (66) 57 / 75; 8 over 8, 128 (16) 35 / 32, 256 (33) 39
+//    / 51;
 //  * one chunk beside 40 decoding sequences, which the two kernels share the card for: 256 tokens behind 1000 (11)
 //    36 / 36, 512 (22) 47 / 47, 735 behind 1300, 24 heads (28) 57 / 74.
-// Contexts are taken to be as long as the table, rows to be the entries' (a call with others may take the slower one). Left
-// to the kernel, which knows the lengths, the choice costs every such call more than a wrong one: a launch for either
-// outcome is 1.1 to 1.6 times as long as the right one.
+// Contexts are taken to be as long as the table, rows to be the entries' (a call with others may take the slower one).
+// Left to the kernel, which knows the lengths, the choice costs every such call more than a wrong one: a launch for
+// either outcome is 1.1 to 1.6 times as long as the right one.
 static bool fp8_attn_tiled(int64_t entries, int64_t tokens, int64_t G, int64_t HKV, int64_t max_q_len,
                            int64_t max_ctx) {
   constexpr int64_t kItems = 200, kFar = 6000, kMixed = 128;

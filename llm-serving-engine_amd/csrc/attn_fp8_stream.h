@@ -20,6 +20,10 @@
 // takes workgroups, the keys are split too (f8_unit): into ranges of one length for all entries, chosen so
 // that all ranges run at once, each leaving its state to a second kernel. With ranges of a fixed 1024 or 2048
 // keys, four sequences behind 7500 to 60000 positions took 44 + 7 us.
+//
+// On MI355X, bytes of the cache over the kernel's time: 64 sequences behind 256 to 2048 positions, 8 K/V heads of 128,
+// 25.4 us, 5.2 TB/s; heads of 64 behind 2048 to 16384, 95 us, 6.0 TB/s; four behind 15000 to 32000, 35.3 us, 5.9 TB/s,
+// and 4.6 us to add the ranges up; one behind 467 positions 6.1 us, all latency.
 #pragma once
 
 #include "attn_fp8.h"

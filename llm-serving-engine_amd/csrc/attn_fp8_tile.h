@@ -27,6 +27,14 @@
 //
 // Where a call has too few items to fill the card, each is cut into parts by its key tiles, and a second kernel
 // adds the parts' states up.
+//
+// On MI355X a tile of 64 keys takes 1.3 us in a workgroup alone on its CU, 1.7 beside another, which is the rate of a
+// large bf16 product (1260 TFLOP/s); what precedes and follows an item's tiles (finding it, three loads that
+// depend on each other, the first scores, the stores) 6.6 us. Three fresh prompts of 1285 to 1321 tokens, 32 heads
+// over 8: 58 us, 724 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 214 to 240 us (by the card),
+// 890 to 995 TFLOP/s.
+// In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or 10 parts takes 267, 328 and
+// 340 us, partial states and all.
 #pragma once
 
 #include <type_traits>

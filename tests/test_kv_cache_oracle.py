@@ -106,3 +106,51 @@ def test_table_refusals(pkg):
     for bad in ((0, 128), (24, 128), (16, 96)):
         with pytest.raises(RuntimeError):
             pkg.ops.fp8_kv_pool(4, bad[0], 8, bad[1], "cpu")
+
+
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotation_is_a_complex_product(interleaved):
+    """Pairs as complex numbers times e^{i angle}, in fp64; half pairs over whole heads also by transformers."""
+    from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
+
+    rng = np.random.default_rng(5)
+    x, positions = rng.standard_normal((7, 3, 64)), np.array([0, 1, 5, 30, 2, 9, 31])
+    for half in (32, 16, 8):
+        angle = np.arange(32)[:, None] / 100.0 ** (np.arange(half) / half)
+        got = kv.rotate(x, np.cos(angle), np.sin(angle), positions, interleaved, np.float64)
+        pair = x[..., :2 * half]
+        z = (pair[..., 0::2] + 1j * pair[..., 1::2] if interleaved else pair[..., :half] + 1j * pair[..., half:])
+        z = z * np.exp(1j * angle[positions])[:, None]
+        want = x.copy()
+        if interleaved:
+            want[..., 0:2 * half:2], want[..., 1:2 * half:2] = z.real, z.imag
+        else:
+            want[..., :half], want[..., half:2 * half] = z.real, z.imag
+        np.testing.assert_allclose(got, want, rtol=0, atol=1e-14)
+        if half == 32 and not interleaved:
+            c, s = (torch.from_numpy(np.tile(f(angle[positions]), 2))[None] for f in (np.cos, np.sin))
+            q = torch.from_numpy(x).transpose(0, 1)[None]
+            hf = apply_rotary_pos_emb(q, q, c, s)[0][0].transpose(0, 1).numpy()
+            np.testing.assert_allclose(got, hf, rtol=0, atol=1e-14)
+
+
+@pytest.mark.parametrize("pieces", [[70], [1] * 70, [5, 40, 1, 24], [16, 16, 38]])
+def test_appended_rows_come_back(pieces):
+    """Rows appended in pieces: each value is off by half a step of its code at most, once more where its group's
+    scale grew; slots behind the last and other blocks are zeros. A row in another's place is far off."""
+    rng = np.random.default_rng(len(pieces))
+    k, v = (rng.standard_normal((70, 2, 64)).astype(np.float32) for _ in range(2))
+    v[30:40] *= 50.0
+    pool = (np.zeros((9, 2, 2, 1024), np.uint8), np.zeros((9, 2, 2, 1024), np.uint8), np.ones((9, 2, 2, 2), np.uint8))
+    table, at = np.array([[7, 2, 5, 0]], np.int32), 0
+    for n in pieces:
+        kv.append(pool, k[at:at + n], v[at:at + n], table, [at], [0], [n], 32)
+        at += n
+    values = kv.unpack(pool, 32)
+    for what, x in enumerate((k, v)):
+        got = values[what][table[0]].reshape(128, 2, 64)
+        step = 2.0 ** (pool[2][..., what].astype(np.int64) - 127)[table[0]].transpose(0, 2, 1).reshape(8, 2)
+        tol = 2.0 ** -4 * np.abs(x) + 2.0 ** -9 * step[np.arange(70) // 16][..., None]
+        assert (np.abs(got[:70] - x) <= tol).all()
+        assert not got[70:].any() and not (np.abs(got[1:71] - x) <= tol).all()
+        assert not values[what][[1, 3, 4, 6, 8]].any()
