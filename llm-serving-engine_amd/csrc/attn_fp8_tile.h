@@ -418,24 +418,25 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
   };
 
   if (tiles > 0) {
-    // The first tile's codes are on their way before its scales are waited for.
+    // The first codes are on their way before the first scales are waited for; K of tile 1 goes to LDS behind the first
+    // scores.
+    uint4 k1[P];
     sc0 = place(blk0, sub0, off0);
     at_k = __builtin_amdgcn_readfirstlane(off0);
     load(a.pool.k, at_k, kc);
     load(a.pool.v, at_k, vc);
+    at_v = __builtin_amdgcn_readlane(off0, 1);
+    load(a.pool.k, at_v, k1);
     __builtin_amdgcn_sched_barrier(0);
     sc1 = place(blk1, sub1, off1);
     scale_k = scale_v = __builtin_amdgcn_readfirstlane(sc0);
+    scale_v_next = __builtin_amdgcn_readlane(sc0, 1);
 #pragma unroll
     for (int x = 0; x < 2 * P; ++x) stage_k(x >> 1, x & 1, 0);
-    load_k(1);
     mask_v(0);
 #pragma unroll
     for (int x = 0; x < 2 * P; ++x) stage_v(x >> 1, x & 1, 0);
     load_v();
-#pragma unroll
-    for (int x = 0; x < 2 * P; ++x) stage_k(x >> 1, x & 1, kSlot);
-    load_k(2);
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       const uint32_t flip = a.scale_log2 < 0.0f ? 0x80008000u : 0u;
@@ -448,6 +449,12 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
     for (int f = 0; f < N; ++f) {
       cur[f & 1] = f8_mfma32(read_k(f, 0), qf[f >> 1], f < 2 ? zero : cur[f & 1]);
     }
+    scale_k = scale_v;
+#pragma unroll
+    for (int i = 0; i < P; ++i) kc[i] = k1[i];
+#pragma unroll
+    for (int x = 0; x < 2 * P; ++x) stage_k(x >> 1, x & 1, kSlot);
+    load_k(2);
 #pragma unroll
     for (int i = 0; i < 32; ++i) mx = fmaxf(mx, cur[i >> 4][i & 15]);
     hide(0);
