@@ -455,9 +455,9 @@ int lse_append_kv_fp8(const struct lse_append_kv_fp8_args* args, void* stream);
  *   on the lengths of the other entries.
  * Non-finite values: as lse_paged_attention's; infinity or NaN in a V row may reach rows of the same entry and K/V
  *   head up to 127 query rows before it, and no others.
- * D = 64 or 128; 1 <= H / H_KV <= 16; block_size % 16 == 0; the strides of q and o multiples of 8, q, o and
- * the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes (it reads the
- * sizes in args only; -1: invalid ones), 16-byte aligned.
+ * D = 64 or 128; 1 <= H / H_KV <= 16; block_size % 16 == 0; max_blocks * block_size <= 2^30; the strides of q and
+ * o multiples of 8, q, o and the pools 16-byte aligned. workspace: lse_paged_attention_fp8_workspace_bytes bytes
+ * (it reads the sizes in args only; -1: invalid ones), 16-byte aligned.
  * Replaces: `paged_attention_forward` (src/llm_serving_engine/kernels/flash_attention.py:287-332) over a pool
  * the reference does not have.
  */

@@ -289,7 +289,8 @@ int check_sizes(const Args& x) {
       x.H_KV < 1 || x.H % x.H_KV || x.H / x.H_KV > 16 || (x.D != 64 && x.D != 128) || x.max_q_len < 0 ||
       x.max_q_len > kMax31 || x.max_blocks < 0 || x.block_size < 16 || x.block_size % 16)
     return LSE_E_SHAPE;
-  return x.block_size > kMax31 || x.max_blocks > kMax31 / x.block_size ? LSE_E_RANGE : LSE_OK;
+  // Contexts of up to 2^30 positions: the kernels round their ends up to whole tiles in 32 bits.
+  return x.block_size > kMax31 || x.max_blocks > ((int64_t)1 << 30) / x.block_size ? LSE_E_RANGE : LSE_OK;
 }
 
 lse::Fp8AttnPlan plan_of(const Args& x) {

@@ -103,6 +103,7 @@ def test_append_refusals(pkg, changes, status):
     (dict(scales=FAKE + 1), E_ALIGN), (dict(table=FAKE + 2), E_ALIGN),
     (dict(blocks=1 << 26), E_RANGE),  # a pool of 2^37 bytes a side
     (dict(max_blocks=1 << 28, t_stride=1 << 28), E_RANGE),
+    (dict(max_blocks=(1 << 26) + 1, t_stride=1 << 28), E_RANGE),
     (dict(max_blocks=500, t_stride=500), E_WORKSPACE),  # splits, and has no workspace
     (dict(entries=0), 0), (dict(tokens=0), 0), (dict(most=0), 0)])
 def test_attention_refusals(pkg, changes, status):
