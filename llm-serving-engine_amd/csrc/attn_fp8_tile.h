@@ -30,11 +30,10 @@
 //
 // On MI355X a tile of 64 keys takes 1.3 us in a workgroup alone on its CU, 1.7 beside another, which is the rate of a
 // large bf16 product (1260 TFLOP/s); what precedes and follows an item's tiles (finding it, three loads that
-// depend on each other, the first scores, the stores) 6.6 us. Three fresh prompts of 1285 to 1321 tokens, 32 heads
-// over 8: 58 us, 724 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 214 to 240 us (by the card),
-// 890 to 995 TFLOP/s.
-// In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or 10 parts takes 267, 328 and
-// 340 us, partial states and all.
+// depend on each other, the first scores, the stores) 6 us. Three fresh prompts of 1285 to 1321 tokens, 32 heads
+// over 8: 56 us, 750 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 211 to 220 us (by the card), 967 to
+// 1006 TFLOP/s. In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or 10 parts took
+// 267, 328 and 340 us, partial states and all, where whole ones took 223.
 #pragma once
 
 #include <type_traits>
@@ -362,7 +361,7 @@ __device__ __forceinline__ void f8_tile(const Fp8AttnArgs& a, int block, unsigne
     } else {
 #pragma unroll
       for (int f = 0; f < N; ++f) {
-        // Ahead of the other workgroup's wave on the SIMD: 5 % less time (64.1 against 61.3 us, three prompts).
+        // Ahead of the other workgroup's wave on the SIMD: 4 % less time (61.3 against 64.1 us, three prompts).
         if (f == 0) __builtin_amdgcn_s_setprio(1);
         if (f == kLate) reference(cur);
         next[f & 1] = f8_mfma32(fr[f % kAhead], qf[f >> 1], f < 2 ? zero : next[f & 1]);
