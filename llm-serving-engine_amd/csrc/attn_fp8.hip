@@ -181,29 +181,33 @@ static int fp8_attn_cus() {
 // Whether a call's long entries go to the row-tiled kernel: where it has, as far as its sizes tell, so many items of
 // them (128 rows of a K/V head) or so many (query row, key) pairs that this is faster. Measured on MI355X, us,
 // row-tiled / key-streaming, 32 heads over 8 unless said:
-//  * fresh prompts, items: 4 x 64 tokens (64) 9.5 / 7.7, 1 x 512 (128) 19 / 17, 2 x 256 (128) 13 / 14, 1 x 1024, 24
-//    heads (192) 30 / 30, 1 x 1024 (256) 29 / 35, 4 x 256 (256) 14 / 25, 8 x 512 (1024) 42 / 95; 8 over 8, 1 x 2048
-//    (128) 38 / 26;
-//  * behind 500 positions: 512 tokens (128) 30 / 23, 1024 (256) 39 / 45, 2048 (512) 74 / 111;
-//  * behind 2000, pairs: 512 tokens (37 million) 46 / 41, 768 (59) 57 / 60, 1024 (82) 65 / 80; 8 over 8, 1024 (21) 34
-//    / 25, 2048 (50) 57 / 51; behind 8000, where the query tiles read more than the L2s hold and pairs count twice:
-//    128 tokens (8) 26 / 26, 256 (17) 28 / 34; behind 16000: 128 (66) 57 / 75; 8 over 8, 128 (16) 35 / 32, 256 (33) 39
-//    / 51;
-//  * one chunk beside 40 decoding sequences, which the two kernels share the card for: 256 tokens behind 1000 (11)
-//    36 / 36, 512 (22) 47 / 47, 735 behind 1300, 24 heads (28) 57 / 74.
+//  * fresh prompts, items: 4 x 64 tokens (64) 8.9 / 8.0, 5 x 64 (80) 9.2 / 11.8, 4 x 128, 24 heads (96) 10.5 / 13.1,
+//    8 over 8, 6 x 128 (48) 10.0 / 8.4; 1 x 384 (96) 15.0 / 15.3, 1 x 512 (128) 17.6 / 17.4, heads of 64 13.5 / 12.3;
+//    1 x 1024, 24 heads (192) 26.6 / 29.6, 1 x 1024 (256) 28 / 35, 8 x 512 (1024) 36 / 95; 8 over 8, 1 x 2048 (128)
+//    36 / 27;
+//  * behind 300 positions: 2 x 192 (96) 17.6 / 15.3, 4 x 128 (128) 16.8 / 18.5; behind 500: 512 tokens (128)
+//    27 / 22, 768 (192) 38 / 33, 1024 (256) 37 / 45;
+//  * behind 2000, pairs: 512 tokens (37 million) 45 / 41, 768 (59) 56 / 60, 1024 (82) 65 / 80; 8 over 8, 1024 (21)
+//    35 / 25, 2048 (50) 54 / 51; behind 16000, where the query tiles read more than the L2s hold and pairs count
+//    twice: 128 (66) 59 / 76; 8 over 8, 128 (16) 37 / 33, 256 (33) 40 / 51;
+//  * one chunk beside 40 decoding sequences, which the two kernels share the card for, behind 1000: 128 tokens (6)
+//    30 / 30, 256 (11) 33 / 35, 512 (22) 41 / 47.
 // Contexts are taken to be as long as the table, rows to be the entries' (a call with others may take the slower one).
 // Left to the kernel, which knows the lengths, the choice costs every such call more than a wrong one: a launch for
 // either outcome is 1.1 to 1.6 times as long as the right one.
 static bool fp8_attn_tiled(int64_t entries, int64_t tokens, int64_t G, int64_t HKV, int64_t max_q_len,
                            int64_t max_ctx) {
-  constexpr int64_t kItems = 200, kFar = 6000, kMixed = 128;
-  constexpr double kPairs = 40e6, kPairsMixed = 20e6;
+  // Items that suffice for contexts of up to 256, of up to 512 and of more positions: where the tiles of the
+  // key-streaming kernel no longer fit the card at once, short items hardly last longer than its.
+  constexpr int64_t kItems256 = 72, kItems512 = 128, kItems = 200, kFar = 6000, kMixed = 128;
+  constexpr double kPairs = 40e6, kPairsMixed = 12e6;
   if (!f8_is_long(max_q_len, (int)G)) return false;
   // The longest entry's items, and those of all rows where the mean entry is long, else of those that short ones
   // cannot have.
   const int64_t q = std::min(max_q_len, tokens), rows = tokens * G;
   const int64_t left = rows >= entries * kF8LongRows ? rows : rows - entries * (kF8LongRows - 1);
-  if (std::max(ceil_div(q * G, (int64_t)kF8TileRows), left / kF8TileRows) * HKV >= kItems) return true;
+  const int64_t enough = max_ctx <= 256 ? kItems256 : max_ctx <= 512 ? kItems512 : kItems;
+  if (std::max(ceil_div(q * G, (int64_t)kF8TileRows), left / kF8TileRows) * HKV >= enough) return true;
   const int64_t keys = std::max<int64_t>(max_ctx - q / 2, 0);
   const double pairs = (double)rows * HKV * keys * (keys < kFar ? 1 : 2);
   return pairs >= ((entries - 1) * HKV >= kMixed ? kPairsMixed : kPairs);

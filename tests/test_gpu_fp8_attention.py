@@ -343,9 +343,11 @@ def _tiled(case, most=None):
         return False
     q, rows = min(most, tokens), tokens * g
     left = rows if rows >= entries * bound["F8LongRows"] else rows - entries * (bound["F8LongRows"] - 1)
-    if max(-(-q * g // 128), left // 128) * h_kv >= bound["Items"]:
+    room = case["table"].shape[1] * case["bs"]
+    enough = bound["Items256" if room <= 256 else "Items512" if room <= 512 else "Items"]
+    if max(-(-q * g // 128), left // 128) * h_kv >= enough:
         return True
-    keys = max(case["table"].shape[1] * case["bs"] - q // 2, 0)
+    keys = max(room - q // 2, 0)
     pairs = rows * h_kv * keys * (1 if keys < bound["Far"] else 2)
     return pairs >= (bound["PairsMixed"] if (entries - 1) * h_kv >= bound["Mixed"] else bound["Pairs"])
 
@@ -376,6 +378,15 @@ def test_parts_of_few_items(pkg, dev, entries, d):
     split too, and a long entry that has one part."""
     case = _long_case(70 + len(entries), entries, h=4, h_kv=1, d=d, block_size=64)
     check_attention(pkg, dev, case, "parts")
+
+
+@pytest.mark.parametrize("entries,h,h_kv,d,tiled", [
+    ([(64, 0, 64)] * 5, 32, 8, 64, True), ([(64, 0, 64)] * 4, 32, 8, 64, False),
+    ([(64, 300, 364)] * 8, 32, 8, 64, True), ([(64, 300, 364)] * 7, 32, 8, 64, False)])
+def test_short_prompts_on_both_sides_of_the_rule(pkg, dev, entries, h, h_kv, d, tiled):
+    case = attention_case(69, entries, h=h, h_kv=h_kv, d=d)
+    assert _tiled(case) == tiled
+    check_attention(pkg, dev, case, f"{len(entries)} prompts")
 
 
 @pytest.mark.parametrize("end", [1, 63, 64, 65, 127, 128, 129, 191, 192, 193, 385, 500])
@@ -420,7 +431,7 @@ def test_long_entries_read_nothing_behind_their_context(pkg, dev):
     np.testing.assert_array_equal(ora.f32_to_bf16_bits(o[:, 144:]), want[:, 144:])
 
 
-@pytest.mark.parametrize("h,h_kv,tiled", [(16, 1, True), (4, 1, False)])
+@pytest.mark.parametrize("h,h_kv,tiled", [(16, 1, True), (4, 1, True), (2, 1, False)])
 def test_many_entries(pkg, dev, h, h_kv, tiled):
     """More entries than a wave looks at in a step: prompts of 64 to 100 tokens among decode rows."""
     rng = np.random.default_rng(63)
