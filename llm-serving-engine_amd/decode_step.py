@@ -141,6 +141,8 @@ class DecodeRunner:
         if self.device.type != "cuda" or d not in (64, 128) or groups > 16:
             raise ValueError(f"an 8-bit cache needs a GPU, heads of 64 or 128 dims and at most 16 query heads per "
                              f"K/V head, got {self.device}, {d}, {groups}")
+        if self.model.dtype != torch.bfloat16:
+            raise ValueError(f"an 8-bit cache needs a bf16 model, got {self.model.dtype}")
         if block_size < ops.KV_GROUP or block_size % ops.KV_GROUP:
             raise ValueError(f"block_size must be a multiple of {ops.KV_GROUP}, got {block_size}")
         self.rope = self._rope_table()

@@ -101,6 +101,18 @@ def test_logits_track_the_bf16_cache(pkg, dev, when):
         tok = want.argmax(-1)
 
 
+def test_sequences_by_index(pkg, dev):
+    """Sequences given by index, in another order than their slice: the same hidden states."""
+    runner = _runner(dev)
+    runner.enable_fp8_kv()
+    runner.prefill(_tokens((3, 40), 6, dev))
+    tok = _tokens((2, 3), 7, dev)
+    want = runner.forward(tok, 40, slice(1, 3)).reshape(2, 3, -1)
+    for rows in ([2, 1], torch.tensor([2, 1], device=dev)):
+        got = runner.forward(tok.flip(0), 40, rows).reshape(2, 3, -1)
+        assert torch.equal(got.flip(0), want)
+
+
 def test_a_step_replays_from_a_graph(pkg, dev):
     """One decode step, captured; replays with eager steps between are the eager step's bits."""
     runner = _runner(dev)
@@ -137,6 +149,10 @@ def test_refusals(pkg, dev):
             call()
     with pytest.raises(ValueError, match="capacity"):
         runner.forward(_tokens((3, 2), 5, dev), 39)
+    full = _runner(dev)
+    full.model.float()
+    with pytest.raises(ValueError, match="bf16 model"):
+        full.enable_fp8_kv()
     wide = _runner(dev, num_attention_heads=32, num_key_value_heads=1, head_dim=64)
     with pytest.raises(ValueError, match="query heads"):
         wide.enable_fp8_kv()
