@@ -628,6 +628,15 @@ def _launch(dev: int, what: str, args: bytes, *more) -> None:
         _lib.check(status, what)
 
 
+# Entries of a `rope_scaling` by kind: those it needs, those it may have.
+_LONG = ("factor", "original_max_position_embeddings")
+_ROPE_SCALING = {
+    "default": ((), ()), "linear": (("factor",), ()),
+    "llama3": ((*_LONG, "low_freq_factor", "high_freq_factor"), ()),
+    "yarn": (_LONG, ("beta_fast", "beta_slow", "attention_factor")),
+}
+
+
 def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dict | None = None,
                device: torch.device | str | int | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """(cos, sin) of positions 0 .. positions - 1, each (positions, rotary / 2) fp32: what `rope` and
@@ -637,13 +646,21 @@ def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dic
     {"rope_type": "linear", "factor"}, {"rope_type": "llama3", "factor", "low_freq_factor",
     "high_freq_factor", "original_max_position_embeddings"} or {"rope_type": "yarn", "factor",
     "original_max_position_embeddings"} with yarn's optional "beta_fast", "beta_slow" and
-    "attention_factor" (which multiplies cos and sin)."""
+    "attention_factor" (which multiplies cos and sin). Other entries would change the table and are refused."""
     _require(rotary >= 2 and rotary % 2 == 0, f"rotary must be even, got {rotary}")
     _require(positions >= 1, f"a table needs at least one position, got {positions}")
+    scaling = scaling or {}
+    kind = scaling.get("rope_type", scaling.get("type", "default"))
+    if kind not in _ROPE_SCALING:
+        raise RuntimeError(f"unknown rope_type {kind!r}")
+    needs, may = _ROPE_SCALING[kind]
+    other = set(scaling) - {"rope_type", "type", "rope_theta", "partial_rotary_factor", *needs, *may}
+    _require(not other, f"unknown entries of {kind} scaling: {sorted(other)}")
+    _require(all(n in scaling for n in needs), f"{kind} scaling needs {needs}")
+    _require(scaling.get("rope_theta", theta) == theta, f"theta is {theta}, the scaling's {scaling.get('rope_theta')}")
     pair = torch.arange(0, rotary, 2, dtype=torch.float64, device=device) / rotary
     freq = 1.0 / theta ** pair
     gain = 1.0
-    kind = (scaling or {}).get("rope_type", (scaling or {}).get("type", "default"))
     if kind == "linear":
         freq = freq / scaling["factor"]
     elif kind == "llama3":
@@ -666,8 +683,6 @@ def rope_table(positions: int, rotary: int, theta: float = 10000.0, scaling: dic
         gain = scaling.get("attention_factor")
         if gain is None:
             gain = 0.1 * math.log(factor) + 1.0 if factor > 1.0 else 1.0
-    elif kind != "default":
-        raise RuntimeError(f"unknown rope_type {kind!r}")
     angle = torch.arange(positions, dtype=torch.float64, device=device)[:, None] * freq
     return (gain * torch.cos(angle)).float(), (gain * torch.sin(angle)).float()
 

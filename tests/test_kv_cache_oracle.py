@@ -108,6 +108,18 @@ def test_table_refusals(pkg):
             pkg.ops.fp8_kv_pool(4, bad[0], 8, bad[1], "cpu")
 
 
+@pytest.mark.parametrize("scaling,what", [
+    (dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=2048, mscale=0.7, mscale_all_dim=1.0), "mscale"),
+    (dict(rope_type="yarn", factor=4.0, original_max_position_embeddings=2048, truncate=False), "truncate"),
+    (dict(rope_type="yarn", factor=4.0), "needs"), (dict(rope_type="linear"), "needs"),
+    (dict(rope_type="llama3", factor=8.0, original_max_position_embeddings=8192), "needs"),
+    (dict(rope_type="linear", factor=2.0, rope_theta=500000.0), "theta"),
+    (dict(rope_type="default", rope_theta=500000.0), "theta")])
+def test_scalings_that_the_table_would_get_wrong(pkg, scaling, what):
+    with pytest.raises(RuntimeError, match=what):
+        pkg.ops.rope_table(16, 64, 10000.0, scaling)
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rotation_is_a_complex_product(interleaved):
     """Pairs as complex numbers times e^{i angle}, in fp64; half pairs over whole heads also by transformers."""
