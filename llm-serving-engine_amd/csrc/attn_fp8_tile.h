@@ -1,5 +1,6 @@
 // Paged attention over the 8-bit K/V cache (fp8_kv.h) of prompts and prompt chunks: the row-tiled kernel beside
-// attn_fp8_stream.h's key-streaming one, with the same semantics. It takes every entry that f8_is_long.
+// attn_fp8_stream.h's key-streaming one, with the same semantics. It takes the entries that f8_is_long of calls
+// that are tiled (fp8_attn_tiled, attn_fp8.hip).
 //
 // A workgroup of four waves owns 128 rows (tokens x the G query heads of one K/V head, token-major, so no G
 // leaves rows idle), each wave 32 of them on v_mfma_f32_32x32x16_bf16, over tiles of 64 keys:
@@ -31,8 +32,8 @@
 // On MI355X a tile of 64 keys takes 1.3 us in a workgroup alone on its CU, 1.7 beside another, which is the rate of a
 // large bf16 product (1260 TFLOP/s); what precedes and follows an item's tiles (finding it, three loads that
 // depend on each other, the first scores, the stores) 6 us. Three fresh prompts of 1285 to 1321 tokens, 32 heads
-// over 8: 56 us, 750 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 211 to 220 us (by the card), 967 to
-// 1006 TFLOP/s. In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or 10 parts took
+// over 8: 56 us, 750 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 207 to 220 us (by the card), 967 to
+// 1030 TFLOP/s. In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or 10 parts took
 // 267, 328 and 340 us, partial states and all, where whole ones took 223.
 #pragma once
 
