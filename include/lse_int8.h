@@ -413,8 +413,9 @@ int lse_rope(const struct lse_rope_args* args, void* stream);
  *   scale of a group = the smallest power of two s >= 2^-126 with |x| <= 448 s for every finite new x (k
  *     after its rotation, in fp32), and no less than the group's former scale where it holds positions
  *     before query_offset[e]; those are kept, requantised if the scale grew;
- *   code = rne_e4m3(x / s); infinity and NaN become NaN. Slots behind the last new position of a group are
- *     zeroed, other groups are not touched.
+ *   code = rne_e4m3(x / s), but none that stands for 2^128 (at s = 2^120, which |x| above 224 x 2^120 takes, 240 is the
+ *     largest); infinity and NaN become NaN. Slots behind the last new position of a group are zeroed, other groups
+ *     are not touched.
  * q (may be NULL), k, v: bf16, element (t, h, d) at t * stride_t + h * stride_h + d. q_out: (tokens, H, D)
  *   bf16; rows of no entry are not written. Positions outside the table's max_blocks blocks, blocks outside
  *   the pool and rows outside the `tokens` rows are dropped; a group of none but such is not touched. Entries

@@ -20,6 +20,7 @@ namespace lse {
 
 constexpr int kKvGroup = 16;      // positions that share a scale
 constexpr int kKvScaleNan = 255;  // e8m0
+constexpr int kKvScaleTop = 247;  // 2^120: the largest scale of finite values, and the first that some codes make infinite
 
 struct Fp8Pool {
   uint8_t *k, *v, *scales;
@@ -56,6 +57,19 @@ __device__ __forceinline__ bf16x8 kv_decode8(uint32_t lo, uint32_t hi, float sca
 __device__ __forceinline__ uint32_t kv_encode4(float a, float b, float c, float d) {
   int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
+}
+
+// Four codes of values below 2^128 at a scale from kKvScaleTop on: those rounded up to 2^128, infinity in bf16, become
+// the largest code below it, less than 2^-4 of the value away (240 for 255.99 at 2^120). NaN stays.
+__device__ __forceinline__ uint32_t kv_keep_finite4(uint32_t w, int byte) {
+  const uint32_t most = 8 * (262 - byte) - 1;  // 2^(255 - byte) is code 8 (262 - byte)
+  uint32_t out = 0;
+#pragma unroll
+  for (int i = 0; i < 32; i += 8) {
+    const uint32_t c = w >> i & 0x7f;
+    out |= (c == 0x7f ? c : min(c, most)) << i;
+  }
+  return out | (w & 0x80808080u);
 }
 
 // Four codes times `ratio` (a power of two up to 1), as codes.

@@ -306,10 +306,14 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
   __syncthreads();
   if (mine) {
     const float inv = kv_scale_inverse(byte);
-    const uint32_t c[4] = {kv_encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
-                           kv_encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv),
-                           kv_encode4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
-                           kv_encode4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)};
+    uint32_t c[4] = {kv_encode4(x[0] * inv, x[1] * inv, x[2] * inv, x[3] * inv),
+                     kv_encode4(x[4] * inv, x[5] * inv, x[6] * inv, x[7] * inv),
+                     kv_encode4(y[0] * inv, y[1] * inv, y[2] * inv, y[3] * inv),
+                     kv_encode4(y[4] * inv, y[5] * inv, y[6] * inv, y[7] * inv)};
+    if (__builtin_expect(byte >= kKvScaleTop, 0)) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) c[i] = kv_keep_finite4(c[i], byte);
+    }
     if (what == 0) {
       auto put = [&](int d, uint32_t w0, uint32_t w1) {
         uint8_t* to = image[0] + ((slot / 4 * (D / 64) + d / 64) * 4 + slot % 4) * 64 + d % 64;

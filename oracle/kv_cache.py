@@ -51,6 +51,15 @@ def scale_byte(amax: np.ndarray) -> np.ndarray:
     return out
 
 
+def keep_finite(codes: np.ndarray, byte: int) -> np.ndarray:
+    """Codes of finite values at the scale 2^(byte - 127): those that stand for 2^128 or more, infinity in fp32 and
+    bf16, become the largest that does not. NaN stays."""
+    below = E4M3[:127] * 2.0 ** (byte - 127) < 2.0 ** 128
+    most = np.flatnonzero(below)[-1]
+    size = codes & 127
+    return np.where((size != 127) & (size > most), codes & 128 | most, codes).astype(np.uint8)
+
+
 def k_index(slot, d, dim: int):
     return ((slot // 4 * (dim // 64) + d // 64) * 4 + slot % 4) * 64 + d % 64
 
@@ -112,7 +121,7 @@ def append(pool, k, v, table, query_offset, q_start, q_len, block_size: int) -> 
                             was = encode(E4M3[was] * ratio)
                         image[index(s, dims, d)] = was
                     for s, x in new.items():
-                        image[index(s, dims, d)] = encode(x.astype(np.float64) * 2.0 ** (127 - byte))
+                        image[index(s, dims, d)] = keep_finite(encode(x.astype(np.float64) * 2.0 ** (127 - byte)), byte)
                     codes[block, h, sub] = image
                     scales[block, h, sub, what] = byte
 
