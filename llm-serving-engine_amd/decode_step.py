@@ -113,28 +113,28 @@ class DecodeRunner:
         if self.fp8_kv is not None:
             raise RuntimeError("the K/V cache is 8-bit")
         dev = self.device
-        num_blocks = self._deal_blocks(block_size, seed)
+        self.tables, num_blocks = self._deal_blocks(block_size, seed)
+        self.block_size = block_size
         shape = (num_blocks + 1, block_size, self.n_kv, self.head_dim)
         self.k_pool = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         self.v_pool = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         for i in range(len(self.layers)):
             self._write_pool(i, self.k_cache[i], self.v_cache[i], 0, self.capacity, slice(None))
 
-    def _deal_blocks(self, block_size: int, seed: int) -> int:
-        """Block tables of `capacity` positions a sequence, in shuffled order; the number of blocks."""
+    def _deal_blocks(self, block_size: int, seed: int) -> tuple[torch.Tensor, int]:
+        """Block tables of `capacity` positions a sequence, in shuffled order, and the number of blocks."""
         per_seq = -(-self.capacity // block_size)
         num_blocks = self.batch * per_seq
         g = torch.Generator().manual_seed(seed)
         perm = torch.randperm(num_blocks, generator=g)
-        self.block_size = block_size
-        self.tables = perm.reshape(self.batch, per_seq).to(torch.int32).to(self.device)
-        return num_blocks
+        return perm.reshape(self.batch, per_seq).to(torch.int32).to(self.device), num_blocks
 
     @torch.no_grad()
     def enable_fp8_kv(self, block_size: int = 16, seed: int = 0) -> None:
         """Holds K/V in an 8-bit paged pool per layer (about half the bytes) from here on: what the contiguous
         cache holds is copied in, it and the bf16 pools are freed, and attention is "paged-fp8". Call before
-        prefill, or after."""
+        prefill, or after. The old caches are freed once the new ones are whole, so both have to fit the card; a
+        call that fails, for want of memory or on its arguments, leaves the runner as it was."""
         if self.fp8_kv is not None:
             raise RuntimeError("the K/V cache is 8-bit already")
         d, groups = self.head_dim, self.n_heads // self.n_kv
@@ -145,19 +145,19 @@ class DecodeRunner:
             raise ValueError(f"an 8-bit cache needs a bf16 model, got {self.model.dtype}")
         if block_size < ops.KV_GROUP or block_size % ops.KV_GROUP:
             raise ValueError(f"block_size must be a multiple of {ops.KV_GROUP}, got {block_size}")
-        self.rope = self._rope_table()
-        num_blocks = self._deal_blocks(block_size, seed)
+        rope = self._rope_table()
+        tables, num_blocks = self._deal_blocks(block_size, seed)
+        pools = [ops.fp8_kv_pool(num_blocks, block_size, self.n_kv, d, self.device) for _ in self.layers]
+        full = lambda v: torch.full((self.batch,), v, dtype=torch.int32, device=self.device)  # noqa: E731
+        q_start = torch.arange(0, self.batch * self.capacity, self.capacity, dtype=torch.int32, device=self.device)
+        plan = tables, full(0), q_start, full(self.capacity), self.capacity
+        for pool, *cache in zip(pools, self.k_cache, self.v_cache):
+            k, v = (c.transpose(1, 2).reshape(-1, self.n_kv, d) for c in cache)
+            ops.append_kv_fp8(None, k, v, None, None, pool, *plan)
+        # Nothing of the runner has changed up to here, and nothing can fail from here on.
+        self.rope, self.tables, self.block_size, self.fp8_kv = rope, tables, block_size, pools
         self.k_pool = self.v_pool = None
-        self._rows = slice(None)
-        plan = self._paged_plan(0, self.capacity, self.batch, self.capacity)
-        pools = []
-        for i in range(len(self.layers)):
-            pools.append(ops.fp8_kv_pool(num_blocks, block_size, self.n_kv, d, self.device))
-            k, v = (c[i].transpose(1, 2).reshape(-1, self.n_kv, d) for c in (self.k_cache, self.v_cache))
-            self.k_cache[i] = self.v_cache[i] = None
-            table, _, offset, q_start, q_len, ntok = plan
-            ops.append_kv_fp8(None, k, v, None, None, pools[i], table, offset, q_start, q_len, ntok)
-        self.fp8_kv = pools
+        self.k_cache, self.v_cache = ([None] * len(self.layers) for _ in range(2))
         self.attention = "paged-fp8"
 
     def _rope_table(self) -> tuple[torch.Tensor, torch.Tensor]:
