@@ -801,7 +801,7 @@ def summarize_profiles(trace_dir: str, fetch_dir: str, write_dir: str) -> None:
         "fetch_factor": round(ff, 4),
         "write_factor": round(wf, 4),
         "median_us_per_call": round(avg_t, 3),
-        "library_sources_sha16": library_sources_digest(),
+        "sweep_sources_sha16": sweep_sources_digest(),
     }, indent=1) + "\n")
     print("\n".join(out))
 
@@ -1207,27 +1207,31 @@ def collections_by_dispatch(rows: list[dict], kernel: str) -> list[dict]:
     return [by[d] for d in sorted(by)]
 
 
-def library_sources_digest() -> str:
-    """First 16 hex digits of the SHA-256 over the HIP sources (file names and contents, sorted):
-    a PMC traffic figure is only reported for the library build it was measured on."""
+# What the kernels of the decode sweep, and the choice among them, are compiled from.
+SWEEP_SOURCES = ("api.hip", "lse_common.h", "skinny.hip", "tiled.hip", "xsplit.hip")
+
+
+def sweep_sources_digest(csrc: Path = CSRC) -> str:
+    """First 16 hex digits of the SHA-256 over the sweep's sources (file names and contents): a PMC traffic figure
+    is only reported for the kernels it was measured on, whatever else the library holds."""
     h = hashlib.sha256()
-    for f in sorted(CSRC.glob("*.hip")) + sorted(CSRC.glob("*.h")):
-        h.update(f.name.encode())
-        h.update(f.read_bytes())
+    for name in SWEEP_SOURCES:
+        h.update(name.encode())
+        h.update((csrc / name).read_bytes())
     return h.hexdigest()[:16]
 
 
 def measured_traffic(dec: dict) -> tuple[float | None, str]:
     """(HBM bytes per decode launch from the committed PMC summary of this same sweep, or None;
-    why None). The summary counts only if it covers the same launches and was measured on a
-    library built from the current sources."""
+    why None). The summary counts only if it covers the same launches and was measured on
+    kernels built from the current sources."""
     try:
         t = json.loads(PROFILE_TRAFFIC.read_text())
     except (OSError, ValueError):
         return None, f"no readable {PROFILE_TRAFFIC.name}"
     if t.get("calls") != dec["launches_per_step"]:
         return None, "the PMC summary covers another set of launches"
-    if t.get("library_sources_sha16") != library_sources_digest():
+    if t.get("sweep_sources_sha16") != sweep_sources_digest():
         return None, "the PMC summary was measured on another build of the kernels"
     return t["hbm_bytes_per_call"], ""
 
