@@ -418,8 +418,10 @@ int lse_rope(const struct lse_rope_args* args, void* stream);
  *     are not touched.
  * q (may be NULL), k, v: bf16, element (t, h, d) at t * stride_t + h * stride_h + d. q_out: (tokens, H, D)
  *   bf16; rows of no entry are not written. Positions outside the table's max_blocks blocks, blocks outside
- *   the pool and rows outside the `tokens` rows are dropped; a group of none but such is not touched. Entries
- *   must own distinct rows, and the blocks they write to must be theirs alone. max_q_len >= every q_len.
+ *   the pool, entries of a negative query_offset and rows outside the `tokens` rows are dropped: their q rows are
+ *   rotated all the same (as lse_rope's, to NaN where the tables lack the position), k and v are not written, and a
+ *   group of none but such is not touched. Entries must own distinct rows, and the blocks they write to must be
+ *   theirs alone. max_q_len >= every q_len.
  * D = 64 or 128; block_size % 16 == 0; strides of rows multiples of 8, pool_stride_block of 16; rows, tables
  *   and pools 16-byte aligned.
  * Replaces: apply_rotary_pos_emb and the K/V writes in `_project_qkv` and `attend_paged`

@@ -137,15 +137,19 @@ struct AppendArgs {
   int one;  // every entry has at most one new token
 };
 
-// An entry's new tokens whose rows are the call's, [m0, m1), and the groups of 16 positions that they touch.
+// An entry's new tokens whose rows are the call's, [m0, m1), and the groups of 16 positions that they touch: where the
+// offset is negative, those before position 0 too, whose q rows are the call's as well. Groups are counted from the
+// one of the offset, in which that is slot `lead`.
 struct NewTokens {
   int offset, start, m0, m1;
-  __device__ __forceinline__ int first_group() const { return (int)(((unsigned)offset + (unsigned)m0) / kKvGroup); }
+  __device__ __forceinline__ int offset_group() const { return offset >> 4; }
+  __device__ __forceinline__ int lead() const { return offset & 15; }
+  __device__ __forceinline__ int first() const { return (int)(((unsigned)lead() + (unsigned)m0) >> 4); }
   __device__ __forceinline__ int groups() const {
-    if (m0 >= m1 || offset < 0) return 0;
-    return (int)(((unsigned)offset + (unsigned)m1 - 1) / kKvGroup) - first_group() + 1;
+    return m0 >= m1 ? 0 : (int)(((unsigned)lead() + (unsigned)m1 - 1) >> 4) - first() + 1;
   }
 };
+static_assert(kKvGroup == 16, "groups by shifts");
 __device__ __forceinline__ NewTokens new_tokens(const AppendArgs& a, int e) {
   const int start = a.q_start[e];
   return {a.query_offset[e], start, (int)min(max(-(int64_t)start, (int64_t)0), (int64_t)0x7fffffff),
@@ -198,15 +202,15 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
   const NewTokens entry = new_tokens(a, e);
   const int offset = entry.offset, n = entry.m1, start = entry.start;
   if (entry.groups() == 0) return;
-  const int group = entry.first_group() + first;
+  const int run = entry.first() + first, group = entry.offset_group() + run;
   // New tokens' slots of the group: [lo, hi), slot s being token s + base of the entry.
-  const int base = group * kKvGroup - offset;
-  const int lo = max(0, -base), hi = min(kKvGroup, n - base);
+  const int base = run * kKvGroup - entry.lead();
+  const int lo = max(0, -base), hi = (int)min((int64_t)kKvGroup, (int64_t)n - base);
 
   // The group's place, and what it held, if it holds earlier positions.
   const int what = threadIdx.x / T, unit = threadIdx.x % U, slot = threadIdx.x % T / U;
   const int block =
-      group < a.max_groups ? a.block_table[(int64_t)e * a.sbt + group / a.pool.per] : -1;
+      offset >= 0 && group < a.max_groups ? a.block_table[(int64_t)e * a.sbt + group / a.pool.per] : -1;
   const bool held = block >= 0 && block < a.pool.blocks;  // dropped otherwise
   const int64_t inner = (int64_t)kvh * a.pool.per + group % a.pool.per;
 
@@ -223,7 +227,7 @@ __global__ void __launch_bounds__(256) append_kv_kernel(AppendArgs a) {
     xb = *reinterpret_cast<const uint4*>(p + dims.b);
   }
   Turn turn{};
-  if (in && turned.turned && (a.q.p || what == 0)) turn = turn_at(a.r, unit, offset + base + slot);
+  if (in && turned.turned && (a.q.p || what == 0)) turn = turn_at(a.r, unit, (int)((unsigned)group * kKvGroup + slot));
   uint8_t* scale_at = a.pool.scales + (int64_t)(held ? block : 0) * a.pool.ss + 2 * inner;
   const int64_t bytes = (int64_t)(held ? block : 0) * a.pool.sb + inner * (16 * D) + 16 * (threadIdx.x % T);
   uint8_t* at = (what == 0 ? a.pool.k : a.pool.v) + bytes;

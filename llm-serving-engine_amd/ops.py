@@ -838,8 +838,9 @@ def append_kv_fp8(
     block_table[e] names; entries own their rows and the blocks they write to. A group of 16 positions
     takes the smallest power-of-two scale that keeps its finite values within 448 scales; positions it held
     before are requantised when its scale grows, and slots behind the last new one are zeroed. Infinities
-    and NaN are held as NaN. Positions outside the table, blocks outside the pool and rows outside q, k
-    and v are dropped. Returns the rotated q (tokens, H, D), of which rows of no entry are not written."""
+    and NaN are held as NaN. Positions outside the table, blocks outside the pool, entries of a negative
+    query_offset and rows outside q, k and v are dropped: their k and v are not written. Returns the rotated q
+    (tokens, H, D), of which rows of no entry are not written."""
     dev = _one_gpu(k, v, *pool, block_table, query_offset, q_start, q_len)
     blocks, n_kv, per, d, stride, s_stride = _check_fp8_pool(pool)
     entries, width, t_stride = _check_plan(block_table, query_offset, q_start, q_len)
