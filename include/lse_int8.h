@@ -84,7 +84,7 @@ enum lse_query_key {
   LSE_Q_NOALLOC_SCRATCH = 5, /* bytes of the static scratch lse_w8a16_gemm_noalloc works in */
 };
 
-#define LSE_ABI_VERSION 14
+#define LSE_ABI_VERSION 15
 #define LSE_NOALLOC_SCRATCH_BYTES (32 << 20)
 #define LSE_K_ALIGN 16
 #define LSE_DECODE_MAX_M 64
@@ -481,6 +481,11 @@ struct lse_paged_attention_fp8_args {
 int64_t lse_paged_attention_fp8_workspace_bytes(const struct lse_paged_attention_fp8_args* args);
 int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, void* workspace,
                             int64_t workspace_bytes, void* stream);
+/* What such a call would run, from the sizes in args alone: row_tiled 1 where the row-tiled kernel takes the entries of
+ * 128 query rows per K/V head or more, in up to `parts` parts each (0 where it takes none); units > 0 where the other
+ * entries' keys are split, into at most that many ranges a K/V head. */
+int lse_paged_attention_fp8_choice(const struct lse_paged_attention_fp8_args* args, int64_t* row_tiled,
+                                   int64_t* parts, int64_t* units);
 
 /* Static properties (enum lse_query_key); -1 for an unknown key. Load-time checks read these,
  * as `ModelRunner.check_custom_kernel_support` (model_runner.py:77-94) checks its kernels. */

@@ -311,6 +311,16 @@ int64_t lse_paged_attention_fp8_workspace_bytes(const struct lse_paged_attention
   return plan_of(*args).ws_bytes;
 }
 
+int lse_paged_attention_fp8_choice(const struct lse_paged_attention_fp8_args* args, int64_t* row_tiled,
+                                   int64_t* parts, int64_t* units) {
+  if (!args || !row_tiled || !parts || !units) return LSE_E_NULL;
+  if (int st = check_sizes(*args)) return st;
+  const bool empty = args->entries == 0 || args->tokens == 0 || args->max_q_len == 0;
+  const lse::Fp8AttnPlan pl = empty ? lse::Fp8AttnPlan{} : plan_of(*args);
+  *row_tiled = pl.tiled, *parts = pl.tiled ? pl.tile_parts : 0, *units = pl.slots;
+  return LSE_OK;
+}
+
 int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, void* workspace,
                             int64_t workspace_bytes, void* stream) {
   if (!args) return LSE_E_NULL;
