@@ -16,7 +16,7 @@ struct Fp8AttnArgs {
   const int32_t *context_len, *query_offset, *q_start, *q_len;
   uint16_t* o;  // bf16, same indexing as q with strides so_h, so_t
   int64_t so_h, so_t;
-  int entries, H, HKV, G, tokens;
+  int entries, HKV, G, tokens;
   int max_ctx;       // positions that the table has room for
   int max_q_len;
   int tiled;         // the row-tiled kernel takes the long entries

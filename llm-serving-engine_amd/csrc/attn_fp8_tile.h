@@ -32,9 +32,9 @@
 // On MI355X a tile of 64 keys takes 1.3 us in a workgroup alone on its CU, 1.7 beside another, which is the rate of a
 // large bf16 product (1260 TFLOP/s); what precedes and follows an item's tiles (finding it, three loads that
 // depend on each other, the first scores, the stores) 6 us. Three fresh prompts of 1285 to 1321 tokens, 32 heads
-// over 8: 56 us, 750 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 207 to 220 us, by the card, 967 to
-// 1030 TFLOP/s. In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or 10 parts took
-// 267, 328 and 340 us, partial states and all, where whole ones took 223.
+// over 8: 56 to 57 us, by the card, 720 to 750 TFLOP/s of the causal half; 1813 tokens behind 6266 positions: 207 to
+// 222 us, 960 to 1030 TFLOP/s. In the latter 56 of 256 CUs have one item instead of two, but every item cut into 4, 9 or
+// 10 parts took 267, 328 and 340 us, partial states and all, where whole ones took 223.
 #pragma once
 
 #include <type_traits>

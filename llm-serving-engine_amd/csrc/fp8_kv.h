@@ -6,7 +6,8 @@
 // 255 = NaN). With a floating code a power of two loses nothing against any other scale, since the codes'
 // relative precision is the same everywhere in their range, and it makes everything but the one rounding
 // exact: code x scale is a bf16 value (the hardware's scaled conversion gives it in half an instruction a
-// value), and a group whose scale grows keeps its codes but for those that fall below the smallest normal.
+// value; at the three scales below 2^-124 the smallest codes are rounded to bf16's subnormals, steps of 2^-133),
+// and a group whose scale grows keeps its codes but for those that fall below the smallest normal.
 //
 // k and v: (blocks, H_KV, S, 16 D) bytes, S = block_size / 16 groups in a block; scales: (blocks, H_KV, S, 2).
 // A group's bytes lie in the order in which the matrix cores take them as 16 contiguous bytes of a lane:
@@ -42,8 +43,8 @@ __device__ __forceinline__ float kv_scale_inverse(int byte) {
   return __builtin_bit_cast(float, byte < 254 ? (uint32_t)(254 - byte) << 23 : 0x00400000u);
 }
 
-// Eight codes to bf16, times a power of two; exact (v_cvt_scalef32_pk_bf16_fp8: of `scale` it takes the
-// exponent field as an e8m0 byte, so kv_scale of bytes 0 and 255, 2^-127 and NaN, serves too).
+// Eight codes to bf16, times a power of two; exact but for bf16's subnormals (v_cvt_scalef32_pk_bf16_fp8: of `scale`
+// it takes the exponent field as an e8m0 byte, so kv_scale of bytes 0 and 255, 2^-127 and NaN, serves too).
 __device__ __forceinline__ bf16x8 kv_decode8(uint32_t lo, uint32_t hi, float scale) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false);

@@ -8,8 +8,8 @@
 //
 // A thread's unit is 16 dims of a token's head: eight pairs, or 16 dims to pass on.
 //
-// On MI355X: a batch of three prompts (about 4000 tokens, 32 heads over 8 of 128) is rotated in 17.9 us (4.5 TB/s of
-// values and tables in and out) and appended in 21.9 us (4.6 TB/s); one decode row, and 64, take 2.6 and 6.9 us on the
+// On MI355X: a batch of three prompts (about 4000 tokens, 32 heads over 8 of 128) is rotated in 18.1 us (4.5 TB/s of
+// values and tables in and out) and appended in 21.9 us (4.6 TB/s); one decode row, and 64, take 2.7 and 7.1 us on the
 // GPU, less than their launches.
 #include <algorithm>
 

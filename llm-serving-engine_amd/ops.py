@@ -773,7 +773,8 @@ def fp8_kv_pool(num_blocks: int, block_size: int, n_kv: int, d: int,
 
 def unpack_fp8_kv(pool: Fp8KV) -> tuple[torch.Tensor, torch.Tensor]:
     """The values a pool stands for, as two bf16 (blocks, block_size, H_KV, D) tensors (the layout of
-    `paged_attention_forward`'s pools; exact, done with torch operations)."""
+    `paged_attention_forward`'s pools; exact but for values below 2^-126, which bf16 holds in steps of 2^-133;
+    done with torch operations)."""
     blocks, n_kv, per, size = pool.k.shape
     d = size // KV_GROUP
     k = pool.k.view(torch.uint8).reshape(blocks, n_kv, per, 4, d // 64, 4, 64).transpose(4, 5)

@@ -107,3 +107,20 @@ def test_infinities_and_nan_are_nan_beside_them(pkg, dev):
         got = got[1].double().cpu().numpy()
         np.testing.assert_array_equal(np.isnan(got), ~np.isfinite(x))
         assert np.isfinite(got[np.isfinite(x)]).all()
+
+
+@pytest.mark.parametrize("byte", [0, 1, 2, 3, 4, 127, 246])
+def test_what_a_code_stands_for(pkg, dev, byte):
+    """Attention over one key gives its V row: code x scale exactly from a scale of 2^-124 on, below that rounded to
+    bf16's subnormals, whose step is 2^-133; the same as unpacking."""
+    pool = pkg.ops.fp8_kv_pool(1, 16, 2, 128, dev)
+    codes = torch.arange(256, dtype=torch.uint8, device=dev).view(2, 128)
+    codes = torch.where(codes & 127 == 127, torch.zeros_like(codes), codes)
+    pool.v.view(torch.uint8).view(1, 2, 1, 128, 16)[0, :, 0, :, 0] = codes
+    pool.scales.view(torch.uint8).fill_(byte)
+    q = torch.zeros(2, 1, 128, dtype=torch.bfloat16, device=dev)
+    one, zero = i32([1], dev), i32([0], dev)
+    o = pkg.ops.paged_attention_fp8(q, pool, i32([[0]], dev), one, zero, zero, one, 1)
+    exact = codes.view(torch.float8_e4m3fn).double() * 2.0 ** (byte - 127)
+    assert ((o[:, 0].double() - exact).abs() <= (0.0 if byte >= 3 else 2.0 ** -134)).all()
+    assert torch.equal(o[:, 0], pkg.ops.unpack_fp8_kv(pool)[1][0, 0])
