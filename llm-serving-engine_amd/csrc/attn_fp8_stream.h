@@ -36,8 +36,8 @@ constexpr int kF8Round = kF8Keys * kF8Waves;
 constexpr int kF8Window = 4 * kF8Round;  // keys of four tiles of every wave, whose blocks and scales it holds
 // Workgroups of a split launch, two per CU: for heads of 128 all there is room for (204 registers; with 168, three, the
 // kernel spills: four sequences behind 7500 to 60000 positions 42 -> 54 us), and with twice as many, half of them wait
-// (48 us). Heads of 64 have room for twice as many, which gains 5 to 10 % where ranges are short (16 sequences behind
-// 2000 to 8192 positions 21.0 -> 20.4 us, 32 37.7 -> 35.1) and loses as much where they are long (4 behind 24000 to 60000
+// (48 us). Heads of 64 have room for twice as many, which gains 3 to 10 % where ranges are short (16 sequences behind
+// 2000 to 8192 positions 21.0 -> 20.4 us, 32 37.7 -> 35.1) and loses 10 to 15 % where they are long (4 behind 24000 to 60000
 // 34.0 -> 39.1, 16 behind 4000 to 32768 56 -> 62), so it is the same for both.
 constexpr int kF8Groups = 512;
 // Fewest keys of a range, and contexts up to which nothing is split: a wave takes 0.5 us a tile, the second
