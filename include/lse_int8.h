@@ -84,7 +84,7 @@ enum lse_query_key {
   LSE_Q_NOALLOC_SCRATCH = 5, /* bytes of the static scratch lse_w8a16_gemm_noalloc works in */
 };
 
-#define LSE_ABI_VERSION 15
+#define LSE_ABI_VERSION 16
 #define LSE_NOALLOC_SCRATCH_BYTES (32 << 20)
 #define LSE_K_ALIGN 16
 #define LSE_DECODE_MAX_M 64
@@ -486,6 +486,82 @@ int lse_paged_attention_fp8(const struct lse_paged_attention_fp8_args* args, voi
  * entries' keys are split, into at most that many ranges a K/V head. */
 int lse_paged_attention_fp8_choice(const struct lse_paged_attention_fp8_args* args, int64_t* row_tiled,
                                    int64_t* parts, int64_t* units);
+
+/*
+ * 4-bit weights. Codes are float4 e2m1 (sign and 0, 0.5, 1, 1.5, 2, 3, 4, 6), and every 32 consecutive k of a row have
+ * one scale, a power of two as an e8m0 byte b = 2^(b - 127) (255 = NaN); K % 32 == 0, K <= LSE_FP4_MAX_K.
+ * Row by row: codes (N, K / 2) bytes, the lower k in the low half, scales (N, K / 32) bytes.
+ * In tiles (lse_pack_fp4), what the products take: with nsteps = ceil(K / 128) and nchunks = ceil(K / 512), codes
+ *   (tiles, nsteps, 1024) bytes, byte 16 l + i of tile (rb, j) holding row 16 rb + l % 16 at k = 128 j + 32 (l / 16) +
+ *   2 i (low half) and the k after it, zeros past N and K; scales (tiles, nchunks, 256) bytes, byte 4 l + t of tile
+ *   (rb, c) that of row 16 rb + l % 16 and the 32 k from 512 c + 128 t + 32 (l / 16) on, 127 past N and K. glu 0:
+ *   tiles = ceil(N / 16). glu 1: N = 2 I stacked rows [gate; up], tiles = 2 ceil(I / 16), tile 2 t holding gate rows
+ *   16 t .. and tile 2 t + 1 the same rows of up. lse_fp4_codes_bytes and lse_fp4_scales_bytes: the tiles' sizes, -1
+ *   for invalid ones.
+ *
+ * lse_quantize_weight_fp4: w (N, K) fp32, row stride ldw (a multiple of 4, 16-byte aligned), row by row:
+ *   scale = the smallest power of two s >= 2^-126 with |w| <= 6 s over the group; code = the nearest to w / s, ties to
+ *   the even code, but none that stands for 2^128 or more; a group with a value that is not finite gets the scale NaN.
+ * Replaces: the bf16 weight `from_pretrained` loads (model_runner.py:50-52), at the switch (model_runner.py:45-46).
+ */
+#define LSE_FP4_MAX_K 2097152
+int64_t lse_fp4_codes_bytes(int64_t N, int64_t K, int64_t glu);
+int64_t lse_fp4_scales_bytes(int64_t N, int64_t K, int64_t glu);
+int lse_quantize_weight_fp4(const float* w, int64_t ldw, void* codes, void* scales, int64_t N, int64_t K,
+                            void* stream);
+int lse_pack_fp4(const void* codes, const void* scales, void* out_codes, void* out_scales, int64_t N, int64_t K,
+                 int64_t glu, void* stream);
+
+/*
+ * Rows in 8 bits: float8 e4m3 codes (M, K) and e8m0 scales (M, K / 32), both contiguous: scale = the smallest power of
+ * two s >= 2^-126 with |x| <= 448 s for every finite x of the group; code = rne_e4m3(x / s), but none that stands for
+ * 2^128; infinity and NaN become NaN. K % 32 == 0.
+ * lse_quantize_rows_fp8: x (M, K) bf16, row stride ldx (a multiple of 8, 16-byte aligned); K <= LSE_FP4_MAX_K.
+ * lse_add_rmsnorm_fp8: lse_add_rmsnorm with y in this form (s, r and y's rounding to bf16 as there, then the codes):
+ *   x, residual (may be NULL): (M, K) bf16, row strides multiples of 8, 16-byte aligned; weight (K) bf16; sum (M, K)
+ *   bf16 contiguous receiving x + residual, or NULL; it may be x or residual where that is contiguous. K <=
+ *   LSE_NORM_MAX_K.
+ * Replaces: `hidden + ...` and the norm that reads it in `decoder_hidden` (model_runner.py:222-223;
+ * LlamaRMSNorm.forward, modeling_llama.py:62-67), and the rounding that the products of 8-bit rows need.
+ */
+struct lse_add_rmsnorm_fp8_args {
+  const void* x;
+  int64_t x_stride;
+  const void* residual;
+  int64_t residual_stride;
+  const void* weight;
+  void *sum, *codes, *scales;
+  int64_t M, K;
+  double eps;
+};
+int lse_quantize_rows_fp8(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, void* stream);
+int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* stream);
+
+/*
+ * Products with a 4-bit weight in tiles:
+ *   glu 0:  y[m,n] = bf16(sum_k x[m,k] w[n,k]),  w = code x scale;
+ *   glu 1:  y[m,n] = bf16(silu(sum_k x[m,k] gate[n,k]) * sum_k x[m,k] up[n,k]), N the columns of y (I).
+ * x_scales NULL: x (M, K) bf16, row stride x_stride (a multiple of 8), exact products and fp32 sums. Otherwise x is
+ *   e4m3 codes, row stride a multiple of 16, and x_scales (M, K / 32) e8m0 bytes, row stride x_scales_stride; the
+ *   products of eight consecutive k are cut off 13 bits below the largest, then added in fp32. x 16-byte aligned,
+ *   strides at most LSE_FP4_MAX_K. y: (M, N) bf16, row stride y_stride.
+ * A row's bits do not depend on the other rows' values. workspace: lse_fp4_gemm_workspace_bytes bytes (it reads the
+ *   sizes in args only; -1: invalid ones; 0 for most calls), 16-byte aligned.
+ * Replaces: `F.linear(x, W)` (torch/nn/modules/linear.py:134) at model_runner.py:322-324,369,418 and
+ * `act_fn(gate_proj(x)) * up_proj(x)` (modeling_llama.py:175, from model_runner.py:223), for 4-bit weights, which the
+ * reference does not have.
+ */
+struct lse_fp4_gemm_args {
+  const void* x;
+  int64_t x_stride;
+  const void* x_scales;
+  int64_t x_scales_stride;
+  const void *codes, *scales;
+  void* y;
+  int64_t y_stride, M, N, K, glu;
+};
+int64_t lse_fp4_gemm_workspace_bytes(const struct lse_fp4_gemm_args* args);
+int lse_fp4_gemm(const struct lse_fp4_gemm_args* args, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* Static properties (enum lse_query_key); -1 for an unknown key. Load-time checks read these,
  * as `ModelRunner.check_custom_kernel_support` (model_runner.py:77-94) checks its kernels. */

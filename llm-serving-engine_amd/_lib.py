@@ -51,15 +51,25 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lse_paged_attention_fp8_workspace_bytes": (_I64, [_P]),
     "lse_paged_attention_fp8": (_INT, [_P, _P, _I64, _P]),
     "lse_paged_attention_fp8_choice": (_INT, [_P, _P, _P, _P]),
+    "lse_fp4_codes_bytes": (_I64, [_I64] * 3),
+    "lse_fp4_scales_bytes": (_I64, [_I64] * 3),
+    "lse_quantize_weight_fp4": (_INT, [_P, _I64, _P, _P, _I64, _I64, _P]),
+    "lse_pack_fp4": (_INT, [_P] * 4 + [_I64] * 3 + [_P]),
+    "lse_quantize_rows_fp8": (_INT, [_P, _I64, _P, _P, _I64, _I64, _P]),
+    "lse_add_rmsnorm_fp8": (_INT, [_P, _P]),
+    "lse_fp4_gemm_workspace_bytes": (_I64, [_P]),
+    "lse_fp4_gemm": (_INT, [_P, _P, _I64, _P]),
     "lse_query": (_I64, [_INT]),
     "lse_status_string": (ctypes.c_char_p, [_INT]),
 }
 
-# The header's argument structs: eight bytes a field, the last of the attention's a double. Packing one takes a
+# The header's argument structs: eight bytes a field, the last of the attention's and the norm's a double. Packing one takes a
 # sixth of the time of passing its fields one by one.
 ROPE_ARGS = struct.Struct("18q")
 APPEND_KV_FP8_ARGS = struct.Struct("34q")
 PAGED_ATTENTION_FP8_ARGS = struct.Struct("26qd")
+ADD_RMSNORM_FP8_ARGS = struct.Struct("10qd")
+FP4_GEMM_ARGS = struct.Struct("12q")
 
 # Mirrors of the header's enums.
 LSE_OK = 0
@@ -68,8 +78,9 @@ MODE_W8A16, MODE_W8A8 = 0, 1
 E_WORKSPACE, E_SCRATCH = -6, -7
 Q_ABI_VERSION, Q_K_ALIGN, Q_DECODE_MAX_M, Q_MAX_K, Q_GFX_ARCH = 0, 1, 2, 3, 4
 Q_NOALLOC_SCRATCH = 5
-ABI_VERSION = 15
+ABI_VERSION = 16
 NORM_MAX_K = 16384
+FP4_MAX_K = 2097152
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None

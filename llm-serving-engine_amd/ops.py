@@ -20,26 +20,35 @@ import torch
 from . import _lib
 
 __all__ = [
+    "Fp4Weight",
     "Fp8KV",
+    "Fp8Rows",
     "add_rmsnorm",
+    "add_rmsnorm_fp8",
     "append_kv_fp8",
     "bf16_decode_linear",
+    "dequantize_fp4",
+    "dequantize_rows_fp8",
     "fp8_kv_pool",
     "pack_bf16_weight",
     "packed_bf16_shape",
     "unpack_bf16_weight",
     "paged_attention_forward",
     "paged_attention_fp8",
+    "pack_fp4",
     "pack_glu",
     "pack_weight",
     "packed_glu_shape",
     "packed_shape",
     "quantize_act_per_token",
+    "quantize_rows_fp8",
+    "quantize_weight_fp4",
     "quantize_weight_per_channel",
     "rmsnorm_quantize",
     "rope",
     "rope_kv",
     "rope_table",
+    "unpack_fp4",
     "unpack_fp8_kv",
     "unpack_glu",
     "unpack_weight",
@@ -47,6 +56,10 @@ __all__ = [
     "w8a8_glu",
     "w8a8_glu_quantized",
     "w8a8_linear",
+    "w4a16_glu",
+    "w4a16_linear",
+    "w4a8_glu",
+    "w4a8_linear",
     "w8a16_glu",
     "w8a16_linear",
     "w8a16_linear_noalloc",
@@ -615,8 +628,8 @@ def _one_gpu(first: torch.Tensor, *others: torch.Tensor) -> int:
     return dev if dev >= 0 else _on_gpu(first)
 
 
-def _launch(dev: int, what: str, args: bytes, *more) -> None:
-    """Calls the entry point `what` with packed args and dev's current stream. A kernel goes to the current
+def _launch(dev: int, what: str, args: bytes | int, *more) -> None:
+    """Calls the entry point `what` with its (packed) args and dev's current stream. A kernel goes to the current
     device, whose default stream has the handle of every other's."""
     fn = getattr(_lib._lib or _lib.library(), what)
     if torch._C._cuda_getDevice() == dev:
@@ -958,3 +971,239 @@ def bf16_decode_linear(x: torch.Tensor, wp: torch.Tensor, n: int) -> torch.Tenso
         "lse_bf16_decode_gemm",
     )
     return y
+
+
+# ---- 4-bit weights, and rows in 8 bits -----------------------------------------------------------
+
+FP4_GROUP = 32  # weights of a row, or values of a row in 8 bits, that share a scale
+FP4_MAGNITUDES = (0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0)  # of the e2m1 codes 0 to 7; 8 more is the sign
+
+
+class Fp4Weight(NamedTuple):
+    """A 4-bit weight in the tiles that the products stream: float4 e2m1 codes with a power of two (e8m0) for every
+    32 consecutive k of a row.
+
+    codes: uint8 (tiles, ceil(K / 128), 1024), scales: float8_e8m0fnu (tiles, ceil(K / 512), 256); n: the columns of
+    the product, k: those of its input. tiles = ceil(n / 16); 2 ceil(n / 16) for the gate and up weights of a
+    `w4a16_glu` or `w4a8_glu`, whose row tiles take turns. Made by `pack_fp4`."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+    n: int
+    k: int
+
+
+class Fp8Rows(NamedTuple):
+    """Rows held in 8 bits: float8 e4m3 codes (..., K) and a power of two (e8m0) for every 32 of a row's values,
+    scales (..., K / 32). Made by `quantize_rows_fp8` and `add_rmsnorm_fp8`."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+def quantize_weight_fp4(w: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """W (N, K) → codes uint8 (N, K / 2), two e2m1 codes a byte with the lower k in the low half, and scales
+    float8_e8m0fnu (N, K / 32): the smallest power of two from 2^-126 up that has its 32 weights within 6 scales;
+    each weight goes to the nearest code, ties to the even one. A group with a value that is not finite gets the scale
+    NaN. K % 32 == 0. Runs on the GPU at load time; W is read as fp32 (bf16 and fp16 widen exactly)."""
+    _require(w.dim() == 2 and w.is_floating_point(), f"weight must be 2-D floating point, got {tuple(w.shape)} {w.dtype}")
+    dev = _on_gpu(w)
+    n, k = w.shape
+    _require(k % FP4_GROUP == 0, f"4-bit weights need K % {FP4_GROUP} == 0, got K = {k}")
+    w32 = w.to(torch.float32).contiguous()
+    if w32.data_ptr() % 16:
+        w32 = w32.clone()
+    codes = torch.empty((n, k // 2), dtype=torch.uint8, device=dev)
+    scales = torch.empty((n, k // FP4_GROUP), dtype=_E8, device=dev)
+    _launch(dev, "lse_quantize_weight_fp4", w32.data_ptr(), k, codes.data_ptr(), scales.data_ptr(), n, k)
+    return codes, scales
+
+
+def _check_fp4_rows(codes: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
+    """(rows, K) of a weight's codes and scales row by row."""
+    if codes.dim() != 2 or codes.dtype is not torch.uint8 or scales.dim() != 2 or scales.dtype is not _E8:
+        raise RuntimeError("codes must be uint8 (N, K / 2), scales float8_e8m0fnu (N, K / 32)")
+    n, k = codes.shape[0], 2 * codes.shape[1]
+    if k % FP4_GROUP or scales.shape != (n, k // FP4_GROUP):
+        raise RuntimeError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are no 4-bit weight")
+    return n, k
+
+
+def pack_fp4(codes: torch.Tensor, scales: torch.Tensor, glu: bool = False) -> Fp4Weight:
+    """A 4-bit weight row by row (`quantize_weight_fp4`'s form) → its tiles, on the GPU. glu: the rows are (2 I, K)
+    [gate; up], for `w4a16_glu` and `w4a8_glu`; n is then I."""
+    dev = _on_gpu(codes, scales)
+    rows, k = _check_fp4_rows(codes, scales)
+    _require(not glu or rows % 2 == 0, "gate and up rows come in equal numbers")
+    codes, scales = codes.contiguous(), scales.contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    n = rows // 2 if glu else rows
+    tiles = -(-n // 16) * (2 if glu else 1)
+    out = Fp4Weight(torch.empty((tiles, -(-k // 128), 1024), dtype=torch.uint8, device=dev),
+                    torch.empty((tiles, -(-k // 512), 256), dtype=_E8, device=dev), n, k)
+    _launch(dev, "lse_pack_fp4", codes.data_ptr(), scales.data_ptr(), out.codes.data_ptr(), out.scales.data_ptr(), rows,
+            k, int(glu))
+    return out
+
+
+def unpack_fp4(weight: Fp4Weight) -> tuple[torch.Tensor, torch.Tensor]:
+    """Inverse of `pack_fp4` (a pure permutation, done with torch views): (codes, scales) row by row."""
+    _, tiles = _check_fp4(weight, None)
+    glu, n, k = tiles != -(-weight.n // 16), weight.n, weight.k
+    c = weight.codes.view(tiles, -1, 4, 16, 16).permute(0, 3, 1, 2, 4).reshape(tiles * 16, -1)[:, :k // 2]
+    s = weight.scales.view(torch.uint8).view(tiles, -1, 4, 16, 4).permute(0, 3, 1, 4, 2)
+    s = s.reshape(tiles * 16, -1)[:, :k // FP4_GROUP]
+    if glu:
+        c, s = (t.reshape(-1, 2, 16, t.shape[1]).transpose(0, 1).reshape(2, -1, t.shape[1])[:, :n].flatten(0, 1)
+                for t in (c, s))
+    else:
+        c, s = c[:n], s[:n]
+    return c.contiguous(), s.contiguous().view(_E8)
+
+
+def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
+    """The values of a 4-bit weight row by row, (N, K) fp32."""
+    n, k = _check_fp4_rows(codes, scales)
+    value = torch.tensor([*FP4_MAGNITUDES, *(-v for v in FP4_MAGNITUDES)], device=codes.device)
+    w = value[torch.stack([codes & 15, codes >> 4], -1).view(n, k).int()]
+    return (w.view(n, -1, FP4_GROUP) * scales.float()[..., None]).view(n, k)
+
+
+def dequantize_rows_fp8(rows: Fp8Rows) -> torch.Tensor:
+    """The values of rows in 8 bits, (..., K) bf16 (each is one)."""
+    v = rows.codes.float().unflatten(-1, (-1, FP4_GROUP)) * rows.scales.float()[..., None]
+    return v.flatten(-2).to(_BF16)
+
+
+def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
+    """x (..., K) bf16 → its rows in 8 bits: for every 32 values of a row the smallest power of two from 2^-126 up that
+    has the finite ones within 448 scales, and their codes, rounded to nearest even (none to 2^128; infinity and NaN
+    become NaN). K % 32 == 0."""
+    dev = _one_gpu(x)
+    if x.dtype is not _BF16:
+        raise RuntimeError(f"rows in 8 bits are made of bf16 rows, got {x.dtype}")
+    k = x.shape[-1]
+    if k % FP4_GROUP:
+        raise RuntimeError(f"rows in 8 bits need K % {FP4_GROUP} == 0, got K = {k}")
+    owner, at, ldx, m = _row_args(x, k) if k else (x, 0, 0, 0)
+    rows = Fp8Rows(torch.empty(x.shape, dtype=_F8, device=x.device),
+                   torch.empty((*x.shape[:-1], k // FP4_GROUP), dtype=_E8, device=x.device))
+    _launch(dev, "lse_quantize_rows_fp8", at, ldx, rows.codes.data_ptr(), rows.scales.data_ptr(), m, k)
+    return rows
+
+
+def add_rmsnorm_fp8(
+    x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float,
+) -> tuple[torch.Tensor, Fp8Rows]:
+    """(s, LlamaRMSNorm(s) in 8 bits) with s = x + residual (x itself when residual is None) in one kernel: the bits of
+    `add_rmsnorm` and `quantize_rows_fp8` after it. x and residual (..., K) bf16, weight (K,) bf16, K % 32 == 0,
+    K <= `_lib.NORM_MAX_K`."""
+    dev = _one_gpu(x, weight) if residual is None else _one_gpu(x, weight, residual)
+    k = x.shape[-1]
+    if x.dtype is not _BF16 or weight.dtype is not _BF16 or weight.shape != (k,):
+        raise RuntimeError(f"RMSNorm takes bf16 x and weight ({k},)")
+    if k % FP4_GROUP or k > _lib.NORM_MAX_K or k == 0:
+        raise RuntimeError(f"a norm into 8 bits needs K % {FP4_GROUP} == 0 up to {_lib.NORM_MAX_K}, got K = {k}")
+    owner, at, ldx, m = _row_args(x, k)
+    s, r_at, ldr, s_at = x, 0, 0, 0
+    if residual is not None:
+        if residual.dtype is not _BF16 or residual.shape != x.shape:
+            raise RuntimeError("the residual must be bf16 and of x's shape")
+        r_owner, r_at, ldr, _ = _row_args(residual, k)
+        s = torch.empty(x.shape, dtype=_BF16, device=x.device)
+        s_at = s.data_ptr()
+    w = weight.contiguous()
+    if w.data_ptr() % 16:  # a piece of a flat parameter buffer
+        w = w.clone()
+    rows = Fp8Rows(torch.empty(x.shape, dtype=_F8, device=x.device),
+                   torch.empty((*x.shape[:-1], k // FP4_GROUP), dtype=_E8, device=x.device))
+    _launch(dev, "lse_add_rmsnorm_fp8", _lib.ADD_RMSNORM_FP8_ARGS.pack(
+        at, ldx, r_at, ldr, w.data_ptr(), s_at, rows.codes.data_ptr(), rows.scales.data_ptr(), m, k, float(eps)))
+    return s, rows
+
+
+def _check_fp4(weight: Fp4Weight, glu: bool | None) -> tuple[int, int]:
+    """(n, tiles) of a 4-bit weight, its tiles checked; glu None: of either kind."""
+    codes, scales, n, k = weight
+    tiles = codes.shape[0]
+    if codes.dtype is not torch.uint8 or scales.dtype is not _E8 or not codes.is_contiguous() \
+            or not scales.is_contiguous() or codes.data_ptr() % 16 or scales.data_ptr() % 16:
+        raise RuntimeError("a 4-bit weight's codes must be uint8 and its scales float8_e8m0fnu, contiguous, 16-byte "
+                           "aligned")
+    if k % FP4_GROUP or codes.shape != (tiles, -(-k // 128), 1024) or scales.shape != (tiles, -(-k // 512), 256):
+        raise RuntimeError(f"codes {tuple(codes.shape)} and scales {tuple(scales.shape)} are no tiles of K = {k}")
+    once = -(-n // 16)
+    if tiles != (once if not glu else 2 * once) and not (glu is None and tiles == 2 * once):
+        raise RuntimeError(f"{tiles} row tiles are no {'gate/up ' if glu else ''}weight of n = {n}")
+    return n, tiles
+
+
+def _fp4_gemm(x: torch.Tensor | Fp8Rows, weight: Fp4Weight, glu: bool) -> torch.Tensor:
+    n, _ = _check_fp4(weight, glu)
+    k = weight.k
+    if isinstance(x, Fp8Rows):
+        codes, scales = x
+        dev = _one_gpu(codes, scales, weight.codes, weight.scales)
+        lead = codes.shape[:-1]
+        if codes.dtype is not _F8 or scales.dtype is not _E8:
+            raise RuntimeError(f"rows in 8 bits are float8_e4m3fn with float8_e8m0fnu scales, got {codes.dtype}, "
+                               f"{scales.dtype}")
+        if codes.shape[-1] != k or scales.shape != (*lead, k // FP4_GROUP):
+            raise RuntimeError(f"rows {tuple(codes.shape)} with scales {tuple(scales.shape)} do not fit K = {k}")
+        codes, scales = codes.reshape(-1, k), scales.reshape(-1, k // FP4_GROUP)
+        m = codes.shape[0]
+        ldx = codes.stride(0) if m > 1 else k
+        if codes.stride(1) != 1 or not k <= ldx <= _lib.FP4_MAX_K or ldx % 16 or codes.data_ptr() % 16:
+            codes, ldx = codes.clone(memory_format=torch.contiguous_format), k
+        lds = scales.stride(0) if m > 1 else k // FP4_GROUP
+        if scales.stride(1) != 1 or not k // FP4_GROUP <= lds <= _lib.FP4_MAX_K:
+            scales, lds = scales.clone(memory_format=torch.contiguous_format), k // FP4_GROUP
+        at, s_at = codes.data_ptr(), scales.data_ptr()
+    else:
+        dev = _one_gpu(x, weight.codes, weight.scales)
+        if x.dtype is not _BF16:
+            raise RuntimeError(f"expected bf16 rows or Fp8Rows, got {x.dtype}")
+        lead = x.shape[:-1]
+        owner, at, ldx, m = _row_args(x, k)
+        if ldx > _lib.FP4_MAX_K:
+            owner = owner.contiguous()
+            at, ldx = owner.data_ptr(), k
+        s_at = lds = 0
+    y = torch.empty((*lead, n), dtype=_BF16, device=weight.codes.device)
+    args = _lib.FP4_GEMM_ARGS.pack(at, ldx, s_at, lds, weight.codes.data_ptr(), weight.scales.data_ptr(), y.data_ptr(),
+                                   n, m, n, k, int(glu))
+    nbytes = (_lib._lib or _lib.library()).lse_fp4_gemm_workspace_bytes(args)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=y.device) if nbytes > 0 else None
+    _launch(dev, "lse_fp4_gemm", args, *_ws_args(ws))
+    return y
+
+
+def w4a16_linear(x: torch.Tensor, weight: Fp4Weight) -> torch.Tensor:
+    """y = bf16(sum_k x[..., k] w[n, k]) for x (..., K) bf16 → y (..., N) bf16: exact products with the 4-bit weight's
+    values, fp32 sums."""
+    if isinstance(x, Fp8Rows):
+        raise RuntimeError("rows in 8 bits go to w4a8_linear")
+    return _fp4_gemm(x, weight, False)
+
+
+def w4a16_glu(x: torch.Tensor, weight: Fp4Weight) -> torch.Tensor:
+    """h = silu(x Gᵀ) * (x Uᵀ) for x (..., K) bf16 and stacked 4-bit weights (`pack_fp4(..., glu=True)`) → (..., I)
+    bf16, rounded once."""
+    if isinstance(x, Fp8Rows):
+        raise RuntimeError("rows in 8 bits go to w4a8_glu")
+    return _fp4_gemm(x, weight, True)
+
+
+def w4a8_linear(rows: Fp8Rows, weight: Fp4Weight) -> torch.Tensor:
+    """`w4a16_linear` over rows in 8 bits, at twice the matrix cores' rate."""
+    if not isinstance(rows, Fp8Rows):
+        raise RuntimeError("w4a8_linear takes Fp8Rows (quantize_rows_fp8, add_rmsnorm_fp8)")
+    return _fp4_gemm(rows, weight, False)
+
+
+def w4a8_glu(rows: Fp8Rows, weight: Fp4Weight) -> torch.Tensor:
+    """`w4a16_glu` over rows in 8 bits, at twice the matrix cores' rate."""
+    if not isinstance(rows, Fp8Rows):
+        raise RuntimeError("w4a8_glu takes Fp8Rows (quantize_rows_fp8, add_rmsnorm_fp8)")
+    return _fp4_gemm(rows, weight, True)
