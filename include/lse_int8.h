@@ -513,9 +513,9 @@ int lse_pack_fp4(const void* codes, const void* scales, void* out_codes, void* o
                  int64_t glu, void* stream);
 
 /*
- * Rows in 8 bits: float8 e4m3 codes (M, K) and e8m0 scales (M, K / 32), both contiguous: scale = the smallest power of
- * two s >= 2^-126 with |x| <= 448 s for every finite x of the group; code = rne_e4m3(x / s), but none that stands for
- * 2^128; infinity and NaN become NaN. K % 32 == 0.
+ * Rows in 8 bits: float8 e4m3 codes (M, K), contiguous, and e8m0 scales (M, K / 32), row stride scales_stride bytes
+ * (the products take multiples of 4): scale = the smallest power of two s >= 2^-126 with |x| <= 448 s for every finite x
+ * of the group; code = rne_e4m3(x / s), but none that stands for 2^128; infinity and NaN become NaN. K % 32 == 0.
  * lse_quantize_rows_fp8: x (M, K) bf16, row stride ldx (a multiple of 8, 16-byte aligned); K <= LSE_FP4_MAX_K.
  * lse_add_rmsnorm_fp8: lse_add_rmsnorm with y in this form (s, r and y's rounding to bf16 as there, then the codes):
  *   x, residual (may be NULL): (M, K) bf16, row strides multiples of 8, 16-byte aligned; weight (K) bf16; sum (M, K)
@@ -531,10 +531,11 @@ struct lse_add_rmsnorm_fp8_args {
   int64_t residual_stride;
   const void* weight;
   void *sum, *codes, *scales;
-  int64_t M, K;
+  int64_t scales_stride, M, K;
   double eps;
 };
-int lse_quantize_rows_fp8(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K, void* stream);
+int lse_quantize_rows_fp8(const void* x, int64_t ldx, void* codes, void* scales, int64_t scales_stride, int64_t M,
+                          int64_t K, void* stream);
 int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* stream);
 
 /*
@@ -542,7 +543,8 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
  *   glu 0:  y[m,n] = bf16(sum_k x[m,k] w[n,k]),  w = code x scale;
  *   glu 1:  y[m,n] = bf16(silu(sum_k x[m,k] gate[n,k]) * sum_k x[m,k] up[n,k]), N the columns of y (I).
  * x_scales NULL: x (M, K) bf16, row stride x_stride (a multiple of 8), exact products and fp32 sums. Otherwise x is
- *   e4m3 codes, row stride a multiple of 16, and x_scales (M, K / 32) e8m0 bytes, row stride x_scales_stride; the
+ *   e4m3 codes, row stride a multiple of 16, and x_scales (M, K / 32) e8m0 bytes, row stride x_scales_stride, which
+ *   is a multiple of 4 and x_scales 4-byte aligned (rows are read in whole dwords, bytes past K / 32 do not count); the
  *   products of eight consecutive k are cut off 13 bits below the largest, then added in fp32. x 16-byte aligned,
  *   strides at most LSE_FP4_MAX_K. y: (M, N) bf16, row stride y_stride.
  * A row's bits do not depend on the other rows' values. workspace: lse_fp4_gemm_workspace_bytes bytes (it reads the

@@ -55,7 +55,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lse_fp4_scales_bytes": (_I64, [_I64] * 3),
     "lse_quantize_weight_fp4": (_INT, [_P, _I64, _P, _P, _I64, _I64, _P]),
     "lse_pack_fp4": (_INT, [_P] * 4 + [_I64] * 3 + [_P]),
-    "lse_quantize_rows_fp8": (_INT, [_P, _I64, _P, _P, _I64, _I64, _P]),
+    "lse_quantize_rows_fp8": (_INT, [_P, _I64, _P, _P, _I64, _I64, _I64, _P]),
     "lse_add_rmsnorm_fp8": (_INT, [_P, _P]),
     "lse_fp4_gemm_workspace_bytes": (_I64, [_P]),
     "lse_fp4_gemm": (_INT, [_P, _P, _I64, _P]),
@@ -68,7 +68,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
 ROPE_ARGS = struct.Struct("18q")
 APPEND_KV_FP8_ARGS = struct.Struct("34q")
 PAGED_ATTENTION_FP8_ARGS = struct.Struct("26qd")
-ADD_RMSNORM_FP8_ARGS = struct.Struct("10qd")
+ADD_RMSNORM_FP8_ARGS = struct.Struct("11qd")
 FP4_GEMM_ARGS = struct.Struct("12q")
 
 # Mirrors of the header's enums.

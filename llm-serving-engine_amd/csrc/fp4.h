@@ -91,9 +91,19 @@ struct Fp4Args {
   int M, N, K;           // N output columns (gate/up: I)
   int nsteps, nchunks;   // ceil(K / 128), ceil(K / 512)
   int nrb;               // row tiles of the weight
-  int xs_dwords;         // the scale bytes of a step are one aligned dword
+};
+
+// How a call runs: bm 0: the streaming kernel; otherwise tiles of bm x bn, K in `splits` ranges of `chunks` chunks.
+struct Fp4Plan {
+  int bm, bn, splits, chunks;
+};
+
+struct Fp4Split {
+  int mblocks, nblocks, splits, chunks;
+  float* part;  // splits > 1: [splits][M][16 nrb] sums
 };
 
 int launch_fp4_stream(const Fp4Args& a, bool rows8, bool glu, hipStream_t stream);
+int launch_fp4_tile(const Fp4Args& a, const Fp4Plan& plan, bool rows8, bool glu, float* part, hipStream_t stream);
 
 }  // namespace lse

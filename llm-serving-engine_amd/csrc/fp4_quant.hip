@@ -107,9 +107,10 @@ __device__ __forceinline__ void bf16x8_to_f32(uint4 q, float (&v)[8]) {
   }
 }
 
-// One thread eight values of a row. codes (M, K), scales (M, K / 32) contiguous.
+// One thread eight values of a row. codes (M, K) contiguous, scales (M, K / 32) of row stride lds.
 __global__ void __launch_bounds__(256)
-fp8_rows_kernel(const uint16_t* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t total, int per_row) {
+fp8_rows_kernel(const uint16_t* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, int64_t total,
+                int per_row) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (at >= total) return;  // whole groups: total and 256 are multiples of 4
   const int64_t m = at / per_row;
@@ -117,7 +118,7 @@ fp8_rows_kernel(const uint16_t* x, int64_t ldx, uint8_t* codes, uint8_t* scales,
   bf16x8_to_f32(*reinterpret_cast<const uint4*>(x + m * ldx + 8 * (at - m * per_row)), v);
   int byte;
   *reinterpret_cast<uint2*>(codes + 8 * at) = fp8_encode8(v, byte);
-  if ((at & 3) == 0) scales[at >> 2] = (uint8_t)byte;
+  if ((at & 3) == 0) scales[m * lds + ((at - m * per_row) >> 2)] = (uint8_t)byte;
 }
 
 constexpr int kNormFp8Threads = 512;
@@ -129,7 +130,7 @@ constexpr int kNormFp8Threads = 512;
 template <int NV>
 __global__ void __launch_bounds__(kNormFp8Threads)
 add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int64_t ldr, const uint16_t* w, float eps,
-                       uint16_t* sum, uint8_t* codes, uint8_t* scales, int K) {
+                       uint16_t* sum, uint8_t* codes, uint8_t* scales, int64_t lds, int K) {
   __shared__ float red[kNormFp8Threads / 64];
   const int64_t m = blockIdx.x;
   float s[NV][8], g[NV][8];
@@ -178,7 +179,7 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
     const uint2 c = fp8_encode8(n, byte);  // every lane: K is a multiple of 32, so groups are whole
     if (k < K) {
       *reinterpret_cast<uint2*>(codes + m * K + k) = c;
-      if ((threadIdx.x & 3) == 0) scales[m * (K / kFp4Group) + k / kFp4Group] = (uint8_t)byte;
+      if ((threadIdx.x & 3) == 0) scales[m * lds + k / kFp4Group] = (uint8_t)byte;
     }
   }
 }
@@ -239,9 +240,9 @@ int lse_pack_fp4(const void* codes, const void* scales, void* out_codes, void* o
   return lse::launch_status();
 }
 
-int lse_quantize_rows_fp8(const void* x, int64_t ldx, void* codes, void* scales, int64_t M, int64_t K,
-                          void* stream) {
-  if (M < 0 || K < 0 || ldx < K || M > kMax31) return LSE_E_SHAPE;
+int lse_quantize_rows_fp8(const void* x, int64_t ldx, void* codes, void* scales, int64_t scales_stride, int64_t M,
+                          int64_t K, void* stream) {
+  if (M < 0 || K < 0 || ldx < K || M > kMax31 || scales_stride < K / lse::kFp4Group) return LSE_E_SHAPE;
   if (K % lse::kFp4Group || ldx % 8) return LSE_E_ALIGN;
   if (K > LSE_FP4_MAX_K) return LSE_E_RANGE;
   if (M == 0 || K == 0) return LSE_OK;
@@ -250,7 +251,7 @@ int lse_quantize_rows_fp8(const void* x, int64_t ldx, void* codes, void* scales,
   const int64_t total = M * (K / 8), blocks = lse::ceil_div(total, 256);
   if (blocks > kMax31) return LSE_E_RANGE;
   hipLaunchKernelGGL(lse::fp8_rows_kernel, dim3((unsigned)blocks), dim3(256), 0, (hipStream_t)stream,
-                     (const uint16_t*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, total, (int)(K / 8));
+                     (const uint16_t*)x, ldx, (uint8_t*)codes, (uint8_t*)scales, scales_stride, total, (int)(K / 8));
   return lse::launch_status();
 }
 
@@ -262,7 +263,9 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
   if (x.K > LSE_NORM_MAX_K) return LSE_E_RANGE;
   if (x.M == 0 || x.K == 0) return LSE_OK;
   if (!x.x || !x.weight || !x.codes || !x.scales) return LSE_E_NULL;
-  if (x.x_stride < x.K || (x.residual && x.residual_stride < x.K) || !(x.eps >= 0.0)) return LSE_E_SHAPE;
+  if (x.x_stride < x.K || (x.residual && x.residual_stride < x.K) ||
+      x.scales_stride < x.K / lse::kFp4Group || !(x.eps >= 0.0))
+    return LSE_E_SHAPE;
   if (x.x_stride % 8 || (x.residual && x.residual_stride % 8) || !aligned16(x.x) || !aligned16(x.residual) ||
       !aligned16(x.weight) || !aligned16(x.sum) || !aligned16(x.codes))
     return LSE_E_ALIGN;
@@ -270,7 +273,7 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, wg, 0, (hipStream_t)stream, (const uint16_t*)x.x, x.x_stride,
                        (const uint16_t*)x.residual, x.residual_stride, (const uint16_t*)x.weight, (float)x.eps,
-                       (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, (int)x.K);
+                       (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, x.scales_stride, (int)x.K);
   };
   if (x.K <= 8 * lse::kNormFp8Threads)
     go(lse::add_rmsnorm_fp8_kernel<1>);

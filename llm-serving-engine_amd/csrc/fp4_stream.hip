@@ -51,9 +51,11 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
                                     (uint32_t)tiles * (uint32_t)a.nchunks * kFp4ScaleBytes);
   const BufferRsrc xres = make_rsrc(static_cast<const char*>(a.x) + (int64_t)m0 * a.ldx * ESZ,
                                     (uint32_t)(((int64_t)(rows - 1) * a.ldx + a.K) * ESZ));
-  const int per = a.K / kFp4Group;
-  const BufferRsrc xsres = A8 ? make_rsrc(a.xs + (int64_t)m0 * a.lds, (uint32_t)((int64_t)(rows - 1) * a.lds + per))
+  const int per4 = (a.K / kFp4Group + 3) & ~3;  // scale bytes of a row in whole dwords
+  const BufferRsrc xsres = A8 ? make_rsrc(a.xs + (int64_t)m0 * a.lds, (uint32_t)((int64_t)(rows - 1) * a.lds + per4))
                               : make_rsrc(a.x, 0);
+  // Scale bytes past K in the last step's dword, which may be anything, become 0.
+  const uint32_t tail = a.K % kFp4Step ? (1u << (8 * (a.K % kFp4Step / kFp4Group))) - 1 : ~0u;
 
   struct Step {
     uint4 w[RT];
@@ -87,17 +89,9 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
         const int b0 = 4 * (4 * c + t);  // the step's first byte of the row
-        if (a.xs_dwords) {
-          s.x[t] = __builtin_amdgcn_raw_buffer_load_b32(
-              xsres, (int)(r16 < rows && b0 < per ? base + b0 : kOutOfRange), 0, 0);
-        } else {
-          s.x[t] = 0;
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            s.x[t] |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(
-                          xsres, (int)(r16 < rows && b0 + i < per ? base + b0 + i : kOutOfRange), 0, 0)
-                      << (8 * i);
-        }
+        s.x[t] = __builtin_amdgcn_raw_buffer_load_b32(
+            xsres, (int)(r16 < rows && b0 < per4 ? base + b0 : kOutOfRange), 0, 0);
+        if (4 * c + t == a.nsteps - 1) s.x[t] &= tail;
       }
     }
   };

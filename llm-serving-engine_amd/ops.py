@@ -1076,6 +1076,15 @@ def dequantize_rows_fp8(rows: Fp8Rows) -> torch.Tensor:
     return v.flatten(-2).to(_BF16)
 
 
+def _empty_rows(x: torch.Tensor, k: int) -> tuple[Fp8Rows, int]:
+    """Rows in 8 bits for x (..., K), and the bytes from a row's scales to the next: the products read whole dwords."""
+    per = k // FP4_GROUP
+    lds = (per + 3) & ~3
+    codes = torch.empty(x.shape, dtype=_F8, device=x.device)
+    scales = torch.empty((*x.shape[:-1], lds), dtype=_E8, device=x.device)
+    return Fp8Rows(codes, scales if lds == per else scales[..., :per]), lds
+
+
 def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
     """x (..., K) bf16 → its rows in 8 bits: for every 32 values of a row the smallest power of two from 2^-126 up that
     has the finite ones within 448 scales, and their codes, rounded to nearest even (none to 2^128; infinity and NaN
@@ -1087,9 +1096,8 @@ def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
     if k % FP4_GROUP:
         raise RuntimeError(f"rows in 8 bits need K % {FP4_GROUP} == 0, got K = {k}")
     owner, at, ldx, m = _row_args(x, k) if k else (x, 0, 0, 0)
-    rows = Fp8Rows(torch.empty(x.shape, dtype=_F8, device=x.device),
-                   torch.empty((*x.shape[:-1], k // FP4_GROUP), dtype=_E8, device=x.device))
-    _launch(dev, "lse_quantize_rows_fp8", at, ldx, rows.codes.data_ptr(), rows.scales.data_ptr(), m, k)
+    rows, lds = _empty_rows(x, k)
+    _launch(dev, "lse_quantize_rows_fp8", at, ldx, rows.codes.data_ptr(), rows.scales.data_ptr(), lds, m, k)
     return rows
 
 
@@ -1116,10 +1124,9 @@ def add_rmsnorm_fp8(
     w = weight.contiguous()
     if w.data_ptr() % 16:  # a piece of a flat parameter buffer
         w = w.clone()
-    rows = Fp8Rows(torch.empty(x.shape, dtype=_F8, device=x.device),
-                   torch.empty((*x.shape[:-1], k // FP4_GROUP), dtype=_E8, device=x.device))
+    rows, lds = _empty_rows(x, k)
     _launch(dev, "lse_add_rmsnorm_fp8", _lib.ADD_RMSNORM_FP8_ARGS.pack(
-        at, ldx, r_at, ldr, w.data_ptr(), s_at, rows.codes.data_ptr(), rows.scales.data_ptr(), m, k, float(eps)))
+        at, ldx, r_at, ldr, w.data_ptr(), s_at, rows.codes.data_ptr(), rows.scales.data_ptr(), lds, m, k, float(eps)))
     return s, rows
 
 
@@ -1139,6 +1146,19 @@ def _check_fp4(weight: Fp4Weight, glu: bool | None) -> tuple[int, int]:
     return n, tiles
 
 
+def _dword_rows(scales: torch.Tensor, per: int) -> tuple[torch.Tensor, int]:
+    """Scales (M, per) whose rows start at, and may be read to, a whole dword, and the bytes from row to row: as they are
+    where they allow it."""
+    m, whole = scales.shape[0], (per + 3) & ~3
+    lds = scales.stride(0) if m > 1 else whole
+    if (scales.stride(1) != 1 or lds % 4 or not whole <= lds <= _lib.FP4_MAX_K or scales.data_ptr() % 4
+            or (whole != per and scales.storage_offset() + (m - 1) * lds + whole > scales.untyped_storage().nbytes())):
+        rows = torch.empty((m, whole), dtype=_E8, device=scales.device)
+        rows[:, :per] = scales
+        return rows, whole
+    return scales, lds
+
+
 def _fp4_gemm(x: torch.Tensor | Fp8Rows, weight: Fp4Weight, glu: bool) -> torch.Tensor:
     n, _ = _check_fp4(weight, glu)
     k = weight.k
@@ -1151,14 +1171,13 @@ def _fp4_gemm(x: torch.Tensor | Fp8Rows, weight: Fp4Weight, glu: bool) -> torch.
                                f"{scales.dtype}")
         if codes.shape[-1] != k or scales.shape != (*lead, k // FP4_GROUP):
             raise RuntimeError(f"rows {tuple(codes.shape)} with scales {tuple(scales.shape)} do not fit K = {k}")
-        codes, scales = codes.reshape(-1, k), scales.reshape(-1, k // FP4_GROUP)
+        per = k // FP4_GROUP
+        codes, scales = codes.reshape(-1, k), scales.reshape(-1, per)
         m = codes.shape[0]
         ldx = codes.stride(0) if m > 1 else k
         if codes.stride(1) != 1 or not k <= ldx <= _lib.FP4_MAX_K or ldx % 16 or codes.data_ptr() % 16:
             codes, ldx = codes.clone(memory_format=torch.contiguous_format), k
-        lds = scales.stride(0) if m > 1 else k // FP4_GROUP
-        if scales.stride(1) != 1 or not k // FP4_GROUP <= lds <= _lib.FP4_MAX_K:
-            scales, lds = scales.clone(memory_format=torch.contiguous_format), k // FP4_GROUP
+        scales, lds = _dword_rows(scales, per)
         at, s_at = codes.data_ptr(), scales.data_ptr()
     else:
         dev = _one_gpu(x, weight.codes, weight.scales)
