@@ -30,6 +30,16 @@ constexpr int kFp4ScaleBytes = 256;
 
 typedef int i32x8 __attribute__((ext_vector_type(8)));
 
+// f(0), f(1), ... f(N - 1), each index a constant.
+template <typename F, int... I>
+__device__ __forceinline__ void unroll_seq(F&& f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void unroll(F&& f) {
+  unroll_seq(f, std::make_integer_sequence<int, N>{});
+}
+
 // Eight weights of a dword times 2^(scale's exponent field - 127), in k order; exact but for products past bf16's range
 // (v_cvt_scalef32_pk_bf16_fp4; measured over every code and scale).
 __device__ __forceinline__ bf16x8 fp4_decode8(uint32_t w, float scale) {
@@ -58,6 +68,20 @@ __device__ __forceinline__ f32x4 mfma_fp4_fp8(uint4 w, uint32_t ws, uint4 lo, ui
   const i32x8 a = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
   const i32x8 b = {(int)lo.x, (int)lo.y, (int)lo.z, (int)lo.w, (int)hi.x, (int)hi.y, (int)hi.z, (int)hi.w};
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, 4, 0, T, (int)ws, 0, (int)xs);
+}
+
+// One dword a lane to LDS byte address base + IMM (+ 4 l for lane l), as dma16_lds.
+template <int IMM>
+__device__ __forceinline__ void dma4_lds(u32x4 r, uint32_t base, uint32_t offset) {
+  uint32_t saved;
+  asm volatile(
+      "s_mov_b32 %0, m0\n\t"
+      "s_add_u32 m0, %1, %4\n\t"
+      "buffer_load_dword %2, %3, 0 offen lds\n\t"
+      "s_mov_b32 m0, %0"
+      : "=&s"(saved)
+      : "s"(base), "v"(offset), "s"(r), "i"(IMM)
+      : "memory", "scc");
 }
 
 // The e8m0 byte of the smallest power of two s >= 2^-126 with amax <= most * s (amax finite), most = 448 or 6:

@@ -14,12 +14,13 @@ lse::Fp4Plan plan_of(const lse_fp4_gemm_args& p) {
   lse::Fp4Plan plan{0, 0, 1, (int)chunks};
   if (p.M <= 64) return plan;
   auto blocks = [&](int bm, int bn) { return lse::ceil_div(p.M, bm) * lse::ceil_div(nrb, bn / 16); };
-  if (blocks(256, 256) >= 192)
+  if (blocks(256, 256) >= 192) {
     plan.bm = plan.bn = 256;
-  else if (blocks(128, 128) >= 256)
-    plan.bm = plan.bn = 128;
-  else
+  } else if (blocks(256, 256) >= 96 && chunks >= 16) {
+    plan.bm = plan.bn = 256, plan.chunks = (int)lse::ceil_div(chunks, 2), plan.splits = 2;
+  } else {
     plan.bm = 64, plan.bn = 128;
+  }
   return plan;
 }
 

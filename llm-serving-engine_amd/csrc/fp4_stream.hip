@@ -125,16 +125,10 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
   Step st[4];
   Scales cur, next;
   load_scales(wave, cur);
-  auto each = [](auto&& f) {
-    f(std::integral_constant<int, 0>{});
-    f(std::integral_constant<int, 1>{});
-    f(std::integral_constant<int, 2>{});
-    f(std::integral_constant<int, 3>{});
-  };
-  each([&](auto t) { load_step(wave, t, st[t]); });
+  unroll<4>([&](auto t) { load_step(wave, t, st[t]); });
   for (int it = 0; it < iters; ++it) {
     const int c = wave + W * (it + 1);
-    each([&](auto t) {
+    unroll<4>([&](auto t) {
       // All but the three later steps' loads have landed, the slab among them.
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * LOADS));
       compute(t, st[t], cur);

@@ -1,11 +1,10 @@
 // Products of many rows with a 4-bit weight (layouts and formats: fp4.h; the arithmetic as in fp4_stream.hip), bound by
 // the matrix cores.
 //
-// A workgroup of WGM x WGN waves computes BM token rows x BN weight rows over K, in stages of 256 bytes of a token row
-// (128 k of bf16, 256 k of 8-bit codes). Token rows go to LDS by direct loads (whole 256-byte row pieces, 16-byte
-// chunks swizzled by row), NST - 1 stages ahead; the weight, a quarter or a half of their bytes, goes straight to the
-// registers of the wave that multiplies it, as far ahead: each wave needs BN / WGN rows of it and no other wave of its
-// row of waves does. One barrier a stage. bf16 rows: a wave decodes its weight tiles (half an instruction a weight,
+// A workgroup of WGM x WGN waves computes BM token rows x BN weight rows over K, in stages of 128 k. Token rows go to LDS
+// by direct loads (whole 256 or 128 byte row pieces, 16-byte chunks swizzled by row), NST - 1 stages ahead; the weight,
+// a quarter or a half of their bytes, goes straight to the registers of the wave that multiplies it, as far ahead: each
+// wave needs BN / WGN rows of it and no other wave of its row of waves does. One barrier a stage. bf16 rows: a wave decodes its weight tiles (half an instruction a weight,
 // shared by its WM token rows) and runs 16x16x32 bf16 instructions. 8-bit rows: codes and scale bytes of both operands
 // go to the scaled 16x16x128 instruction as they are.
 //
@@ -13,6 +12,9 @@
 // token blocks x consecutive weight panels, so that what it runs at once shares token rows and weights in its L2.
 // K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order.
 // A result depends on K and the split alone, never on other rows.
+//
+// The direct loads are issued by inline assembly (dma16_lds), so that the only waits on them are the ones written here:
+// tracked, the compiler waited for all of them before most LDS reads. It still counts the weights' loads, in order.
 #include <algorithm>
 
 #include "fp4.h"
@@ -26,20 +28,17 @@ __global__ void __launch_bounds__(64 * WGM * WGN)
 fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   static_assert(WM % 16 == 0 && WN % 16 == 0 && (!GLU || TN % 2 == 0), "whole tiles, and pairs of row tiles");
-  static_assert(NST == 2 || NST == 4, "stage slots");
   constexpr int ESZ = A8 ? 1 : 2;
-  constexpr int SUB = A8 ? 2 : 1;            // 128-k steps of a stage
-  constexpr int CS = 4 / SUB;                // stages of a 512-k chunk
-  constexpr int U = CS > NST ? CS : NST;     // stages of the unrolled loop body: whole chunks, whole rings
-  constexpr int XI = BM / (4 * W);           // 1 KB loads (4 rows) of a wave and stage
-  constexpr int XSI = A8 ? (BM + 32 * W - 1) / (32 * W) : 0;  // scale loads (32 rows) of a wave and stage
-  static_assert(BM % (4 * W) == 0, "whole 1 KB loads per wave");
-  constexpr int SLOT = BM * 16;              // uint4 of a stage's rows
-  constexpr int XS = A8 ? 64 * W * XSI : 1;  // dwords of a stage's scales: two a row
-  __shared__ uint4 x0[SLOT], x1[SLOT], x2[NST > 2 ? SLOT : 1], x3[NST > 2 ? SLOT : 1];
-  __shared__ uint32_t s0[XS], s1[XS], s2[NST > 2 ? XS : 1], s3[NST > 2 ? XS : 1];
-  auto slot = [&](int i) -> uint4* { return i == 0 ? x0 : i == 1 ? x1 : i == 2 ? x2 : x3; };
-  auto sslot = [&](int i) -> uint32_t* { return i == 0 ? s0 : i == 1 ? s1 : i == 2 ? s2 : s3; };
+  constexpr int ROWB = kFp4Step * ESZ, CH = ROWB / 16;  // bytes of a token row and stage, its 16-byte chunks
+  constexpr int RPL = 1024 / ROWB;                      // rows of a 1 KB load
+  constexpr int XI = BM / (RPL * W);                    // such loads of a wave and stage
+  constexpr int XSI = A8 ? (BM + 64 * W - 1) / (64 * W) : 0;  // loads of 64 rows' scale dwords, likewise
+  static_assert(BM % (RPL * W) == 0 && RPL * W % 16 == 0, "whole loads per wave, whose lanes' chunks do not differ");
+  constexpr int SLOT = BM * CH;                         // uint4 of a stage's rows
+  constexpr int XS = A8 ? 64 * W * XSI : 1;             // dwords of a stage's scales
+  __shared__ uint4 xlds[NST * SLOT];
+  __shared__ uint32_t slds[NST * XS];
+  auto swz = [](int r) { return A8 ? (r & 7) ^ ((r >> 3) & 1) : r & 15; };
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -54,59 +53,63 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const int gm = min(p.mblocks - first, kFp4GroupM), tg = t - group * kFp4GroupM * p.nblocks;
   const int m0 = (first + tg % gm) * BM, rb0 = tg / gm * (BN / 16);
   const int rows = min(BM, a.M - m0);
-  // Chunks [c0, c1) of K, and its stages counted from c0.
+  // Chunks [c0, c1) of K, and its steps (stages) counted from c0.
   const int c0 = sp * p.chunks, c1 = min(c0 + p.chunks, a.nchunks);
-  const int nsteps = min(4 * c1, a.nsteps) - 4 * c0, stages = (nsteps + SUB - 1) / SUB;
+  const int stages = min(4 * c1, a.nsteps) - 4 * c0;
 
-  const BufferRsrc xres = make_rsrc(static_cast<const char*>(a.x) + (int64_t)m0 * a.ldx * ESZ,
-                                    (uint32_t)(((int64_t)(rows - 1) * a.ldx + a.K) * ESZ));
+  const u32x4 xres = make_rsrc4(static_cast<const char*>(a.x) + (int64_t)m0 * a.ldx * ESZ,
+                                (uint32_t)(((int64_t)(rows - 1) * a.ldx + a.K) * ESZ));
   const int per4 = (a.K / kFp4Group + 3) & ~3;  // scale bytes of a row in whole dwords
-  const BufferRsrc sres = A8 ? make_rsrc(a.xs + (int64_t)m0 * a.lds, (uint32_t)((int64_t)(rows - 1) * a.lds + per4))
-                             : make_rsrc(a.x, 0);
-  // This wave's row tiles; those past the weight repeat its last one, and are not stored.
-  const uint8_t *wp[TN], *wsp[TN];
+  const u32x4 sres = A8 ? make_rsrc4(a.xs + (int64_t)m0 * a.lds, (uint32_t)((int64_t)(rows - 1) * a.lds + per4))
+                        : make_rsrc4(a.x, 0);
+  // This wave's row tiles; those past the weight repeat its last one, and are not stored. A tile's step is a scalar
+  // offset from the panel's first tile, so its loads need no address arithmetic of their own.
+  const int tiles = min(BN / 16, a.nrb - rb0);
+  const BufferRsrc wres = make_rsrc(a.codes + (int64_t)rb0 * a.nsteps * kFp4TileBytes,
+                                    (uint32_t)tiles * (uint32_t)a.nsteps * kFp4TileBytes);
+  const BufferRsrc wsres = make_rsrc(a.scales + (int64_t)rb0 * a.nchunks * kFp4ScaleBytes,
+                                     (uint32_t)tiles * (uint32_t)a.nchunks * kFp4ScaleBytes);
+  uint32_t wp[TN], wsp[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const int rb = min(rb0 + wn * TN + j, a.nrb - 1);
-    wp[j] = a.codes + ((int64_t)rb * a.nsteps + 4 * c0) * kFp4TileBytes + 16 * lane;
-    wsp[j] = a.scales + ((int64_t)rb * a.nchunks + c0) * kFp4ScaleBytes + 4 * lane;
+    const uint32_t tile = min(wn * TN + j, tiles - 1);
+    wp[j] = (tile * a.nsteps + 4 * c0) * kFp4TileBytes;
+    wsp[j] = (tile * a.nchunks + c0) * kFp4ScaleBytes;
   }
 
-  // Load i of a wave: rows 4 (wave + W i) .. + 3, lane l its physical chunk l % 16 of row l / 16. W is even, so a lane's
-  // logical chunk depends on i where 4 W i is no multiple of 16.
-  auto load_x = [&](int s, int sl) {
-#pragma unroll
-    for (int i = 0; i < XI; ++i) {
-      const int r = 4 * (wave + W * i) + (lane >> 4), kb = (4 * c0 * kFp4Step * ESZ) + 256 * s + 16 * (r16 ^ (r & 15));
-      const bool ok = s < stages && r < rows && kb < a.K * ESZ;
-      buffer_load16_lds(xres, slot(sl) + 64 * (wave + W * i), ok ? (uint32_t)(r * a.ldx * ESZ + kb) : kOutOfRange);
-    }
-#pragma unroll
-    for (int i = 0; i < XSI; ++i) {
-      const int at = 64 * (wave + W * i) + lane, r = at >> 1, b0 = 16 * c0 + 8 * s + 4 * (at & 1);
-      const bool ok = s < stages && r < rows && b0 < per4;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (LdsPtr)(sslot(sl) + 64 * (wave + W * i)), 4,
-                                               ok ? (uint32_t)(r * a.lds + b0) : kOutOfRange, 0, 0, 0);
+  // Load i of a wave: rows RPL (wave + W i) .. , lane l physical chunk l % CH of row l / CH, whose logical chunk is the
+  // same for every i. Rows past the call's lie past the resource, and read zeros; so does, by its offset, what is past K.
+  const int xr = RPL * wave + lane / CH, xkb = 16 * ((lane % CH) ^ swz(xr));
+  const int kbytes = (a.K - 4 * c0 * kFp4Step) * ESZ;  // of a row from c0 on
+  const uint32_t xoff = (uint32_t)(xr * a.ldx * ESZ + 4 * c0 * kFp4Step * ESZ + xkb);
+  const uint32_t xstep = (uint32_t)(RPL * W * a.ldx * ESZ);
+  const uint32_t soff = (uint32_t)((64 * wave + lane) * a.lds + 16 * c0), sstep = (uint32_t)(64 * W * a.lds);
+  const uint32_t xat = lds_addr(xlds + 64 * wave), sat = lds_addr(slds + 64 * wave);
+  auto load_x = [&](int s, auto slot) {
+    const uint32_t off = ROWB * s + xkb < kbytes ? xoff + ROWB * s : kOutOfRange;
+    unroll<XI>([&](auto i) { dma16_lds<16 * slot * SLOT + 1024 * W * i>(xres, xat, off + i * xstep); });
+    if constexpr (A8) {
+      const uint32_t so = 4 * (4 * c0 + s) < per4 ? soff + 4 * s : kOutOfRange;
+      unroll<XSI>([&](auto i) { dma4_lds<4 * slot * XS + 256 * W * i>(sres, sat, so + i * sstep); });
     }
   };
   struct Weights {
-    uint4 w[SUB][TN];
+    u32x4 w[TN];
   };
-  auto load_w = [&](int s, Weights& st) {
+  auto load_w = [&](int j, Weights& st) {  // step j of the range; past it the last, whose rows are zeros then
+    const uint32_t at = min(j, stages - 1) * kFp4TileBytes;
 #pragma unroll
-    for (int u = 0; u < SUB; ++u) {
-      const int j = min(SUB * s + u, nsteps - 1);
-#pragma unroll
-      for (int n = 0; n < TN; ++n) st.w[u][n] = *reinterpret_cast<const uint4*>(wp[n] + (int64_t)j * kFp4TileBytes);
-    }
+    for (int n = 0; n < TN; ++n)
+      st.w[n] = __builtin_amdgcn_raw_buffer_load_b128(wres, 16 * lane, (int)(wp[n] + at), 0);
   };
   struct Scales {
     uint32_t w[TN];
   };
   auto load_s = [&](int c, Scales& sc) {  // chunk c0 + c
+    const uint32_t at = min(c, c1 - c0 - 1) * kFp4ScaleBytes;
 #pragma unroll
     for (int n = 0; n < TN; ++n)
-      sc.w[n] = *reinterpret_cast<const uint32_t*>(wsp[n] + (int64_t)min(c, c1 - c0 - 1) * kFp4ScaleBytes);
+      sc.w[n] = __builtin_amdgcn_raw_buffer_load_b32(wsres, 4 * lane, (int)(wsp[n] + at), 0);
   };
 
   f32x4 acc[TM][TN];
@@ -117,75 +120,68 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
 
   // Scale bytes past K in the last step's dword, which may be anything, become 0.
   const uint32_t tail = a.K % kFp4Step ? (1u << (8 * (a.K % kFp4Step / kFp4Group))) - 1 : ~0u;
-  auto compute = [&](int s, auto sl, auto phase, const Weights& st, const Scales& sc) {
-    const uint4* xs = slot(sl) + (wm * WM + r16) * 16;
+  // Step j from slot, the chunk's step t.
+  auto compute = [&](int j, auto slot, auto t, const Weights& st, const Scales& sc) {
+    const uint4* xs = xlds + slot * SLOT + (wm * WM + r16) * CH;
     if constexpr (A8) {
+      const uint32_t mask = 4 * c0 + j == a.nsteps - 1 ? tail : ~0u;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const uint2 sd = *reinterpret_cast<const uint2*>(sslot(sl) + 2 * (wm * WM + 16 * i + r16));
-        auto step = [&](auto u, uint32_t d) {
-          if (SUB * s + u >= nsteps) return;
-          if (4 * c0 + SUB * s + u == a.nsteps - 1) d &= tail;
-          const uint4 lo = xs[256 * i + ((8 * u + g) ^ r16)], hi = xs[256 * i + ((8 * u + 4 + g) ^ r16)];
+        const uint32_t d = (slds[slot * XS + wm * WM + 16 * i + r16] & mask) >> (8 * g);
+        const uint4 lo = xs[16 * CH * i + (g ^ swz(r16))], hi = xs[16 * CH * i + ((4 + g) ^ swz(r16))];
 #pragma unroll
-          for (int j = 0; j < TN; ++j)
-            acc[i][j] = mfma_fp4_fp8<(SUB * phase + u) % 4>(st.w[u][j], sc.w[j], lo, hi, d >> (8 * g), acc[i][j]);
-        };
-        step(std::integral_constant<int, 0>{}, sd.x);
-        step(std::integral_constant<int, 1>{}, sd.y);
+        for (int n = 0; n < TN; ++n)
+          acc[i][n] = mfma_fp4_fp8<t>(__builtin_bit_cast(uint4, st.w[n]), sc.w[n], lo, hi, d, acc[i][n]);
       }
     } else {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         bf16x8 w[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          const uint32_t w4[4] = {st.w[0][j].x, st.w[0][j].y, st.w[0][j].z, st.w[0][j].w};
-          w[j] = fp4_decode8(w4[q], fp4_scale(sc.w[j], phase % 4));
-        }
+        for (int n = 0; n < TN; ++n) w[n] = fp4_decode8(st.w[n][q], fp4_scale(sc.w[n], t));
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const bf16x8 xv = as_bf16x8(xs[256 * i + ((4 * g + q) ^ r16)]);
+          const bf16x8 xv = as_bf16x8(xs[16 * CH * i + ((4 * g + q) ^ swz(r16))]);
 #pragma unroll
-          for (int j = 0; j < TN; ++j) acc[i][j] = mfma16x16x32(w[j], xv, acc[i][j]);
+          for (int n = 0; n < TN; ++n) acc[i][n] = mfma16x16x32(w[n], xv, acc[i][n]);
         }
       }
     }
   };
 
-  constexpr int LOADS = XI + XSI + SUB * TN;
+  // NST register sets of weights, each refilled when its step is done. Issued after a stage's rows when that stage
+  // begins: the rows of the NST - 2 later stages, and the weights of the NST - 1.
+  constexpr int XLOADS = XI + XSI, LATER = (NST - 1) * TN + (NST - 2) * XLOADS;
+  static_assert(LATER < 64, "vmcnt holds at most 63");
+  constexpr int U = NST == 3 ? 12 : 4;  // stages of the loop body: whole chunks, whole rings
+  static_assert(U % NST == 0, "whole rings");
   Weights st[NST];
-  Scales sc[U / CS], next[U / CS];
+  Scales sc, next;
+  load_s(0, sc);
+  unroll<NST - 1>([&](auto i) { load_x(i, i); });
 #pragma unroll
-  for (int c = 0; c < U / CS; ++c) load_s(c, sc[c]);
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i) {
-    load_x(i, i);
-    load_w(i, st[i]);
-  }
-  for (int base = 0; base < stages; base += U) {
-    auto stage = [&](auto u) {
-      constexpr int sl = u % NST, ahead = (u + NST - 1) % NST;
+  for (int i = 0; i < NST; ++i) load_w(i, st[i]);
+  auto body = [&](int base, auto whole) {
+    unroll<U>([&](auto u) {
+      constexpr int slot = u % NST, ahead = (u + NST - 1) % NST;
       const int s = base + u;
-      if (s >= stages) return;
+      if (!whole && s >= stages) return;
+      asm volatile("" ::: "memory");  // the reads of the stage before stay before the barrier
       // This wave's rows of stage s have landed and its reads of the slot that the loads below go to are done; after
       // the barrier every wave's are.
-      __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm((NST - 2) * LOADS));
+      __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(LATER));
       __builtin_amdgcn_s_barrier();
-      load_x(s + NST - 1, ahead);
-      load_w(s + NST - 1, st[ahead]);
-      if constexpr (u == 0) {
-#pragma unroll
-        for (int c = 0; c < U / CS; ++c) load_s((base + U) / CS + c, next[c]);
-      }
-      compute(s, std::integral_constant<int, sl>{}, u, st[sl], sc[u / CS]);
-    };
-    [&]<int... I>(std::integer_sequence<int, I...>) {
-      (stage(std::integral_constant<int, I>{}), ...);
-    }(std::make_integer_sequence<int, U>{});
-#pragma unroll
-    for (int c = 0; c < U / CS; ++c) sc[c] = next[c];
-  }
+      if constexpr (u % 4 == 0) load_s(s / 4 + 1, next);
+      load_x(s + NST - 1, std::integral_constant<int, ahead>{});
+      compute(s, std::integral_constant<int, slot>{}, std::integral_constant<int, u % 4>{}, st[slot], sc);
+      load_w(s + NST, st[slot]);
+      if constexpr (u % 4 == 3) sc = next;
+    });
+  };
+  // Whole groups without tests between their stages, which would make the compiler wait for every load; then the rest.
+  int base = 0;
+  for (; base + U <= stages; base += U) body(base, std::true_type{});
+  if (base < stages) body(base, std::false_type{});
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
 
   // D tile (i, j): lane holds weight rows 4 g + r (r = 0..3) of token row r16.
@@ -260,8 +256,6 @@ static int launch(const Fp4Args& a, const Fp4Plan& plan, float* part, hipStream_
   };
   if (plan.bm == 256)
     go(fp4_tile_kernel<A8, 256, 256, 2, 4, 2, GLU>, 512);
-  else if (plan.bm == 128)
-    go(fp4_tile_kernel<A8, 128, 128, 2, 2, 2, GLU>, 256);
   else
     go(fp4_tile_kernel<A8, 64, 128, 1, 4, 4, GLU>, 256);
   if (p.splits > 1) {
