@@ -84,6 +84,19 @@ __device__ __forceinline__ void dma4_lds(u32x4 r, uint32_t base, uint32_t offset
       : "memory", "scc");
 }
 
+// Rows of one step in LDS: 256 (bf16) or 128 (codes) bytes, their 16-byte chunk c at c ^ fp4_swz(row), rows in 16s. A
+// wave reads a chunk of 16 rows, lane l of row l % 16 chunk 4 (l / 16) + i (bf16) or 4 i + l / 16 (codes), and the LDS
+// serves a 16-byte read as four groups of 16 lanes: 0-3, 12-15 and 20-27, 4-11, 16-19 and 28-31, and the same 32 lanes
+// on. So rows {0-3, 12-15} of one l / 16 meet rows {4-11} of its neighbour, and either set has to fill whole pairs of
+// the places that the neighbour's chunk changes (by 4, or 1). With row & 15, or the other kernels' spread of 128-byte
+// rows, a read cost 4 conflict cycles more (SQ_LDS_BANK_CONFLICT).
+template <bool A8>
+__host__ __device__ constexpr int fp4_swz(int row) {
+  if (!A8) return (row & 15) ^ ((row & 4) << 1);
+  const int q = row >> 1 & 7;
+  return ((q >> 2 ^ q >> 1) & 1) << 2 | (q >> 2) << 1 | (q & 1);
+}
+
 // The e8m0 byte of the smallest power of two s >= 2^-126 with amax <= most * s (amax finite), most = 448 or 6:
 // (1 + m) 2^p, one more than amax's exponent - p where its mantissa is above m.
 __device__ __forceinline__ int fp8_scale_byte(float amax) {  // 1.75 x 2^8
@@ -117,7 +130,8 @@ struct Fp4Args {
   int nrb;               // row tiles of the weight
 };
 
-// How a call runs: bm 0: the streaming kernel; otherwise tiles of bm x bn, K in `splits` ranges of `chunks` chunks.
+// How a call runs: bm 0: the streaming kernel, bn / 16 row tiles a workgroup; otherwise tiles of bm x bn, K in `splits`
+// ranges of `chunks` chunks.
 struct Fp4Plan {
   int bm, bn, splits, chunks;
 };
@@ -127,7 +141,7 @@ struct Fp4Split {
   float* part;  // splits > 1: [splits][M][16 nrb] sums
 };
 
-int launch_fp4_stream(const Fp4Args& a, bool rows8, bool glu, hipStream_t stream);
+int launch_fp4_stream(const Fp4Args& a, int rt, bool rows8, bool glu, hipStream_t stream);
 int launch_fp4_tile(const Fp4Args& a, const Fp4Plan& plan, bool rows8, bool glu, float* part, hipStream_t stream);
 
 }  // namespace lse

@@ -1,4 +1,6 @@
 // The C entry points of the products with 4-bit weights: argument checks, and which kernel a call takes.
+#include <algorithm>
+
 #include "fp4.h"
 
 namespace {
@@ -8,20 +10,61 @@ constexpr int64_t kMax31 = 2147483647;
 
 int64_t row_tiles(const lse_fp4_gemm_args& p) { return (p.glu ? 2 : 1) * lse::ceil_div(p.N, 16); }
 
-// Which kernel a call takes, from its sizes alone.
+// Microseconds that a call takes apart from the weight's way from HBM, for the tile kernels by stages (128 k of one tile
+// on each CU), for the streaming kernel by what a CU reads through its L1: fitted to about 150 timed calls of both kinds
+// of rows (M 1 to 2048, N 1024 to 28672, K 4096 and 14336), of which the better kernel was missed by 5 % in the mean.
+struct Tile {
+  int bm, bn;
+  int slots;             // workgroups that run at once on 256 CUs
+  double one[2], all[2]; // of a stage, bf16 and 8-bit rows: one workgroup a CU, and all slots taken
+};
+constexpr Tile kTiles[] = {{32, 128, 512, {0.37, 0.33}, {0.65, 0.45}},
+                           {64, 128, 512, {0.55, 0.42}, {0.92, 0.62}},
+                           {128, 256, 256, {1.50, 0.96}, {1.50, 0.96}},
+                           {256, 256, 256, {2.80, 1.62}, {2.80, 1.62}}};
+constexpr double kLaunchUs = 2.5, kHbmBytesPerUs = 4.5e6, kL1BytesPerUs = 52e3, kSecondPassUs = 3.0,
+                 kPartBytesPerUs = 4e6;
+constexpr int64_t kMaxPartBytes = 64 << 20;
+
+// Which kernel a call takes, from its sizes alone: the one whose time is estimated the shortest.
 lse::Fp4Plan plan_of(const lse_fp4_gemm_args& p) {
+  const bool rows8 = p.x_scales != nullptr;
   const int64_t nrb = row_tiles(p), chunks = lse::ceil_div(p.K, lse::kFp4Chunk);
-  lse::Fp4Plan plan{0, 0, 1, (int)chunks};
-  if (p.M <= 64) return plan;
-  auto blocks = [&](int bm, int bn) { return lse::ceil_div(p.M, bm) * lse::ceil_div(nrb, bn / 16); };
-  if (blocks(256, 256) >= 192) {
-    plan.bm = plan.bn = 256;
-  } else if (blocks(256, 256) >= 96 && chunks >= 16) {
-    plan.bm = plan.bn = 256, plan.chunks = (int)lse::ceil_div(chunks, 2), plan.splits = 2;
-  } else {
-    plan.bm = 64, plan.bn = 128;
+  const int narrow = p.glu ? 2 : 1;
+  // Few rows: the narrowest panels, since x costs next to nothing.
+  lse::Fp4Plan best{0, 16 * narrow, 1, (int)chunks};
+  if (p.M <= (rows8 ? 8 : 4)) return best;
+  const int64_t stages = lse::ceil_div(p.K, lse::kFp4Step);
+  const double weight = 16.0 * nrb * stages * 68, hbm = weight / kHbmBytesPerUs;
+  double least = 1e30;
+  auto take = [&](double us, int bm, int bn, int64_t splits, int64_t per) {
+    if (us < least) least = us, best = {bm, bn, (int)splits, (int)per};
+  };
+  const int64_t groups = lse::ceil_div(p.M, 16);
+  for (int rt = 4; rt >= narrow; rt /= 2) {
+    const double workgroups = (double)lse::ceil_div(nrb, rt) * groups;
+    const double rows = p.M < 16 ? p.M : 16;
+    const double bytes = stages * (rows * (rows8 ? 132.0 : 256.0) + rt * 16 * 68.0);
+    const double us = kLaunchUs + std::max(hbm, std::max(1.0, workgroups / 256) * bytes / kL1BytesPerUs);
+    take(us, 0, 16 * rt, 1, chunks);
   }
-  return plan;
+  for (const Tile& t : kTiles) {
+    if (p.M <= 16 && (t.bm > 32 || !rows8)) continue;
+    const int64_t tiles = lse::ceil_div(p.M, t.bm) * lse::ceil_div(nrb, t.bn / 16);
+    for (int64_t splits = 1; splits <= 8; splits *= 2) {
+      const int64_t per = lse::ceil_div(chunks, splits), ranges = lse::ceil_div(chunks, per);
+      if (splits > 1 && (ranges != splits || per < 2)) break;
+      const double part = 64.0 * nrb * p.M * splits;
+      if (splits > 1 && part > kMaxPartBytes) break;
+      const int64_t blocks = tiles * splits, full = blocks / t.slots, rest = blocks % t.slots;
+      const double last = rest == 0 ? 0.0 : rest <= 256 ? t.one[rows8] : t.all[rows8];
+      double us = std::min<double>(stages, 4 * per) * (full * t.all[rows8] + last);
+      us = kLaunchUs + std::max(hbm, us);
+      if (splits > 1) us += kSecondPassUs + 2 * part / kPartBytesPerUs;
+      take(us, t.bm, t.bn, splits, per);
+    }
+  }
+  return best;
 }
 
 }  // namespace
@@ -63,7 +106,7 @@ int lse_fp4_gemm(const struct lse_fp4_gemm_args* args, void* workspace, int64_t 
   a.nsteps = (int)lse::ceil_div(p.K, lse::kFp4Step), a.nchunks = (int)lse::ceil_div(p.K, lse::kFp4Chunk);
   a.nrb = (int)row_tiles(p);
   const lse::Fp4Plan plan = plan_of(p);
-  if (plan.bm == 0) return lse::launch_fp4_stream(a, rows8, p.glu != 0, (hipStream_t)stream);
+  if (plan.bm == 0) return lse::launch_fp4_stream(a, plan.bn / 16, rows8, p.glu != 0, (hipStream_t)stream);
   if (plan.splits > 1 && (!workspace || workspace_bytes < lse_fp4_gemm_workspace_bytes(args) || !aligned16(workspace)))
     return LSE_E_WORKSPACE;
   return lse::launch_fp4_tile(a, plan, rows8, p.glu != 0, (float*)workspace, (hipStream_t)stream);

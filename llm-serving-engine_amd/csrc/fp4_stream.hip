@@ -17,14 +17,11 @@
 
 namespace lse {
 
-constexpr int kFp4Waves = 8;
-
 // XR: rows of a slab (16, or fewer where the call has fewer). RT: row tiles of a workgroup.
-template <bool A8, int XR, int RT, bool GLU>
-__global__ void __launch_bounds__(64 * kFp4Waves)
+template <bool A8, int XR, int RT, int W, bool GLU>
+__global__ void __launch_bounds__(64 * W)
 fp4_stream_kernel(Fp4Args a, int panels, int groups) {
   static_assert(!GLU || RT % 2 == 0, "gate/up panels hold whole pairs of row tiles");
-  constexpr int W = kFp4Waves;
   constexpr int ESZ = A8 ? 1 : 2;
   constexpr int ROWB = kFp4Step * ESZ;       // bytes of a slab row
   constexpr int CH = ROWB / 16;              // its 16-byte chunks
@@ -34,7 +31,7 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
   __shared__ uint4 x0[W * WAVE], x1[W * WAVE], x2[W * WAVE], x3[W * WAVE];
   __shared__ f32x4 red[W][RT][64];
   auto slab = [&](int t) -> uint4* { return t == 0 ? x0 : t == 1 ? x1 : t == 2 ? x2 : x3; };
-  auto swz = [](int r) { return A8 ? (r & 7) ^ ((r >> 3) & 1) : r & 15; };
+  constexpr auto swz = fp4_swz<A8>;
 
   // Workgroup (panel, token group): panel = 8 q + xcd, the groups of a panel 8 apart.
   const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
@@ -96,21 +93,29 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
     }
   };
 
+  // Where this lane's operands lie in a slab. The compiler is kept from taking the sums apart: it follows an LDS access
+  // to its array, and so tells the slab that a load fills from those that are read, through a few additions only.
+  int at[A8 ? 2 : 4];
+#pragma unroll
+  for (int i = 0; i < (A8 ? 2 : 4); ++i) {
+    const int row = r16 & (XR - 1);
+    at[i] = wave * WAVE + row * CH + ((A8 ? 4 * i + g : 4 * g + i) ^ swz(row));
+    asm volatile("" : "+v"(at[i]));
+  }
+
   f32x4 acc[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) acc[rt] = f32x4{0, 0, 0, 0};
   auto compute = [&](auto t, const Step& st, const Scales& s) {
-    const int row = r16 & (XR - 1);
-    const uint4* xw = slab(t) + wave * WAVE + row * CH;
     if constexpr (A8) {
-      const uint4 lo = xw[g ^ swz(row)], hi = xw[(4 + g) ^ swz(row)];
+      const uint4 lo = slab(t)[at[0]], hi = slab(t)[at[1]];
       const uint32_t xs = s.x[t] >> (8 * g);
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) acc[rt] = mfma_fp4_fp8<t>(st.w[rt], s.w[rt], lo, hi, xs, acc[rt]);
     } else {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const bf16x8 xv = as_bf16x8(xw[(4 * g + i) ^ swz(row)]);
+        const bf16x8 xv = as_bf16x8(slab(t)[at[i]]);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt) {
           const uint32_t w4[4] = {st.w[rt].x, st.w[rt].y, st.w[rt].z, st.w[rt].w};
@@ -125,9 +130,12 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
   Step st[4];
   Scales cur, next;
   load_scales(wave, cur);
-  unroll<4>([&](auto t) { load_step(wave, t, st[t]); });
-  for (int it = 0; it < iters; ++it) {
-    const int c = wave + W * (it + 1);
+  unroll<4>([&](auto t) {
+    load_step(wave, t, st[t]);
+    __builtin_amdgcn_sched_barrier(0);
+  });
+  for (int it = 1; it < iters; ++it) {
+    const int c = wave + W * it;
     unroll<4>([&](auto t) {
       // All but the three later steps' loads have landed, the slab among them.
       __builtin_amdgcn_s_waitcnt(vmcnt_imm(3 * LOADS));
@@ -136,10 +144,14 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
       __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(63));
       if constexpr (t == 0) load_scales(c, next);
       load_step(c, t, st[t]);
+      __builtin_amdgcn_sched_barrier(0);  // the loads stay in this order, by which they are counted
     });
     cur = next;
   }
-  __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  unroll<4>([&](auto t) {
+    __builtin_amdgcn_s_waitcnt(vmcnt_imm((3 - t) * LOADS));
+    compute(t, st[t], cur);
+  });
 
   // The waves' sums, added in wave order: wave i adds tile i (gate/up: pair i).
 #pragma unroll
@@ -172,22 +184,23 @@ fp4_stream_kernel(Fp4Args a, int panels, int groups) {
 }
 
 template <bool A8, bool GLU>
-static int launch(const Fp4Args& a, hipStream_t stream) {
-  const int groups = (int)ceil_div(a.M, 16);
-  // The widest panel that leaves a workgroup for each of the 256 CUs.
-  int rt = 4;
-  while (rt > (GLU ? 2 : 1) && ceil_div(a.nrb, rt) * groups < 256) rt /= 2;
-  const int panels = (int)ceil_div(a.nrb, rt);
+static int launch(const Fp4Args& a, int rt, hipStream_t stream) {
+  const int groups = (int)ceil_div(a.M, 16), panels = (int)ceil_div(a.nrb, rt);
   const int64_t blocks = ceil_div(panels, 8) * 8 * groups;
   if (blocks > 2147483647) return LSE_E_RANGE;
-  auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * kFp4Waves), 0, stream, a, panels, groups);
+  auto go = [&](auto kernel, int waves) {
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(64 * waves), 0, stream, a, panels, groups);
     return launch_status();
   };
-  constexpr int FEW = A8 ? 8 : 4;
-  auto width = [&](auto RTc) {
-    constexpr int RT = decltype(RTc)::value;
-    return a.M <= FEW ? go(fp4_stream_kernel<A8, FEW, RT, GLU>) : go(fp4_stream_kernel<A8, 16, RT, GLU>);
+  constexpr int FEW = A8 ? 8 : 4, NARROW = GLU ? 2 : 1;
+  if (a.M <= FEW) return go(fp4_stream_kernel<A8, FEW, NARROW, 8, GLU>, 8);
+  // Four waves hold half the LDS, so that two workgroups share a CU; where there is one for each CU at most, 8-bit rows
+  // are better off with eight (64 rows through 4096 x 4096 6.5 against 7.3 us; bf16 rows 7.4 either way).
+  const bool four = !A8 || panels * groups > 256;
+  auto width = [&](auto RT) {
+    if constexpr (A8)
+      if (!four) return go(fp4_stream_kernel<A8, 16, RT, 8, GLU>, 8);
+    return go(fp4_stream_kernel<A8, 16, RT, 4, GLU>, 4);
   };
   if (rt == 4) return width(std::integral_constant<int, 4>{});
   if constexpr (!GLU)
@@ -195,9 +208,9 @@ static int launch(const Fp4Args& a, hipStream_t stream) {
   return width(std::integral_constant<int, 2>{});
 }
 
-int launch_fp4_stream(const Fp4Args& a, bool rows8, bool glu, hipStream_t stream) {
-  if (rows8) return glu ? launch<true, true>(a, stream) : launch<true, false>(a, stream);
-  return glu ? launch<false, true>(a, stream) : launch<false, false>(a, stream);
+int launch_fp4_stream(const Fp4Args& a, int rt, bool rows8, bool glu, hipStream_t stream) {
+  if (rows8) return glu ? launch<true, true>(a, rt, stream) : launch<true, false>(a, rt, stream);
+  return glu ? launch<false, true>(a, rt, stream) : launch<false, false>(a, rt, stream);
 }
 
 }  // namespace lse

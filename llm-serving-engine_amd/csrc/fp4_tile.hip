@@ -13,8 +13,10 @@
 // K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order.
 // A result depends on K and the split alone, never on other rows.
 //
-// The direct loads are issued by inline assembly (dma16_lds), so that the only waits on them are the ones written here:
-// tracked, the compiler waited for all of them before most LDS reads. It still counts the weights' loads, in order.
+// The compiler counts the weights' loads and waits for them in order, so it has to count the direct loads too, without
+// taking them for writes of the slot that is being read: one array a slot, indexes that it does not take apart (at[]).
+// With two slots (the widest tiles) it still waited for all of them in every stage; there they are issued by inline
+// assembly (dma16_lds), and the only wait on them is the one written here, with nothing later in flight but weights.
 #include <algorithm>
 
 #include "fp4.h"
@@ -36,9 +38,24 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   static_assert(BM % (RPL * W) == 0 && RPL * W % 16 == 0, "whole loads per wave, whose lanes' chunks do not differ");
   constexpr int SLOT = BM * CH;                         // uint4 of a stage's rows
   constexpr int XS = A8 ? 64 * W * XSI : 1;             // dwords of a stage's scales
-  __shared__ uint4 xlds[NST * SLOT];
-  __shared__ uint32_t slds[NST * XS];
-  auto swz = [](int r) { return A8 ? (r & 7) ^ ((r >> 3) & 1) : r & 15; };
+  // One array a slot, so that the compiler tells the slot a load fills from the one that is read.
+  __shared__ uint4 x0[SLOT], x1[SLOT], x2[NST > 2 ? SLOT : 1], x3[NST > 3 ? SLOT : 1], x4[NST > 4 ? SLOT : 1],
+      x5[NST > 4 ? SLOT : 1], x6[NST > 6 ? SLOT : 1], x7[NST > 6 ? SLOT : 1];
+  __shared__ uint32_t s0[XS], s1[XS], s2[NST > 2 ? XS : 1], s3[NST > 3 ? XS : 1], s4[NST > 4 ? XS : 1],
+      s5[NST > 4 ? XS : 1], s6[NST > 6 ? XS : 1], s7[NST > 6 ? XS : 1];
+  auto slot_x = [&](auto i) -> uint4* {
+    if constexpr (i < 4)
+      return i == 0 ? x0 : i == 1 ? x1 : i == 2 ? x2 : x3;
+    else
+      return i == 4 ? x4 : i == 5 ? x5 : i == 6 ? x6 : x7;
+  };
+  auto slot_s = [&](auto i) -> uint32_t* {
+    if constexpr (i < 4)
+      return i == 0 ? s0 : i == 1 ? s1 : i == 2 ? s2 : s3;
+    else
+      return i == 4 ? s4 : i == 5 ? s5 : i == 6 ? s6 : s7;
+  };
+  constexpr auto swz = fp4_swz<A8>;
 
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -57,11 +74,13 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const int c0 = sp * p.chunks, c1 = min(c0 + p.chunks, a.nchunks);
   const int stages = min(4 * c1, a.nsteps) - 4 * c0;
 
-  const u32x4 xres = make_rsrc4(static_cast<const char*>(a.x) + (int64_t)m0 * a.ldx * ESZ,
-                                (uint32_t)(((int64_t)(rows - 1) * a.ldx + a.K) * ESZ));
+  const void* xbase = static_cast<const char*>(a.x) + (int64_t)m0 * a.ldx * ESZ;
+  const uint32_t xbytes = (uint32_t)(((int64_t)(rows - 1) * a.ldx + a.K) * ESZ);
   const int per4 = (a.K / kFp4Group + 3) & ~3;  // scale bytes of a row in whole dwords
-  const u32x4 sres = A8 ? make_rsrc4(a.xs + (int64_t)m0 * a.lds, (uint32_t)((int64_t)(rows - 1) * a.lds + per4))
-                        : make_rsrc4(a.x, 0);
+  const void* sbase = A8 ? a.xs + (int64_t)m0 * a.lds : a.x;
+  const uint32_t sbytes = A8 ? (uint32_t)((int64_t)(rows - 1) * a.lds + per4) : 0;
+  const BufferRsrc xres = make_rsrc(xbase, xbytes), sres = make_rsrc(sbase, sbytes);
+  const u32x4 xres4 = make_rsrc4(xbase, xbytes), sres4 = make_rsrc4(sbase, sbytes);
   // This wave's row tiles; those past the weight repeat its last one, and are not stored. A tile's step is a scalar
   // offset from the panel's first tile, so its loads need no address arithmetic of their own.
   const int tiles = min(BN / 16, a.nrb - rb0);
@@ -84,13 +103,24 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const uint32_t xoff = (uint32_t)(xr * a.ldx * ESZ + 4 * c0 * kFp4Step * ESZ + xkb);
   const uint32_t xstep = (uint32_t)(RPL * W * a.ldx * ESZ);
   const uint32_t soff = (uint32_t)((64 * wave + lane) * a.lds + 16 * c0), sstep = (uint32_t)(64 * W * a.lds);
-  const uint32_t xat = lds_addr(xlds + 64 * wave), sat = lds_addr(slds + 64 * wave);
   auto load_x = [&](int s, auto slot) {
     const uint32_t off = ROWB * s + xkb < kbytes ? xoff + ROWB * s : kOutOfRange;
-    unroll<XI>([&](auto i) { dma16_lds<16 * slot * SLOT + 1024 * W * i>(xres, xat, off + i * xstep); });
+    if constexpr (NST == 2) {
+      unroll<XI>([&](auto i) { dma16_lds<1024 * W * i>(xres4, lds_addr(slot_x(slot) + 64 * wave), off + i * xstep); });
+    } else {
+#pragma unroll
+      for (int i = 0; i < XI; ++i) buffer_load16_lds(xres, slot_x(slot) + 64 * (wave + W * i), off + i * xstep);
+    }
     if constexpr (A8) {
       const uint32_t so = 4 * (4 * c0 + s) < per4 ? soff + 4 * s : kOutOfRange;
-      unroll<XSI>([&](auto i) { dma4_lds<4 * slot * XS + 256 * W * i>(sres, sat, so + i * sstep); });
+      if constexpr (NST == 2) {
+        unroll<XSI>([&](auto i) { dma4_lds<256 * W * i>(sres4, lds_addr(slot_s(slot) + 64 * wave), so + i * sstep); });
+      } else {
+#pragma unroll
+        for (int i = 0; i < XSI; ++i)
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (LdsPtr)(slot_s(slot) + 64 * (wave + W * i)), 4, so + i * sstep,
+                                                   0, 0, 0);
+      }
     }
   };
   struct Weights {
@@ -120,15 +150,23 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
 
   // Scale bytes past K in the last step's dword, which may be anything, become 0.
   const uint32_t tail = a.K % kFp4Step ? (1u << (8 * (a.K % kFp4Step / kFp4Group))) - 1 : ~0u;
+  // Where this lane's operands of the wave's first token tile lie in a slot. The compiler is kept from taking the sums
+  // apart: it follows an LDS access to its array through a few additions only.
+  int at[A8 ? 2 : 4], sat = wm * WM + r16;
+#pragma unroll
+  for (int i = 0; i < (A8 ? 2 : 4); ++i) {
+    at[i] = (wm * WM + r16) * CH + ((A8 ? 4 * i + g : 4 * g + i) ^ swz(r16));
+    asm volatile("" : "+v"(at[i]));
+  }
+  asm volatile("" : "+v"(sat));
   // Step j from slot, the chunk's step t.
   auto compute = [&](int j, auto slot, auto t, const Weights& st, const Scales& sc) {
-    const uint4* xs = xlds + slot * SLOT + (wm * WM + r16) * CH;
     if constexpr (A8) {
       const uint32_t mask = 4 * c0 + j == a.nsteps - 1 ? tail : ~0u;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
-        const uint32_t d = (slds[slot * XS + wm * WM + 16 * i + r16] & mask) >> (8 * g);
-        const uint4 lo = xs[16 * CH * i + (g ^ swz(r16))], hi = xs[16 * CH * i + ((4 + g) ^ swz(r16))];
+        const uint32_t d = (slot_s(slot)[sat + 16 * i] & mask) >> (8 * g);
+        const uint4 lo = slot_x(slot)[at[0] + 16 * CH * i], hi = slot_x(slot)[at[1] + 16 * CH * i];
 #pragma unroll
         for (int n = 0; n < TN; ++n)
           acc[i][n] = mfma_fp4_fp8<t>(__builtin_bit_cast(uint4, st.w[n]), sc.w[n], lo, hi, d, acc[i][n]);
@@ -141,7 +179,7 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
         for (int n = 0; n < TN; ++n) w[n] = fp4_decode8(st.w[n][q], fp4_scale(sc.w[n], t));
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
-          const bf16x8 xv = as_bf16x8(xs[16 * CH * i + ((4 * g + q) ^ swz(r16))]);
+          const bf16x8 xv = as_bf16x8(slot_x(slot)[at[q] + 16 * CH * i]);
 #pragma unroll
           for (int n = 0; n < TN; ++n) acc[i][n] = mfma16x16x32(w[n], xv, acc[i][n]);
         }
@@ -153,8 +191,8 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   // begins: the rows of the NST - 2 later stages, and the weights of the NST - 1.
   constexpr int XLOADS = XI + XSI, LATER = (NST - 1) * TN + (NST - 2) * XLOADS;
   static_assert(LATER < 64, "vmcnt holds at most 63");
-  constexpr int U = NST == 3 ? 12 : 4;  // stages of the loop body: whole chunks, whole rings
-  static_assert(U % NST == 0, "whole rings");
+  constexpr int U = NST % 3 == 0 ? 12 : NST > 4 ? 8 : 4;  // stages of the loop body: whole chunks, whole rings
+  static_assert(U % NST == 0 && (NST == 2 || NST == 3 || NST == 4 || NST == 6 || NST == 8), "whole rings");
   Weights st[NST];
   Scales sc, next;
   load_s(0, sc);
@@ -256,8 +294,12 @@ static int launch(const Fp4Args& a, const Fp4Plan& plan, float* part, hipStream_
   };
   if (plan.bm == 256)
     go(fp4_tile_kernel<A8, 256, 256, 2, 4, 2, GLU>, 512);
-  else
+  else if (plan.bm == 128)
+    go(fp4_tile_kernel<A8, 128, 256, 2, 4, 2, GLU>, 512);
+  else if (plan.bm == 64)
     go(fp4_tile_kernel<A8, 64, 128, 1, 4, 4, GLU>, 256);
+  else
+    go(fp4_tile_kernel<A8, 32, 128, 1, 4, 4, GLU>, 256);
   if (p.splits > 1) {
     if (int st = launch_status()) return st;
     const int64_t quads = (int64_t)a.M * ceil_div(a.N, 4);
