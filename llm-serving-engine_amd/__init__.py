@@ -8,6 +8,7 @@ from . import ops
 from ._lib import LIB_PATH, library
 from .checkpoint import load_int8_checkpoint, save_int8_checkpoint
 from .config import ModelConfig
+from .fp4_linear import Fp4GateUp, Fp4GluMLP, Fp4Linear, Fp8RMSNorm
 from .int8_linear import (
     Int8GateUp,
     Int8GluMLP,
@@ -21,6 +22,10 @@ from .quantize import check_int8_support, quantize_model_
 
 __all__ = [
     "LIB_PATH",
+    "Fp4GateUp",
+    "Fp4GluMLP",
+    "Fp4Linear",
+    "Fp8RMSNorm",
     "Int8GateUp",
     "Int8GluMLP",
     "Int8Linear",

@@ -29,6 +29,7 @@ import torch
 from torch import nn
 
 from . import ops
+from .fp4_linear import Fp4GateUp, Fp4Linear
 from .int8_linear import (Int8GateUp, Int8GluMLP, Int8Linear, Int8RMSNormQuant, PackedBf16Linear,
                           group_qkv)
 
@@ -55,6 +56,9 @@ def _quantized_tensors(model: nn.Module) -> tuple[dict[str, torch.Tensor], str]:
     and the model's mode."""
     out: dict[str, torch.Tensor] = {}
     modes = set()
+
+    if any(isinstance(m, (Fp4Linear, Fp4GateUp)) for m in model.modules()):
+        raise RuntimeError("the int8 checkpoint format holds no 4-bit weights")
 
     def put(prefix: str, mod: Int8Linear) -> None:
         out[f"{prefix}.qweight"] = mod.unpacked_qweight().cpu()

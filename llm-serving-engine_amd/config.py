@@ -2,8 +2,8 @@
 
 Field names, defaults and env-var names follow the reference so a deployment's environment
 carries over. `quantize` takes "none", "int8" (weight-only W8A16, the reference's meaning at
-model_runner.py:45-46) or "w8a8" (dynamic per-token activations). The int8 kernels compute in
-bf16, so `dtype` must be "bfloat16" whenever `quantize` is not "none".
+model_runner.py:45-46), "w8a8" (dynamic per-token activations), "w4a16" (4-bit weights) or "w4a8" (4-bit weights, rows in
+8 bits). The kernels compute in bf16, so `dtype` must be "bfloat16" whenever `quantize` is not "none".
 """
 
 from __future__ import annotations
@@ -11,7 +11,7 @@ from __future__ import annotations
 import os
 from dataclasses import dataclass
 
-QUANTIZE_MODES = ("none", "int8", "w8a8")
+QUANTIZE_MODES = ("none", "int8", "w8a8", "w4a16", "w4a8")
 
 
 def _env_str(name: str, default: str) -> str:
@@ -27,7 +27,7 @@ class ModelConfig:
     model_name_or_path: str = "unsloth/Llama-3.2-3B-Instruct"
     device: str = "cuda"
     dtype: str = "float16"
-    quantize: str = "none"  # "none", "int8" (W8A16) or "w8a8"
+    quantize: str = "none"  # "none", "int8" (W8A16), "w8a8", "w4a16" or "w4a8"
     use_custom_kernels: bool = True
     use_cuda_graphs: bool = True
 

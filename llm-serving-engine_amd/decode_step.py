@@ -18,6 +18,9 @@ applies o_proj (`attention_output`, model_runner.py:365-369).
     weight stream whose epilogue applies the MLP's SiLU-mul, so the (M, 28672) projection never
     leaves the kernel. Per-channel quantization of a row-stacked weight equals quantizing each
     part;
+  * "fp4" (`quantize("w4a16")` or `quantize("w4a8")`): `Fp4Linear` and `Fp4GateUp` in the same places, 4-bit weights with
+    a power of two for every 32; in "w4a8" the norms give rows in 8 bits with the residual's addition
+    (`ops.add_rmsnorm_fp8`), and o_proj and down_proj round theirs (`ops.quantize_rows_fp8`);
   * "int8-torch": the same quantized weights, applied by an eager torch restatement of each
     module's own arithmetic instead of the HIP kernels (`restate`: W8A16 s·Σ x·q in fp32, W8A8
     per-token quantization, exact integer sums and (acc·sx)·s; gate/up as fp32 g and u with
@@ -30,7 +33,7 @@ output), so each layer's kernels can be checked on the very input they saw (erro
 compound over layers).
 lm_head stays bf16 in every back end: the vendor BLAS's `nn.Linear` on "bf16" and "int8-torch",
 `PackedBf16Linear` (the same bf16 weight in the packed tile layout, `quantize_model_`'s default)
-on "int8", in either quantization mode. Attention has two implementations: "torch", fp32 over a
+on "int8" and "fp4", in every quantization mode. Attention has two implementations: "torch", fp32 over a
 contiguous per-layer KV cache (the reference's `contiguous_attention` path,
 model_runner.py:400-418), the same arithmetic for both linear back ends so only the linears
 differ; "paged", the HIP paged attention (`ops.paged_attention_forward`, the reference's
@@ -49,8 +52,9 @@ import torch
 from torch import nn
 from torch.nn.modules import module as nn_module
 
-from . import _lib, ops
-from .int8_linear import Int8GateUp, Int8Linear, PackedBf16Linear
+from . import _lib, fp4_linear, ops
+from .fp4_linear import Fp4GateUp, Fp4Linear
+from .int8_linear import Int8GateUp, Int8Linear, PackedBf16Linear, QuantizedRows
 
 LLAMA3_8B = dict(
     hidden_size=4096,
@@ -97,6 +101,7 @@ class DecodeRunner:
         self.k_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         self.v_cache = [torch.zeros(shape, dtype=torch.bfloat16, device=dev) for _ in self.layers]
         self.int8: list[dict[str, Int8Linear]] | None = None
+        self.fp4: list[dict[str, Fp4Linear | Fp4GateUp]] | None = None
         self.head: PackedBf16Linear | None = None
         self.trace: list | None = None
         self.backend = "bf16"
@@ -223,32 +228,39 @@ class DecodeRunner:
 
     @torch.no_grad()
     def quantize(self, mode: str = "int8") -> None:
-        """Builds the int8 projections from the bf16 weights (kept, for the bf16 back end)."""
-        self.int8 = []
+        """Builds the int8 ("int8", "w8a8") or 4-bit ("w4a16", "w4a8") projections from the bf16 weights (kept, for
+        the bf16 back end)."""
+        fp4 = mode in fp4_linear.MODES
+        linear, gate_up = (_fp4, Fp4GateUp) if fp4 else (_int8, Int8GateUp)
+        built = []
         for layer in self.layers:
             attn, mlp = layer.self_attn, layer.mlp
             qkv = torch.cat([attn.q_proj.weight, attn.k_proj.weight, attn.v_proj.weight])
-            self.int8.append({
-                "qkv": _int8(qkv, mode),
-                "o": _int8(attn.o_proj.weight, mode),
-                "gate_up": Int8GateUp.from_linears(mlp.gate_proj, mlp.up_proj, mode),
-                "down": _int8(mlp.down_proj.weight, mode),
+            built.append({
+                "qkv": linear(qkv, mode),
+                "o": linear(attn.o_proj.weight, mode),
+                "gate_up": gate_up.from_linears(mlp.gate_proj, mlp.up_proj, mode),
+                "down": linear(mlp.down_proj.weight, mode),
             })
             del qkv
+        if fp4:
+            self.fp4 = built
+        else:
+            self.int8 = built
         head = self.model.lm_head
         self.head = head if isinstance(head, PackedBf16Linear) else PackedBf16Linear.from_linear(head)
         torch.cuda.empty_cache()
 
     def use(self, backend: str) -> None:
-        if backend not in ("bf16", "int8", "int8-torch"):
+        if backend not in ("bf16", "int8", "int8-torch", "fp4"):
             raise ValueError(f"unknown back end {backend!r}")
-        if backend != "bf16" and self.int8 is None:
+        if backend != "bf16" and (self.fp4 if backend == "fp4" else self.int8) is None:
             raise RuntimeError("quantize() first")
         self.backend = backend
 
     def _lin(self, i: int, name: str, x: torch.Tensor) -> torch.Tensor:
-        mod = self.int8[i][name]
-        if self.backend != "int8":
+        mod = (self.fp4 if self.backend == "fp4" else self.int8)[i][name]
+        if self.backend == "int8-torch":
             return restate(mod, x)
         y = mod(x)
         if self.trace is not None:
@@ -331,7 +343,13 @@ class DecodeRunner:
         return q.transpose(1, 2).reshape(nseq * ntok, self.n_heads, self.head_dim)
 
     def _add_norm(self, norm: nn.Module, x: torch.Tensor, residual: torch.Tensor | None):
-        """(x + residual, norm(x + residual)), as one kernel where it can be."""
+        """(x + residual, norm(x + residual)), as one kernel where it can be; "w4a8" projections read the second as rows
+        in 8 bits."""
+        rows8 = (self.backend == "fp4" and norm is not self.model.model.norm
+                 and self.fp4[0]["qkv"].mode == "w4a8")
+        if rows8 and self._fused and x.dtype == torch.bfloat16:
+            hidden, rows = ops.add_rmsnorm_fp8(x, residual, norm.weight, norm.variance_epsilon)
+            return hidden, QuantizedRows(rows.codes, rows.scales, x.shape, x.dtype)
         if self._fused and x.dtype == torch.bfloat16 and (residual is None
                                                           or residual.dtype == torch.bfloat16):
             return ops.add_rmsnorm(x, residual, norm.weight, norm.variance_epsilon)
@@ -394,8 +412,8 @@ class DecodeRunner:
         return self.lm_head()(hidden[0])
 
     def lm_head(self) -> nn.Module:
-        """The back end's lm_head: the packed bf16 one on "int8", the model's own otherwise."""
-        return self.head if self.backend == "int8" and self.head is not None else self.model.lm_head
+        """The back end's lm_head: the packed bf16 one on "int8" and "fp4", the model's own otherwise."""
+        return self.head if self.backend in ("int8", "fp4") and self.head is not None else self.model.lm_head
 
     # ---- linear-only timing -------------------------------------------------------------------
 
@@ -419,7 +437,7 @@ class DecodeRunner:
                           (p.gate_proj, x_h), (p.up_proj, x_h), (SiluMul(p.act_fn), x_gu),
                           (p.down_proj, x_i)]
             else:
-                d = self.int8[i]
+                d = (self.fp4 if self.backend == "fp4" else self.int8)[i]
                 calls += [(d["qkv"], x_h), (d["o"], x_h), (d["gate_up"], x_h), (d["down"], x_i)]
         return calls
 
@@ -432,6 +450,9 @@ class DecodeRunner:
             if isinstance(mod, Int8GateUp):  # both weights in, the SiLU-mul product out
                 n = 2 * mod.intermediate_size
                 total += k * n + 4 * n + 2 * m * k + 2 * m * (n // 2)
+            elif isinstance(mod, (Fp4GateUp, Fp4Linear)):  # codes and scales, rows in and out
+                n = mod.intermediate_size if isinstance(mod, Fp4GateUp) else mod.out_features
+                total += mod.qweight.numel() + mod.scales.numel() + 2 * m * k + 2 * m * n
             elif isinstance(mod, SiluMul):  # (M, 2I) in, (M, I) out
                 total += 2 * m * k + m * k
             elif isinstance(mod, Int8Linear):
@@ -498,6 +519,10 @@ def restate(mod: nn.Module, x: torch.Tensor) -> torch.Tensor:
         inter = mod.intermediate_size
         return (torch.nn.functional.silu(gu[..., :inter]) * gu[..., inter:]).to(torch.bfloat16)
     return _restate_f32(mod.mode, x, q, s).to(torch.bfloat16)
+
+
+def _fp4(weight: torch.Tensor, mode: str) -> Fp4Linear:
+    return Fp4Linear.from_quantized(*ops.quantize_weight_fp4(weight), mode)
 
 
 def _int8(weight: torch.Tensor, mode: str) -> Int8Linear:

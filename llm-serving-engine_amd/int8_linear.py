@@ -172,7 +172,7 @@ class QKVGroup:
                  members: list[Int8Linear]) -> None:
         self.qweight, self.scales, self.mode = qweight, scales, mode
         self.members = list(members)
-        self.n = int(scales.shape[0])
+        self.n = sum(m.out_features for m in members)
         self.offsets: dict[int, tuple[int, int]] = {}
         at = 0
         for mod in members:
@@ -210,6 +210,9 @@ class QKVGroup:
             m._buffers["qweight"] = self.qweight[a // 16:b // 16]
             m._buffers["scales"] = self.scales[a:b]
 
+    def _product(self, x) -> torch.Tensor:
+        return _int8_product(self.mode, x, self.qweight, self.scales, self.n)
+
     def columns(self, mod: Int8Linear, x) -> torch.Tensor:
         key = id(mod)
         hit = (self._out is not None and x is self._input and key in self._pending
@@ -217,7 +220,7 @@ class QKVGroup:
         if not hit:
             if not self._members_are_views():
                 self._restack()
-            self._out = _int8_product(self.mode, x, self.qweight, self.scales, self.n)
+            self._out = self._product(x)
             self._input, self._version = x, self._version_of(x)
             self._pending = set(self.offsets)
         out = self._out
@@ -228,29 +231,38 @@ class QKVGroup:
         return out[..., a:b]
 
 
-def group_qkv(attn: nn.Module) -> QKVGroup | None:
-    """Makes `attn`'s q_proj, k_proj and v_proj (Int8Linear, one mode, one input width, row counts
-    multiples of 16, biases all present or all absent) views of one stacked packed weight run by
-    a `QKVGroup`. Returns the group, or None when they do not qualify (they then stay separate)."""
+def group_qkv_as(attn: nn.Module, kind: type, make) -> QKVGroup | None:
+    """Makes `attn`'s q_proj, k_proj and v_proj (all `kind`, one mode, one input width, row counts multiples of 16,
+    biases all present or all absent) members of the group that make([q, k, v]) gives. Returns it, or None when they do
+    not qualify (they then stay separate)."""
     mods = [getattr(attn, n, None) for n in ("q_proj", "k_proj", "v_proj")]
-    if not all(isinstance(m, Int8Linear) for m in mods):
+    if not all(isinstance(m, kind) for m in mods):
         return None
     if (len({m.mode for m in mods}) != 1 or len({m.in_features for m in mods}) != 1
             or any(m.out_features % 16 for m in mods)
             or len({m.bias is None for m in mods}) != 1):
         return None
-    qweight = torch.cat([m.qweight for m in mods])  # row tiles stack: still the tile layout
-    scales = torch.cat([m.scales for m in mods])
-    at = 0
-    for m in mods:
-        rb = m.out_features // 16
-        m._buffers["qweight"] = qweight[at // 16:at // 16 + rb]
-        m._buffers["scales"] = scales[at:at + m.out_features]
-        at += m.out_features
-    group = QKVGroup(qweight, scales, mods[0].mode, mods)
+    group = make(mods)
     for m in mods:
         m.__dict__["_qkv_group"] = group
     return group
+
+
+def group_qkv(attn: nn.Module) -> QKVGroup | None:
+    """Makes `attn`'s q_proj, k_proj and v_proj (Int8Linear, as `group_qkv_as` takes them) views of one stacked packed
+    weight run by a `QKVGroup`."""
+    def make(mods: list[Int8Linear]) -> QKVGroup:
+        qweight = torch.cat([m.qweight for m in mods])  # row tiles stack: still the tile layout
+        scales = torch.cat([m.scales for m in mods])
+        at = 0
+        for m in mods:
+            rb = m.out_features // 16
+            m._buffers["qweight"] = qweight[at // 16:at // 16 + rb]
+            m._buffers["scales"] = scales[at:at + m.out_features]
+            at += m.out_features
+        return QKVGroup(qweight, scales, mods[0].mode, mods)
+
+    return group_qkv_as(attn, Int8Linear, make)
 
 
 def check_linear_supported(linear: nn.Linear) -> None:

@@ -983,8 +983,8 @@ class Fp4Weight(NamedTuple):
     """A 4-bit weight in the tiles that the products stream: float4 e2m1 codes with a power of two (e8m0) for every
     32 consecutive k of a row.
 
-    codes: uint8 (tiles, ceil(K / 128), 1024), scales: float8_e8m0fnu (tiles, ceil(K / 512), 256); n: the columns of
-    the product, k: those of its input. tiles = ceil(n / 16); 2 ceil(n / 16) for the gate and up weights of a
+    codes: uint8 (tiles, ceil(K / 128), 1024), scales: float8_e8m0fnu, or its bytes as uint8, (tiles, ceil(K / 512),
+    256); n: the columns of the product, k: those of its input. tiles = ceil(n / 16); 2 ceil(n / 16) for the gate and up weights of a
     `w4a16_glu` or `w4a8_glu`, whose row tiles take turns. Made by `pack_fp4`."""
 
     codes: torch.Tensor
@@ -1145,7 +1145,7 @@ def _check_fp4(weight: Fp4Weight, glu: bool | None) -> tuple[int, int]:
     """(n, tiles) of a 4-bit weight, its tiles checked; glu None: of either kind."""
     codes, scales, n, k = weight
     tiles = codes.shape[0]
-    if (codes.dtype is not torch.uint8 or scales.dtype is not _E8 or not codes.is_contiguous()
+    if (codes.dtype is not torch.uint8 or scales.dtype not in (_E8, torch.uint8) or not codes.is_contiguous()
             or not scales.is_contiguous() or (codes.data_ptr() | scales.data_ptr()) % 16):
         raise RuntimeError("a 4-bit weight's codes must be uint8 and its scales float8_e8m0fnu, contiguous, 16-byte "
                            "aligned")

@@ -1,4 +1,4 @@
-"""Swaps a loaded Llama-family model's projections for `Int8Linear`, in place.
+"""Swaps a loaded Llama-family model's projections for `Int8Linear` or `Fp4Linear`, in place.
 
 This is the work the reference's int8 switch stands in for: `ModelRunner.__init__` raises
 `NotImplementedError("int8 weight-only quantization")` before loading
@@ -17,8 +17,12 @@ import gc
 import torch
 from torch import nn
 
-from .int8_linear import (MODES, Int8GluMLP, Int8Linear, Int8RMSNormQuant, PackedBf16Linear,
+from . import fp4_linear
+from .fp4_linear import Fp4GluMLP, Fp4Linear, Fp8RMSNorm, group_qkv_fp4
+from .int8_linear import (MODES as INT8_MODES, Int8GluMLP, Int8Linear, Int8RMSNormQuant, PackedBf16Linear,
                           fusable_mlp, group_qkv)
+
+MODES = INT8_MODES + fp4_linear.MODES
 
 ATTENTION_PROJECTIONS = ("q_proj", "k_proj", "v_proj", "o_proj")
 MLP_PROJECTIONS = ("gate_proj", "up_proj", "down_proj")
@@ -49,35 +53,41 @@ def quantize_model_(model: nn.Module, mode: str = "int8", fuse_mlp: bool = True,
     `fuse_qkv` the layer's q, k and v projections share one stacked weight (`QKVGroup`): the
     three module calls the runner makes on one input run as one GEMM. In the W8A8 mode
     (`fuse_norm`, default on for "w8a8") the layer's two RMSNorms become `Int8RMSNormQuant`,
-    which quantizes the normed rows once for all their projections. With `pack_lm_head` a bf16
+    which quantizes the normed rows once for all their projections. The modes "w4a16" and "w4a8" put
+    `Fp4Linear` and `Fp4GluMLP` (4-bit weights, a power of two for every 32) in the same places, and in "w4a8"
+    `Fp8RMSNorm` for the norms, whose rows leave in 8 bits. With `pack_lm_head` a bf16
     `lm_head` without bias becomes `PackedBf16Linear` (same bf16 values, tile layout; a tied
     lm_head keeps its embedding and adds the packed copy). Returns the same model object."""
     if mode not in MODES:
         raise ValueError(f"mode must be one of {MODES}, got {mode!r}")
+    rows8 = mode in ("w8a8", "w4a8")
     if fuse_norm is None:
-        fuse_norm = mode == "w8a8"
-    if fuse_norm and mode != "w8a8":
-        raise ValueError("fuse_norm feeds pre-quantized rows to W8A8 projections only")
+        fuse_norm = rows8
+    if fuse_norm and not rows8:
+        raise ValueError("fuse_norm feeds pre-quantized rows to W8A8 and W4A8 projections only")
     check_int8_support(model)
+    linear_as, mlp_as, norm_as, group = (
+        (Fp4Linear, Fp4GluMLP, Fp8RMSNorm, group_qkv_fp4) if mode in fp4_linear.MODES
+        else (Int8Linear, Int8GluMLP, Int8RMSNormQuant, group_qkv))
     for layer in model.model.layers:
         swaps = [(layer.self_attn, ATTENTION_PROJECTIONS)]
         if fuse_mlp and fusable_mlp(layer.mlp):
-            layer.mlp = Int8GluMLP.from_mlp(layer.mlp, mode)
+            layer.mlp = mlp_as.from_mlp(layer.mlp, mode)
         else:
             swaps.append((layer.mlp, MLP_PROJECTIONS))
         for parent, names in swaps:
             for name in names:
                 linear = getattr(parent, name)
                 if isinstance(linear, nn.Linear):
-                    setattr(parent, name, Int8Linear.from_linear(linear, mode))
+                    setattr(parent, name, linear_as.from_linear(linear, mode))
                     del linear
         if fuse_qkv:
-            group_qkv(layer.self_attn)
+            group(layer.self_attn)
         if fuse_norm:
             for name in ("input_layernorm", "post_attention_layernorm"):
                 norm = getattr(layer, name)
-                if not isinstance(norm, Int8RMSNormQuant):
-                    setattr(layer, name, Int8RMSNormQuant(norm))
+                if not isinstance(norm, norm_as):
+                    setattr(layer, name, norm_as(norm))
     head = getattr(model, "lm_head", None)
     if (pack_lm_head and isinstance(head, nn.Linear) and head.bias is None
             and head.weight.dtype == torch.bfloat16):
