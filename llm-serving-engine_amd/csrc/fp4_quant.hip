@@ -123,11 +123,29 @@ fp8_rows_kernel(const uint16_t* x, int64_t ldx, uint8_t* codes, uint8_t* scales,
 
 constexpr int kNormFp8Threads = 512;
 
-// One workgroup per row, thread t holding elements 8 t + 4096 i (i < NV): s = bf16(x + res) (or x), n = bf16(w *
-// bf16(s * r)), r = 1 / sqrt(mean(s^2) + eps), the roundings of LlamaRMSNorm (modeling_llama.py:62-67), then n's
-// codes and scales. The sum of squares: each thread's in order, then a fixed tree. `sum` may be x or res: a thread
-// reads all of its elements before it writes any.
-template <int NV>
+typedef unsigned u32x2_t __attribute__((ext_vector_type(2)));
+
+// 16-byte loads, and 16- or 8-byte stores, of what a call reads and writes once.
+template <bool STREAM>
+__device__ __forceinline__ uint4 load16_once(const void* p) {
+  return STREAM ? load16_stream(p) : *static_cast<const uint4*>(p);
+}
+template <bool STREAM, typename V>
+__device__ __forceinline__ void store_once(void* p, V v) {
+  if constexpr (STREAM)
+    __builtin_nontemporal_store(v, static_cast<V*>(p));
+  else
+    *static_cast<V*>(p) = v;
+}
+
+// One workgroup per row, of as many waves as its first 4096 values keep busy, thread t holding elements 8 t + 4096 i
+// (i < NV): s = bf16(x + res) (or x), n = bf16(w * bf16(s * r)), r = 1 / sqrt(mean(s^2) + eps), the roundings of
+// LlamaRMSNorm (modeling_llama.py:62-67), then n's codes and scales. The sum of squares: each thread's in order, then a
+// fixed tree, add_rmsnorm_kernel's order. `sum` may be x or res: a thread reads all of its elements before it writes any.
+// Bound by HBM: STREAM, for calls that move much of what the cache behind L2 holds, keeps it from being filled with what
+// is not read again (4160 rows of 4096 30.9 -> 27.6 us, 4.3 TB/s of a copy's 4.7; 2048 of 14336 52.2 -> 51.0), which
+// smaller calls are better off with in the cache (4160 of 1024 16.9 against 21.4, repeated).
+template <int NV, bool STREAM>
 __global__ void __launch_bounds__(kNormFp8Threads)
 add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int64_t ldr, const uint16_t* w, float eps,
                        uint16_t* sum, uint8_t* codes, uint8_t* scales, int64_t lds, int K) {
@@ -139,11 +157,11 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
   for (int i = 0; i < NV; ++i) {
     const int k = 8 * (threadIdx.x + kNormFp8Threads * i);
     const uint4 zero = make_uint4(0, 0, 0, 0);
-    bf16x8_to_f32(k < K ? *reinterpret_cast<const uint4*>(x + m * ldx + k) : zero, s[i]);
+    bf16x8_to_f32(k < K ? load16_once<STREAM>(x + m * ldx + k) : zero, s[i]);
     bf16x8_to_f32(k < K ? *reinterpret_cast<const uint4*>(w + k) : zero, g[i]);
     if (res) {
       float r[8];
-      bf16x8_to_f32(k < K ? *reinterpret_cast<const uint4*>(res + m * ldr + k) : zero, r);
+      bf16x8_to_f32(k < K ? load16_once<STREAM>(res + m * ldr + k) : zero, r);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[i][j] = bf16_to_f32(f32_to_bf16(s[i][j] + r[j]));
     }
@@ -155,9 +173,8 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
     for (int i = 0; i < NV; ++i) {
       const int k = 8 * (threadIdx.x + kNormFp8Threads * i);
       if (k < K)
-        *reinterpret_cast<uint4*>(sum + m * K + k) =
-            make_uint4(pack_bf16x2(s[i][0], s[i][1]), pack_bf16x2(s[i][2], s[i][3]), pack_bf16x2(s[i][4], s[i][5]),
-                       pack_bf16x2(s[i][6], s[i][7]));
+        store_once<STREAM>(sum + m * K + k, u32x4{pack_bf16x2(s[i][0], s[i][1]), pack_bf16x2(s[i][2], s[i][3]),
+                                                  pack_bf16x2(s[i][4], s[i][5]), pack_bf16x2(s[i][6], s[i][7])});
     }
   }
 #pragma unroll
@@ -166,7 +183,8 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
   __syncthreads();
   float total = red[0];
 #pragma unroll
-  for (int i = 1; i < kNormFp8Threads / 64; ++i) total += red[i];
+  for (int i = 1; i < kNormFp8Threads / 64; ++i)
+    if (64 * i < blockDim.x) total += red[i];
   const float r = 1.0f / __builtin_sqrtf(total / (float)K + eps);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
@@ -178,7 +196,7 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
     int byte;
     const uint2 c = fp8_encode8(n, byte);  // every lane: K is a multiple of 32, so groups are whole
     if (k < K) {
-      *reinterpret_cast<uint2*>(codes + m * K + k) = c;
+      store_once<STREAM>(codes + m * K + k, u32x2_t{c.x, c.y});
       if ((threadIdx.x & 3) == 0) scales[m * lds + k / kFp4Group] = (uint8_t)byte;
     }
   }
@@ -269,18 +287,26 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
   if (x.x_stride % 8 || (x.residual && x.residual_stride % 8) || !aligned16(x.x) || !aligned16(x.residual) ||
       !aligned16(x.weight) || !aligned16(x.sum) || !aligned16(x.codes))
     return LSE_E_ALIGN;
-  const dim3 grid((unsigned)x.M), wg(lse::kNormFp8Threads);
+  const int64_t waves = std::min<int64_t>(lse::ceil_div(x.K, 512), lse::kNormFp8Threads / 64);
+  const dim3 grid((unsigned)x.M), wg((unsigned)(64 * waves));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, wg, 0, (hipStream_t)stream, (const uint16_t*)x.x, x.x_stride,
                        (const uint16_t*)x.residual, x.residual_stride, (const uint16_t*)x.weight, (float)x.eps,
                        (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, x.scales_stride, (int)x.K);
   };
+  auto width = [&](auto nv) {
+    constexpr int NV = decltype(nv)::value;
+    if (x.M * x.K * 7 > (64 << 20))
+      go(lse::add_rmsnorm_fp8_kernel<NV, true>);
+    else
+      go(lse::add_rmsnorm_fp8_kernel<NV, false>);
+  };
   if (x.K <= 8 * lse::kNormFp8Threads)
-    go(lse::add_rmsnorm_fp8_kernel<1>);
+    width(std::integral_constant<int, 1>{});
   else if (x.K <= 16 * lse::kNormFp8Threads)
-    go(lse::add_rmsnorm_fp8_kernel<2>);
+    width(std::integral_constant<int, 2>{});
   else
-    go(lse::add_rmsnorm_fp8_kernel<4>);
+    width(std::integral_constant<int, 4>{});
   return lse::launch_status();
 }
 
