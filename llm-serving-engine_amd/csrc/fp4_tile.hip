@@ -39,22 +39,10 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   constexpr int SLOT = BM * CH;                         // uint4 of a stage's rows
   constexpr int XS = A8 ? 64 * W * XSI : 1;             // dwords of a stage's scales
   // One array a slot, so that the compiler tells the slot a load fills from the one that is read.
-  __shared__ uint4 x0[SLOT], x1[SLOT], x2[NST > 2 ? SLOT : 1], x3[NST > 3 ? SLOT : 1], x4[NST > 4 ? SLOT : 1],
-      x5[NST > 4 ? SLOT : 1], x6[NST > 6 ? SLOT : 1], x7[NST > 6 ? SLOT : 1];
-  __shared__ uint32_t s0[XS], s1[XS], s2[NST > 2 ? XS : 1], s3[NST > 3 ? XS : 1], s4[NST > 4 ? XS : 1],
-      s5[NST > 4 ? XS : 1], s6[NST > 6 ? XS : 1], s7[NST > 6 ? XS : 1];
-  auto slot_x = [&](auto i) -> uint4* {
-    if constexpr (i < 4)
-      return i == 0 ? x0 : i == 1 ? x1 : i == 2 ? x2 : x3;
-    else
-      return i == 4 ? x4 : i == 5 ? x5 : i == 6 ? x6 : x7;
-  };
-  auto slot_s = [&](auto i) -> uint32_t* {
-    if constexpr (i < 4)
-      return i == 0 ? s0 : i == 1 ? s1 : i == 2 ? s2 : s3;
-    else
-      return i == 4 ? s4 : i == 5 ? s5 : i == 6 ? s6 : s7;
-  };
+  __shared__ uint4 x0[SLOT], x1[SLOT], x2[NST > 2 ? SLOT : 1], x3[NST > 2 ? SLOT : 1];
+  __shared__ uint32_t s0[XS], s1[XS], s2[NST > 2 ? XS : 1], s3[NST > 2 ? XS : 1];
+  auto slot_x = [&](auto i) -> uint4* { return i == 0 ? x0 : i == 1 ? x1 : i == 2 ? x2 : x3; };
+  auto slot_s = [&](auto i) -> uint32_t* { return i == 0 ? s0 : i == 1 ? s1 : i == 2 ? s2 : s3; };
   constexpr auto swz = fp4_swz<A8>;
 
   const int lane = threadIdx.x & 63;
@@ -191,8 +179,8 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   // begins: the rows of the NST - 2 later stages, and the weights of the NST - 1.
   constexpr int XLOADS = XI + XSI, LATER = (NST - 1) * TN + (NST - 2) * XLOADS;
   static_assert(LATER < 64, "vmcnt holds at most 63");
-  constexpr int U = NST % 3 == 0 ? 12 : NST > 4 ? 8 : 4;  // stages of the loop body: whole chunks, whole rings
-  static_assert(U % NST == 0 && (NST == 2 || NST == 3 || NST == 4 || NST == 6 || NST == 8), "whole rings");
+  constexpr int U = 4;  // stages of the loop body: a chunk, and whole rings
+  static_assert(NST == 2 || NST == 4, "whole rings");
   Weights st[NST];
   Scales sc, next;
   load_s(0, sc);
@@ -212,6 +200,25 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
       if constexpr (u % 4 == 0) load_s(s / 4 + 1, next);
       load_x(s + NST - 1, std::integral_constant<int, ahead>{});
       compute(s, std::integral_constant<int, slot>{}, std::integral_constant<int, u % 4>{}, st[slot], sc);
+      // The order of the stage's LDS reads (0x100) and matrix instructions (0x008), where a wave has so many of both that
+      // the compiler reads a tile and waits for it at once: bf16 rows 2 tiles ahead of their instructions (2048 rows by
+      // two 14336 x 4096 weights: 349 -> 340 us), 8-bit rows (two chunks and a scale a tile) likewise (202 -> 198 us).
+      // The 128 token rows of 8 bits, half as many tiles a wave, ran 1 % slower so and keep the compiler's order.
+      if constexpr (!A8 && TN == 4) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+        unroll<4 * TM - 2>([&](auto) {
+          __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        });
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN, 0);
+      } else if constexpr (A8 && TN == 4 && TM > 4) {
+        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
+        unroll<TM - 2>([&](auto) {
+          __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+        });
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN, 0);
+      }
       load_w(s + NST, st[slot]);
       if constexpr (u % 4 == 3) sc = next;
     });
