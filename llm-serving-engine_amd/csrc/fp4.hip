@@ -11,19 +11,20 @@ constexpr int64_t kMax31 = 2147483647;
 int64_t row_tiles(const lse_fp4_gemm_args& p) { return (p.glu ? 2 : 1) * lse::ceil_div(p.N, 16); }
 
 // Microseconds that a call takes apart from the weight's way from HBM, for the tile kernels by stages (128 k of one tile
-// on each CU), for the streaming kernel by what a CU reads through its L1: fitted to about 150 timed calls of both kinds
-// of rows (M 1 to 2048, N 1024 to 28672, K 4096 and 14336), of which the better kernel was missed by 5 % in the mean.
+// on each CU), for the streaming kernel by what a CU reads through its L1. Fitted to 94 sizes of both kinds of rows and
+// both epilogues (M 9 to 8192, N 1024 to 28672, K 1536 to 14336), each timed with every plan below: the one chosen here
+// is 1 % slower than the fastest in the mean, 13 % at most.
 struct Tile {
   int bm, bn;
-  int slots;             // workgroups that run at once on 256 CUs
-  double one[2], all[2]; // of a stage, bf16 and 8-bit rows: one workgroup a CU, and all slots taken
+  int slots[2];           // workgroups that run at once on 256 CUs, bf16 and 8-bit rows
+  double one[2], all[2];  // of a stage: one workgroup a CU, and all slots taken
 };
-constexpr Tile kTiles[] = {{32, 128, 512, {0.37, 0.33}, {0.65, 0.45}},
-                           {64, 128, 512, {0.55, 0.42}, {0.92, 0.62}},
-                           {128, 256, 256, {1.50, 0.96}, {1.50, 0.96}},
-                           {256, 256, 256, {2.80, 1.62}, {2.80, 1.62}}};
-constexpr double kLaunchUs = 2.5, kHbmBytesPerUs = 4.5e6, kL1BytesPerUs = 52e3, kSecondPassUs = 3.0,
-                 kPartBytesPerUs = 4e6;
+constexpr Tile kTiles[] = {{32, 128, {256, 512}, {0.29, 0.26}, {0.29, 0.45}},
+                           {64, 128, {256, 512}, {0.46, 0.37}, {0.46, 0.64}},
+                           {128, 256, {256, 256}, {1.50, 0.96}, {1.50, 0.96}},
+                           {256, 256, {0, 256}, {0, 1.57}, {0, 1.57}}};  // bf16 rows: 3.1, no better than two of 128
+constexpr double kLaunchUs = 2.5, kStreamBytesPerUs = 4.3e6, kTileBytesPerUs = 5e6, kL1BytesPerUs = 65e3;
+constexpr double kSecondPassUs = 3.0, kPartBytesPerUs = 4e6;
 constexpr int64_t kMaxPartBytes = 64 << 20;
 
 // Which kernel a call takes, from its sizes alone: the one whose time is estimated the shortest.
@@ -35,31 +36,31 @@ lse::Fp4Plan plan_of(const lse_fp4_gemm_args& p) {
   lse::Fp4Plan best{0, 16 * narrow, 1, (int)chunks};
   if (p.M <= (rows8 ? 8 : 4)) return best;
   const int64_t stages = lse::ceil_div(p.K, lse::kFp4Step);
-  const double weight = 16.0 * nrb * stages * 68, hbm = weight / kHbmBytesPerUs;
+  const double weight = 16.0 * nrb * stages * 68;
   double least = 1e30;
   auto take = [&](double us, int bm, int bn, int64_t splits, int64_t per) {
     if (us < least) least = us, best = {bm, bn, (int)splits, (int)per};
   };
   const int64_t groups = lse::ceil_div(p.M, 16);
   for (int rt = 4; rt >= narrow; rt /= 2) {
-    const double workgroups = (double)lse::ceil_div(nrb, rt) * groups;
+    const int64_t rounds = lse::ceil_div(lse::ceil_div(nrb, rt) * groups, 256);
     const double rows = p.M < 16 ? p.M : 16;
     const double bytes = stages * (rows * (rows8 ? 132.0 : 256.0) + rt * 16 * 68.0);
-    const double us = kLaunchUs + std::max(hbm, std::max(1.0, workgroups / 256) * bytes / kL1BytesPerUs);
+    const double us = kLaunchUs + std::max(weight / kStreamBytesPerUs, rounds * bytes / kL1BytesPerUs);
     take(us, 0, 16 * rt, 1, chunks);
   }
   for (const Tile& t : kTiles) {
-    if (p.M <= 16 && (t.bm > 32 || !rows8)) continue;
+    if (t.slots[rows8] == 0 || (p.M <= 16 && (t.bm > 32 || !rows8))) continue;
     const int64_t tiles = lse::ceil_div(p.M, t.bm) * lse::ceil_div(nrb, t.bn / 16);
     for (int64_t splits = 1; splits <= 8; splits *= 2) {
       const int64_t per = lse::ceil_div(chunks, splits), ranges = lse::ceil_div(chunks, per);
       if (splits > 1 && (ranges != splits || per < 2)) break;
       const double part = 64.0 * nrb * p.M * splits;
       if (splits > 1 && part > kMaxPartBytes) break;
-      const int64_t blocks = tiles * splits, full = blocks / t.slots, rest = blocks % t.slots;
+      const int64_t blocks = tiles * splits, full = blocks / t.slots[rows8], rest = blocks % t.slots[rows8];
       const double last = rest == 0 ? 0.0 : rest <= 256 ? t.one[rows8] : t.all[rows8];
       double us = std::min<double>(stages, 4 * per) * (full * t.all[rows8] + last);
-      us = kLaunchUs + std::max(hbm, us);
+      us = kLaunchUs + std::max(weight / kTileBytesPerUs, us);
       if (splits > 1) us += kSecondPassUs + 2 * part / kPartBytesPerUs;
       take(us, t.bm, t.bn, splits, per);
     }

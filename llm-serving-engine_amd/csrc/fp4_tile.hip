@@ -1,21 +1,27 @@
 // Products of many rows with a 4-bit weight (layouts and formats: fp4.h; the arithmetic as in fp4_stream.hip), bound by
 // the matrix cores.
 //
-// A workgroup of WGM x WGN waves computes BM token rows x BN weight rows over K, in stages of 128 k. Token rows go to LDS
-// by direct loads (whole 256 or 128 byte row pieces, 16-byte chunks swizzled by row), NST - 1 stages ahead; the weight,
-// a quarter or a half of their bytes, goes straight to the registers of the wave that multiplies it, as far ahead: each
-// wave needs BN / WGN rows of it and no other wave of its row of waves does. One barrier a stage. bf16 rows: a wave decodes its weight tiles (half an instruction a weight,
+// A workgroup of WGM x WGN waves (KG groups of so many) computes BM token rows x BN weight rows over K, in stages of
+// 128 k a group, which take them in turn. Token rows go to LDS by direct loads (whole 256 or 128 byte row pieces, 16-byte
+// chunks swizzled by row), NST - 1 stages ahead; the weight, a quarter or a half of their bytes, goes straight to the
+// registers of the wave that multiplies it, as far ahead: each wave needs BN / WGN rows of it and no other wave of its
+// row of waves does. One barrier a stage. bf16 rows: a wave decodes its weight tiles (half an instruction a weight,
 // shared by its WM token rows) and runs 16x16x32 bf16 instructions. 8-bit rows: codes and scale bytes of both operands
 // go to the scaled 16x16x128 instruction as they are.
 //
 // Tile order: blocks are dealt to the 8 XCDs in turn; each XCD gets a contiguous range of tiles, in groups of kGroupM
 // token blocks x consecutive weight panels, so that what it runs at once shares token rows and weights in its L2.
 // K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order.
-// A result depends on K and the split alone, never on other rows.
+// A result depends on K, the groups and the split alone, never on other rows.
+//
+// The small tiles fill a card with one workgroup a CU, a wave a SIMD, whose decoding, LDS reads and matrix instructions
+// then wait for each other: with bf16 rows they take two groups (256 rows by 4096 x 4096: 14.1 -> 11.1 us; 777 by
+// 2330 x 4128: 22.3 -> 20.1). What bounds them then is the CU's way from L2, 50 to 60 bytes a ns: 17 or 25 KB a stage.
+// 8-bit rows, half the bytes and no decoding, ran slower with two (12.5 -> 12.9) and keep one, with four slots.
 //
 // The compiler counts the weights' loads and waits for them in order, so it has to count the direct loads too, without
 // taking them for writes of the slot that is being read: one array a slot, indexes that it does not take apart (at[]).
-// With two slots (the widest tiles) it still waited for all of them in every stage; there they are issued by inline
+// With two slots it still waited for all of them in every stage; there they are issued by inline
 // assembly (dma16_lds), and the only wait on them is the one written here, with nothing later in flight but weights.
 #include <algorithm>
 
@@ -25,9 +31,10 @@ namespace lse {
 
 constexpr int kFp4GroupM = 4;
 
-template <bool A8, int BM, int BN, int WGM, int WGN, int NST, bool GLU>
-__global__ void __launch_bounds__(64 * WGM * WGN)
+template <bool A8, int BM, int BN, int WGM, int WGN, int KG, int NST, bool GLU>
+__global__ void __launch_bounds__(64 * WGM * WGN * KG)
 fp4_tile_kernel(Fp4Args a, Fp4Split p) {
+  static_assert(KG == 1 || KG == 2, "whole chunks");
   constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
   static_assert(WM % 16 == 0 && WN % 16 == 0 && (!GLU || TN % 2 == 0), "whole tiles, and pairs of row tiles");
   constexpr int ESZ = A8 ? 1 : 2;
@@ -39,14 +46,15 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   constexpr int SLOT = BM * CH;                         // uint4 of a stage's rows
   constexpr int XS = A8 ? 64 * W * XSI : 1;             // dwords of a stage's scales
   // One array a slot, so that the compiler tells the slot a load fills from the one that is read.
-  __shared__ uint4 x0[SLOT], x1[SLOT], x2[NST > 2 ? SLOT : 1], x3[NST > 2 ? SLOT : 1];
-  __shared__ uint32_t s0[XS], s1[XS], s2[NST > 2 ? XS : 1], s3[NST > 2 ? XS : 1];
+  __shared__ uint4 x0[KG * SLOT], x1[KG * SLOT], x2[NST > 2 ? KG * SLOT : 1], x3[NST > 2 ? KG * SLOT : 1];
+  __shared__ uint32_t s0[KG * XS], s1[KG * XS], s2[NST > 2 ? KG * XS : 1], s3[NST > 2 ? KG * XS : 1];
   auto slot_x = [&](auto i) -> uint4* { return i == 0 ? x0 : i == 1 ? x1 : i == 2 ? x2 : x3; };
   auto slot_s = [&](auto i) -> uint32_t* { return i == 0 ? s0 : i == 1 ? s1 : i == 2 ? s2 : s3; };
   constexpr auto swz = fp4_swz<A8>;
 
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kg = KG == 1 ? 0 : all / W, wave = KG == 1 ? all : all % W;  // the wave's group, and its place there
   const int wm = wave / WGN, wn = wave % WGN;
   const int r16 = lane & 15, g = lane >> 4;
 
@@ -60,7 +68,7 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const int rows = min(BM, a.M - m0);
   // Chunks [c0, c1) of K, and its steps (stages) counted from c0.
   const int c0 = sp * p.chunks, c1 = min(c0 + p.chunks, a.nchunks);
-  const int stages = min(4 * c1, a.nsteps) - 4 * c0;
+  const int steps = min(4 * c1, a.nsteps) - 4 * c0;
 
   const void* xbase = static_cast<const char*>(a.x) + (int64_t)m0 * a.ldx * ESZ;
   const uint32_t xbytes = (uint32_t)(((int64_t)(rows - 1) * a.ldx + a.K) * ESZ);
@@ -92,30 +100,34 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const uint32_t xstep = (uint32_t)(RPL * W * a.ldx * ESZ);
   const uint32_t soff = (uint32_t)((64 * wave + lane) * a.lds + 16 * c0), sstep = (uint32_t)(64 * W * a.lds);
   auto load_x = [&](int s, auto slot) {
+    s = KG * s + kg;
     const uint32_t off = ROWB * s + xkb < kbytes ? xoff + ROWB * s : kOutOfRange;
     if constexpr (NST == 2) {
-      unroll<XI>([&](auto i) { dma16_lds<1024 * W * i>(xres4, lds_addr(slot_x(slot) + 64 * wave), off + i * xstep); });
+      const uint32_t to = lds_addr(slot_x(slot) + kg * SLOT + 64 * wave);
+      unroll<XI>([&](auto i) { dma16_lds<1024 * W * i>(xres4, to, off + i * xstep); });
     } else {
 #pragma unroll
-      for (int i = 0; i < XI; ++i) buffer_load16_lds(xres, slot_x(slot) + 64 * (wave + W * i), off + i * xstep);
+      for (int i = 0; i < XI; ++i)
+        buffer_load16_lds(xres, slot_x(slot) + kg * SLOT + 64 * (wave + W * i), off + i * xstep);
     }
     if constexpr (A8) {
       const uint32_t so = 4 * (4 * c0 + s) < per4 ? soff + 4 * s : kOutOfRange;
       if constexpr (NST == 2) {
-        unroll<XSI>([&](auto i) { dma4_lds<256 * W * i>(sres4, lds_addr(slot_s(slot) + 64 * wave), so + i * sstep); });
+        const uint32_t to4 = lds_addr(slot_s(slot) + kg * XS + 64 * wave);
+        unroll<XSI>([&](auto i) { dma4_lds<256 * W * i>(sres4, to4, so + i * sstep); });
       } else {
 #pragma unroll
         for (int i = 0; i < XSI; ++i)
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (LdsPtr)(slot_s(slot) + 64 * (wave + W * i)), 4, so + i * sstep,
-                                                   0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(sres, (LdsPtr)(slot_s(slot) + kg * XS + 64 * (wave + W * i)), 4,
+                                                   so + i * sstep, 0, 0, 0);
       }
     }
   };
   struct Weights {
     u32x4 w[TN];
   };
-  auto load_w = [&](int j, Weights& st) {  // step j of the range; past it the last, whose rows are zeros then
-    const uint32_t at = min(j, stages - 1) * kFp4TileBytes;
+  auto load_w = [&](int s, Weights& st) {  // stage s; past the range its last step, which is not used then
+    const uint32_t at = min(KG * s + kg, steps - 1) * kFp4TileBytes;
 #pragma unroll
     for (int n = 0; n < TN; ++n)
       st.w[n] = __builtin_amdgcn_raw_buffer_load_b128(wres, 16 * lane, (int)(wp[n] + at), 0);
@@ -140,17 +152,22 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const uint32_t tail = a.K % kFp4Step ? (1u << (8 * (a.K % kFp4Step / kFp4Group))) - 1 : ~0u;
   // Where this lane's operands of the wave's first token tile lie in a slot. The compiler is kept from taking the sums
   // apart: it follows an LDS access to its array through a few additions only.
-  int at[A8 ? 2 : 4], sat = wm * WM + r16;
+  int at[A8 ? 2 : 4], sat = kg * XS + wm * WM + r16;
 #pragma unroll
   for (int i = 0; i < (A8 ? 2 : 4); ++i) {
-    at[i] = (wm * WM + r16) * CH + ((A8 ? 4 * i + g : 4 * g + i) ^ swz(r16));
+    at[i] = kg * SLOT + (wm * WM + r16) * CH + ((A8 ? 4 * i + g : 4 * g + i) ^ swz(r16));
     asm volatile("" : "+v"(at[i]));
   }
   asm volatile("" : "+v"(sat));
-  // Step j from slot, the chunk's step t.
-  auto compute = [&](int j, auto slot, auto t, const Weights& st, const Scales& sc) {
+  // Stage j from slot, whose step is the chunk's t + kg.
+  auto compute = [&](int j, auto slot, auto t, const Weights& st, const Scales& chunk) {
+    Scales sc = chunk;
+    if constexpr (KG > 1) {
+#pragma unroll
+      for (int n = 0; n < TN; ++n) sc.w[n] >>= 8 * kg;
+    }
     if constexpr (A8) {
-      const uint32_t mask = 4 * c0 + j == a.nsteps - 1 ? tail : ~0u;
+      const uint32_t mask = 4 * c0 + KG * j + kg == a.nsteps - 1 ? tail : ~0u;
 #pragma unroll
       for (int i = 0; i < TM; ++i) {
         const uint32_t d = (slot_s(slot)[sat + 16 * i] & mask) >> (8 * g);
@@ -179,7 +196,8 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   // begins: the rows of the NST - 2 later stages, and the weights of the NST - 1.
   constexpr int XLOADS = XI + XSI, LATER = (NST - 1) * TN + (NST - 2) * XLOADS;
   static_assert(LATER < 64, "vmcnt holds at most 63");
-  constexpr int U = 4;  // stages of the loop body: a chunk, and whole rings
+  constexpr int U = 4, SC = 4 / KG;  // stages of the loop body: whole chunks, of SC stages, and whole rings
+  const int stages = (steps + KG - 1 - kg) / KG, most = (steps + KG - 1) / KG, least = steps / KG;
   static_assert(NST == 2 || NST == 4, "whole rings");
   Weights st[NST];
   Scales sc, next;
@@ -191,15 +209,16 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
     unroll<U>([&](auto u) {
       constexpr int slot = u % NST, ahead = (u + NST - 1) % NST;
       const int s = base + u;
-      if (!whole && s >= stages) return;
+      if (!whole && s >= most) return;
       asm volatile("" ::: "memory");  // the reads of the stage before stay before the barrier
       // This wave's rows of stage s have landed and its reads of the slot that the loads below go to are done; after
       // the barrier every wave's are.
       __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(LATER));
       __builtin_amdgcn_s_barrier();
-      if constexpr (u % 4 == 0) load_s(s / 4 + 1, next);
+      if constexpr (u % SC == 0) load_s(s / SC + 1, next);
       load_x(s + NST - 1, std::integral_constant<int, ahead>{});
-      compute(s, std::integral_constant<int, slot>{}, std::integral_constant<int, u % 4>{}, st[slot], sc);
+      if (whole || KG == 1 || s < stages)
+        compute(s, std::integral_constant<int, slot>{}, std::integral_constant<int, KG * (u % SC)>{}, st[slot], sc);
       // The order of the stage's LDS reads (0x100) and matrix instructions (0x008), where a wave has so many of both that
       // the compiler reads a tile and waits for it at once: bf16 rows 2 tiles ahead of their instructions (2048 rows by
       // two 14336 x 4096 weights: 349 -> 340 us), 8-bit rows (two chunks and a scale a tile) likewise (202 -> 198 us).
@@ -220,14 +239,36 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN, 0);
       }
       load_w(s + NST, st[slot]);
-      if constexpr (u % 4 == 3) sc = next;
+      if constexpr (u % SC == SC - 1) sc = next;
     });
   };
   // Whole groups without tests between their stages, which would make the compiler wait for every load; then the rest.
   int base = 0;
-  for (; base + U <= stages; base += U) body(base, std::true_type{});
-  if (base < stages) body(base, std::false_type{});
+  for (; base + U <= least; base += U) body(base, std::true_type{});
+  if (base < most) body(base, std::false_type{});
   __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
+  if constexpr (KG == 2) {
+    // The second group's sums go through the slots to the first, which adds them to its own.
+    constexpr int PER = 64 * W * TN;
+    static_assert(PER * ((TM + NST - 1) / NST) <= KG * SLOT, "the sums fit the slots");
+    auto sums = [&](auto i) {
+      return reinterpret_cast<f32x4*>(slot_x(std::integral_constant<int, i % NST>{})) + i / NST * PER + 64 * wave * TN +
+             lane;
+    };
+    __syncthreads();
+    if (kg) {
+      unroll<TM>([&](auto i) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) sums(i)[64 * j] = acc[i][j];
+      });
+    }
+    __syncthreads();
+    if (kg) return;
+    unroll<TM>([&](auto i) {
+#pragma unroll
+      for (int j = 0; j < TN; ++j) acc[i][j] += sums(i)[64 * j];
+    });
+  }
 
   // D tile (i, j): lane holds weight rows 4 g + r (r = 0..3) of token row r16.
   const bool yvec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 7) == 0;
@@ -299,14 +340,15 @@ static int launch(const Fp4Args& a, const Fp4Plan& plan, float* part, hipStream_
   auto go = [&](auto kernel, int threads) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, a, p);
   };
-  if (plan.bm == 256)
-    go(fp4_tile_kernel<A8, 256, 256, 2, 4, 2, GLU>, 512);
-  else if (plan.bm == 128)
-    go(fp4_tile_kernel<A8, 128, 256, 2, 4, 2, GLU>, 512);
-  else if (plan.bm == 64)
-    go(fp4_tile_kernel<A8, 64, 128, 1, 4, 4, GLU>, 256);
-  else
-    go(fp4_tile_kernel<A8, 32, 128, 1, 4, 4, GLU>, 256);
+  if constexpr (A8) {
+    if (plan.bm == 256) go(fp4_tile_kernel<A8, 256, 256, 2, 4, 1, 2, GLU>, 512);
+  }
+  if (plan.bm == 128)
+    go(fp4_tile_kernel<A8, 128, 256, 2, 4, 1, 2, GLU>, 512);
+  if (plan.bm == 64)
+    go(fp4_tile_kernel<A8, 64, 128, 1, 4, A8 ? 1 : 2, A8 ? 4 : 2, GLU>, A8 ? 256 : 512);
+  if (plan.bm == 32)
+    go(fp4_tile_kernel<A8, 32, 128, 1, 4, A8 ? 1 : 2, A8 ? 4 : 2, GLU>, A8 ? 256 : 512);
   if (p.splits > 1) {
     if (int st = launch_status()) return st;
     const int64_t quads = (int64_t)a.M * ceil_div(a.N, 4);

@@ -15,13 +15,17 @@ pytestmark = pytest.mark.gpu
 KINDS = [(1, 40, 640), (13, 100, 1184), (40, 3600, 544), (100, 64, 96), (300, 500, 1056), (700, 1100, 640)]
 
 
+SPLIT = [(300, 1030, 14336, False), (260, 2050, 14400, False), (130, 530, 28704, True)]  # K over 2 to 8 workgroups
+
+
 @pytest.mark.parametrize("rows", [False, True], ids=["bf16", "fp8"])
-@pytest.mark.parametrize("m,n,k,glu", [(200, 1030, 14336, False), (40, 4096, 14368, False), (200, 512, 14400, True)])
+@pytest.mark.parametrize("m,n,k,glu", [(200, 1030, 14336, False), (40, 4096, 14368, False), (200, 512, 14400, True), *SPLIT])
 def test_split_k(pkg, m, n, k, glu, rows):
     from llm_serving_engine_amd import _lib
 
     args = _lib.FP4_GEMM_ARGS.pack(16, k, 16 if rows else 0, k // 32 + 3 & ~3, 16, 16, 16, n, m, n, k, int(glu))
-    assert pkg.library().lse_fp4_gemm_workspace_bytes(args) > 0
+    if (m, n, k, glu) in SPLIT:
+        assert pkg.library().lse_fp4_gemm_workspace_bytes(args) > 0
     _check(pkg, m, n, k, rows, glu, seed=m)
 
 
