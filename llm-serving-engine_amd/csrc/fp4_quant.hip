@@ -19,10 +19,11 @@ __device__ __forceinline__ uint32_t fp4_code(float v) {
   return c && v < 0.0f ? c | 8 : c;
 }
 
-constexpr int kFp4ScaleTop = 253;  // 2^126, the largest scale of finite values: its codes 6 and 7 stand for 2^128 and more
+// 2^126, the largest scale of finite values: its codes 6 and 7 stand for 2^128 and more.
+constexpr int kFp4ScaleTop = 253;
 
 // One thread a group of 32 of one row: w fp32, stride ldw. A group with a value that is not finite gets the scale
-// 255 (NaN): e2m1 has no code for it. Finite weights stay finite.
+// 255 (NaN): e2m1 has no code for it. Finite weights stay finite. 14336 x 4096: 52 us a call, 5.1 TB/s.
 __global__ void __launch_bounds__(256)
 fp4_quantize_kernel(const float* w, int64_t ldw, uint8_t* codes, uint8_t* scales, int64_t groups, int per_row) {
   const int64_t at = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -58,7 +59,7 @@ fp4_quantize_kernel(const float* w, int64_t ldw, uint8_t* codes, uint8_t* scales
 }
 
 // One thread 16 bytes of a code tile (a group) and one scale byte of a scale tile; threads past the code tiles' K fill
-// the scale tiles up. codes (rows, K / 2), scales (rows, K / 32); glu: rows = 2 I.
+// the scale tiles up. codes (rows, K / 2), scales (rows, K / 32); glu: rows = 2 I. 14336 x 4096: 14 us a call.
 __global__ void __launch_bounds__(256)
 fp4_pack_kernel(const uint8_t* codes, const uint8_t* scales, uint8_t* out_codes, uint8_t* out_scales, int64_t total,
                 int rows, int K, int nsteps, int nchunks, int glu) {
@@ -107,7 +108,9 @@ __device__ __forceinline__ void bf16x8_to_f32(uint4 q, float (&v)[8]) {
   }
 }
 
-// One thread eight values of a row. codes (M, K) contiguous, scales (M, K / 32) of row stride lds.
+// One thread eight values of a row, four threads a group, whose largest value they share by shuffles. Bound by HBM, 3
+// bytes a value: 2048 rows of 14336 15.7 us, 5.6 TB/s (some of it from the cache behind L2); 64 of 4096 2.7, a launch.
+// codes (M, K) contiguous, scales (M, K / 32) of row stride lds.
 __global__ void __launch_bounds__(256)
 fp8_rows_kernel(const uint16_t* x, int64_t ldx, uint8_t* codes, uint8_t* scales, int64_t lds, int64_t total,
                 int per_row) {
@@ -141,10 +144,13 @@ __device__ __forceinline__ void store_once(void* p, V v) {
 // One workgroup per row, of as many waves as its first 4096 values keep busy, thread t holding elements 8 t + 4096 i
 // (i < NV): s = bf16(x + res) (or x), n = bf16(w * bf16(s * r)), r = 1 / sqrt(mean(s^2) + eps), the roundings of
 // LlamaRMSNorm (modeling_llama.py:62-67), then n's codes and scales. The sum of squares: each thread's in order, then a
-// fixed tree, add_rmsnorm_kernel's order. `sum` may be x or res: a thread reads all of its elements before it writes any.
-// Bound by HBM: STREAM, for calls that move much of what the cache behind L2 holds, keeps it from being filled with what
-// is not read again (4160 rows of 4096 30.9 -> 27.6 us, 4.3 TB/s of a copy's 4.7; 2048 of 14336 52.2 -> 51.0), which
-// smaller calls are better off with in the cache (4160 of 1024 16.9 against 21.4, repeated).
+// fixed tree, add_rmsnorm_kernel's order, so that the codes are those of its rows. `sum` may be x or res: a thread reads
+// all of its elements before it writes any.
+// Bound by HBM, 7 bytes a value: 4160 rows of 4096 24.3 us, 4.9 TB/s, a copy's rate; 2048 of 14336 42.0; 33 of 4096 4.8, a
+// launch. Waves that would hold no element are not started (4160 of 1024: 16.9 -> 9.7 us). STREAM, for calls that move a
+// good part of the 256 MB behind L2, keeps from there what is not read again: 2048 of 14336 46.0 -> 42.0, 4160 of 4096 29.9
+// -> 24.3 after other work and 24.1 by itself either way; smaller calls are better off without (3200 of 4096 17.5 against
+// 19.4, 2560 14.9 against 16.6).
 template <int NV, bool STREAM>
 __global__ void __launch_bounds__(kNormFp8Threads)
 add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int64_t ldr, const uint16_t* w, float eps,
@@ -296,7 +302,7 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
   };
   auto width = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
-    if (x.M * x.K * 7 > (64 << 20))
+    if (x.M * x.K * 7 > (96 << 20))
       go(lse::add_rmsnorm_fp8_kernel<NV, true>);
     else
       go(lse::add_rmsnorm_fp8_kernel<NV, false>);

@@ -9,10 +9,17 @@
 // shared by its WM token rows) and runs 16x16x32 bf16 instructions. 8-bit rows: codes and scale bytes of both operands
 // go to the scaled 16x16x128 instruction as they are.
 //
-// Tile order: blocks are dealt to the 8 XCDs in turn; each XCD gets a contiguous range of tiles, in groups of kGroupM
-// token blocks x consecutive weight panels, so that what it runs at once shares token rows and weights in its L2.
+// Tile order: blocks are dealt to the 8 XCDs in turn; each XCD gets a contiguous range of tiles, in groups of
+// kFp4GroupM token blocks x consecutive weight panels, so that what it runs at once shares token rows and weights in
+// its L2.
 // K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order.
 // A result depends on K, the groups and the split alone, never on other rows.
+//
+// What it measured: bf16 rows, 128 x 256 tiles, 2048 by two of 14336 x 4096 340 us, 1410 TFLOP/s, by 4096 x 14336 161,
+// 1490 (a large library product 1330 to 1380), matrix cores busy for two thirds of the time; 8-bit rows, 256 x 256, 2048
+// by two of 14336 x 4096 201 us, 2390 TFLOP/s, 128 x 256, by 4096 x 14336 98, 2450 (a library's fp8 2590 to 2930), busy
+// 60 %: the LDS reads and decoding of a wave do not all hide behind the other wave of its SIMD, whose stage ends at the
+// same barrier. Deeper rings (3, 4, 6 slots) gain nothing, a second barrier in mid-stage spills.
 //
 // The small tiles fill a card with one workgroup a CU, a wave a SIMD, whose decoding, LDS reads and matrix instructions
 // then wait for each other: with bf16 rows they take two groups (256 rows by 4096 x 4096: 14.1 -> 11.1 us; 777 by
@@ -21,8 +28,8 @@
 //
 // The compiler counts the weights' loads and waits for them in order, so it has to count the direct loads too, without
 // taking them for writes of the slot that is being read: one array a slot, indexes that it does not take apart (at[]).
-// With two slots it still waited for all of them in every stage; there they are issued by inline
-// assembly (dma16_lds), and the only wait on them is the one written here, with nothing later in flight but weights.
+// With two slots it still waited for all of them in every stage; there they are issued by inline assembly (dma16_lds),
+// and the only wait on them is the one written here, with nothing later in flight but weights.
 #include <algorithm>
 
 #include "fp4.h"
@@ -302,7 +309,8 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   }
 }
 
-// Adds the splits' sums of four neighbouring columns in order, and rounds them (gate/up: silu and product first).
+// Adds the splits' sums of four neighbouring columns in order, and rounds them (gate/up: silu and product first). A launch
+// and the sums' way through L2: 64 x 4096 of 4 splits 2.4 us.
 template <bool GLU>
 __global__ void __launch_bounds__(256) fp4_reduce_kernel(Fp4Args a, Fp4Split p) {
   const int quads = (a.N + 3) / 4;

@@ -127,6 +127,18 @@ def test_norm(pkg, m, k, residual):
     assert bool((off <= 2.0 ** -6 * n64.double().abs()).all()) and float((off > 0).double().mean()) < 1e-3
 
 
+@pytest.mark.parametrize("m,k", [(3700, 4096), (1900, 8000), (900, 16384)])
+def test_norm_of_large_calls(pkg, m, k):
+    """More than 96 MiB of traffic: the same bits as in two steps."""
+    assert 7 * m * k > 96 << 20
+    x, r, w = activations(m, k, 1).cuda(), activations(m, k, 2).cuda(), activations(1, k, 3)[0].cuda()
+    s, rows = pkg.ops.add_rmsnorm_fp8(x, r, w, 1e-5)
+    s2, normed = pkg.ops.add_rmsnorm(x, r, w, 1e-5)
+    assert torch.equal(s, s2)
+    for a, b in zip(rows, pkg.ops.quantize_rows_fp8(normed)):
+        assert torch.equal(_bytes(a), _bytes(b))
+
+
 def test_norm_of_rows_that_are_not_finite(pkg):
     x = activations(4, 256, 5)
     x[1, 7], x[2, 9] = float("inf"), float("nan")
