@@ -63,8 +63,8 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lse_status_string": (ctypes.c_char_p, [_INT]),
 }
 
-# The header's argument structs: eight bytes a field, the last of the attention's and the norm's a double. Packing one takes a
-# sixth of the time of passing its fields one by one.
+# The header's argument structs: eight bytes a field, the last of the attention's and the norm's a double. Packing one
+# takes a sixth of the time of passing its fields one by one.
 ROPE_ARGS = struct.Struct("18q")
 APPEND_KV_FP8_ARGS = struct.Struct("34q")
 PAGED_ATTENTION_FP8_ARGS = struct.Struct("26qd")

@@ -2,8 +2,8 @@
 
 Field names, defaults and env-var names follow the reference so a deployment's environment
 carries over. `quantize` takes "none", "int8" (weight-only W8A16, the reference's meaning at
-model_runner.py:45-46), "w8a8" (dynamic per-token activations), "w4a16" (4-bit weights) or "w4a8" (4-bit weights, rows in
-8 bits). The kernels compute in bf16, so `dtype` must be "bfloat16" whenever `quantize` is not "none".
+model_runner.py:45-46), "w8a8" (dynamic per-token activations), "w4a16" (4-bit weights) or "w4a8"
+(4-bit weights, rows in 8 bits). The kernels compute in bf16, so `dtype` must be "bfloat16" whenever `quantize` is not "none".
 """
 
 from __future__ import annotations

@@ -347,11 +347,11 @@ class DecodeRunner:
         in 8 bits."""
         rows8 = (self.backend == "fp4" and norm is not self.model.model.norm
                  and self.fp4[0]["qkv"].mode == "w4a8")
-        if rows8 and self._fused and x.dtype == torch.bfloat16:
+        fused = self._fused and x.dtype == torch.bfloat16 and (residual is None or residual.dtype == torch.bfloat16)
+        if rows8 and fused:
             hidden, rows = ops.add_rmsnorm_fp8(x, residual, norm.weight, norm.variance_epsilon)
             return hidden, QuantizedRows(rows.codes, rows.scales, x.shape, x.dtype)
-        if self._fused and x.dtype == torch.bfloat16 and (residual is None
-                                                          or residual.dtype == torch.bfloat16):
+        if fused:
             return ops.add_rmsnorm(x, residual, norm.weight, norm.variance_epsilon)
         hidden = x if residual is None else residual + x
         return hidden, norm(hidden)

@@ -5,9 +5,9 @@ They stand in the same places: `Fp4Linear` for the projections that the referenc
 (transformers modeling_llama.py:163-176), `Fp8RMSNorm` for a decoder layer's two norms (modeling_llama.py:53-67).
 Weights are float4 e2m1 codes with a power of two for every 32 of a row (`ops.quantize_weight_fp4`), held as the tiles
 that the kernels stream (`ops.pack_fp4`); both are buffers of bytes, so `model.dtype` stays bf16 and a change of the
-model's dtype leaves them alone. "w4a16" multiplies bf16 rows,
-"w4a8" rows in 8 bits (float8 e4m3 with a power of two for every 32 values), which the norms make once for all
-projections that read them and the other projections make themselves.
+model's dtype leaves them alone. "w4a16" multiplies bf16 rows, "w4a8" rows in 8 bits (float8 e4m3 with a power of two
+for every 32 values), which the norms make once for all projections that read them and the other projections make
+themselves.
 """
 
 from __future__ import annotations

@@ -984,8 +984,8 @@ class Fp4Weight(NamedTuple):
     32 consecutive k of a row.
 
     codes: uint8 (tiles, ceil(K / 128), 1024), scales: float8_e8m0fnu, or its bytes as uint8, (tiles, ceil(K / 512),
-    256); n: the columns of the product, k: those of its input. tiles = ceil(n / 16); 2 ceil(n / 16) for the gate and up weights of a
-    `w4a16_glu` or `w4a8_glu`, whose row tiles take turns. Made by `pack_fp4`."""
+    256); n: the columns of the product, k: those of its input. tiles = ceil(n / 16); 2 ceil(n / 16) for the gate and up
+    weights of a `w4a16_glu` or `w4a8_glu`, whose row tiles take turns. Made by `pack_fp4`."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -1071,7 +1071,8 @@ def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
 
 
 def dequantize_rows_fp8(rows: Fp8Rows) -> torch.Tensor:
-    """The values of rows in 8 bits, (..., K) bf16 (each is one)."""
+    """The values of rows in 8 bits, (..., K) bf16: exact, but that the two smallest scales have values below
+    bf16's subnormals, which round to them."""
     v = rows.codes.float().unflatten(-1, (-1, FP4_GROUP)) * rows.scales.float()[..., None]
     return v.flatten(-2).to(_BF16)
 

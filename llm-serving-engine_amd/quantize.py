@@ -17,9 +17,9 @@ import gc
 import torch
 from torch import nn
 
-from . import fp4_linear
-from .fp4_linear import Fp4GluMLP, Fp4Linear, Fp8RMSNorm, group_qkv_fp4
-from .int8_linear import (MODES as INT8_MODES, Int8GluMLP, Int8Linear, Int8RMSNormQuant, PackedBf16Linear,
+from . import _lib, fp4_linear
+from .fp4_linear import Fp4GateUp, Fp4GluMLP, Fp4Linear, Fp8RMSNorm, group_qkv_fp4
+from .int8_linear import (MODES as INT8_MODES, Int8GateUp, Int8GluMLP, Int8Linear, Int8RMSNormQuant, PackedBf16Linear,
                           fusable_mlp, group_qkv)
 
 MODES = INT8_MODES + fp4_linear.MODES
@@ -41,6 +41,23 @@ def check_int8_support(model: nn.Module) -> None:
         raise RuntimeError(f"int8 kernels need a CUDA (HIP) device, got {p.device}")
     if p.dtype != torch.bfloat16:
         raise RuntimeError(f"int8 kernels compute in bfloat16, the model is {p.dtype}")
+
+
+def _check_kinds(model: nn.Module, mode: str, fuse_norm: bool) -> None:
+    """Refuses before anything is swapped what would fail half-way or when the model runs: a model with 4-bit weights,
+    and for a 4-bit mode int8 ones and widths that do not fit."""
+    for layer in model.model.layers:
+        for name, mod in layer.named_modules():
+            if isinstance(mod, (Fp4Linear, Fp4GateUp)):
+                raise RuntimeError(f"{name} holds a {mod.mode} weight already")
+            if mode not in fp4_linear.MODES:
+                continue
+            if isinstance(mod, (Int8Linear, Int8GateUp)):
+                raise RuntimeError(f"{name} holds an {mod.mode} weight already")
+            if isinstance(mod, nn.Linear) and name.split(".")[-1] in ATTENTION_PROJECTIONS + MLP_PROJECTIONS:
+                fp4_linear.check_fp4_supported(mod)
+        if mode in fp4_linear.MODES and fuse_norm and (width := layer.input_layernorm.weight.numel()) > _lib.NORM_MAX_K:
+            raise RuntimeError(f"a norm into 8 bits takes up to {_lib.NORM_MAX_K} values, the model's have {width}")
 
 
 @torch.no_grad()
@@ -66,6 +83,7 @@ def quantize_model_(model: nn.Module, mode: str = "int8", fuse_mlp: bool = True,
     if fuse_norm and not rows8:
         raise ValueError("fuse_norm feeds pre-quantized rows to W8A8 and W4A8 projections only")
     check_int8_support(model)
+    _check_kinds(model, mode, fuse_norm)
     linear_as, mlp_as, norm_as, group = (
         (Fp4Linear, Fp4GluMLP, Fp8RMSNorm, group_qkv_fp4) if mode in fp4_linear.MODES
         else (Int8Linear, Int8GluMLP, Int8RMSNormQuant, group_qkv))

@@ -196,6 +196,34 @@ def test_quantized_llama(pkg, mode):
         pkg.save_int8_checkpoint(model, "/nonexistent/never-written.safetensors")
 
 
+def test_quantized_llama_is_refused_whole(pkg):
+    """What a mode cannot take is refused before any projection is swapped."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    def model(hidden, intermediate, layers=1):
+        return LlamaForCausalLM(LlamaConfig(
+            hidden_size=hidden, intermediate_size=intermediate, num_hidden_layers=layers, num_attention_heads=2,
+            num_key_value_heads=1, vocab_size=64)).to(torch.bfloat16).cuda()
+
+    def kinds(m):
+        return [type(x) for x in m.modules()]
+
+    for m, mode, word in ((model(64, 80), "w4a16", "in_features"), (model(48, 64), "w4a8", "in_features"),
+                          (pkg.quantize_model_(model(64, 64), "int8"), "w4a8", "already"),
+                          (pkg.quantize_model_(model(64, 64), "w8a8"), "w4a16", "already"),
+                          (pkg.quantize_model_(model(64, 64), "w4a16"), "int8", "already"),
+                          (pkg.quantize_model_(model(64, 64), "w4a8"), "w4a16", "already"),
+                          (pkg.quantize_model_(model(64, 64), "w4a8"), "w4a8", "already")):
+        before = kinds(m)
+        with pytest.raises(RuntimeError, match=word):
+            pkg.quantize_model_(m, mode)
+        assert kinds(m) == before
+    wide = model(64, 64)
+    wide.model.layers[0].input_layernorm.weight = torch.nn.Parameter(torch.ones(16416, dtype=torch.bfloat16).cuda())
+    with pytest.raises(RuntimeError, match="16384"):
+        pkg.quantize_model_(wide, "w4a8")
+
+
 @pytest.mark.parametrize("rows", [False, True])
 @pytest.mark.parametrize("m,n,k", [(1, 256, 1024), (16, 64, 640), (40, 2048, 512), (100, 128, 4096), (200, 256, 14336), (300, 512, 1024)])
 def test_products_replay_from_a_graph_on_another_stream(pkg, rows, m, n, k):
