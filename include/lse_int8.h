@@ -517,7 +517,8 @@ int lse_pack_fp4(const void* codes, const void* scales, void* out_codes, void* o
  * (the products take multiples of 4): scale = the smallest power of two s >= 2^-126 with |x| <= 448 s for every finite x
  * of the group; code = rne_e4m3(x / s), but none that stands for 2^128; infinity and NaN become NaN. K % 32 == 0.
  * lse_quantize_rows_fp8: x (M, K) bf16, row stride ldx (a multiple of 8, 16-byte aligned); K <= LSE_FP4_MAX_K.
- * lse_add_rmsnorm_fp8: lse_add_rmsnorm with y in this form (s, r and y's rounding to bf16 as there, then the codes):
+ * lse_add_rmsnorm_fp8: lse_add_rmsnorm with y in this form: its roundings, but the mean and r in 64 bits and s r the
+ *   nearest fp32, then the codes of what lse_add_rmsnorm would round to bf16:
  *   x, residual (may be NULL): (M, K) bf16, row strides multiples of 8, 16-byte aligned; weight (K) bf16; sum (M, K)
  *   bf16 contiguous receiving x + residual, or NULL; it may be x or residual where that is contiguous. K <=
  *   LSE_NORM_MAX_K.

@@ -142,23 +142,24 @@ __device__ __forceinline__ void store_once(void* p, V v) {
 }
 
 // One workgroup per row, of as many waves as its first 4096 values keep busy, thread t holding elements 8 t + 4096 i
-// (i < NV): s = bf16(x + res) (or x), n = bf16(w * bf16(s * r)), r = 1 / sqrt(mean(s^2) + eps), the roundings of
-// LlamaRMSNorm (modeling_llama.py:62-67), then n's codes and scales. The sum of squares: each thread's in order, then a
-// fixed tree, add_rmsnorm_kernel's order, so that the codes are those of its rows. `sum` may be x or res: a thread reads
-// all of its elements before it writes any.
-// Bound by HBM, 7 bytes a value: 4160 rows of 4096 24.3 us, 4.9 TB/s, a copy's rate; 2048 of 14336 42.0; 33 of 4096 4.8, a
+// (i < NV): s = bf16(x + res) (or x), n = bf16(w * bf16(fp32(s * r))), r = 1 / sqrt(mean(s^2) + eps), the roundings of
+// LlamaRMSNorm (modeling_llama.py:62-67), then n's codes and scales. A code has two or three bits after its first, so one
+// bf16 step too far, which an r of 24 bits gives now and then, can become a quarter or an eighth of the value: the sum of
+// squares (of exact squares, each thread's in order, then a fixed tree) and r are held in 64 bits and s r is the nearest
+// fp32, for 5 % of the time. `sum` may be x or res: a thread reads all of its elements before it writes any.
+// Bound by HBM, 7 bytes a value: 4160 rows of 4096 25.5 us, 4.7 TB/s, a copy's rate; 2048 of 14336 42.8; 33 of 4096 4.8, a
 // launch. Waves that would hold no element are not started (4160 of 1024: 16.9 -> 9.7 us). STREAM, for calls that move a
-// good part of the 256 MB behind L2, keeps from there what is not read again: 2048 of 14336 46.0 -> 42.0, 4160 of 4096 29.9
-// -> 24.3 after other work and 24.1 by itself either way; smaller calls are better off without (3200 of 4096 17.5 against
-// 19.4, 2560 14.9 against 16.6).
+// good part of the 256 MB behind L2, keeps from there what is not read again (with r in 32 bits: 2048 of 14336 46.0 ->
+// 42.0, 4160 of 4096 29.9 -> 24.3 after other work and 24.1 by itself either way); smaller calls are better off without
+// (3200 of 4096 17.5 against 19.4, 2560 14.9 against 16.6).
 template <int NV, bool STREAM>
 __global__ void __launch_bounds__(kNormFp8Threads)
-add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int64_t ldr, const uint16_t* w, float eps,
-                       uint16_t* sum, uint8_t* codes, uint8_t* scales, int64_t lds, int K) {
-  __shared__ float red[kNormFp8Threads / 64];
+add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int64_t ldr, const uint16_t* w, double eps,
+                       uint16_t* sum, uint8_t* codes, uint8_t* scales, int64_t lds, int K, double inv_k) {
+  __shared__ double red[kNormFp8Threads / 64];
   const int64_t m = blockIdx.x;
   float s[NV][8], g[NV][8];
-  float ss = 0.0f;
+  double ss = 0.0;
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = 8 * (threadIdx.x + kNormFp8Threads * i);
@@ -172,7 +173,7 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
       for (int j = 0; j < 8; ++j) s[i][j] = bf16_to_f32(f32_to_bf16(s[i][j] + r[j]));
     }
 #pragma unroll
-    for (int j = 0; j < 8; ++j) ss = __builtin_fmaf(s[i][j], s[i][j], ss);
+    for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)s[i][j], (double)s[i][j], ss);
   }
   if (sum) {
 #pragma unroll
@@ -187,18 +188,29 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
   for (int off = 32; off > 0; off >>= 1) ss += __shfl_xor(ss, off, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = ss;
   __syncthreads();
-  float total = red[0];
+  double total = red[0];
 #pragma unroll
   for (int i = 1; i < kNormFp8Threads / 64; ++i)
     if (64 * i < blockDim.x) total += red[i];
-  const float r = 1.0f / __builtin_sqrtf(total / (float)K + eps);
+  const double t = total * inv_k + eps;
+  double r;
+  if (t > 0x1p-100 && t < 0x1p100) {  // one step of Newton's in 64 bits from 32 gives 40
+    const double y = __builtin_amdgcn_rsqf((float)t);
+    r = __builtin_fma(y * 0.5, __builtin_fma(-t * y, y, 1.0), y);
+  } else {
+    r = 1.0 / __builtin_sqrt(t);
+  }
+  // r = rh + rl with 16 bits in rh: s rh is exact, and s r to the nearest fp32 by one fma.
+  const float rh = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)r) & 0xffffff00u);
+  const float rl = (float)(r - rh);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = 8 * (threadIdx.x + kNormFp8Threads * i);
     float n[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      n[j] = bf16_to_f32(f32_to_bf16(g[i][j] * bf16_to_f32(f32_to_bf16(s[i][j] * r))));
+    for (int j = 0; j < 8; ++j) n[j] = __builtin_fmaf(s[i][j], rl, s[i][j] * rh);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) n[j] = bf16_to_f32(f32_to_bf16(g[i][j] * bf16_to_f32(f32_to_bf16(n[j]))));
     int byte;
     const uint2 c = fp8_encode8(n, byte);  // every lane: K is a multiple of 32, so groups are whole
     if (k < K) {
@@ -297,8 +309,8 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
   const dim3 grid((unsigned)x.M), wg((unsigned)(64 * waves));
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, wg, 0, (hipStream_t)stream, (const uint16_t*)x.x, x.x_stride,
-                       (const uint16_t*)x.residual, x.residual_stride, (const uint16_t*)x.weight, (float)x.eps,
-                       (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, x.scales_stride, (int)x.K);
+                       (const uint16_t*)x.residual, x.residual_stride, (const uint16_t*)x.weight, x.eps,
+                       (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, x.scales_stride, (int)x.K, 1.0 / (double)x.K);
   };
   auto width = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;

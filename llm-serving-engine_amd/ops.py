@@ -1116,9 +1116,9 @@ def quantize_rows_fp8(x: torch.Tensor) -> Fp8Rows:
 def add_rmsnorm_fp8(
     x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float,
 ) -> tuple[torch.Tensor, Fp8Rows]:
-    """(s, LlamaRMSNorm(s) in 8 bits) with s = x + residual (x itself when residual is None) in one kernel: the bits of
-    `add_rmsnorm` and `quantize_rows_fp8` after it. x and residual (..., K) bf16, weight (K,) bf16, K % 32 == 0,
-    K <= `_lib.NORM_MAX_K`."""
+    """(s, LlamaRMSNorm(s) in 8 bits) with s = x + residual (x itself when residual is None) in one kernel: `add_rmsnorm`
+    and `quantize_rows_fp8` after it, but that the mean and its root are held in 64 bits. x and residual (..., K) bf16,
+    weight (K,) bf16, K % 32 == 0, K <= `_lib.NORM_MAX_K`."""
     dev = _one_gpu(x, weight) if residual is None else _one_gpu(x, weight, residual)
     k = x.shape[-1]
     if x.dtype is not _BF16 or weight.dtype is not _BF16 or weight.shape != (k,):

@@ -17,7 +17,7 @@ FP4 = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], dtype=torch.float64
 def scale_bytes(groups: torch.Tensor, top: float) -> torch.Tensor:
     """groups (..., 32) in 64 bits → bytes (...)."""
     amax = torch.where(torch.isfinite(groups), groups.abs(), 0.0).amax(-1)
-    powers = torch.exp2(torch.arange(-126, 128, dtype=torch.float64)) * top
+    powers = torch.exp2(torch.arange(-126, 128, dtype=torch.float64, device=groups.device)) * top
     return torch.searchsorted(powers, amax.contiguous()) + 1  # the first power with amax <= it; byte 1 is 2^-126
 
 
@@ -107,8 +107,8 @@ def glu(gate: torch.Tensor, up: torch.Tensor) -> torch.Tensor:
 
 
 def add_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tensor, eps: float):
-    """(s, n): s = bf16(x + residual), n = bf16(w bf16(s / sqrt(mean(s^2) + eps))), both bf16."""
+    """(s, n): s = bf16(x + residual), n = bf16(w bf16(fp32(s / sqrt(mean(s^2) + eps)))), both bf16."""
     s = x if residual is None else (x.double() + residual.double()).to(torch.bfloat16)
     h = s.double()
-    t = (h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps)).to(torch.bfloat16)
+    t = (h / torch.sqrt((h * h).mean(-1, keepdim=True) + eps)).float().to(torch.bfloat16)
     return s, (weight.double() * t.double()).to(torch.bfloat16)
