@@ -16,13 +16,12 @@ int64_t row_tiles(const lse_fp4_gemm_args& p) { return (p.glu ? 2 : 1) * lse::ce
 // is 1 % slower than the fastest in the mean, 13 % at most.
 struct Tile {
   int bm, bn;
-  int slots[2];           // workgroups that run at once on 256 CUs, bf16 and 8-bit rows
-  double one[2], all[2];  // of a stage: one workgroup a CU, and all slots taken
+  int slots;        // workgroups that run at once on 256 CUs
+  double one, all;  // of a stage: one workgroup a CU, and all slots taken
 };
-constexpr Tile kTiles[] = {{32, 128, {256, 512}, {0.29, 0.26}, {0.29, 0.45}},
-                           {64, 128, {256, 512}, {0.46, 0.37}, {0.46, 0.64}},
-                           {128, 256, {256, 256}, {1.50, 0.96}, {1.50, 0.96}},
-                           {256, 256, {0, 256}, {0, 1.57}, {0, 1.57}}};  // bf16 rows: 3.1, no better than two of 128
+constexpr Tile kTiles[2][3] = {
+    {{32, 128, 256, 0.29, 0.29}, {64, 128, 256, 0.46, 0.46}, {64, 256, 512, 0.82, 1.50}},   // bf16 rows
+    {{32, 128, 512, 0.26, 0.45}, {64, 128, 512, 0.37, 0.64}, {128, 256, 512, 0.85, 1.62}}};  // 8-bit rows
 constexpr double kLaunchUs = 2.5, kStreamBytesPerUs = 4.3e6, kTileBytesPerUs = 5e6, kL1BytesPerUs = 65e3;
 constexpr double kSecondPassUs = 3.0, kPartBytesPerUs = 4e6;
 constexpr int64_t kMaxPartBytes = 64 << 20;
@@ -49,17 +48,17 @@ lse::Fp4Plan plan_of(const lse_fp4_gemm_args& p) {
     const double us = kLaunchUs + std::max(weight / kStreamBytesPerUs, rounds * bytes / kL1BytesPerUs);
     take(us, 0, 16 * rt, 1, chunks);
   }
-  for (const Tile& t : kTiles) {
-    if (t.slots[rows8] == 0 || (p.M <= 16 && (t.bm > 32 || !rows8))) continue;
+  for (const Tile& t : kTiles[rows8]) {
+    if (p.M <= 16 && (t.bm > 32 || !rows8)) continue;
     const int64_t tiles = lse::ceil_div(p.M, t.bm) * lse::ceil_div(nrb, t.bn / 16);
     for (int64_t splits = 1; splits <= 8; splits *= 2) {
       const int64_t per = lse::ceil_div(chunks, splits), ranges = lse::ceil_div(chunks, per);
       if (splits > 1 && (ranges != splits || per < 2)) break;
       const double part = 64.0 * nrb * p.M * splits;
       if (splits > 1 && part > kMaxPartBytes) break;
-      const int64_t blocks = tiles * splits, full = blocks / t.slots[rows8], rest = blocks % t.slots[rows8];
-      const double last = rest == 0 ? 0.0 : rest <= 256 ? t.one[rows8] : t.all[rows8];
-      double us = std::min<double>(stages, 4 * per) * (full * t.all[rows8] + last);
+      const int64_t blocks = tiles * splits, full = blocks / t.slots, rest = blocks % t.slots;
+      const double last = rest == 0 ? 0.0 : rest <= 256 ? t.one : t.all;
+      double us = std::min<double>(stages, 4 * per) * (full * t.all + last);
       us = kLaunchUs + std::max(weight / kTileBytesPerUs, us);
       if (splits > 1) us += kSecondPassUs + 2 * part / kPartBytesPerUs;
       take(us, t.bm, t.bn, splits, per);

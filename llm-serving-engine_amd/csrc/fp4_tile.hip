@@ -1,13 +1,13 @@
 // Products of many rows with a 4-bit weight (layouts and formats: fp4.h; the arithmetic as in fp4_stream.hip), bound by
 // the matrix cores.
 //
-// A workgroup of WGM x WGN waves (KG groups of so many) computes BM token rows x BN weight rows over K, in stages of
-// 128 k a group, which take them in turn. Token rows go to LDS by direct loads (whole 256 or 128 byte row pieces, 16-byte
-// chunks swizzled by row), NST - 1 stages ahead; the weight, a quarter or a half of their bytes, goes straight to the
-// registers of the wave that multiplies it, as far ahead: each wave needs BN / WGN rows of it and no other wave of its
-// row of waves does. One barrier a stage. bf16 rows: a wave decodes its weight tiles (half an instruction a weight,
-// shared by its WM token rows) and runs 16x16x32 bf16 instructions. 8-bit rows: codes and scale bytes of both operands
-// go to the scaled 16x16x128 instruction as they are.
+// A workgroup of four waves (KG groups of four) computes BM token rows x BN weight rows over K, in stages of 128 k a
+// group, which take them in turn. Token rows go to LDS by direct loads (whole 256 or 128 byte row pieces, 16-byte chunks
+// swizzled by row), NST - 1 stages ahead; the weight, a quarter or a half of their bytes, goes straight to the registers
+// of the wave that multiplies it, as far ahead: each wave needs BN / 4 rows of it and no other wave of its group does.
+// One barrier a stage. bf16 rows: a wave decodes its weight tiles (half an instruction a weight, shared by the BM token
+// rows) and runs 16x16x32 bf16 instructions. 8-bit rows: codes and scale bytes of both operands go to the scaled
+// 16x16x128 instruction as they are.
 //
 // Tile order: blocks are dealt to the 8 XCDs in turn; each XCD gets a contiguous range of tiles, in groups of
 // kFp4GroupM token blocks x consecutive weight panels, so that what it runs at once shares token rows and weights in
@@ -15,13 +15,14 @@
 // K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order.
 // A result depends on K, the groups and the split alone, never on other rows.
 //
-// What it measured: bf16 rows, 128 x 256 tiles, 2048 by two of 14336 x 4096 340 us, 1410 TFLOP/s, by 4096 x 14336 161,
-// 1490 (a large library product 1330 to 1380), matrix cores busy for two thirds of the time; 8-bit rows, 256 x 256, 2048
-// by two of 14336 x 4096 201 us, 2390 TFLOP/s, 128 x 256, by 4096 x 14336 98, 2450 (a library's fp8 2590 to 2930), busy
-// 60 %: the LDS reads and decoding of a wave do not all hide behind the other wave of its SIMD, whose stage ends at the
-// same barrier. Deeper rings (3, 4, 6 slots) gain nothing, a second barrier in mid-stage spills.
+// What it measured: bf16 rows, 64 x 256 tiles, 2048 by two of 14336 x 4096 342 us, 1405 TFLOP/s, by 4096 x 14336 166,
+// 1450 (a large library product 1330 to 1380); 8-bit rows, 128 x 256 tiles, 2048 by two of 14336 x 4096 182 us, 2640
+// TFLOP/s, by 4096 x 14336 92, 2610 (a library's fp8 2590 to 2930). The matrix cores bound these, but for the time around
+// the barriers: two workgroups of four waves share a CU, so that one runs while the other waits. One of eight waves, of
+// twice the tile, gave 205 us with 8-bit rows (256 x 256) and 345 with bf16 ones (128 x 256). Deeper rings (3, 4, 6 slots)
+// gain nothing, a second barrier in mid-stage spills.
 //
-// The small tiles fill a card with one workgroup a CU, a wave a SIMD, whose decoding, LDS reads and matrix instructions
+// A small tile's workgroup is often alone on its CU, a wave a SIMD, whose decoding, LDS reads and matrix instructions
 // then wait for each other: with bf16 rows they take two groups (256 rows by 4096 x 4096: 14.1 -> 11.1 us; 777 by
 // 2330 x 4128: 22.3 -> 20.1). What bounds them then is the CU's way from L2, 50 to 60 bytes a ns: 17 or 25 KB a stage.
 // 8-bit rows, half the bytes and no decoding, ran slower with two (12.5 -> 12.9) and keep one, with four slots.
@@ -38,12 +39,12 @@ namespace lse {
 
 constexpr int kFp4GroupM = 4;
 
-template <bool A8, int BM, int BN, int WGM, int WGN, int KG, int NST, bool GLU>
-__global__ void __launch_bounds__(64 * WGM * WGN * KG)
+template <bool A8, int BM, int BN, int KG, int NST, bool GLU>
+__global__ void __launch_bounds__(256 * KG, 2)
 fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   static_assert(KG == 1 || KG == 2, "whole chunks");
-  constexpr int W = WGM * WGN, WM = BM / WGM, WN = BN / WGN, TM = WM / 16, TN = WN / 16;
-  static_assert(WM % 16 == 0 && WN % 16 == 0 && (!GLU || TN % 2 == 0), "whole tiles, and pairs of row tiles");
+  constexpr int W = 4, TM = BM / 16, TN = BN / W / 16;  // waves of a group, their tiles
+  static_assert(BM % 16 == 0 && BN % (16 * W) == 0 && (!GLU || TN % 2 == 0), "whole tiles, and pairs of row tiles");
   constexpr int ESZ = A8 ? 1 : 2;
   constexpr int ROWB = kFp4Step * ESZ, CH = ROWB / 16;  // bytes of a token row and stage, its 16-byte chunks
   constexpr int RPL = 1024 / ROWB;                      // rows of a 1 KB load
@@ -62,7 +63,6 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const int lane = threadIdx.x & 63;
   const int all = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kg = KG == 1 ? 0 : all / W, wave = KG == 1 ? all : all % W;  // the wave's group, and its place there
-  const int wm = wave / WGN, wn = wave % WGN;
   const int r16 = lane & 15, g = lane >> 4;
 
   const int sp = blockIdx.x % p.splits;
@@ -94,7 +94,7 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   uint32_t wp[TN], wsp[TN];
 #pragma unroll
   for (int j = 0; j < TN; ++j) {
-    const uint32_t tile = min(wn * TN + j, tiles - 1);
+    const uint32_t tile = min(wave * TN + j, tiles - 1);
     wp[j] = (tile * a.nsteps + 4 * c0) * kFp4TileBytes;
     wsp[j] = (tile * a.nchunks + c0) * kFp4ScaleBytes;
   }
@@ -159,10 +159,10 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const uint32_t tail = a.K % kFp4Step ? (1u << (8 * (a.K % kFp4Step / kFp4Group))) - 1 : ~0u;
   // Where this lane's operands of the wave's first token tile lie in a slot. The compiler is kept from taking the sums
   // apart: it follows an LDS access to its array through a few additions only.
-  int at[A8 ? 2 : 4], sat = kg * XS + wm * WM + r16;
+  int at[A8 ? 2 : 4], sat = kg * XS + r16;
 #pragma unroll
   for (int i = 0; i < (A8 ? 2 : 4); ++i) {
-    at[i] = kg * SLOT + (wm * WM + r16) * CH + ((A8 ? 4 * i + g : 4 * g + i) ^ swz(r16));
+    at[i] = kg * SLOT + r16 * CH + ((A8 ? 4 * i + g : 4 * g + i) ^ swz(r16));
     asm volatile("" : "+v"(at[i]));
   }
   asm volatile("" : "+v"(sat));
@@ -226,22 +226,16 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
       load_x(s + NST - 1, std::integral_constant<int, ahead>{});
       if (whole || KG == 1 || s < stages)
         compute(s, std::integral_constant<int, slot>{}, std::integral_constant<int, KG * (u % SC)>{}, st[slot], sc);
-      // The order of the stage's LDS reads (0x100) and matrix instructions (0x008), where a wave has so many of both that
-      // the compiler reads a tile and waits for it at once: bf16 rows 2 tiles ahead of their instructions (2048 rows by
-      // two 14336 x 4096 weights: 349 -> 340 us), 8-bit rows (two chunks and a scale a tile) likewise (202 -> 198 us).
-      // The 128 token rows of 8 bits, half as many tiles a wave, ran 1 % slower so and keep the compiler's order.
-      if constexpr (!A8 && TN == 4) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-        unroll<4 * TM - 2>([&](auto) {
+      // The order of the stage's LDS reads (0x100) and matrix instructions (0x008) of the wide tiles, where a wave has so
+      // many of both that the compiler reads a tile and waits for it at once: bf16 rows 2 tiles ahead of their
+      // instructions (2048 rows by two 14336 x 4096 weights, tiles of eight waves: 349 -> 340 us), 8-bit rows (two
+      // chunks and a scale a tile) likewise (202 -> 198 us).
+      if constexpr (TN == 4) {
+        constexpr int READS = A8 ? 3 : 1, TILES = A8 ? TM : 4 * TM;
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * READS, 0);
+        unroll<TILES - 2>([&](auto) {
           __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-        });
-        __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN, 0);
-      } else if constexpr (A8 && TN == 4 && TM > 4) {
-        __builtin_amdgcn_sched_group_barrier(0x100, 6, 0);
-        unroll<TM - 2>([&](auto) {
-          __builtin_amdgcn_sched_group_barrier(0x008, TN, 0);
-          __builtin_amdgcn_sched_group_barrier(0x100, 3, 0);
+          __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
         });
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN, 0);
       }
@@ -281,11 +275,11 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   const bool yvec = (a.ldy & 3) == 0 && ((uintptr_t)a.y & 7) == 0;
 #pragma unroll
   for (int i = 0; i < TM; ++i) {
-    const int m = m0 + wm * WM + 16 * i + r16;
+    const int m = m0 + 16 * i + r16;
     if (m >= a.M) continue;
 #pragma unroll
     for (int j = 0; j < TN; ++j) {
-      const int rb = rb0 + wn * TN + j;
+      const int rb = rb0 + wave * TN + j;
       if (p.splits > 1) {
         if (rb < a.nrb)
           *reinterpret_cast<f32x4*>(p.part + ((int64_t)sp * a.M + m) * (16 * a.nrb) + 16 * rb + 4 * g) = acc[i][j];
@@ -349,14 +343,14 @@ static int launch(const Fp4Args& a, const Fp4Plan& plan, float* part, hipStream_
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(threads), 0, stream, a, p);
   };
   if constexpr (A8) {
-    if (plan.bm == 256) go(fp4_tile_kernel<A8, 256, 256, 2, 4, 1, 2, GLU>, 512);
+    if (plan.bm == 128) go(fp4_tile_kernel<true, 128, 256, 1, 2, GLU>, 256);
+    if (plan.bm == 64) go(fp4_tile_kernel<true, 64, 128, 1, 4, GLU>, 256);
+    if (plan.bm == 32) go(fp4_tile_kernel<true, 32, 128, 1, 4, GLU>, 256);
+  } else {
+    if (plan.bn == 256) go(fp4_tile_kernel<false, 64, 256, 1, 2, GLU>, 256);
+    if (plan.bn == 128 && plan.bm == 64) go(fp4_tile_kernel<false, 64, 128, 2, 2, GLU>, 512);
+    if (plan.bn == 128 && plan.bm == 32) go(fp4_tile_kernel<false, 32, 128, 2, 2, GLU>, 512);
   }
-  if (plan.bm == 128)
-    go(fp4_tile_kernel<A8, 128, 256, 2, 4, 1, 2, GLU>, 512);
-  if (plan.bm == 64)
-    go(fp4_tile_kernel<A8, 64, 128, 1, 4, A8 ? 1 : 2, A8 ? 4 : 2, GLU>, A8 ? 256 : 512);
-  if (plan.bm == 32)
-    go(fp4_tile_kernel<A8, 32, 128, 1, 4, A8 ? 1 : 2, A8 ? 4 : 2, GLU>, A8 ? 256 : 512);
   if (p.splits > 1) {
     if (int st = launch_status()) return st;
     const int64_t quads = (int64_t)a.M * ceil_div(a.N, 4);
