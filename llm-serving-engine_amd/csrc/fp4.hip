@@ -10,10 +10,10 @@ constexpr int64_t kMax31 = 2147483647;
 
 int64_t row_tiles(const lse_fp4_gemm_args& p) { return (p.glu ? 2 : 1) * lse::ceil_div(p.N, 16); }
 
-// Microseconds that a call takes apart from the weight's way from HBM, for the tile kernels by stages (128 k of one tile
-// on each CU), for the streaming kernel by what a CU reads through its L1. Fitted to 94 sizes of both kinds of rows and
-// both epilogues (M 9 to 8192, N 1024 to 28672, K 1536 to 14336), each timed with every plan below: the one chosen here
-// is 1 % slower than the fastest in the mean, 13 % at most.
+// Microseconds that a call takes apart from the weight's way from HBM, for the tile kernels by stages (128 k of one
+// tile on each CU), for the streaming kernel by what a CU reads through its L1. Fitted to 84 sizes of both kinds of rows
+// and both epilogues (M 9 to 4096, N 1024 to 28672, K 1536 to 14336), each timed with the plans below that suit it: the
+// one chosen here is 0.6 % slower than the fastest in the mean, 11 % at most.
 struct Tile {
   int bm, bn;
   int slots;        // workgroups that run at once on 256 CUs

@@ -310,7 +310,8 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
   auto go = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, grid, wg, 0, (hipStream_t)stream, (const uint16_t*)x.x, x.x_stride,
                        (const uint16_t*)x.residual, x.residual_stride, (const uint16_t*)x.weight, x.eps,
-                       (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, x.scales_stride, (int)x.K, 1.0 / (double)x.K);
+                       (uint16_t*)x.sum, (uint8_t*)x.codes, (uint8_t*)x.scales, x.scales_stride, (int)x.K,
+                       1.0 / (double)x.K);
   };
   auto width = [&](auto nv) {
     constexpr int NV = decltype(nv)::value;
