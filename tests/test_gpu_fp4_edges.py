@@ -12,7 +12,8 @@ from test_gpu_fp4_gemm import _bound, _check
 
 pytestmark = pytest.mark.gpu
 
-KINDS = [(1, 40, 640), (13, 100, 1184), (40, 3600, 544), (100, 64, 96), (300, 500, 1056), (700, 1100, 640)]
+KINDS = [(1, 40, 640), (13, 100, 1184), (40, 3600, 544), (100, 64, 96), (300, 500, 1056), (700, 1100, 640),
+         (1050, 6100, 544)]
 
 
 SPLIT = [(300, 1030, 14336, False), (260, 2050, 14400, False), (130, 530, 28704, True)]  # K over 2 to 8 workgroups

@@ -72,7 +72,18 @@ def test_glu(pkg, m, n, k, rows):
     _check(pkg, m, n, k, rows, True)
 
 
-@pytest.mark.parametrize("m,n,k", [(1, 300, 4128), (13, 100, 1184), (70, 333, 2048), (300, 500, 1600)])
+# The widest tiles, at their edges in every direction.
+LARGE = [(1000, 6150, 1184), (2100, 3601, 160), (700, 3601, 2080), (1023, 2070, 96), (301, 6150, 672)]
+
+
+@pytest.mark.parametrize("glu", [False, True], ids=["linear", "glu"])
+@pytest.mark.parametrize("rows", [False, True], ids=["bf16", "fp8"])
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_large(pkg, m, n, k, rows, glu):
+    _check(pkg, m, n, k, rows, glu)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 300, 4128), (13, 100, 1184), (70, 333, 2048), (300, 500, 1600), (1000, 6150, 1184)])
 @pytest.mark.parametrize("rows", [False, True], ids=["bf16", "fp8"])
 def test_every_place_exactly(pkg, m, n, k, rows):
     """Five values of a row, so every output is a multiple of 1/8 below 32: exact in bf16, whatever the order."""
