@@ -200,8 +200,9 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   };
 
   // NST register sets of weights, each refilled when its step is done. Issued after a stage's rows when that stage
-  // begins: the rows of the NST - 2 later stages, and the weights of the NST - 1.
-  constexpr int XLOADS = XI + XSI, LATER = (NST - 1) * TN + (NST - 2) * XLOADS;
+  // begins: the rows of the NST - 2 later stages, and the weights of the NST - 1. The compiler drops weight loads that
+  // no later stage of the last, partial group uses, so there only the rows count.
+  constexpr int XLOADS = XI + XSI, ROWS_LATER = (NST - 2) * XLOADS, LATER = (NST - 1) * TN + ROWS_LATER;
   static_assert(LATER < 64, "vmcnt holds at most 63");
   constexpr int U = 4, SC = 4 / KG;  // stages of the loop body: whole chunks, of SC stages, and whole rings
   const int stages = (steps + KG - 1 - kg) / KG, most = (steps + KG - 1) / KG, least = steps / KG;
@@ -210,6 +211,7 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
   Scales sc, next;
   load_s(0, sc);
   unroll<NST - 1>([&](auto i) { load_x(i, i); });
+  if constexpr (NST > 2) __builtin_amdgcn_sched_barrier(0);  // rows before weights, as LATER has it
 #pragma unroll
   for (int i = 0; i < NST; ++i) load_w(i, st[i]);
   auto body = [&](int base, auto whole) {
@@ -220,7 +222,7 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
       asm volatile("" ::: "memory");  // the reads of the stage before stay before the barrier
       // This wave's rows of stage s have landed and its reads of the slot that the loads below go to are done; after
       // the barrier every wave's are.
-      __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(LATER));
+      __builtin_amdgcn_s_waitcnt(vmcnt_lgkm0_imm(whole ? LATER : ROWS_LATER));
       __builtin_amdgcn_s_barrier();
       if constexpr (u % SC == 0) load_s(s / SC + 1, next);
       load_x(s + NST - 1, std::integral_constant<int, ahead>{});
@@ -239,6 +241,8 @@ fp4_tile_kernel(Fp4Args a, Fp4Split p) {
         });
         __builtin_amdgcn_sched_group_barrier(0x008, 2 * TN, 0);
       }
+      // The stage's rows are issued before its weights, as LATER has it; two slots' assembly keeps its place by itself.
+      if constexpr (NST > 2) __builtin_amdgcn_sched_barrier(0);
       load_w(s + NST, st[slot]);
       if constexpr (u % SC == SC - 1) sc = next;
     });
