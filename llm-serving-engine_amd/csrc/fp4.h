@@ -77,6 +77,7 @@ __device__ __forceinline__ void dma4_lds(u32x4 r, uint32_t base, uint32_t offset
   asm volatile(
       "s_mov_b32 %0, m0\n\t"
       "s_add_u32 m0, %1, %4\n\t"
+      "s_nop 0\n\t"
       "buffer_load_dword %2, %3, 0 offen lds\n\t"
       "s_mov_b32 m0, %0"
       : "=&s"(saved)

@@ -220,7 +220,8 @@ __device__ __forceinline__ uint32_t lds_addr(const void* lds) {
 }
 
 // One load to LDS byte address base + IMM (+ 16 l for lane l); NT: the streaming (nt) cache
-// policy, for data read once per call.
+// policy, for data read once per call. A load to LDS needs one wait state after a scalar
+// instruction that writes M0, which the compiler cannot put into the block.
 template <int IMM, bool NT = false>
 __device__ __forceinline__ void dma16_lds(u32x4 r, uint32_t base, uint32_t offset) {
   uint32_t saved;
@@ -228,6 +229,7 @@ __device__ __forceinline__ void dma16_lds(u32x4 r, uint32_t base, uint32_t offse
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_add_u32 m0, %1, %4\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %3, 0 offen nt lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)
@@ -237,6 +239,7 @@ __device__ __forceinline__ void dma16_lds(u32x4 r, uint32_t base, uint32_t offse
     asm volatile(
         "s_mov_b32 %0, m0\n\t"
         "s_add_u32 m0, %1, %4\n\t"
+        "s_nop 0\n\t"
         "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
         "s_mov_b32 m0, %0"
         : "=&s"(saved)

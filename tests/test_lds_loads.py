@@ -88,3 +88,19 @@ def test_a_stages_rows_have_landed_at_its_barrier(pkg, tmp_path):
         assert _most_at_a_barrier(code) <= (slots - 2) * loads, name
         tiles += 1
     assert tiles == 12
+
+
+def _loads_right_after_m0(code) -> list[int]:
+    """Loads to LDS with no instruction between them and the scalar one that wrote M0, where their address is: they need
+    one wait state there."""
+    return [b[0] for a, b in zip(code, code[1:])
+            if re.match(r"s_\w+", a[1]) and re.match(r"m0\b", a[2]) and b[1].startswith(("buffer_load", "global_load"))
+            and (re.search(r"\blds\b", b[2]) or "_lds_" in b[1])]
+
+
+def test_the_address_of_a_load_to_lds_is_there_before_it(pkg, tmp_path):
+    early = [(0, "s_add_u32", "m0, s1, 0x400", None), (4, "buffer_load_dword", "v1, s[0:3], 0 offen lds", None)]
+    assert _loads_right_after_m0(early) == [4]
+    assert not _loads_right_after_m0([early[0], (2, "s_nop", "0", None), early[1]])
+    found = {name: _loads_right_after_m0(code) for name, code in _listing(pkg, tmp_path).items()}
+    assert not {name: len(at) for name, at in found.items() if at}
