@@ -550,8 +550,9 @@ int lse_add_rmsnorm_fp8(const struct lse_add_rmsnorm_fp8_args* args, void* strea
  *   strides at most LSE_FP4_MAX_K. y: (M, N) bf16, row stride y_stride.
  * Equal calls give equal bits, and a row's do not depend on the other rows' values. Which kernel a call takes, and in
  *   what order it adds up, follows from M, N, K, glu and the kind of rows: the same row in a call of another M may differ
- *   by the fp32 sums' order. Rows of y past M and columns past N are not written. workspace: lse_fp4_gemm_workspace_bytes bytes (it reads the
- *   sizes in args only; -1: invalid ones; 0 for most calls), 16-byte aligned.
+ *   by the fp32 sums' order. Rows of y past M and columns past N are not written.
+ * workspace: lse_fp4_gemm_workspace_bytes bytes (0 for most calls), 16-byte aligned. That function reads M, N, K, glu and
+ *   whether x_scales is NULL, by which it knows rows in 8 bits; -1: invalid ones.
  * Replaces: `F.linear(x, W)` (torch/nn/modules/linear.py:134) at model_runner.py:322-324,369,418 and
  * `act_fn(gate_proj(x)) * up_proj(x)` (modeling_llama.py:175, from model_runner.py:223), for 4-bit weights, which the
  * reference does not have.

@@ -73,7 +73,7 @@ extern "C" {
 
 int64_t lse_fp4_gemm_workspace_bytes(const struct lse_fp4_gemm_args* args) {
   if (!args || args->M < 0 || args->N < 0 || args->K < 0 || args->M > kMax31 || args->N > kMax31 - 64 ||
-      args->K > LSE_FP4_MAX_K || args->K % lse::kFp4Group)
+      args->K > LSE_FP4_MAX_K || args->K % lse::kFp4Group || (args->glu != 0 && args->glu != 1))
     return -1;
   if (args->M == 0 || args->N == 0 || args->K == 0) return 0;
   const int64_t nrb = row_tiles(*args);
