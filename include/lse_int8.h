@@ -84,7 +84,7 @@ enum lse_query_key {
   LSE_Q_NOALLOC_SCRATCH = 5, /* bytes of the static scratch lse_w8a16_gemm_noalloc works in */
 };
 
-#define LSE_ABI_VERSION 16
+#define LSE_ABI_VERSION 17
 #define LSE_NOALLOC_SCRATCH_BYTES (32 << 20)
 #define LSE_K_ALIGN 16
 #define LSE_DECODE_MAX_M 64
@@ -568,6 +568,11 @@ struct lse_fp4_gemm_args {
 };
 int64_t lse_fp4_gemm_workspace_bytes(const struct lse_fp4_gemm_args* args);
 int lse_fp4_gemm(const struct lse_fp4_gemm_args* args, void* workspace, int64_t workspace_bytes, void* stream);
+/* What such a call would run, from the fields that lse_fp4_gemm_workspace_bytes reads: tiles of tile_rows token rows x
+ * tile_columns weight rows (gate/up: of both), K in `splits` ranges, or, tile_rows 0, the kernel for few rows, tile_columns
+ * weight rows a workgroup. All 0 where M, N or K is. */
+int lse_fp4_gemm_choice(const struct lse_fp4_gemm_args* args, int64_t* tile_rows, int64_t* tile_columns,
+                        int64_t* splits);
 
 /* Static properties (enum lse_query_key); -1 for an unknown key. Load-time checks read these,
  * as `ModelRunner.check_custom_kernel_support` (model_runner.py:77-94) checks its kernels. */

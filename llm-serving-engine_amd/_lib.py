@@ -59,6 +59,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "lse_add_rmsnorm_fp8": (_INT, [_P, _P]),
     "lse_fp4_gemm_workspace_bytes": (_I64, [_P]),
     "lse_fp4_gemm": (_INT, [_P, _P, _I64, _P]),
+    "lse_fp4_gemm_choice": (_INT, [_P] * 4),
     "lse_query": (_I64, [_INT]),
     "lse_status_string": (ctypes.c_char_p, [_INT]),
 }
@@ -78,7 +79,7 @@ MODE_W8A16, MODE_W8A8 = 0, 1
 E_WORKSPACE, E_SCRATCH = -6, -7
 Q_ABI_VERSION, Q_K_ALIGN, Q_DECODE_MAX_M, Q_MAX_K, Q_GFX_ARCH = 0, 1, 2, 3, 4
 Q_NOALLOC_SCRATCH = 5
-ABI_VERSION = 16
+ABI_VERSION = 17
 NORM_MAX_K = 16384
 FP4_MAX_K = 2097152
 

@@ -67,27 +67,41 @@ lse::Fp4Plan plan_of(const lse_fp4_gemm_args& p) {
   return best;
 }
 
+// LSE_OK if the sizes are a product's (K may be 0).
+int check_sizes(const lse_fp4_gemm_args& p) {
+  if (p.M < 0 || p.N < 0 || p.K < 0 || p.M > kMax31 || p.N > kMax31 - 64 || (p.glu != 0 && p.glu != 1))
+    return LSE_E_SHAPE;
+  if (p.K % lse::kFp4Group) return LSE_E_ALIGN;
+  return p.K > LSE_FP4_MAX_K ? LSE_E_RANGE : LSE_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
 int64_t lse_fp4_gemm_workspace_bytes(const struct lse_fp4_gemm_args* args) {
-  if (!args || args->M < 0 || args->N < 0 || args->K < 0 || args->M > kMax31 || args->N > kMax31 - 64 ||
-      args->K > LSE_FP4_MAX_K || args->K % lse::kFp4Group || (args->glu != 0 && args->glu != 1))
-    return -1;
+  if (!args || check_sizes(*args)) return -1;
   if (args->M == 0 || args->N == 0 || args->K == 0) return 0;
   const int64_t nrb = row_tiles(*args);
   const lse::Fp4Plan plan = plan_of(*args);
   return plan.splits > 1 ? plan.splits * args->M * 16 * nrb * 4 : 0;
 }
 
+int lse_fp4_gemm_choice(const struct lse_fp4_gemm_args* args, int64_t* tile_rows, int64_t* tile_columns,
+                        int64_t* splits) {
+  if (!args || !tile_rows || !tile_columns || !splits) return LSE_E_NULL;
+  if (const int st = check_sizes(*args)) return st;
+  lse::Fp4Plan plan{};
+  if (args->M && args->N && args->K) plan = plan_of(*args);
+  *tile_rows = plan.bm, *tile_columns = plan.bn, *splits = plan.splits;
+  return LSE_OK;
+}
+
 int lse_fp4_gemm(const struct lse_fp4_gemm_args* args, void* workspace, int64_t workspace_bytes, void* stream) {
   if (!args) return LSE_E_NULL;
   const lse_fp4_gemm_args& p = *args;
-  if (p.M < 0 || p.N < 0 || p.K < 0 || p.M > kMax31 || p.N > kMax31 - 64 || (p.glu != 0 && p.glu != 1))
-    return LSE_E_SHAPE;
-  if (p.K % lse::kFp4Group) return LSE_E_ALIGN;
-  if (p.K == 0 || p.K > LSE_FP4_MAX_K) return LSE_E_RANGE;
+  if (const int st = check_sizes(p)) return st;
+  if (p.K == 0) return LSE_E_RANGE;
   if (p.M == 0 || p.N == 0) return LSE_OK;
   const bool rows8 = p.x_scales != nullptr;
   if (!p.x || !p.codes || !p.scales || !p.y) return LSE_E_NULL;
