@@ -194,21 +194,32 @@ add_rmsnorm_fp8_kernel(const uint16_t* x, int64_t ldx, const uint16_t* res, int6
     if (64 * i < blockDim.x) total += red[i];
   const double t = total * inv_k + eps;
   double r;
-  if (t > 0x1p-100 && t < 0x1p100) {  // one step of Newton's in 64 bits from 32 gives 40
+  const bool narrow = t > 0x1p-100 && t < 0x1p100;
+  if (narrow) {  // one step of Newton's in 64 bits from 32 gives 40
     const double y = __builtin_amdgcn_rsqf((float)t);
     r = __builtin_fma(y * 0.5, __builtin_fma(-t * y, y, 1.0), y);
   } else {
     r = 1.0 / __builtin_sqrt(t);
   }
-  // r = rh + rl with 16 bits in rh: s rh is exact, and s r to the nearest fp32 by one fma.
+  // r = rh + rl with 16 bits in rh: s rh is exact, and s r to the nearest fp32 by one fma. Where fp32 holds r badly or not
+  // at all (rows below 2^-126, or of the largest values), in 64 bits.
   const float rh = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, (float)r) & 0xffffff00u);
   const float rl = (float)(r - rh);
 #pragma unroll
   for (int i = 0; i < NV; ++i) {
     const int k = 8 * (threadIdx.x + kNormFp8Threads * i);
     float n[8];
+    if (narrow) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) n[j] = __builtin_fmaf(s[i][j], rl, s[i][j] * rh);
+      for (int j = 0; j < 8; ++j) n[j] = __builtin_fmaf(s[i][j], rl, s[i][j] * rh);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        float v = s[i][j];
+        asm volatile("" : "+v"(v));  // or the compiler keeps every s in 64 bits from the sum of squares to here
+        n[j] = (float)(v * r);
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; ++j) n[j] = bf16_to_f32(f32_to_bf16(g[i][j] * bf16_to_f32(f32_to_bf16(n[j]))));
     int byte;
