@@ -40,8 +40,9 @@ __device__ __forceinline__ void unroll(F&& f) {
   unroll_seq(f, std::make_integer_sequence<int, N>{});
 }
 
-// Eight weights of a dword times 2^(scale's exponent field - 127), in k order; exact but for products past bf16's range
-// (v_cvt_scalef32_pk_bf16_fp4; measured over every code and scale).
+// Eight weights of a dword times 2^(scale's exponent field - 127), in k order: exact from bf16's subnormals up, infinite
+// from 2^128 on, and NaN, codes of zero too, where the field is 255 (v_cvt_scalef32_pk_bf16_fp4;
+// tests/test_gpu_fp4_codes.py takes every code and scale through the products).
 __device__ __forceinline__ bf16x8 fp4_decode8(uint32_t w, float scale) {
   typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
   const bf16x2 a = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0);
@@ -51,8 +52,8 @@ __device__ __forceinline__ bf16x8 fp4_decode8(uint32_t w, float scale) {
   return bf16x8{a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
 }
 
-// Byte t of a scale dword as a float of that exponent field (0, which stands for 2^-127, and 255 too: the
-// conversion reads the field alone).
+// Byte t of a scale dword as a float of that exponent field. The conversion reads the field alone and as an e8m0 byte: 0
+// is 2^-127, where the float is zero, and 255 NaN, where it is infinity.
 __device__ __forceinline__ float fp4_scale(uint32_t dword, int t) {
   return __builtin_bit_cast(float, (dword >> (8 * t) & 0xff) << 23);
 }
@@ -62,7 +63,8 @@ __device__ __forceinline__ float fp4_scale(uint32_t dword, int t) {
 // 16 (l / 16) .. + 15 (lo) and 64 + 16 (l / 16) .. + 15 (hi); byte T of ws and byte 0 of xs scale the 32 k from
 // 32 (l / 16) on. D as the 16x16x32 instruction's. The instruction cuts the products of eight consecutive k off 13
 // bits below the largest of them (toward zero; measured) and adds the rest in fp32: 2^-14 of the result in the mean
-// of random ones, far below the steps of 2^-4 that the 8-bit operand was rounded to.
+// of random ones, far below the steps of 2^-4 that the 8-bit operand was rounded to. One bf16 output in a hundred goes to
+// its neighbour by it (64 x 4096 x 4096: 1.6493e-3 off the 64-bit product in the norm, its nearest bf16 values 1.6492e-3).
 template <int T>
 __device__ __forceinline__ f32x4 mfma_fp4_fp8(uint4 w, uint32_t ws, uint4 lo, uint4 hi, uint32_t xs, f32x4 c) {
   const i32x8 a = {(int)w.x, (int)w.y, (int)w.z, (int)w.w, 0, 0, 0, 0};
