@@ -1051,12 +1051,13 @@ def unpack_fp4(weight: Fp4Weight) -> tuple[torch.Tensor, torch.Tensor]:
     """Inverse of `pack_fp4` (a pure permutation, done with torch views): (codes, scales) row by row."""
     _, tiles = _check_fp4(weight, None)
     glu, n, k = tiles != -(-weight.n // 16), weight.n, weight.k
-    c = weight.codes.view(tiles, -1, 4, 16, 16).permute(0, 3, 1, 2, 4).reshape(tiles * 16, -1)[:, :k // 2]
-    s = weight.scales.view(torch.uint8).view(tiles, -1, 4, 16, 4).permute(0, 3, 1, 4, 2)
-    s = s.reshape(tiles * 16, -1)[:, :k // FP4_GROUP]
+    steps, chunks = weight.codes.shape[1], weight.scales.shape[1]
+    c = weight.codes.view(tiles, steps, 4, 16, 16).permute(0, 3, 1, 2, 4).reshape(tiles * 16, 64 * steps)[:, :k // 2]
+    s = weight.scales.view(torch.uint8).view(tiles, chunks, 4, 16, 4).permute(0, 3, 1, 4, 2)
+    s = s.reshape(tiles * 16, 16 * chunks)[:, :k // FP4_GROUP]
     if glu:
-        c, s = (t.reshape(-1, 2, 16, t.shape[1]).transpose(0, 1).reshape(2, -1, t.shape[1])[:, :n].flatten(0, 1)
-                for t in (c, s))
+        c, s = (t.reshape(tiles // 2, 2, 16, t.shape[1]).transpose(0, 1).reshape(2, tiles * 8, t.shape[1])[:, :n]
+                .flatten(0, 1) for t in (c, s))
     else:
         c, s = c[:n], s[:n]
     return c.contiguous(), s.contiguous().view(_E8)
@@ -1067,7 +1068,7 @@ def dequantize_fp4(codes: torch.Tensor, scales: torch.Tensor) -> torch.Tensor:
     n, k = _check_fp4_rows(codes, scales)
     value = torch.tensor([*FP4_MAGNITUDES, *(-v for v in FP4_MAGNITUDES)], device=codes.device)
     w = value[torch.stack([codes & 15, codes >> 4], -1).view(n, k).int()]
-    return (w.view(n, -1, FP4_GROUP) * scales.float()[..., None]).view(n, k)
+    return (w.view(n, k // FP4_GROUP, FP4_GROUP) * scales.float()[..., None]).view(n, k)
 
 
 def dequantize_rows_fp8(rows: Fp8Rows) -> torch.Tensor:
