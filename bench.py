@@ -77,8 +77,9 @@ def parse() -> argparse.Namespace:
     p.add_argument("--no-secondary", action="store_true", help="skip prefill and W8A8 figures")
     p.add_argument("--only", choices=["decode", "prefill", "w8a8", "glu", "attention",
                                       "lm-head", "decode-step", "decode-step-linears", "tp8",
-                                      "mid"],
-                   help="one family; decode-step is config 4 (a 32-layer model's decode step)")
+                                      "mid", "modes"],
+                   help="one family; decode-step is config 4 (a 32-layer model's decode step), modes "
+                        "the int8 and 4-bit modes side by side")
     p.add_argument("--summarize-profiles", nargs=3, metavar=("TRACE", "FETCH", "WRITE"),
                    help="summarize rocprofv3 output dirs of the decode sweep into profiles/")
     p.add_argument("--summarize-attention", metavar="TRACE",
@@ -1316,6 +1317,54 @@ def bench_decode_step_linears(pkg, dev, steps: int, layers: int = 32, batch: int
             "int8_linear_gbps": round(nbytes / t / 1e9, 1), "int8_linear_bytes": nbytes}
 
 
+MODE_MS = (1, 4, 16, 64, 256, 2048)
+
+
+def bench_modes(pkg, dev, steps: int, layers: int = 32, context: int = 1024) -> dict:
+    """The four quantization modes side by side on a random-init Llama-3-8B-architecture model, as `DecodeRunner` runs
+    them. `layer_us`: a decoder layer without its attention (both norms with their residual's addition, the four
+    products, and whatever rounds their rows, which o_proj and down_proj get in bf16 in every mode), over four layers'
+    weights in turn. `step_us`: a whole decode step of 32 layers and the lm_head, every sequence behind `context`
+    positions of an 8-bit K/V cache. Graph replays."""
+    import torch
+
+    from llm_serving_engine_amd.decode_step import DecodeRunner, random_llama
+
+    model = random_llama(layers, seed=4000, device=dev)
+    runners = {m: DecodeRunner(model, m, context + 16) for m in (1, 64)}
+    for r in runners.values():
+        r.enable_fp8_kv()
+    res: dict = {"layer_us": {}, "step_us": {}}
+    gen = torch.Generator().manual_seed(4002)
+    hid, inter = model.config.hidden_size, model.config.intermediate_size
+    for mode in ("int8", "w8a8", "w4a16", "w4a8"):
+        first, *others = runners.values()
+        first.quantize(mode)
+        backend = "fp4" if mode.startswith("w4") else "int8"
+        for r in others:
+            r.int8, r.fp4, r.head = first.int8, first.fp4, first.head
+        for r in runners.values():
+            r.use(backend)
+        first._fused = first._fusable()
+        row = res["layer_us"][mode] = {}
+        for m in MODE_MS:
+            x, y = (torch.randn(m, n, generator=gen).to(torch.bfloat16).to(dev) for n in (hid, inter))
+
+            def some_layers(x=x, y=y):
+                for i, layer in enumerate(first.layers[:4]):
+                    first._lin(i, "qkv", first._add_norm(layer.input_layernorm, x, x)[1])
+                    first._lin(i, "o", x)
+                    first._lin(i, "gate_up", first._add_norm(layer.post_attention_layernorm, x, x)[1])
+                    first._lin(i, "down", y)
+
+            row[f"M{m}"] = round(time_graph(some_layers, steps) / 4 * 1e6, 1)
+        row = res["step_us"][mode] = {}
+        for m, r in runners.items():
+            tokens = torch.zeros(m, dtype=torch.long, device=dev)
+            row[f"batch{m}"] = round(time_graph(lambda r=r, tokens=tokens: r.step(tokens, context), steps) * 1e6, 1)
+    return res
+
+
 def bench_decode_step(pkg, dev, steps: int, layers: int = 32, batch: int = 64,
                       context: int = 1024, decode_steps: int = 4) -> dict:
     """Config 4: a random-init Llama-3-8B-architecture model (lm_head bf16), `batch` sequences
@@ -1509,6 +1558,9 @@ def main() -> None:
         return
     if args.only == "mid":
         print(json.dumps({"mid_range": bench_mid_range(pkg, dev, args.steps, gen)}))
+        return
+    if args.only == "modes":
+        print(json.dumps({"modes": bench_modes(pkg, dev, args.steps)}))
         return
     if args.only == "tp8":
         print(json.dumps({"tp8_shard_shapes": bench_tp8_shards(pkg, dev, args.steps, gen),
