@@ -12,11 +12,12 @@
 // Tile order: blocks are dealt to the 8 XCDs in turn; each XCD gets a contiguous range of tiles, in groups of
 // kFp4GroupM token blocks x consecutive weight panels, so that what it runs at once shares token rows and weights in
 // its L2.
-// K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order.
+// K may be split over `splits` workgroups, whose fp32 sums a second kernel adds in order. They are neighbours in the grid,
+// so an XCD then has one range of K, of tiles out of two, four or all of the eight ranges of tiles.
 // A result depends on K, the groups and the split alone, never on other rows.
 //
-// What it measured: bf16 rows, 64 x 256 tiles, 2048 by two of 14336 x 4096 342 us, 1405 TFLOP/s, by 4096 x 14336 166,
-// 1450 (a large library product 1330 to 1380); 8-bit rows, 128 x 256 tiles, 2048 by two of 14336 x 4096 182 us, 2640
+// What it measured: bf16 rows, 64 x 256 tiles, 2048 by two of 14336 x 4096 343 us, 1400 TFLOP/s, by 4096 x 14336 166,
+// 1450 (a large library product 1330 to 1380); 8-bit rows, 128 x 256 tiles, 2048 by two of 14336 x 4096 184 us, 2610
 // TFLOP/s, by 4096 x 14336 92, 2610 (a library's fp8 2590 to 2930). The matrix cores bound these, but for the time around
 // the barriers: two workgroups of four waves share a CU, so that one runs while the other waits. One of eight waves, of
 // twice the tile, gave 205 us with 8-bit rows (256 x 256) and 345 with bf16 ones (128 x 256). Deeper rings (3, 4, 6 slots)
@@ -24,7 +25,7 @@
 //
 // A small tile's workgroup is often alone on its CU, a wave a SIMD, whose decoding, LDS reads and matrix instructions
 // then wait for each other: with bf16 rows they take two groups (256 rows by 4096 x 4096: 14.1 -> 11.1 us; 777 by
-// 2330 x 4128: 22.3 -> 20.1). What bounds them then is the CU's way from L2, 50 to 60 bytes a ns: 17 or 25 KB a stage.
+// 2330 x 4128: 22.3 -> 20.1). By their times 17 or 25 KB a stage then come from L2 at 50 to 60 bytes a ns.
 // 8-bit rows, half the bytes and no decoding, ran slower with two (12.5 -> 12.9) and keep one, with four slots.
 //
 // The compiler counts the weights' loads and waits for them in order, so it has to count the direct loads too, without
