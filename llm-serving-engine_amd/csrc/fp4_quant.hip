@@ -243,7 +243,9 @@ constexpr int64_t kMax31 = 2147483647;
 extern "C" {
 
 int64_t lse_fp4_codes_bytes(int64_t N, int64_t K, int64_t glu) {
-  if (N < 0 || K < 0 || K % lse::kFp4Group || (glu && N % 2) || N > kMax31 || K > LSE_FP4_MAX_K) return -1;
+  if (N < 0 || K < 0 || (glu != 0 && glu != 1) || (glu && N % 2) || K % lse::kFp4Group || N > kMax31 - 64 ||
+      K > LSE_FP4_MAX_K)
+    return -1;
   const int64_t tiles = glu ? 2 * lse::ceil_div(N / 2, 16) : lse::ceil_div(N, 16);
   return tiles * lse::ceil_div(K, lse::kFp4Step) * lse::kFp4TileBytes;
 }

@@ -36,3 +36,10 @@ def test_rows_in_8_bits_have_a_plan_of_their_own(pkg):
 def test_the_products_kinds_are_refused_alike(pkg, glu):
     assert _bytes(pkg, glu=glu) == -1 and _bytes(pkg, m=0, glu=glu) == -1
     assert _gemm(pkg, dict(glu=glu)) == E_SHAPE
+
+
+def test_tiles_sizes_are_of_weights_that_can_be_packed(pkg):
+    lib = pkg.library()
+    for size in (lib.lse_fp4_codes_bytes, lib.lse_fp4_scales_bytes):
+        assert size(100, 544, 1) > 0 and size(0, 544, 1) == size(100, 0, 0) == 0
+        assert size(100, 544, 2) == size(100, 544, -1) == size(99, 544, 1) == size((1 << 31) - 16, 544, 0) == -1
