@@ -17,6 +17,11 @@ TILE = re.compile(r"fp4_tile_kernelILb([01])ELi(\d+)ELi(\d+)ELi(\d+)ELi(\d+)ELb(
 LINE = re.compile(r"\s+([a-z]\w+)\s*(.*?)\s*// ([0-9A-F]+):(.*)")
 
 
+@pytest.fixture(scope="module")
+def listing(pkg, tmp_path_factory):
+    return _listing(pkg, tmp_path_factory.mktemp("code"))
+
+
 def _listing(pkg, folder) -> dict[str, list[tuple[int, str, str, int | None]]]:
     """The kernels of the built library: (address, instruction, operands, branch target) in order."""
     objdump = shutil.which("llvm-objdump") or "/opt/rocm/lib/llvm/bin/llvm-objdump"
@@ -77,9 +82,9 @@ def test_the_walk_counts_loads():
     assert _most_at_a_barrier(code) == 2
 
 
-def test_a_stages_rows_have_landed_at_its_barrier(pkg, tmp_path):
+def test_a_stages_rows_have_landed_at_its_barrier(listing):
     tiles = 0
-    for name, code in _listing(pkg, tmp_path).items():
+    for name, code in listing.items():
         if not (m := TILE.search(name)):
             continue
         rows8, bm, _, _, slots, _ = map(int, m.groups())
@@ -98,9 +103,9 @@ def _loads_right_after_m0(code) -> list[int]:
             and (re.search(r"\blds\b", b[2]) or "_lds_" in b[1])]
 
 
-def test_the_address_of_a_load_to_lds_is_there_before_it(pkg, tmp_path):
+def test_the_address_of_a_load_to_lds_is_there_before_it(listing):
     early = [(0, "s_add_u32", "m0, s1, 0x400", None), (4, "buffer_load_dword", "v1, s[0:3], 0 offen lds", None)]
     assert _loads_right_after_m0(early) == [4]
     assert not _loads_right_after_m0([early[0], (2, "s_nop", "0", None), early[1]])
-    found = {name: _loads_right_after_m0(code) for name, code in _listing(pkg, tmp_path).items()}
+    found = {name: _loads_right_after_m0(code) for name, code in listing.items()}
     assert not {name: len(at) for name, at in found.items() if at}
