@@ -75,16 +75,13 @@ __device__ __forceinline__ f32x4 mfma_fp4_fp8(uint4 w, uint32_t ws, uint4 lo, ui
 // One dword a lane to LDS byte address base + IMM (+ 4 l for lane l), as dma16_lds.
 template <int IMM>
 __device__ __forceinline__ void dma4_lds(u32x4 r, uint32_t base, uint32_t offset) {
-  uint32_t saved;
   asm volatile(
-      "s_mov_b32 %0, m0\n\t"
-      "s_add_u32 m0, %1, %4\n\t"
+      "s_add_u32 m0, %0, %3\n\t"
       "s_nop 0\n\t"
-      "buffer_load_dword %2, %3, 0 offen lds\n\t"
-      "s_mov_b32 m0, %0"
-      : "=&s"(saved)
+      "buffer_load_dword %1, %2, 0 offen lds"
+      :
       : "s"(base), "v"(offset), "s"(r), "i"(IMM)
-      : "memory", "scc");
+      : "memory", "scc", "m0");
 }
 
 // Rows of one step in LDS: 256 (bf16) or 128 (codes) bytes, their 16-byte chunk c at c ^ fp4_swz(row), rows in 16s. A

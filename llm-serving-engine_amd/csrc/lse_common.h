@@ -205,7 +205,7 @@ __device__ __forceinline__ void buffer_load16_lds(BufferRsrc r, void* lds, uint3
 // The same load with the buffer descriptor as four dwords, issued from inline assembly. The
 // compiler then does not track the LDS write, so it inserts no waits of its own between these
 // loads and later LDS reads: the caller orders them with explicit s_waitcnt vmcnt counts and
-// barriers (vmcnt drops when the data is in LDS). M0 carries the LDS address and is restored.
+// barriers (vmcnt drops when the data is in LDS). M0 carries the LDS address; the compiler sets it anew where it needs it.
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ u32x4 make_rsrc4(const void* base, uint32_t bytes) {
@@ -221,30 +221,27 @@ __device__ __forceinline__ uint32_t lds_addr(const void* lds) {
 
 // One load to LDS byte address base + IMM (+ 16 l for lane l); NT: the streaming (nt) cache
 // policy, for data read once per call. A load to LDS needs one wait state after a scalar
-// instruction that writes M0, which the compiler cannot put into the block.
+// instruction that writes M0, which the compiler cannot put into the block. With M0 saved and
+// restored around each load instead of clobbered, prompts took 0.5 to 1 % longer, 64 rows by
+// 4096 x 28672 2.5 % (28.7 against 29.5 us).
 template <int IMM, bool NT = false>
 __device__ __forceinline__ void dma16_lds(u32x4 r, uint32_t base, uint32_t offset) {
-  uint32_t saved;
   if constexpr (NT) {
     asm volatile(
-        "s_mov_b32 %0, m0\n\t"
-        "s_add_u32 m0, %1, %4\n\t"
+        "s_add_u32 m0, %0, %3\n\t"
         "s_nop 0\n\t"
-        "buffer_load_dwordx4 %2, %3, 0 offen nt lds\n\t"
-        "s_mov_b32 m0, %0"
-        : "=&s"(saved)
+        "buffer_load_dwordx4 %1, %2, 0 offen nt lds"
+        :
         : "s"(base), "v"(offset), "s"(r), "i"(IMM)
-        : "memory", "scc");
+        : "memory", "scc", "m0");
   } else {
     asm volatile(
-        "s_mov_b32 %0, m0\n\t"
-        "s_add_u32 m0, %1, %4\n\t"
+        "s_add_u32 m0, %0, %3\n\t"
         "s_nop 0\n\t"
-        "buffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
-        "s_mov_b32 m0, %0"
-        : "=&s"(saved)
+        "buffer_load_dwordx4 %1, %2, 0 offen lds"
+        :
         : "s"(base), "v"(offset), "s"(r), "i"(IMM)
-        : "memory", "scc");
+        : "memory", "scc", "m0");
   }
 }
 
